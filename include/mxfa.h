@@ -52,7 +52,7 @@ typedef enum {
     MXFA_ERR_ALIGN = -5,       /* a device pointer is not 16-byte aligned */
     MXFA_ERR_LAUNCH = -6,      /* the HIP runtime rejected a launch */
     MXFA_ERR_DEVICE = -7,      /* no usable gfx950 device */
-    MXFA_ERR_WORKSPACE = -8,   /* a workspace smaller than mxfa_{bwd,prefill}_workspace_bytes(shape) */
+    MXFA_ERR_WORKSPACE = -8,   /* a workspace smaller than mxfa_{bwd,prefill,prefill_batch}_workspace_bytes(shape) */
     MXFA_ERR_CODE_OBJECT = -9, /* the gfx950 code object is missing, malformed, for another
                                   processor, or lacks a kernel */
     MXFA_ERR_SCRATCH = -10     /* mxfa_run_bwd_noalloc: the shape needs more than
@@ -381,6 +381,142 @@ int mxfa_run_prefill_ws(const mxfa_prefill_shape *shape, const void *q, const vo
 int mxfa_run_prefill_paged_ws(const mxfa_prefill_shape *shape, const void *q, const void *kcache,
                               const void *vcache, void *out, const int *block_table, int block_size,
                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- Rotary positions. Pair i of a head's first rotary_dim elements, (x1, x2)
+ * = (x[i], x[i + rotary_dim / 2]) or, interleaved, (x[2i], x[2i + 1]), turns by
+ * a = position * frequencies[i] (radians; the product is formed in 64 bits):
+ *     y1 = factor (x1 cos a - x2 sin a),  y2 = factor (x2 cos a + x1 sin a);
+ * the other elements are copied. inverse = 1 turns by -a with the same factor:
+ * the transpose, which takes the gradients of the outputs to the inputs'. */
+typedef struct {
+    int B, Hq, Hkv, N; /* heads of Q and of K; Hkv = 0: Q alone */
+    int head_dim;      /* a multiple of 8, at most 256 */
+    int rotary_dim;    /* even, 2 .. head_dim */
+    int interleaved;   /* 0 or 1 */
+    int inverse;       /* 0 or 1 */
+    int dtype;         /* mxfa_dtype */
+    int pos0;          /* without positions: token n is at pos0 + n */
+    float factor;      /* multiplies cosines and sines (1: a plain rotation) */
+    /* strides in elements between batches, heads and tokens, of Q, K and their
+     * outputs; rows are contiguous and start on 16-byte boundaries. Dimensions
+     * of one element have no stride (any value). Outputs' strides are >= 0. */
+    long long q_bs, q_hs, q_ts, k_bs, k_hs, k_ts;
+    long long qo_bs, qo_hs, qo_ts, ko_bs, ko_hs, ko_ts;
+    long long pos_bs; /* positions: elements between batches (0: shared) */
+} mxfa_rotary_shape;
+int mxfa_check_rotary(const mxfa_rotary_shape *shape);
+/* One launch for Q and K. positions: int32 on the device, N per batch, any
+ * sign; NULL: pos0 + n. frequencies: rotary_dim / 2 doubles on the device.
+ * An output may be its own input (the same pointer and strides); an output
+ * that overlaps its input otherwise gives MXFA_ERR_UNSUPPORTED, and Q and K
+ * outputs must not overlap each other or the other's input (not checked: they
+ * may be columns of the same rows). */
+int mxfa_run_rotary(const mxfa_rotary_shape *shape, const void *q, const void *k, void *q_out, void *k_out,
+                    const int *positions, const double *frequencies, void *stream);
+
+/* ---- A batch of sequences over a paged KV cache. Sequence s has the rows
+ * cu_q[s] .. cu_q[s + 1] - 1 of the batch's new tokens (cu_q[0] = 0; int32 on
+ * the device, n_seq + 1 of them) and lens[s] positions in all, the new ones
+ * the last: its i-th new token is at lens[s] - (cu_q[s + 1] - cu_q[s]) + i.
+ * Position t's K and V are in cache row block_table[s * table_stride + t /
+ * block_size] * block_size + t % block_size. The device arrays are read when
+ * the kernels run, so a captured launch follows what they hold at each replay.
+ * Nothing outside the buffers is accessed whatever they hold: rows past n_tok,
+ * positions past the table and blocks outside the pool are left out when
+ * written; when read, such a block counts as the nearest one in the pool and
+ * positions past the table as not there, and the sequence's outputs are then
+ * not specified. Rows past cu_q[n_seq] are left as they were. */
+typedef struct {
+    int n_tok;        /* rows of q / qkv and of the output */
+    int n_seq;        /* sequences */
+    int max_q;        /* attention: at least the most new tokens of a sequence;
+                         rows past it are left as they were */
+    int n_head, n_kv_head, head_dim;
+    int block_size;   /* tokens per block, a power of two */
+    int n_blocks;     /* blocks in the caches */
+    int max_blocks;   /* entries of a block_table row */
+    int table_stride; /* elements between block_table rows, >= max_blocks */
+    int q_stride;     /* elements between rows of q / qkv */
+    int kv_stride;    /* elements between cache rows */
+    int out_stride;   /* elements between output rows */
+    int dtype;        /* mxfa_dtype */
+    float scale;      /* attention: 0 -> 1/sqrt(head_dim) */
+} mxfa_batch_shape;
+/* As mxfa_run_prefill_batch checks it. */
+int mxfa_check_batch(const mxfa_batch_shape *shape);
+
+/* Attention of the batch's new tokens over the cache: the token at position t
+ * of its sequence attends to the positions 0 .. t (K and V of the new tokens
+ * included, as mxfa_run_cache_append writes them). Query row r holds head h at
+ * elements [h * head_dim, (h + 1) * head_dim), a cache row KV head h, the
+ * output row likewise; head_dim 64 (fp32, bf16) or 128 (bf16). A row that sees
+ * no position (a token at a negative one) is zeros, its lse -infinity. lse:
+ * NULL, or n_tok x n_head floats. A position that a row does not see never
+ * reaches it, whatever its K and V hold. The workspace
+ * (mxfa_prefill_batch_workspace_bytes, 16-byte aligned, no contents needed) is
+ * used until the call completes: calls that may overlap need their own. The
+ * key ranges of long sequences are joined in a fixed order: equal calls give
+ * equal bits. */
+size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *shape);
+int mxfa_run_prefill_batch(const mxfa_batch_shape *shape, const void *q, const void *kcache, const void *vcache,
+                           void *out, float *lse, const int *block_table, const int *cu_q, const int *lens,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* The cache append: row r of qkv holds token r's n_head query heads, then its
+ * n_kv_head key heads, then its value heads; Q turns into q_out row r, K turns
+ * into kcache and V is copied into vcache, at the rows of the tokens'
+ * positions. rotary_dim = 0 (frequencies NULL): copies only. head_dim as for
+ * mxfa_rotary_shape. q_out may be qkv (the same pointer and stride); any other
+ * overlap of q_out, kcache or vcache with qkv or each other is the caller's to
+ * avoid. */
+typedef struct {
+    int rotary_dim, interleaved;
+    float factor;
+    const double *frequencies; /* device, rotary_dim / 2 */
+} mxfa_append_rotary;
+int mxfa_run_cache_append(const mxfa_batch_shape *shape, const mxfa_append_rotary *rotary, const void *qkv,
+                          void *q_out, void *kcache, void *vcache, const int *block_table, const int *cu_q,
+                          const int *lens, void *stream);
+
+/* ---- The pages of a cache: block tables (int32, table_stride elements between
+ * rows), lengths and use counts of the blocks (int32 per block, how many table
+ * rows hold it), all on the device. A sequence of lens[s] tokens holds its
+ * row's first ceil(lens[s] / block_size) entries. */
+typedef struct {
+    int n_seq, max_blocks, table_stride, block_size, n_blocks;
+} mxfa_pages_shape;
+int mxfa_check_pages(const mxfa_pages_shape *shape);
+/* The sequences rows[0 .. n - 1] end: the counts of their blocks go down, their
+ * table entries become -1 and their lengths 0. Rows outside 0 .. n_seq - 1 are
+ * skipped; a row named twice ends once. */
+int mxfa_run_pages_free(const mxfa_pages_shape *shape, int *block_table, int *lens, int *refs, const int *rows, int n,
+                        void *stream);
+/* Row children[i] becomes a continuation of row parents[i]: it shares the
+ * parent's whole blocks (their counts go up), and a last block that is not
+ * full is to be copied to the lowest block that nobody uses (in the order of
+ * the pairs). pairs[2j], pairs[2j + 1]: the j-th copy's source and destination
+ * (n pairs of space); counts[0]: the copies, counts[1]: the refused pairs;
+ * status[i]: 0, or 1 where the pair was refused and nothing done for it: a
+ * row out of range, a child whose length is not 0, a child that an earlier
+ * pair names, a parent longer than its row, or no block left. Parents count
+ * as they were before the call. */
+int mxfa_run_pages_fork(const mxfa_pages_shape *shape, int *block_table, int *lens, int *refs, const int *parents,
+                        const int *children, int n, int *pairs, int *status, int *counts, void *stream);
+/* The used blocks to the pool's low end: with L blocks in use, the j-th used
+ * one at or above L moves to the j-th unused one below it. Writes the tables
+ * and counts as they are after the moves (new_table may be block_table;
+ * new_refs may not be refs), the moves to pairs (n_blocks / 2 pairs of space,
+ * at least one), and to counts how many and L. Until the blocks that were left
+ * are used again, the old tables stay valid too. */
+int mxfa_run_pages_compact(const mxfa_pages_shape *shape, const int *block_table, const int *lens, const int *refs,
+                           int *new_table, int new_stride, int *new_refs, int *pairs, int *counts, void *stream);
+/* Copies block pairs[2j] to block pairs[2j + 1], j < n_pairs (and < *count,
+ * where count is not NULL: a device int), in each of n_pools pools pool_bytes
+ * apart, of n_blocks blocks of block_bytes bytes. Pairs with a number outside
+ * the pool are skipped. No destination may be another pair's source or
+ * destination (not checked; the two calls above give none). */
+int mxfa_run_pages_copy(void *pools, int n_pools, long long pool_bytes, int n_blocks, long long block_bytes,
+                        const int *pairs, int n_pairs, const int *count, void *stream);
 
 #ifdef __cplusplus
 }

@@ -59,6 +59,9 @@ EXPORTS = (
     "mxfa_run_prefill_paged", "mxfa_prefill_workspace_bytes", "mxfa_run_prefill_ws", "mxfa_run_prefill_paged_ws",
     "mxfa_set_bwd_options", "mxfa_get_bwd_options", "mxfa_bwd_delta_fallbacks", "mxfa_bwd_reduce_timeouts",
     "mxfa_run_bwd_noalloc", "mxfa_bwd_noalloc_scratch_bytes",
+    "mxfa_check_rotary", "mxfa_run_rotary", "mxfa_check_batch", "mxfa_prefill_batch_workspace_bytes",
+    "mxfa_run_prefill_batch", "mxfa_run_cache_append", "mxfa_check_pages", "mxfa_run_pages_free",
+    "mxfa_run_pages_fork", "mxfa_run_pages_compact", "mxfa_run_pages_copy",
 )
 # Every symbol include/mxfa_probes.h declares.
 PROBE_EXPORTS = (
@@ -90,6 +93,28 @@ class MxfaPrefillShape(ctypes.Structure):
                 ("head_dim", ctypes.c_int), ("pos0", ctypes.c_int), ("q_stride", ctypes.c_int),
                 ("kv_stride", ctypes.c_int), ("out_stride", ctypes.c_int), ("dtype", ctypes.c_int),
                 ("scale", ctypes.c_float)]
+
+
+class MxfaRotaryShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("B", "Hq", "Hkv", "N", "head_dim", "rotary_dim", "interleaved", "inverse",
+                                            "dtype", "pos0")] + [("factor", ctypes.c_float)] + \
+               [(n, ctypes.c_longlong) for n in ("q_bs", "q_hs", "q_ts", "k_bs", "k_hs", "k_ts", "qo_bs", "qo_hs",
+                                                 "qo_ts", "ko_bs", "ko_hs", "ko_ts", "pos_bs")]
+
+
+class MxfaBatchShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_tok", "n_seq", "max_q", "n_head", "n_kv_head", "head_dim", "block_size",
+                                            "n_blocks", "max_blocks", "table_stride", "q_stride", "kv_stride",
+                                            "out_stride", "dtype")] + [("scale", ctypes.c_float)]
+
+
+class MxfaAppendRotary(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("factor", ctypes.c_float),
+                ("frequencies", ctypes.c_void_p)]
+
+
+class MxfaPagesShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "max_blocks", "table_stride", "block_size", "n_blocks")]
 
 
 _lib = None
@@ -160,6 +185,20 @@ def load_library(path: str | None = None):
     lib.mxfa_probe_copy.argtypes = [vp, vp, ctypes.c_size_t, vp]
     lib.mxfa_probe_dq_atomic.argtypes = [fp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                          ctypes.POINTER(ctypes.c_double), vp]
+    rp, bp, gp = (ctypes.POINTER(t) for t in (MxfaRotaryShape, MxfaBatchShape, MxfaPagesShape))
+    ci, cl = ctypes.c_int, ctypes.c_longlong
+    lib.mxfa_check_rotary.argtypes = [rp]
+    lib.mxfa_run_rotary.argtypes = [rp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mxfa_check_batch.argtypes = [bp]
+    lib.mxfa_prefill_batch_workspace_bytes.argtypes = [bp]
+    lib.mxfa_prefill_batch_workspace_bytes.restype = ctypes.c_size_t
+    lib.mxfa_run_prefill_batch.argtypes = [bp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.mxfa_run_cache_append.argtypes = [bp, ctypes.POINTER(MxfaAppendRotary), vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mxfa_check_pages.argtypes = [gp]
+    lib.mxfa_run_pages_free.argtypes = [gp, vp, vp, vp, vp, ci, vp]
+    lib.mxfa_run_pages_fork.argtypes = [gp, vp, vp, vp, vp, vp, ci, vp, vp, vp, vp]
+    lib.mxfa_run_pages_compact.argtypes = [gp, vp, vp, vp, vp, ci, vp, vp, vp, vp]
+    lib.mxfa_run_pages_copy.argtypes = [vp, ci, cl, ci, cl, vp, ci, vp, vp]
     op = ctypes.POINTER(MxfaBwdOptions)
     lib.mxfa_set_bwd_options.argtypes = [op]
     lib.mxfa_get_bwd_options.argtypes = [op]
@@ -168,7 +207,7 @@ def load_library(path: str | None = None):
     for name in EXPORTS + PROBE_EXPORTS:
         if name not in ("mxfa_version", "mxfa_strerror", "mxfa_bwd_workspace_bytes",
                         "mxfa_naive_scratch_bytes", "mxfa_bwd_noalloc_scratch_bytes",
-                        "mxfa_prefill_workspace_bytes"):
+                        "mxfa_prefill_workspace_bytes", "mxfa_prefill_batch_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_int
     if path is None:
         _lib = lib
@@ -186,6 +225,7 @@ class _NoBinding:
     def _other(*args):
         return NotImplemented
     attention_fwd = attention_bwd = prefill = _other
+    rotary = cache_append = prefill_batch = pages_free = pages_fork = pages_compact = pages_copy = _other
 
 
 def _calls():
@@ -208,7 +248,9 @@ def _calls():
             return _native
         ext.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
             "mxfa_run_flash_lse", "mxfa_run_bwd_ws", "mxfa_bwd_workspace_bytes", "mxfa_run_prefill",
-            "mxfa_run_prefill_ws", "mxfa_run_prefill_paged", "mxfa_run_prefill_paged_ws")))
+            "mxfa_run_prefill_ws", "mxfa_run_prefill_paged", "mxfa_run_prefill_paged_ws", "mxfa_run_rotary",
+            "mxfa_run_cache_append", "mxfa_run_prefill_batch", "mxfa_prefill_batch_workspace_bytes",
+            "mxfa_run_pages_free", "mxfa_run_pages_fork", "mxfa_run_pages_compact", "mxfa_run_pages_copy")))
         _native = ext
     return _native
 
@@ -766,6 +808,402 @@ def run_prefill_split(q, kcache, vcache, out, pos0: int, n_head: int, n_kv_head:
            lib.mxfa_run_prefill_ws(ctypes.byref(sh), qp, kp, vp, op, ctypes.c_void_p(workspace.data_ptr()),
                                    have, _stream(stream)))
     return workspace
+
+
+# ------------------------------------------------------------ rotary positions --
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int = 4096, fast_turns: float = 32.0, slow_turns: float = 1.0, device="cuda"):
+    """The angles per position (radians, float64, dim / 2 of them) that run_rotary
+    and run_cache_append take, and the factor of the rotation, as (frequencies,
+    factor): base^(-2i / dim), and for contexts `factor` times as long as
+    the model's own
+
+    * scaling="linear": positions compressed, every frequency divided by factor;
+    * "base": base times factor^(dim / (dim - 2)), which leaves the fastest pair
+      as it is and divides the slowest by factor;
+    * "yarn": divided by factor where a pair turns at most slow_turns times over
+      original_length positions, left where it turns fast_turns times or more,
+      in between in proportion to the pair's index; the rotation's factor is
+      0.1 ln(factor) + 1.
+
+    Computed on the host, once per model."""
+    import math
+    torch = _torch()
+    if dim < 2 or dim % 2:
+        raise ValueError(f"dim {dim}: must be even and positive")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError("base must be above 1 and factor at least 1")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    if scaling == "base":
+        if dim == 2:
+            raise ValueError('scaling="base" needs more than one pair')
+        base = base * factor ** (dim / (dim - 2))
+    f = base ** (-i / dim)
+    amount = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        def pair(turns):  # the pair that turns so often over original_length
+            return dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo, hi = max(math.floor(pair(fast_turns)), 0), min(math.ceil(pair(slow_turns)), dim - 1)
+        ramp = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        f = f / factor * ramp + f * (1 - ramp)
+        amount = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"scaling {scaling!r}: None, 'linear', 'base' or 'yarn' expected")
+    return f.to(device), amount
+
+
+def _on(device):
+    """Runs launches on `device` (its current stream) where it is not the
+    calling thread's."""
+    torch = _torch()
+    import contextlib
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _dev(t, name, dtype=None, like=None):
+    """A device tensor of the dtype, on `like`'s device."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name}: must be a device tensor (got {t.device}); there is no CPU path")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name}: on {t.device}, the other tensors on {like.device}")
+    return t
+
+
+def _ints(t, name, n, like):
+    """A contiguous int32 vector of at least n elements."""
+    torch = _torch()
+    _dev(t, name, torch.int32, like)
+    if t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1) or t.numel() < n:
+        raise ValueError(f"{name}: expected a contiguous int32 vector of at least {n} elements, got shape "
+                         f"{tuple(t.shape)} strides {t.stride()}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _freqs(frequencies, dim_max, like):
+    """(pointer, rotary_dim) of a frequencies vector."""
+    torch = _torch()
+    _dev(frequencies, "frequencies", torch.float64, like)
+    if frequencies.dim() != 1 or not frequencies.is_contiguous() or not 1 <= frequencies.numel() <= dim_max // 2:
+        raise ValueError(f"frequencies: expected a contiguous vector of 1 to {dim_max // 2} elements (half of what is "
+                         f"rotated), got shape {tuple(frequencies.shape)}")
+    return ctypes.c_void_p(frequencies.data_ptr()), 2 * frequencies.numel()
+
+
+def _heads(t, name):
+    """[B, H, N, d], or [N, H, d] (tokens first) as B = 1: (pointer, sizes, strides)."""
+    if t.dim() == 3:
+        n, h, d = t.shape
+        sizes, strides = (1, h, n, d), (0, t.stride(1), t.stride(0))
+    elif t.dim() == 4:
+        sizes, strides = tuple(t.shape), t.stride()[:3]
+    else:
+        raise ValueError(f"{name}: expected [B, H, N, d] or [N, H, d], got {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: rows must be contiguous (strides {t.stride()})")
+    return ctypes.c_void_p(t.data_ptr()), sizes, strides
+
+
+def run_rotary(q, k, q_out, k_out, frequencies, positions=None, pos0: int = 0, interleaved: bool = False,
+               factor: float = 1.0, inverse: bool = False, stream=None):
+    """mxfa_run_rotary: rotary positions of Q and K (k and k_out None: Q alone)
+    in one launch. Pair i of a head's first 2 len(frequencies) elements, (x[i],
+    x[i + len(frequencies)]) or with interleaved (x[2i], x[2i + 1]), turns by
+    position * frequencies[i] and is multiplied by factor; the rest is copied.
+
+    q, k and their outputs: [B, H, N, d], or [N, H, d] with the tokens first;
+    rows contiguous, any other strides (views of a fused QKV buffer; an output
+    may be its input), starting on 16 bytes. bf16 or fp32, d a multiple of 8 up
+    to 256. frequencies: float64 on the device (rotary_frequencies).
+    positions: int32, [N] or [B, N]; None: token n at pos0 + n. inverse: the
+    transpose (gradients of the outputs to gradients of the inputs)."""
+    torch = _torch()
+    if stream is None:
+        rc = _calls().rotary(q, k, q_out, k_out, frequencies, positions, pos0, interleaved, factor, inverse)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_rotary", rc)
+    _dev(q, "q")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"q: dtype {q.dtype}; bf16 or float32 expected")
+    qp, (B, Hq, N, d), qs = _heads(q, "q")
+    qop, osz, qos = _heads(_dev(q_out, "q_out", q.dtype, q), "q_out")
+    if osz != (B, Hq, N, d):
+        raise ValueError(f"q_out: shape {tuple(q_out.shape)} does not match q's {tuple(q.shape)}")
+    if (k is None) != (k_out is None):
+        raise ValueError("k and k_out: both or neither")
+    kp = kop = None
+    Hkv, ks, kos = 0, (0, 0, 0), (0, 0, 0)
+    if k is not None:
+        kp, (Bk, Hkv, Nk, dk), ks = _heads(_dev(k, "k", q.dtype, q), "k")
+        if (Bk, Nk, dk) != (B, N, d):
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} disagree")
+        kop, osz, kos = _heads(_dev(k_out, "k_out", q.dtype, q), "k_out")
+        if osz != (B, Hkv, N, d):
+            raise ValueError(f"k_out: shape {tuple(k_out.shape)} does not match k's {tuple(k.shape)}")
+    fp, dim = _freqs(frequencies, d, q)
+    pp, pbs = None, 0
+    if positions is not None:
+        _dev(positions, "positions", torch.int32, q)
+        if tuple(positions.shape) not in ((N,), (B, N)) or (N > 1 and positions.stride(-1) != 1):
+            raise ValueError(f"positions: expected [{N}] or [{B}, {N}] with contiguous rows, got "
+                             f"{tuple(positions.shape)} strides {positions.stride()}")
+        pp, pbs = ctypes.c_void_p(positions.data_ptr()), positions.stride(0) if positions.dim() == 2 else 0
+    sh = MxfaRotaryShape(B, Hq, Hkv, N, d, dim, int(bool(interleaved)), int(bool(inverse)),
+                         MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, pos0, factor, *qs, *ks, *qos, *kos, pbs)
+    with _on(q.device):
+        _check("mxfa_run_rotary", load_library().mxfa_run_rotary(ctypes.byref(sh), qp, kp, qop, kop, pp, fp,
+                                                                 _stream(stream)))
+
+
+# ------------------------------------------------- a batch over a paged cache --
+
+def _block_table(block_table, n_seq, like):
+    """A 2-D int32 table of contiguous rows: (pointer, entries of a row, row stride)."""
+    torch = _torch()
+    _dev(block_table, "block_table", torch.int32, like)
+    if block_table.dim() != 2 or block_table.shape[1] < 1 or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table: expected a 2-D int32 tensor with contiguous rows, got shape "
+                         f"{tuple(block_table.shape)} strides {block_table.stride()}")
+    if block_table.shape[0] != n_seq:
+        raise ValueError(f"block_table: {block_table.shape[0]} rows for {n_seq} sequences")
+    wide = block_table.shape[1]
+    return ctypes.c_void_p(block_table.data_ptr()), wide, block_table.stride(0) if n_seq > 1 else wide
+
+
+def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head, n_kv_head,
+                head_dim, scale):
+    torch = _torch()
+    _dev(q, "q")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"q: dtype {q.dtype}; bf16 or float32 expected")
+    if n_head < 1 or n_kv_head < 1 or head_dim < 1 or block_size < 1:
+        raise ValueError("n_head, n_kv_head, head_dim and block_size must be positive")
+    n_tok = q.shape[0] if q.dim() == 2 else -1
+    qp, qs = _rows(q, "q", q.dtype, 1, q_cols * head_dim)
+    kp, ks = _rows(_dev(kcache, "kcache", q.dtype, q), "kcache", q.dtype, block_size, n_kv_head * head_dim)
+    vp, vs = _rows(_dev(vcache, "vcache", q.dtype, q), "vcache", q.dtype, block_size, n_kv_head * head_dim)
+    if ks != vs or kcache.shape[0] != vcache.shape[0]:
+        raise ValueError(f"kcache and vcache must share their rows and row stride ({kcache.shape[0]}, {ks} and "
+                         f"{vcache.shape[0]}, {vs})")
+    op, os_ = _rows(_dev(out, "out", q.dtype, q), "out", q.dtype, n_tok, n_head * head_dim)
+    n_seq = lens.numel() if isinstance(lens, torch.Tensor) else 0
+    lp = _ints(lens, "lens", 1, q)
+    cp = _ints(cu_q, "cu_q", n_seq + 1, q)
+    tp, wide, ts = _block_table(block_table, n_seq, q)
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, kcache.shape[0] // block_size,
+                        wide, ts, qs, ks, os_, MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
+    return sh, qp, kp, vp, op, tp, cp, lp
+
+
+def run_cache_append(qkv, q_out, kcache, vcache, block_table, block_size: int, cu_q, lens, n_head: int, n_kv_head: int,
+                     head_dim: int = 64, frequencies=None, interleaved: bool = False, factor: float = 1.0,
+                     stream=None):
+    """mxfa_run_cache_append: the new tokens of a batch of sequences enter the paged
+    cache, with rotary positions, in one launch: of each row of qkv the query
+    heads turn into q_out (which may be qkv), the key heads turn into kcache and
+    the value heads are copied into vcache, at the row of the token's position.
+    This is what run_prefill_batch (or run_prefill_paged) then reads.
+
+    qkv: [n_tok, >= (n_head + 2 n_kv_head) head_dim], q_out: [n_tok, >= n_head
+    head_dim], kcache, vcache: [pool rows, >= n_kv_head head_dim] with one row
+    stride; block_table: int32 [n_seq, entries]; cu_q: int32 [n_seq + 1], where
+    each sequence's rows of qkv begin and the last end; lens: int32 [n_seq],
+    the sequences' lengths with their new tokens. frequencies: as for
+    run_rotary; None copies without turning. bf16 or fp32."""
+    if stream is None:
+        rc = _calls().cache_append(qkv, q_out, kcache, vcache, block_table, block_size, cu_q, lens, n_head, n_kv_head,
+                                   head_dim, frequencies, interleaved, factor)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_cache_append", rc)
+    sh, qp, kp, vp, op, tp, cp, lp = _batch_args(qkv, n_head + 2 * n_kv_head, kcache, vcache, q_out, block_table,
+                                                 block_size, cu_q, lens, 1, n_head, n_kv_head, head_dim, 0.0)
+    fp, dim = (None, 0) if frequencies is None else _freqs(frequencies, head_dim, qkv)
+    rot = MxfaAppendRotary(dim, int(bool(interleaved)), factor, fp)
+    with _on(qkv.device):
+        _check("mxfa_run_cache_append",
+               load_library().mxfa_run_cache_append(ctypes.byref(sh), ctypes.byref(rot), qp, op, kp, vp, tp, cp, lp,
+                                                    _stream(stream)))
+
+
+def prefill_batch_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head: int, n_kv_head: int, head_dim: int = 64,
+                                  bf16: bool = True) -> int:
+    """mxfa_prefill_batch_workspace_bytes: what run_prefill_batch needs for such a
+    batch, whatever its lengths (0 for one it does not take)."""
+    w = n_head * head_dim
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, 1, 1, w, n_kv_head * head_dim, w,
+                        MXFA_BF16 if bf16 else MXFA_F32, 0.0)
+    return int(load_library().mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh)))
+
+
+def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q, lens, max_q: int, n_head: int,
+                      n_kv_head: int, head_dim: int = 64, scale: float = 0.0, lse=None, workspace=None, stream=None):
+    """mxfa_run_prefill_batch: attention of a batch of sequences' new tokens (one
+    token, a chunk, or both side by side) over the paged cache: a token attends
+    to its sequence's positions up to its own, which the cache holds
+    (run_cache_append). Lengths and tables are read on the device.
+
+    q: [n_tok, >= n_head head_dim] (may be the columns of a fused QKV buffer),
+    out likewise; the caches, block_table, cu_q and lens as for
+    run_cache_append; max_q: at least the most new tokens any sequence has
+    (rows past it are not computed). lse: None, or float32 [n_tok, n_head] for
+    the rows' log-sum-exp. workspace: a contiguous device tensor of
+    prefill_batch_workspace_bytes bytes (allocated when None); returned. Calls
+    that may overlap need their own. bf16 with head_dim 64 or 128, or fp32 with
+    64."""
+    torch = _torch()
+    if stream is None:
+        rc = _calls().prefill_batch(q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head,
+                                    n_kv_head, head_dim, scale, lse, workspace)
+        if rc is not NotImplemented:
+            if isinstance(rc, int):
+                _check("mxfa_run_prefill_batch", rc)
+            return rc
+    sh, qp, kp, vp, op, tp, cp, lp = _batch_args(q, n_head, kcache, vcache, out, block_table, block_size, cu_q, lens,
+                                                 max_q, n_head, n_kv_head, head_dim, scale)
+    ep = None
+    if lse is not None:
+        _dev(lse, "lse", torch.float32, q)
+        if tuple(lse.shape) != (sh.n_tok, n_head) or not lse.is_contiguous():
+            raise ValueError(f"lse: expected a contiguous [{sh.n_tok}, {n_head}], got {tuple(lse.shape)}")
+        ep = ctypes.c_void_p(lse.data_ptr())
+    lib = load_library()
+    _check("mxfa_check_batch", lib.mxfa_check_batch(ctypes.byref(sh)))
+    with _on(q.device):
+        if workspace is None:
+            workspace = torch.empty(int(lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh))), dtype=torch.uint8,
+                                    device=q.device)
+            if stream is not None:
+                workspace.record_stream(stream)
+        elif not _dev(workspace, "workspace", None, q).is_contiguous():
+            raise ValueError("workspace: expected a contiguous device tensor")
+        _check("mxfa_run_prefill_batch",
+               lib.mxfa_run_prefill_batch(ctypes.byref(sh), qp, kp, vp, op, ep, tp, cp, lp,
+                                          ctypes.c_void_p(workspace.data_ptr()),
+                                          workspace.numel() * workspace.element_size(), _stream(stream)))
+    return workspace
+
+
+# ------------------------------------------------------- the pages of a cache --
+
+def _pages_args(block_table, block_size, lens, refs):
+    torch = _torch()
+    _dev(lens, "lens", torch.int32)
+    tp, wide, ts = _block_table(block_table, lens.numel(), lens)
+    sh = MxfaPagesShape(lens.numel(), wide, ts, block_size, refs.numel() if isinstance(refs, torch.Tensor) else 0)
+    return sh, tp, _ints(lens, "lens", 1, lens), _ints(refs, "refs", 1, lens)
+
+
+def run_pages_free(block_table, block_size: int, lens, refs, rows, stream=None):
+    """mxfa_run_pages_free: the sequences named in rows (int32) end: the use counts
+    (refs, int32 per block of the pool) of the blocks they hold go down by one,
+    their block_table entries become -1 and their lens 0. Row numbers out of
+    range are skipped, a row named twice ends once."""
+    if stream is None:
+        rc = _calls().pages_free(block_table, block_size, lens, refs, rows)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_pages_free", rc)
+    sh, tp, lp, rp = _pages_args(block_table, block_size, lens, refs)
+    n = _ints(rows, "rows", 0, lens)
+    with _on(lens.device):
+        _check("mxfa_run_pages_free", load_library().mxfa_run_pages_free(ctypes.byref(sh), tp, lp, rp, n, rows.numel(),
+                                                                         _stream(stream)))
+
+
+def run_pages_fork(block_table, block_size: int, lens, refs, parents, children, pairs, status, counts, stream=None):
+    """mxfa_run_pages_fork: row children[i] (an empty one) becomes a continuation of
+    row parents[i]: it shares the parent's whole blocks, and a last block that is
+    not full is given a copy, in the lowest block that nobody uses. The copies
+    are written to pairs (int32 [n, 2]: source, destination) and their number to
+    counts[0]; run_pages_copy(pool, block_size, pairs, counts) then makes them,
+    in each pool of the cache. status[i] (int32 [n]): 0, or 1 where a pair was
+    refused (a row out of range, a child that is not empty or that an earlier
+    pair names, no block left); counts[1] (int32 [2]): how many were."""
+    torch = _torch()
+    if stream is None:
+        rc = _calls().pages_fork(block_table, block_size, lens, refs, parents, children, pairs, status, counts)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_pages_fork", rc)
+    sh, tp, lp, rp = _pages_args(block_table, block_size, lens, refs)
+    n = parents.numel() if isinstance(parents, torch.Tensor) else 0
+    pa, ch = _ints(parents, "parents", 0, lens), _ints(children, "children", n, lens)
+    if children.numel() != n:
+        raise ValueError(f"{n} parents and {children.numel()} children")
+    st, ct = _ints(status, "status", n, lens), _ints(counts, "counts", 2, lens)
+    pp = _pairs_ptr(pairs, n, lens)
+    with _on(lens.device):
+        _check("mxfa_run_pages_fork",
+               load_library().mxfa_run_pages_fork(ctypes.byref(sh), tp, lp, rp, pa, ch, n, pp, st, ct, _stream(stream)))
+
+
+def _pairs_ptr(pairs, n, like):
+    torch = _torch()
+    _dev(pairs, "pairs", torch.int32, like)
+    if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.shape[0] < n or not pairs.is_contiguous():
+        raise ValueError(f"pairs: expected a contiguous int32 [at least {n}, 2], got {tuple(pairs.shape)}")
+    return ctypes.c_void_p(pairs.data_ptr())
+
+
+def run_pages_compact(block_table, block_size: int, lens, refs, new_table, new_refs, pairs, counts, stream=None):
+    """mxfa_run_pages_compact: the blocks in use move to the pool's low end, in
+    their order, as few of them as that takes. Writes the block tables
+    (new_table, which may be block_table) and use counts (new_refs, which may not
+    be refs) as they are after the moves, the moves to pairs (int32 [at least
+    max(1, n_blocks // 2), 2]) and to counts (int32 [2]) their number and that
+    of the blocks in use. run_pages_copy(pool, block_size, pairs, counts) then
+    makes the moves, in each pool of the cache; the old tables stay valid until
+    the blocks that were left are used again."""
+    if stream is None:
+        rc = _calls().pages_compact(block_table, block_size, lens, refs, new_table, new_refs, pairs, counts)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_pages_compact", rc)
+    sh, tp, lp, rp = _pages_args(block_table, block_size, lens, refs)
+    ntp, wide, nts = _block_table(new_table, lens.numel(), lens)
+    if wide != sh.max_blocks:
+        raise ValueError(f"new_table: {wide} entries to a row, block_table {sh.max_blocks}")
+    nr = _ints(new_refs, "new_refs", sh.n_blocks, lens)
+    pp, ct = _pairs_ptr(pairs, max(1, sh.n_blocks // 2), lens), _ints(counts, "counts", 2, lens)
+    with _on(lens.device):
+        _check("mxfa_run_pages_compact",
+               load_library().mxfa_run_pages_compact(ctypes.byref(sh), tp, lp, rp, ntp, nts, nr, pp, ct, _stream(stream)))
+
+
+def run_pages_copy(pools, block_size: int, pairs, count=None, stream=None):
+    """mxfa_run_pages_copy: block pairs[j, 0] is copied to block pairs[j, 1], in one
+    pool [rows, width] or in several [pools, rows, width] (K and V of every
+    layer, say) of contiguous rows, block j being rows j block_size .. (j + 1)
+    block_size - 1. count: an int32 device tensor whose first element says how
+    many of the pairs count (run_pages_fork's and run_pages_compact's counts);
+    None: all. Pairs with a number outside the pool are skipped; no destination
+    may be another pair's source or destination. Any dtype; a block is a
+    multiple of 16 bytes."""
+    if stream is None:
+        rc = _calls().pages_copy(pools, block_size, pairs, count)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_pages_copy", rc)
+    _dev(pools, "pools")
+    if block_size < 1:
+        raise ValueError(f"block_size {block_size}: must be positive")
+    if pools.dim() not in (2, 3) or pools.numel() == 0 or not pools[(0,) * (pools.dim() - 2)].is_contiguous() or \
+            pools.shape[-2] < block_size:
+        raise ValueError(f"pools: expected [rows, width] or [pools, rows, width] of contiguous rows and at least a "
+                         f"block of them, got shape {tuple(pools.shape)} strides {pools.stride()}")
+    es, many = pools.element_size(), pools.dim() == 3
+    pp = _pairs_ptr(pairs, 0, pools)
+    cp = None if count is None else _ints(count, "count", 1, pools)
+    with _on(pools.device):
+        _check("mxfa_run_pages_copy",
+               load_library().mxfa_run_pages_copy(ctypes.c_void_p(pools.data_ptr()), pools.shape[0] if many else 1,
+                                                  pools.stride(0) * es if many else 0, pools.shape[-2] // block_size,
+                                                  block_size * pools.shape[-1] * es, pp, pairs.shape[0], cp,
+                                                  _stream(stream)))
 
 
 # ------------------------------------------------------------ conveniences --

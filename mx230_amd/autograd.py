@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from . import attention_bwd, attention_fwd
+from . import attention_bwd, attention_fwd, run_rotary
 
 
 class FlashAttentionFunction(torch.autograd.Function):
@@ -44,13 +44,54 @@ def flash_attention(q, k, v, causal: bool = False, scale: float = 0.0):
     return FlashAttentionFunction.apply(q, k, v, causal, scale)
 
 
+def _rows16(x):
+    """x, or a copy where its rows are not contiguous 16-byte aligned ones."""
+    es = x.element_size()
+    if x.shape[-1] > 1 and x.stride(-1) != 1 or x.data_ptr() % 16 or \
+            any(n > 1 and s * es % 16 for n, s in zip(x.shape[:-1], x.stride()[:-1])):
+        return x.contiguous()
+    return x
+
+
+class RotaryFunction(torch.autograd.Function):
+    """Q and K with rotary positions; the gradient is the transposed rotation."""
+
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, pos0: int, interleaved: bool, factor: float):
+        ctx.save_for_backward(frequencies, positions)
+        ctx.args = pos0, interleaved, factor
+        q, k = _rows16(q), _rows16(k)
+        qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+        run_rotary(q, k, qo, ko, frequencies, positions, pos0, interleaved, factor)
+        return qo, ko
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        frequencies, positions = ctx.saved_tensors
+        pos0, interleaved, factor = ctx.args
+        dq, dk = _rows16(dq), _rows16(dk)
+        gq, gk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (dq, dk))
+        run_rotary(dq, dk, gq, gk, frequencies, positions, pos0, interleaved, factor, inverse=True)
+        return gq, gk, None, None, None, None, None
+
+
+def rotary_embedding(q, k, frequencies, positions=None, pos0: int = 0, interleaved: bool = False, factor: float = 1.0):
+    """Differentiable rotary positions of Q and K [B, H, N, d] (any strides; the
+    results are contiguous), as :func:`mx230_amd.run_rotary` takes them. The
+    positions and frequencies must stay as they are until the backward has run."""
+    return RotaryFunction.apply(q, k, frequencies, positions, pos0, interleaved, factor)
+
+
 class CausalSelfAttention(torch.nn.Module):
     """A transformer attention block around :func:`flash_attention`: fused QKV
     projection, grouped-query heads, output projection (the GEMMs on either side
-    are plain torch; the attention core is the HIP path)."""
+    are plain torch; the attention core is the HIP path). rotary: None, or the
+    (frequencies, factor) of :func:`mx230_amd.rotary_frequencies`, by which Q and
+    K are turned at positions 0 .. N - 1 before the attention."""
 
     def __init__(self, dim: int, n_heads: int, n_kv_heads: int | None = None, head_dim: int = 64,
-                 causal: bool = True):
+                 causal: bool = True, rotary=None, interleaved: bool = False):
         super().__init__()
         self.n_heads = n_heads
         self.n_kv_heads = n_kv_heads or n_heads
@@ -58,6 +99,9 @@ class CausalSelfAttention(torch.nn.Module):
             raise ValueError("n_heads must be a multiple of n_kv_heads")
         self.head_dim = head_dim
         self.causal = causal
+        self.interleaved = interleaved
+        # float64 angles, which a .to(dtype) of the module must not round: no buffer
+        self.rotary = rotary
         self.qkv = torch.nn.Linear(dim, (n_heads + 2 * self.n_kv_heads) * head_dim, bias=False)
         self.out = torch.nn.Linear(n_heads * head_dim, dim, bias=False)
 
@@ -69,5 +113,7 @@ class CausalSelfAttention(torch.nn.Module):
         q = q.view(b, n, hq, d).transpose(1, 2)
         k = k.view(b, n, hk, d).transpose(1, 2)
         v = v.view(b, n, hk, d).transpose(1, 2)
+        if self.rotary is not None:
+            q, k = rotary_embedding(q, k, self.rotary[0], interleaved=self.interleaved, factor=self.rotary[1])
         o = flash_attention(q, k, v, self.causal)
         return self.out(o.transpose(1, 2).reshape(b, n, hq * d))

@@ -43,6 +43,16 @@
     X(mxfa_dkv_reduce_bf16) X(mxfa_dkv_reduce_f32)                                            \
     /* naive baselines (fa_naive.hip) */                                                      \
     X(mxfa_naive_scores) X(mxfa_naive_softmax) X(mxfa_naive_av) X(mxfa_naive_bwd)            \
+    /* attention of a batch over a paged cache (fa_batch.hip) */                              \
+    X(mxfa_batch_b64_few) X(mxfa_batch_b64_many) X(mxfa_batch_b64_join)                       \
+    X(mxfa_batch_b128_few) X(mxfa_batch_b128_many) X(mxfa_batch_b128_join)                    \
+    X(mxfa_batch_f64_few) X(mxfa_batch_f64_many) X(mxfa_batch_f64_join)                       \
+    /* rotary positions and the cache append (fa_rotary.hip): 16-byte, 8-byte, single-element chunks */ \
+    X(mxfa_rotary_b) X(mxfa_rotary_b4) X(mxfa_rotary_b1) X(mxfa_rotary_f) X(mxfa_rotary_f1)   \
+    X(mxfa_append_b) X(mxfa_append_b4) X(mxfa_append_b1) X(mxfa_append_f) X(mxfa_append_f1)   \
+    /* the pages of a cache (fa_pages.hip) */                                                 \
+    X(mxfa_pages_free) X(mxfa_pages_fork_plan) X(mxfa_pages_fork_rows)                        \
+    X(mxfa_pages_compact_plan) X(mxfa_pages_compact_table) X(mxfa_pages_copy)                 \
     /* probes (probe.hip) */                                                                  \
     X(mxfa_probe_mfma_bf16) X(mxfa_probe_mfma_f32) X(mxfa_probe_mfma32_bf16)                  \
     X(mxfa_probe_read_f4) X(mxfa_probe_copy_f4) X(mxfa_probe_dq_atomic_add)                   \

@@ -4,4 +4,7 @@
 #include "fa_fwd.hip"
 #include "fa_bwd.hip"
 #include "fa_naive.hip"
+#include "fa_batch.hip"
+#include "fa_rotary.hip"
+#include "fa_pages.hip"
 #include "probe.hip"

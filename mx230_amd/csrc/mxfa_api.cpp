@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstring>
 
+#include "fa_cache.h"
 #include "fa_launch.h"
 
 namespace {
@@ -555,6 +556,335 @@ int mxfa_run_prefill_paged_ws(const mxfa_prefill_shape *s, const void *q, const 
     const int rc = paged_params(s, q, kcache, vcache, out, block_table, block_size, &p);
     if (rc != MXFA_OK) return rc;
     return run_prefill_maybe_split(s, p, workspace, workspace_bytes, stream);
+}
+
+// ---- rotary positions, the cache append and the pages of a cache
+
+namespace {
+
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int check_ints(std::initializer_list<const void *> ps) {
+    for (const void *p : ps) {
+        if (p == nullptr) return MXFA_ERR_NULL;
+    }
+    for (const void *p : ps) {
+        if (!aligned4(p)) return MXFA_ERR_ALIGN;
+    }
+    return MXFA_OK;
+}
+
+bool power_of_two(int x) { return x > 0 && (x & (x - 1)) == 0; }
+
+int log2_of(int x) {
+    int s = 0;
+    while ((1 << s) < x) ++s;
+    return s;
+}
+
+int check_rotated(int head_dim, int rotary_dim, int interleaved, float factor) {
+    if (head_dim < 8 || rotary_dim < 2 || rotary_dim > head_dim) return MXFA_ERR_SHAPE;
+    if (interleaved != 0 && interleaved != 1) return MXFA_ERR_SHAPE;
+    if (std::isnan(factor) || std::isinf(factor)) return MXFA_ERR_SHAPE;
+    if (head_dim % 8 != 0 || head_dim > 256 || rotary_dim % 2 != 0) return MXFA_ERR_UNSUPPORTED;
+    return MXFA_OK;
+}
+
+// The head views of a rotary call; strides of dimensions of one element count
+// as 0. False where a stride is out of range.
+struct Extent {
+    double lo, hi;  // bytes from the base pointer
+};
+bool view_extent(int B, int H, int N, int d, long long bs, long long hs, long long ts, int esz, Extent *e) {
+    const double reach[3] = {(double)(B - 1) * (double)bs, (double)(H - 1) * (double)hs, (double)(N - 1) * (double)ts};
+    e->lo = 0.0;
+    e->hi = (double)d;
+    for (double r : reach) {
+        if (std::fabs(r) > 1099511627776.0) return false;
+        (r < 0 ? e->lo : e->hi) += r;
+    }
+    e->lo *= esz;
+    e->hi *= esz;
+    return true;
+}
+
+}  // namespace
+
+int mxfa_check_rotary(const mxfa_rotary_shape *s) {
+    if (s == nullptr) return MXFA_ERR_NULL;
+    if (s->dtype != MXFA_F32 && s->dtype != MXFA_BF16) return MXFA_ERR_DTYPE;
+    if (s->B < 1 || s->Hq < 1 || s->Hkv < 0 || s->N < 1) return MXFA_ERR_SHAPE;
+    if (s->inverse != 0 && s->inverse != 1) return MXFA_ERR_SHAPE;
+    const int rc = check_rotated(s->head_dim, s->rotary_dim, s->interleaved, s->factor);
+    if (rc != MXFA_OK) return rc;
+    // positions stay inside int, and so do the threads of a batch's row
+    if ((long long)s->pos0 + s->N > 0x7fffffffLL) return MXFA_ERR_SHAPE;
+    const long long units = mxfa::rotary_row_units(s->head_dim, s->rotary_dim, s->dtype == MXFA_BF16);
+    if (units * s->N > 0x7fffffffLL - 256 || s->B > kMaxGridY || (long long)s->Hq + s->Hkv > kMaxGridY)
+        return MXFA_ERR_SHAPE;
+    if (s->B > 1 && s->pos_bs < 0) return MXFA_ERR_SHAPE;
+    const int esz = s->dtype == MXFA_BF16 ? 2 : 4, d = s->head_dim;
+    const long long in[2][3] = {{s->q_bs, s->q_hs, s->q_ts}, {s->k_bs, s->k_hs, s->k_ts}};
+    const long long out[2][3] = {{s->qo_bs, s->qo_hs, s->qo_ts}, {s->ko_bs, s->ko_hs, s->ko_ts}};
+    for (int t = 0; t < (s->Hkv > 0 ? 2 : 1); ++t) {
+        const int n[3] = {s->B, t ? s->Hkv : s->Hq, s->N};
+        for (int i = 0; i < 3; ++i) {
+            if (n[i] == 1) continue;
+            // an output's rows are rows of their own
+            if (out[t][i] < d) return MXFA_ERR_SHAPE;
+            if ((in[t][i] * esz) % 16 != 0 || (out[t][i] * esz) % 16 != 0) return MXFA_ERR_ALIGN;
+        }
+        // and do not overlap: each stride steps past what the smaller ones reach
+        int order[3] = {0, 1, 2};
+        std::sort(order, order + 3, [&](int a, int b) { return out[t][a] < out[t][b]; });
+        double reach = d;
+        for (int i : order) {
+            if (n[i] == 1) continue;
+            if ((double)out[t][i] < reach) return MXFA_ERR_SHAPE;
+            reach += (double)out[t][i] * (n[i] - 1);
+        }
+        Extent e;
+        if (!view_extent(n[0], n[1], n[2], d, in[t][0], in[t][1], in[t][2], esz, &e) ||
+            !view_extent(n[0], n[1], n[2], d, out[t][0], out[t][1], out[t][2], esz, &e))
+            return MXFA_ERR_SHAPE;
+    }
+    return MXFA_OK;
+}
+
+int mxfa_run_rotary(const mxfa_rotary_shape *s, const void *q, const void *k, void *q_out, void *k_out,
+                    const int *positions, const double *frequencies, void *stream) {
+    int rc = mxfa_check_rotary(s);
+    if (rc != MXFA_OK) return rc;
+    rc = s->Hkv > 0 ? check_ptrs({q, k, q_out, k_out}) : check_ptrs({q, q_out});
+    if (rc != MXFA_OK) return rc;
+    if (frequencies == nullptr) return MXFA_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(frequencies) % 8 != 0 || !aligned4(positions)) return MXFA_ERR_ALIGN;
+    mxfa::RotaryParams p;
+    std::memset(&p, 0, sizeof(p));
+    const int esz = s->dtype == MXFA_BF16 ? 2 : 4;
+    const void *in[2] = {q, k};
+    void *out[2] = {q_out, k_out};
+    const long long is[2][3] = {{s->q_bs, s->q_hs, s->q_ts}, {s->k_bs, s->k_hs, s->k_ts}};
+    const long long os[2][3] = {{s->qo_bs, s->qo_hs, s->qo_ts}, {s->ko_bs, s->ko_hs, s->ko_ts}};
+    for (int t = 0; t < (s->Hkv > 0 ? 2 : 1); ++t) {
+        const int n[3] = {s->B, t ? s->Hkv : s->Hq, s->N};
+        long long i3[3], o3[3];
+        bool same = in[t] == out[t];
+        for (int i = 0; i < 3; ++i) {
+            i3[i] = n[i] == 1 ? 0 : is[t][i];
+            o3[i] = n[i] == 1 ? 0 : os[t][i];
+            same = same && i3[i] == o3[i];
+        }
+        Extent a, b;
+        view_extent(n[0], n[1], n[2], s->head_dim, i3[0], i3[1], i3[2], esz, &a);
+        view_extent(n[0], n[1], n[2], s->head_dim, o3[0], o3[1], o3[2], esz, &b);
+        const double pi = (double)reinterpret_cast<uintptr_t>(in[t]), po = (double)reinterpret_cast<uintptr_t>(out[t]);
+        if (!same && pi + a.lo < po + b.hi && po + b.lo < pi + a.hi) return MXFA_ERR_UNSUPPORTED;
+        p.x[t] = mxfa::HeadView{in[t], out[t], i3[0], i3[1], i3[2], o3[0], o3[1], o3[2]};
+        p.H[t] = n[1];
+    }
+    p.B = s->B;
+    p.N = s->N;
+    p.d = s->head_dim;
+    p.dim = s->rotary_dim;
+    p.interleaved = s->interleaved;
+    p.pos0 = s->pos0;
+    p.positions = positions;
+    p.pos_bs = s->B > 1 ? s->pos_bs : 0;
+    p.freq = frequencies;
+    p.factor = s->factor;
+    p.sin_sign = s->inverse ? -1.0f : 1.0f;
+    return from_hip(mxfa::launch_rotary(p, s->dtype == MXFA_BF16, static_cast<hipStream_t>(stream)));
+}
+
+namespace {
+
+// What the append and the attention of a batch have in common; qw: the columns
+// of a q / qkv row.
+int check_batch(const mxfa_batch_shape *s, long long qw) {
+    if (s->dtype != MXFA_F32 && s->dtype != MXFA_BF16) return MXFA_ERR_DTYPE;
+    if (s->n_tok < 1 || s->n_seq < 1 || s->n_head < 1 || s->n_kv_head < 1 || s->head_dim < 1 || s->n_blocks < 1 ||
+        s->max_blocks < 1 || s->table_stride < s->max_blocks)
+        return MXFA_ERR_SHAPE;
+    if (s->n_head % s->n_kv_head != 0) return MXFA_ERR_SHAPE;
+    if (!power_of_two(s->block_size) || s->block_size > (1 << 24)) return MXFA_ERR_UNSUPPORTED;
+    const long long ow = (long long)s->n_head * s->head_dim, kw = (long long)s->n_kv_head * s->head_dim;
+    if (s->q_stride < qw || s->out_stride < ow || s->kv_stride < kw) return MXFA_ERR_SHAPE;
+    const int esz = s->dtype == MXFA_BF16 ? 2 : 4;
+    if (((long long)s->q_stride * esz) % 16 || ((long long)s->kv_stride * esz) % 16 ||
+        ((long long)s->out_stride * esz) % 16)
+        return MXFA_ERR_ALIGN;
+    return MXFA_OK;
+}
+
+mxfa::BatchParams batch_params(const mxfa_batch_shape *s, const void *q, void *k, void *v, void *o, const int *table,
+                               const int *cu_q, const int *lens) {
+    mxfa::BatchParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.o = o;
+    p.table = table;
+    p.cu_q = cu_q;
+    p.lens = lens;
+    p.n_tok = s->n_tok;
+    p.n_seq = s->n_seq;
+    p.max_q = s->max_q;
+    p.Hq = s->n_head;
+    p.Hkv = s->n_kv_head;
+    p.group = s->n_head / s->n_kv_head;
+    p.d = s->head_dim;
+    p.q_rs = s->q_stride;
+    p.kv_rs = s->kv_stride;
+    p.o_rs = s->out_stride;
+    p.bs_shift = log2_of(s->block_size);
+    p.n_blocks = s->n_blocks;
+    p.max_blocks = s->max_blocks;
+    p.table_stride = s->table_stride;
+    return p;
+}
+
+}  // namespace
+
+int mxfa_check_batch(const mxfa_batch_shape *s) {
+    if (s == nullptr) return MXFA_ERR_NULL;
+    const int rc = check_batch(s, (long long)s->n_head * s->head_dim);
+    if (rc != MXFA_OK) return rc;
+    if (s->max_q < 1) return MXFA_ERR_SHAPE;
+    if (!(s->scale >= 0.0f) || std::isinf(s->scale)) return MXFA_ERR_SHAPE;
+    if (s->head_dim != 64 && s->head_dim != 128) return MXFA_ERR_UNSUPPORTED;
+    if (s->dtype == MXFA_F32 && s->head_dim != 64) return MXFA_ERR_UNSUPPORTED;
+    // rows of a KV head, and the work-groups of a launch, are counted in ints
+    const long long group = s->n_head / s->n_kv_head;
+    if ((long long)s->n_tok * group > 0x7fffffffLL - 64) return MXFA_ERR_SHAPE;
+    const mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    if (mxfa::batch_groups(p, s->dtype == MXFA_BF16) > 0x7fffffffLL / 512) return MXFA_ERR_SHAPE;
+    return MXFA_OK;
+}
+
+size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *s) {
+    if (mxfa_check_batch(s) != MXFA_OK) return 0;
+    return mxfa::batch_workspace_bytes(batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr),
+                                       s->dtype == MXFA_BF16);
+}
+
+int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void *kcache, const void *vcache, void *out,
+                           float *lse, const int *block_table, const int *cu_q, const int *lens, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+    int rc = mxfa_check_batch(s);
+    if (rc != MXFA_OK) return rc;
+    rc = check_ptrs({q, kcache, vcache, out, workspace});
+    if (rc != MXFA_OK) return rc;
+    rc = check_ints({block_table, cu_q, lens});
+    if (rc != MXFA_OK) return rc;
+    if (!aligned4(lse)) return MXFA_ERR_ALIGN;
+    mxfa::BatchParams p = batch_params(s, q, const_cast<void *>(kcache), const_cast<void *>(vcache), out, block_table,
+                                       cu_q, lens);
+    p.lse = lse;
+    p.scale_log2 = (s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * mxfa::kLog2e;
+    if (workspace_bytes < mxfa::batch_workspace_bytes(p, s->dtype == MXFA_BF16)) return MXFA_ERR_WORKSPACE;
+    return from_hip(mxfa::launch_batch(p, s->dtype == MXFA_BF16, workspace, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_cache_append(const mxfa_batch_shape *s, const mxfa_append_rotary *r, const void *qkv, void *q_out,
+                          void *kcache, void *vcache, const int *block_table, const int *cu_q, const int *lens,
+                          void *stream) {
+    if (s == nullptr || r == nullptr) return MXFA_ERR_NULL;
+    int rc = check_batch(s, ((long long)s->n_head + 2LL * s->n_kv_head) * s->head_dim);
+    if (rc != MXFA_OK) return rc;
+    if (r->rotary_dim == 0) {
+        if (s->head_dim % 8 != 0 || s->head_dim > 256) return MXFA_ERR_UNSUPPORTED;
+    } else {
+        rc = check_rotated(s->head_dim, r->rotary_dim, r->interleaved, r->factor);
+        if (rc != MXFA_OK) return rc;
+        if (r->frequencies == nullptr) return MXFA_ERR_NULL;
+        if (reinterpret_cast<uintptr_t>(r->frequencies) % 8 != 0) return MXFA_ERR_ALIGN;
+    }
+    if ((long long)s->n_head + 2LL * s->n_kv_head > kMaxGridY) return MXFA_ERR_SHAPE;
+    if ((double)s->n_tok * mxfa::rotary_row_units(s->head_dim, r->rotary_dim, s->dtype == MXFA_BF16) > 0x7fffffff - 512.0)
+        return MXFA_ERR_SHAPE;  // a launch's threads
+    rc = check_ptrs({qkv, q_out, kcache, vcache});
+    if (rc != MXFA_OK) return rc;
+    rc = check_ints({block_table, cu_q, lens});
+    if (rc != MXFA_OK) return rc;
+    mxfa::BatchParams p = batch_params(s, qkv, kcache, vcache, q_out, block_table, cu_q, lens);
+    p.freq = r->frequencies;
+    p.dim = r->rotary_dim;
+    p.interleaved = r->interleaved;
+    p.factor = r->factor;
+    return from_hip(mxfa::launch_append(p, s->dtype == MXFA_BF16, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_check_pages(const mxfa_pages_shape *s) {
+    if (s == nullptr) return MXFA_ERR_NULL;
+    if (s->n_seq < 1 || s->n_blocks < 1 || s->max_blocks < 1 || s->table_stride < s->max_blocks) return MXFA_ERR_SHAPE;
+    if (s->n_seq > kMaxGridY) return MXFA_ERR_SHAPE;
+    // the plans count blocks in ints, a few thousand past the last
+    if (s->n_blocks > (1 << 30)) return MXFA_ERR_SHAPE;
+    if (!power_of_two(s->block_size) || s->block_size > (1 << 24)) return MXFA_ERR_UNSUPPORTED;
+    return MXFA_OK;
+}
+
+namespace {
+mxfa::PagesParams pages_params(const mxfa_pages_shape *s, const int *table, const int *lens, const int *refs) {
+    return mxfa::PagesParams{const_cast<int *>(table), const_cast<int *>(lens), const_cast<int *>(refs), s->n_seq,
+                             s->max_blocks, s->table_stride, log2_of(s->block_size), s->n_blocks};
+}
+}  // namespace
+
+int mxfa_run_pages_free(const mxfa_pages_shape *s, int *block_table, int *lens, int *refs, const int *rows, int n,
+                        void *stream) {
+    int rc = mxfa_check_pages(s);
+    if (rc != MXFA_OK) return rc;
+    if (n < 0 || n > (1 << 20)) return MXFA_ERR_SHAPE;
+    rc = n > 0 ? check_ints({block_table, lens, refs, rows}) : check_ints({block_table, lens, refs});
+    if (rc != MXFA_OK || n == 0) return rc;
+    return from_hip(mxfa::launch_pages_free(pages_params(s, block_table, lens, refs), rows, n,
+                                            static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_pages_fork(const mxfa_pages_shape *s, int *block_table, int *lens, int *refs, const int *parents,
+                        const int *children, int n, int *pairs, int *status, int *counts, void *stream) {
+    int rc = mxfa_check_pages(s);
+    if (rc != MXFA_OK) return rc;
+    if (n < 0 || n > (1 << 20)) return MXFA_ERR_SHAPE;
+    rc = check_ints({block_table, lens, refs, counts});
+    if (rc == MXFA_OK && n > 0) rc = check_ints({parents, children, pairs, status});
+    if (rc != MXFA_OK) return rc;
+    return from_hip(mxfa::launch_pages_fork(pages_params(s, block_table, lens, refs), parents, children, n, pairs,
+                                            status, counts, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_pages_compact(const mxfa_pages_shape *s, const int *block_table, const int *lens, const int *refs,
+                           int *new_table, int new_stride, int *new_refs, int *pairs, int *counts, void *stream) {
+    int rc = mxfa_check_pages(s);
+    if (rc != MXFA_OK) return rc;
+    if (new_stride < s->max_blocks) return MXFA_ERR_SHAPE;
+    rc = check_ints({block_table, lens, refs, new_table, new_refs, pairs, counts});
+    if (rc != MXFA_OK) return rc;
+    // the counts are read again after the new ones are written
+    if (refs < new_refs + s->n_blocks && new_refs < refs + s->n_blocks) return MXFA_ERR_UNSUPPORTED;
+    return from_hip(mxfa::launch_pages_compact(pages_params(s, block_table, lens, refs), new_table, new_stride,
+                                               new_refs, pairs, counts, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_pages_copy(void *pools, int n_pools, long long pool_bytes, int n_blocks, long long block_bytes,
+                        const int *pairs, int n_pairs, const int *count, void *stream) {
+    if (n_pools < 1 || n_blocks < 1 || n_pairs < 0 || block_bytes < 1) return MXFA_ERR_SHAPE;
+    // below 2^42 bytes in all, so that no offset leaves 64 bits
+    if ((double)block_bytes * n_blocks > 4398046511104.0 || (n_pools > 1 && (double)pool_bytes * n_pools > 4398046511104.0))
+        return MXFA_ERR_SHAPE;
+    if (n_pools > 1 && pool_bytes < block_bytes * n_blocks) return MXFA_ERR_SHAPE;
+    int rc = check_ptrs({pools});
+    if (rc != MXFA_OK) return rc;
+    if (block_bytes % 16 != 0 || (n_pools > 1 && pool_bytes % 16 != 0)) return MXFA_ERR_ALIGN;
+    if (!aligned4(count)) return MXFA_ERR_ALIGN;
+    if (n_pairs == 0) return MXFA_OK;
+    rc = check_ints({pairs});
+    if (rc != MXFA_OK) return rc;
+    return from_hip(mxfa::launch_pages_copy(pools, n_pools, n_pools > 1 ? pool_bytes : 0, n_blocks, block_bytes, pairs,
+                                            n_pairs, count, static_cast<hipStream_t>(stream)));
 }
 
 int mxfa_probe_sink_len(void) { return mxfa::probe_sink_len(); }
