@@ -11,7 +11,7 @@
 // group. Two forms take them in units of rows:
 //   * few (at most 16 rows): every wave holds the same rows and takes 64-key
 //     stages of its own; bound by the reads of K and V;
-//   * many: 64 rows, 16 per wave, the waves sharing each stage; bound by the
+//   * many: 128 rows (fp32: 64), 32 (16) per wave, the waves sharing each stage; bound by the
 //     matrix products.
 // The host knows neither lengths nor units: a work-group finds its item (a
 // unit's share of its keys) from cu_q and lens itself (find_item). A unit is
@@ -20,6 +20,7 @@
 // are then joined by a second launch, in a fixed order.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "fa_cache.h"
 #include "fa_device.h"
@@ -27,19 +28,15 @@
 
 namespace mxfa {
 
-constexpr int kBatchFew = 16, kBatchMany = 64;  // rows of a unit
+constexpr int kBatchFew = 16;  // rows of the few-row form's units
 // the fewest stages of a share, per form: shorter ones cost more in the join
 // than they save
 constexpr int kFewLeast = 4, kManyLeast = 4;
 
-template <bool FEW>
-constexpr int batch_rows() {
-    return FEW ? kBatchFew : kBatchMany;
-}
-template <bool FEW>
-constexpr int batch_least() {
-    return FEW ? kFewLeast : kManyLeast;
-}
+// Rows of the many-row form's units: 16 per wave and query tile.
+__host__ __device__ constexpr int batch_tiles(bool bf16) { return bf16 ? 2 : 1; }
+__host__ __device__ constexpr int batch_many_rows(bool bf16) { return 64 * batch_tiles(bf16); }
+
 // Slots of the workspace: the shares of split units. A unit of n stages is
 // split where n > quota, into ceil(n / quota) < 2 n / quota shares, and quota
 // >= all stages / target, so there are at most 2 target of them.
@@ -47,6 +44,10 @@ __host__ __device__ constexpr long long batch_slots(int target) { return 2LL * t
 __host__ __device__ constexpr size_t batch_part_floats(int target, int rows, int d) {
     return (size_t)batch_slots(target) * rows * (d + 2);
 }
+
+// The device code builds on the forward's stages (fa_fwd.hip, the same
+// translation unit in the code object).
+#if defined(__HIP_DEVICE_COMPILE__)
 
 // ------------------------------------------------- fp32 on its own instructions
 
@@ -61,6 +62,10 @@ struct PolF32 {
     using T = float;
     using Frag = f32x4;
     static constexpr int EPC = 4, NC = 4, ROWS = 64;
+    __device__ static __forceinline__ void chunk_at(int P, int &row, int &chunk) {
+        row = P >> 4;
+        chunk = (P & 15) ^ (row & 15);
+    }
     __device__ static __forceinline__ constexpr int arow(int t, int m) { return 16 * t + m; }
     __device__ static __forceinline__ constexpr int bidx(int t, int g, int r) { return 16 * t + 4 * g + r; }
     __device__ static __forceinline__ int chunk_off(int row, int chunk) { return row * 256 + ((chunk ^ (row & 15)) << 4); }
@@ -93,6 +98,53 @@ struct PolF32 {
     }
 };
 
+// bf16 inputs on v_mfma_f32_16x16x32_bf16 as PolBF16, from LDS tiles whose
+// rows lie whole, one after another, so that a wave's staging load reads whole
+// rows of the cache (4 rows of 256 bytes or 8 of 128; PolBF16's column groups
+// take 32 bytes of each of 32 rows). Chunk c of row r (bits r0, r1, ...) is at
+// slot c ^ swz(r). The 16 rows of a score operand differ in r0, r1, r3, r4, a
+// transposing read of V takes two neighbouring chunks of rows differing in r0
+// and r1 (two lane groups: r3), and with the bit patterns below each of these
+// covers all banks, in 128- and in 256-byte halves. r2 and r5 (tile t or half h,
+// block) stay out of it: plain additions.
+template <int D_>
+struct PolRows {
+    using Base = PolBF16<D_>;
+    static constexpr int D = D_, EPC = 8, NC = Base::NC, ROWS = 64, CPR = D / 8;
+    using T = u16;
+    using Frag = typename Base::Frag;
+    using ChainB = typename Base::ChainB;
+    __device__ static __forceinline__ int arow(int t, int m) { return Base::arow(t, m); }
+    __device__ static __forceinline__ int bidx(int t, int g, int r) { return Base::bidx(t, g, r); }
+    __device__ static __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) { return Base::mma(a, b, c); }
+    __device__ static __forceinline__ ChainB pack(const f32x4 &a, const f32x4 &b) { return Base::pack(a, b); }
+    __device__ static __forceinline__ int swz(int r) {
+        const int r0 = r & 1, r1 = (r >> 1) & 1, r3 = (r >> 3) & 1, r4 = (r >> 4) & 1;
+        return D == 128 ? (2 * r0) ^ (4 * r1) ^ (9 * r3) ^ r4 : (5 * r0) ^ (2 * r1) ^ (4 * r3) ^ r4;
+    }
+    __device__ static __forceinline__ void lds_row_frags(Frag (&f)[NC], const T *tile, int n, int g) {
+        const char *base = reinterpret_cast<const char *>(tile) + n * (2 * D);
+        const int x = (g ^ swz(n)) << 4;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) f[c] = *reinterpret_cast<const Frag *>(base + (x ^ (64 * c)));
+    }
+    __device__ static __forceinline__ f32x4 chain(f32x4 acc, const ChainB &b, const T *tile, int y0, int blk, int g,
+                                                  int l16) {
+        const int r0 = blk + 8 * g + (l16 >> 2);
+        const char *base = reinterpret_cast<const char *>(tile) + r0 * (2 * D) + ((l16 & 1) << 3);
+        const int x = (((l16 >> 1) & 1) ^ swz(r0)) << 4;
+        const int off = x ^ (2 * y0);
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(base + off));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(base + off + 4 * (2 * D)));
+        return mma(__builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), b, acc);
+    }
+    // the chunk at 16-byte position P of the tile, and its row
+    __device__ static __forceinline__ void chunk_at(int P, int &row, int &chunk) {
+        row = P / CPR;
+        chunk = (P % CPR) ^ swz(row);
+    }
+};
+
 // A row's elements that a lane holds as operand B of the scores.
 template <class Pol>
 __device__ __forceinline__ void row_frags(typename Pol::Frag (&f)[Pol::NC], const typename Pol::T *row, int g) {
@@ -103,44 +155,34 @@ __device__ __forceinline__ void row_frags(typename Pol::Frag (&f)[Pol::NC], cons
 
 // ------------------------------------------------------------- staging of pages
 
-// A sequence's stages of keys into LDS, NT threads to a tile; keys past the
-// last count as the last, and blocks outside the pool as the nearest in it, so
-// no read leaves the caches.
-template <class Pol, int NT>
-struct BatchStage {
-    RowPlan<Pol, NT> plan;
-    PagedRows<Pol, NT> rows;
-    static constexpr int LOADS = RowPlan<Pol, NT>::NK;
-    __device__ explicit BatchStage(int tid) : plan(tid) {}
-    __device__ __forceinline__ void fetch(const int *table, int shift, unsigned last_block, int k0, int Nk) {
-        rows.fetch(table, shift, k0, Nk, plan);
-#pragma unroll
-        for (int r = 0; r < PagedRows<Pol, NT>::NR; ++r) rows.blk[r] = (int)min((unsigned)rows.blk[r], last_block);
-    }
-    __device__ __forceinline__ void load(typename Pol::T *tile, const typename Pol::T *X, int k0, int Nk, int shift,
-                                         int wave, int stride) const {
-        rows.stage_one(tile, X, k0, Nk, shift, plan, wave, stride);
+// Cache row of position t of a sequence whose block is `blk`, as an index: blocks
+// outside the pool count as the nearest in it, so no read leaves the caches.
+struct BatchRows {
+    const int *table;
+    int shift, keys;
+    unsigned last;
+    __device__ __forceinline__ int block_at(int t) const { return min(t, keys - 1) >> shift; }
+    __device__ __forceinline__ unsigned row(int blk, int t) const {
+        const unsigned off = (unsigned)min(t, keys - 1) & ((1u << shift) - 1u);
+        return (min((unsigned)blk, last) << shift) + off;
     }
 };
-// fp32: a load of NT threads covers NT / 16 whole rows. Each wave's lanes hold
-// the blocks of the stage's 64 rows, passed on where a load needs them.
-template <int NT>
-struct BatchStage<PolF32, NT> {
-    static constexpr int LOADS = 64 * 16 / NT;
-    int tid, blk;
-    __device__ explicit BatchStage(int t) : tid(t), blk(0) {}
-    __device__ __forceinline__ void fetch(const int *table, int shift, unsigned last_block, int k0, int Nk) {
-        blk = (int)min((unsigned)table[min(k0 + (tid & 63), Nk - 1) >> shift], last_block);
-    }
-    __device__ __forceinline__ void load(float *tile, const float *X, int k0, int Nk, int shift, int wave,
-                                         int stride) const {
+
+// The loads of one 64-key tile by NT threads: load k fills 16-byte positions k NT
+// + tid, whole rows of the cache; row_of(r) is the cache row of the tile's row r.
+template <class Pol, int NT>
+struct BatchStage {
+    static constexpr int CPR = Pol::D / Pol::EPC, LOADS = 64 * CPR / NT;
+    template <class RowOf>
+    __device__ static __forceinline__ void load(typename Pol::T *tile, const typename Pol::T *X, int tid, int wave,
+                                                unsigned stride_bytes, RowOf row_of) {
         const uint32_t base = lds_addr(tile) + wave * 64 * 16;
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) {
-            const int row = (k * NT + tid) >> 4, c = (tid & 15) ^ (row & 15);
-            const int b = __shfl(blk, row, 64), t = min(k0 + row, Nk - 1);
-            const size_t at = (((size_t)b << shift) + (size_t)(t & ((1 << shift) - 1))) * (size_t)stride;
-            lds_dma16(base + k * NT * 16, X + at + 4 * c);
+            int row, c;
+            Pol::chunk_at(k * NT + tid, row, c);
+            lds_dma16(base + k * NT * 16, reinterpret_cast<const char *>(X) +
+                                              (unsigned long long)row_of(row) * stride_bytes + 16 * c);
         }
     }
 };
@@ -156,7 +198,7 @@ struct BatchSeq {
     int units, stages;
 };
 
-template <bool FEW>
+template <bool FEW, int ROWS>
 __device__ __forceinline__ BatchSeq batch_seq(const BatchParams &p, int s) {
     BatchSeq b{0, 0, 0, 0, 0, 0};
     if (s >= p.n_seq) return b;
@@ -172,12 +214,12 @@ __device__ __forceinline__ BatchSeq batch_seq(const BatchParams &p, int s) {
     b.rows = mine ? (int)rows : 0;
     b.keys = (int)min(min((long long)b.pos + max(count, 0), (long long)len), cap);
     b.keys = max(b.keys, 0);
-    b.units = (b.rows + batch_rows<FEW>() - 1) / batch_rows<FEW>();
+    b.units = (b.rows + ROWS - 1) / ROWS;
     b.stages = (b.keys + 63) / 64;
     return b;
 }
 
-__device__ __forceinline__ long long wave_sum(long long x) {
+__device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) x += __shfl_xor(x, k, 64);
     return x;
@@ -203,24 +245,26 @@ struct BatchItem {
 // shares x KV heads, so that neighbouring work-groups, which the dispatcher
 // spreads over the XCDs, have the heads and an XCD's share of them the same
 // head's keys.
-template <bool FEW, bool JOIN>
+template <bool FEW, int ROWS, bool JOIN>
 __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem &it) {
     const int lane = threadIdx.x & 63;
-    BatchSeq b = batch_seq<FEW>(p, lane);
-    long long all = (long long)b.units * max(b.stages, 1);
+    BatchSeq b = batch_seq<FEW, ROWS>(p, lane);
+    // the sum of all stages in fp32, rounded up by more than its rounding
+    float all = (float)b.units * (float)max(b.stages, 1);
     for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
-        const BatchSeq c = batch_seq<FEW>(p, s0 + lane);
-        all += (long long)c.units * max(c.stages, 1);
+        const BatchSeq c = batch_seq<FEW, ROWS>(p, s0 + lane);
+        all += (float)c.units * (float)max(c.stages, 1);
     }
-    all = wave_sum(all) * p.Hkv;
-    const int target = p.target[FEW ? 0 : 1];
-    const long long quota = max((all + target - 1) / target, (long long)batch_least<FEW>());
+    all = wave_sum(all) * (float)p.Hkv;
+    const float even = fminf(all * p.per_item[FEW ? 0 : 1] * 1.001f + 1.0f, 1e9f);
+    const unsigned quota = max((unsigned)even, (unsigned)(FEW ? kFewLeast : kManyLeast));
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-        if (s0 > 0) b = batch_seq<FEW>(p, s0 + lane);
-        const int shares = (long long)b.stages > quota ? (int)((b.stages + quota - 1) / quota) : 1;
-        const int per = JOIN ? (shares > 1 ? b.units * p.Hkv : 0) : b.units * p.Hkv * shares;
-        const int mine = shares > 1 ? b.units * p.Hkv * shares : 0;
+        if (s0 > 0) b = batch_seq<FEW, ROWS>(p, s0 + lane);
+        const int shares = (unsigned)b.stages > quota ? (int)(((unsigned)b.stages + quota - 1) / quota) : 1;
+        const int unit_items = b.units * p.Hkv;
+        const int mine = shares > 1 ? unit_items * shares : 0;
+        const int per = JOIN ? (shares > 1 ? unit_items : 0) : unit_items * shares;
         const int upto = wave_prefix(per, lane), slots_upto = wave_prefix(mine, lane);
         const unsigned long long at = __builtin_amdgcn_ballot_w64(before + upto > w);
         if (at != 0) {
@@ -233,27 +277,38 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
             it.s.units = __builtin_amdgcn_readlane(b.units, l);
             it.s.stages = __builtin_amdgcn_readlane(b.stages, l);
             it.shares = __builtin_amdgcn_readlane(shares, l);
-            int i = w - before - __builtin_amdgcn_readlane(upto - per, l);
+            unsigned i = w - before - __builtin_amdgcn_readlane(upto - per, l);
             it.slot = slots + __builtin_amdgcn_readlane(slots_upto - mine, l);
+            const unsigned heads = p.Hkv, per_unit = i / heads;
+            it.head = i - per_unit * heads;
             if (JOIN) {
-                it.slot += i / p.Hkv * it.shares * p.Hkv + i % p.Hkv;  // the unit's shares are Hkv apart
+                it.slot += per_unit * it.shares * heads + it.head;  // the unit's shares are `heads` apart
                 it.share = 0;
+                it.unit = it.s.units - 1 - (int)per_unit;
             } else {
                 it.slot += i;
+                const unsigned u = per_unit / (unsigned)it.shares;
+                it.share = per_unit - u * it.shares;
+                it.unit = it.s.units - 1 - (int)u;
             }
-            it.head = i % p.Hkv;
-            i /= p.Hkv;
-            if (!JOIN) {
-                it.share = i % it.shares;
-                i /= it.shares;
-            }
-            it.unit = it.s.units - 1 - i;
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         slots += __builtin_amdgcn_readlane(slots_upto, 63);
     }
     return false;
+}
+
+// The share's stages of the unit's n.
+__device__ __forceinline__ void share_stages(const BatchItem &it, int n, int &lo, int &hi) {
+    // n < 2^25 stages and at most 2^11 shares: the products pass 32 bits
+    if (it.shares == 1) {
+        lo = 0;
+        hi = n;
+    } else {
+        lo = (int)((unsigned long long)(unsigned)it.share * (unsigned)n / (unsigned)it.shares);
+        hi = (int)((unsigned long long)(unsigned)(it.share + 1) * (unsigned)n / (unsigned)it.shares);
+    }
 }
 
 // Row r of a unit's sequence: its elements in q or o, and its index in lse.
@@ -278,27 +333,26 @@ template <class Pol>
 __device__ __forceinline__ int batch_col(int i, int g) {
     return sizeof(typename Pol::T) == 2 ? 16 * i + 4 * g : 16 * g + 4 * i;
 }
-template <class Pol, int XT>
-__device__ __forceinline__ f32x4 batch_quad(const f32x4 (&acc)[XT][1], int i) {
+template <class Pol, int XT, int QT>
+__device__ __forceinline__ f32x4 batch_quad(const f32x4 (&acc)[XT][QT], int i, int qt) {
     if constexpr (sizeof(typename Pol::T) == 2) {
-        return acc[i][0];
+        return acc[i][qt];
     } else {
-        return f32x4{acc[0][0][i], acc[1][0][i], acc[2][0][i], acc[3][0][i]};
+        return f32x4{acc[0][qt][i], acc[1][qt][i], acc[2][qt][i], acc[3][qt][i]};
     }
 }
 
 // A unit's share in plain fp32 arithmetic, keys a row does not see left out
 // altogether: taken where a value was not finite, since in the matrix products
 // an infinity or NaN in the V of a key that a row does not see reaches it as 0
-// x inf. 4 threads per row. o: a row's running (max, sum) and output go where
+// x inf. 4 threads per row, rows from row0 of the unit. A row's running (max, sum) and output go where
 // the form's would: to the workspace slot, or finished.
 template <class T, int D, int ROWS>
-__device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchItem &it, int key0, int key1, float *part,
-                                            float *ml) {
+__device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchItem &it, int row0, int key0, int key1,
+                                            float *part, float *ml) {
     constexpr int E = D / 4;
-    const int tid = threadIdx.x;
-    if (tid >= 4 * ROWS) return;
-    const int r = it.unit * ROWS + (tid >> 2), c = E * (tid & 3);
+    const int rl = (int)(threadIdx.x >> 2) + row0, c = E * (int)(threadIdx.x & 3);
+    const int r = it.unit * ROWS + rl;
     const bool have = r < it.s.rows;
     const int row = min(r, it.s.rows - 1);
     const T *Q = static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D) + c;
@@ -334,23 +388,23 @@ __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchIte
     for (int e = 0; e < E; e += 4) {
         const f32x4 o{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
         if (it.shares > 1) {
-            store4<float>(part + (size_t)(tid >> 2) * D + c + e, o, 1.0f);
+            store4<float>(part + (size_t)rl * D + c + e, o, 1.0f);
         } else {
             batch_store<T>(p, it, r, D, c + e, o, m, l);
         }
     }
-    if (it.shares > 1 && c == 0) *reinterpret_cast<float2 *>(ml + 2 * (tid >> 2)) = make_float2(m, l);
+    if (it.shares > 1 && c == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m, l);
 }
 
 // The workspace of an item's share: ROWS rows of D floats, and their (max, sum).
-template <bool FEW>
+template <bool FEW, int ROWS>
 __device__ __forceinline__ float *batch_part(const BatchParams &p, int slot, int d) {
-    return p.part[FEW ? 0 : 1] + (size_t)slot * batch_rows<FEW>() * d;
+    return p.part[FEW ? 0 : 1] + (size_t)slot * ROWS * d;
 }
-template <bool FEW>
+template <bool FEW, int ROWS>
 __device__ __forceinline__ float *batch_ml(const BatchParams &p, int slot, int d) {
-    return p.part[FEW ? 0 : 1] + (size_t)batch_slots(p.target[FEW ? 0 : 1]) * batch_rows<FEW>() * d +
-           (size_t)slot * batch_rows<FEW>() * 2;
+    const int f = FEW ? 0 : 1;
+    return p.part[f] + (size_t)batch_slots(p.target[f]) * ROWS * d + (size_t)slot * ROWS * 2;
 }
 
 // ------------------------------------------------------------------ the few rows
@@ -359,6 +413,7 @@ template <class Pol, int NW>
 union BatchFewSmem {
     struct {
         typename Pol::T k[NW][Pol::ROWS * Pol::D], v[NW][Pol::ROWS * Pol::D];
+        int blk[NW][2][64];
     } t;
     struct {
         float acc[NW][kBatchFew][Pol::D + 4];
@@ -368,63 +423,80 @@ union BatchFewSmem {
 };
 
 // Each of the NW waves takes every NW-th stage of the share, staged into its
-// own tiles with no barrier; the waves' maxima, sums and O meet in LDS.
+// own tiles with no barrier; the waves' maxima, sums and O meet in LDS. The
+// stage's blocks come through LDS too, two stages ahead: as loads into
+// registers the compiler would wait for them with vmcnt(0), and with them for
+// every staging load in flight.
 template <class Pol, int NW>
 __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
     using T = typename Pol::T;
-    constexpr int D = Pol::D, XT = D / 16;
+    using Stage = BatchStage<Pol, 64>;
+    constexpr int D = Pol::D, XT = D / 16, ROWS = kBatchFew, NL = Stage::LOADS;
     __shared__ __attribute__((aligned(16))) BatchFewSmem<Pol, NW> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    if (!find_item<true, false>(p, blockIdx.x, it)) return;
+    if (!find_item<true, ROWS, false>(p, blockIdx.x, it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
-    const int *table = p.table + (long long)it.seq * p.table_stride;
-    const unsigned last_block = p.n_blocks - 1;
+    const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, it.s.keys, (unsigned)(p.n_blocks - 1)};
+    const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
     T *sk = sm.t.k[wave], *sv = sm.t.v[wave];
-    const int Nk = it.s.keys, n = it.s.stages;
-    const int s_lo = (int)((long long)it.share * n / it.shares), s_hi = (int)((long long)(it.share + 1) * n / it.shares);
+    const int Nk = it.s.keys;
+    int s_lo, s_hi;
+    share_stages(it, it.s.stages, s_lo, s_hi);
 
-    BatchStage<Pol, 64> stage(lane);
-    constexpr int NL = BatchStage<Pol, 64>::LOADS;
-    int st = s_lo + wave;
-    if (st < s_hi) {
-        stage.fetch(table, p.bs_shift, last_block, st * 64, Nk);
-        stage.load(sk, K, st * 64, Nk, p.bs_shift, 0, p.kv_rs);
-        stage.load(sv, V, st * 64, Nk, p.bs_shift, 0, p.kv_rs);
-    }
+    // stage `st` is the wave's n-th: its blocks in buffer n & 1
+    auto fetch = [&](int st, int n) __attribute__((always_inline)) {
+        lds_dma4(lds_addr(sm.t.blk[wave][n & 1]), rows.table + rows.block_at(st * 64 + lane));
+    };
+    auto load = [&](T *tile, const T *X, int st, int n) __attribute__((always_inline)) {
+        const int *blk = sm.t.blk[wave][n & 1];
+        Stage::load(tile, X, lane, 0, stride,
+                    [&](int r) __attribute__((always_inline)) { return rows.row(blk[r], st * 64 + r); });
+    };
+    int st = s_lo + wave, n = 0;
+    if (st < s_hi) fetch(st, 0);
     const int row = min(l16, it.s.rows - 1);
     const int qpos = it.s.pos + row / p.group;
     typename Pol::Frag qf[1][Pol::NC];
     row_frags<Pol>(qf[0], static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
+    if (st < s_hi) {
+        wait_loads<0>();
+        if (st + NW < s_hi) fetch(st + NW, 1);
+        load(sk, K, st, 0);
+        load(sv, V, st, 0);
+    }
     f32x4 acc[XT][1];
 #pragma unroll
     for (int xt = 0; xt < XT; ++xt) acc[xt][0] = zero4();
     float m[1] = {-INFINITY}, lsum[1] = {0.f};
     // The wave's next stage: its K goes out once this one's K has been read, its
-    // V once this one's V has, so one tile is in flight at any time. At least
-    // NL loads follow K's when it is waited for (this stage's V), and V's (the
-    // next K): vmcnt counts in order.
-    for (; st < s_hi; st += NW) {
-        const bool more = st + NW < s_hi;
-        if (more) stage.fetch(table, p.bs_shift, last_block, (st + NW) * 64, Nk);
+    // V once this one's V has, so K and V are in flight together but for the
+    // time their tile is read. vmcnt counts in order: NL loads (this stage's V)
+    // follow K, NL + 1 (the blocks after next and the next K) follow V.
+    for (; st < s_hi; st += NW, ++n) {
+        const bool more = st + NW < s_hi, after = st + 2 * NW < s_hi;
         wait_loads<NL>();
         fwd_stage<Pol, 1, true, true, false, true>(
             acc, m, lsum, qf, sk, sv, st * 64, qpos - l16, Nk, g, l16, p.scale_log2,
             [&]() __attribute__((always_inline)) {
                 wait_lds();
-                if (more) stage.load(sk, K, (st + NW) * 64, Nk, p.bs_shift, 0, p.kv_rs);
+                if (more) {
+                    // the buffer this stage's blocks were in: its V is out already
+                    fetch(after ? st + 2 * NW : st, n);
+                    load(sk, K, st + NW, n + 1);
+                }
             },
             [&]() __attribute__((always_inline)) {
                 if (more) {
-                    wait_loads<NL>();
+                    wait_loads<NL + 1>();
                 } else {
                     wait_loads<0>();
                 }
             });
         wait_lds();
-        if (more) stage.load(sv, V, (st + NW) * 64, Nk, p.bs_shift, 0, p.kv_rs);
+        if (more) load(sv, V, st + NW, n + 1);
     }
     const float lw = xg_sum(lsum[0]);
     float z = 0.f * lw;
@@ -437,16 +509,16 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
     if (bad && lane == 0) sm.merge.bad = 1;
 #pragma unroll
     for (int i = 0; i < XT; ++i)
-        *reinterpret_cast<f32x4 *>(&sm.merge.acc[wave][l16][batch_col<Pol>(i, g)]) = batch_quad<Pol>(acc, i);
+        *reinterpret_cast<f32x4 *>(&sm.merge.acc[wave][l16][batch_col<Pol>(i, g)]) = batch_quad<Pol>(acc, i, 0);
     if (g == 0) *reinterpret_cast<float2 *>(sm.merge.ml[wave][l16]) = make_float2(m[0], lw);
     __syncthreads();
     float *part = nullptr, *ml = nullptr;
     if (it.shares > 1) {
-        part = batch_part<true>(p, it.slot, D);
-        ml = batch_ml<true>(p, it.slot, D);
+        part = batch_part<true, ROWS>(p, it.slot, D);
+        ml = batch_ml<true, ROWS>(p, it.slot, D);
     }
     if (sm.merge.bad) {
-        batch_plain<T, D, kBatchFew>(p, it, s_lo * 64, s_hi * 64, part, ml);
+        if (tid < 4 * ROWS) batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
         return;
     }
     for (int i = tid; i < it.s.rows * (D / 4); i += 64 * NW) {
@@ -473,11 +545,13 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
 
 // ----------------------------------------------------------------- the many rows
 
-template <class Pol>
+template <class Pol, int QT>
 __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
     using T = typename Pol::T;
-    constexpr int D = Pol::D, XT = D / 16, BK = Pol::ROWS;
+    using Stage = BatchStage<Pol, 256>;
+    constexpr int D = Pol::D, XT = D / 16, BK = Pol::ROWS, ROWS = 64 * QT;
     constexpr bool kLazy = sizeof(T) == 2;  // fp32 scores are summed from zero
+    constexpr bool kPrio = sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) T sK[2][BK * D];
     __shared__ __attribute__((aligned(16))) T sV[2][BK * D];
     __shared__ int flags[4];
@@ -485,100 +559,139 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    if (!find_item<false, false>(p, blockIdx.x, it)) return;
+    if (!find_item<false, ROWS, false>(p, blockIdx.x, it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
-    const int *table = p.table + (long long)it.seq * p.table_stride;
-    const unsigned last_block = p.n_blocks - 1;
 
-    const int r0 = it.unit * kBatchMany;
-    const int r = r0 + wave * 16 + l16, row = min(r, it.s.rows - 1);
-    const int qpos = it.s.pos + row / p.group;
+    const int r0 = it.unit * ROWS, rw = r0 + wave * 16 * QT;  // the unit's and the wave's first row
+    const int last_row = it.s.rows - 1;
+    RowPos<QT> qpos;
+    typename Pol::Frag qf[QT][Pol::NC];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int row = min(rw + 16 * qt + l16, last_row);
+        qpos.at[qt] = it.s.pos + row / p.group;
+        row_frags<Pol>(qf[qt], static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
+    }
     // positions of the unit's first and last row, and of the wave's last
     const int pos_lo = it.s.pos + r0 / p.group;
-    const int pos_hi = it.s.pos + min(r0 + kBatchMany - 1, it.s.rows - 1) / p.group;
-    const int pos_w = it.s.pos + min(r0 + wave * 16 + 15, it.s.rows - 1) / p.group;
-    typename Pol::Frag qf[1][Pol::NC];
-    row_frags<Pol>(qf[0], static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
-    f32x4 acc[XT][1];
+    const int pos_hi = it.s.pos + min(r0 + ROWS - 1, last_row) / p.group;
+    const int pos_w = it.s.pos + min(rw + 16 * QT - 1, last_row) / p.group;
+    f32x4 acc[XT][QT];
+    float m[QT], lsum[QT];
 #pragma unroll
-    for (int xt = 0; xt < XT; ++xt) acc[xt][0] = zero4();
-    float m[1] = {-INFINITY}, lsum[1] = {0.f};
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) acc[xt][qt] = zero4();
+        m[qt] = -INFINITY;
+        lsum[qt] = 0.f;
+    }
 
     const int Nk = min(it.s.keys, max(pos_hi + 1, 0)), n = (Nk + BK - 1) / BK;
-    const int s_lo = (int)((long long)it.share * n / it.shares), s_hi = (int)((long long)(it.share + 1) * n / it.shares);
-    BatchStage<Pol, 256> stage(tid);
+    const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, Nk, (unsigned)(p.n_blocks - 1)};
+    const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
+    int s_lo, s_hi;
+    share_stages(it, n, s_lo, s_hi);
+    // each wave's lanes hold the blocks of the 64 rows of the stage to be staged
+    // next, fetched a stage ahead, and pass the cache rows on where a load needs
+    // them
+    int blk = 0;
+    auto fetch = [&](int st) __attribute__((always_inline)) { blk = rows.table[rows.block_at(st * BK + lane)]; };
     auto stage_next = [&](T *sk, T *sv, int st) __attribute__((always_inline)) {
-        stage.load(sk, K, st * BK, Nk, p.bs_shift, wave, p.kv_rs);
-        stage.load(sv, V, st * BK, Nk, p.bs_shift, wave, p.kv_rs);
-        if (st + 1 < s_hi) stage.fetch(table, p.bs_shift, last_block, (st + 1) * BK, Nk);
+        const unsigned mine = rows.row(blk, st * BK + lane);
+        auto row_of = [&](int r) __attribute__((always_inline)) { return (unsigned)__shfl((int)mine, r, 64); };
+        Stage::load(sk, K, tid, wave, stride, row_of);
+        Stage::load(sv, V, tid, wave, stride, row_of);
+        if (st + 1 < s_hi) fetch(st + 1);
     };
     if (s_lo < s_hi) {
-        stage.fetch(table, p.bs_shift, last_block, s_lo * BK, Nk);
+        fetch(s_lo);
         stage_next(sK[0], sV[0], s_lo);
     }
     wait_stage();
     __syncthreads();
-    // stages before `whole` hold no key that a row of the unit does not see
+    // stages before `whole` hold no key that a row of the unit does not see: in
+    // pairs, the LDS buffer a compile-time constant (fwd_entry's reasons)
     const int whole = min(s_hi, min(Nk, pos_lo + 1) / BK);
-    for (int st = s_lo; st < s_hi; ++st) {
-        const int cur = (st - s_lo) & 1;
-        if (st + 1 < s_hi) stage_next(sK[cur ^ 1], sV[cur ^ 1], st + 1);
-        const int k0 = st * BK;
-        if (k0 <= pos_w && r0 + wave * 16 < it.s.rows) {  // else no row of the wave sees the stage
-            if (st < whole) {
-                if (st == s_lo || !kLazy) {
-                    fwd_stage<Pol, 1, true, false>(acc, m, lsum, qf, sK[cur], sV[cur], k0, qpos - l16, Nk, g, l16,
-                                                   p.scale_log2);
-                } else if constexpr (kLazy) {
-                    fwd_stage_lazy<Pol, 1, true, false>(acc, m, lsum, qf, sK[cur], sV[cur], k0, qpos - l16, Nk, g,
-                                                        l16, p.scale_log2);
-                }
+    const bool some = rw <= last_row;  // the wave has rows
+    auto main_stage = [&](auto buf, auto first, int st) __attribute__((always_inline)) {
+        constexpr int B = decltype(buf)::value;
+        if (st + 1 < s_hi) stage_next(sK[B ^ 1], sV[B ^ 1], st + 1);
+        if (some) {
+            if constexpr (decltype(first)::value || !kLazy) {
+                fwd_stage<Pol, QT, true, false, kPrio>(acc, m, lsum, qf, sK[B], sV[B], st * BK, qpos, Nk, g, l16,
+                                                       p.scale_log2);
             } else {
-                fwd_stage<Pol, 1, true, true, false, true>(acc, m, lsum, qf, sK[cur], sV[cur], k0, qpos - l16, Nk, g,
-                                                           l16, p.scale_log2);
+                fwd_stage_lazy<Pol, QT, true, false, kPrio>(acc, m, lsum, qf, sK[B], sV[B], st * BK, qpos, Nk, g, l16,
+                                                            p.scale_log2);
             }
         }
         wait_stage();
         __syncthreads();
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    int st = s_lo;
+    if (st < whole) main_stage(B0{}, std::true_type{}, st++);
+    for (; st + 1 < whole; st += 2) {
+        main_stage(B1{}, std::false_type{}, st);
+        main_stage(B0{}, std::false_type{}, st + 1);
     }
-    const float ltot = xg_sum(lsum[0]);
-    float z = 0.f * ltot;
+    if (st < whole) main_stage(B1{}, std::false_type{}, st++);
+    for (; st < s_hi; ++st) {
+        const int cur = (st - s_lo) & 1;
+        if (st + 1 < s_hi) stage_next(sK[cur ^ 1], sV[cur ^ 1], st + 1);
+        if (some && st * BK <= pos_w)  // else no row of the wave sees the stage
+            fwd_stage<Pol, QT, true, true, kPrio, true>(acc, m, lsum, qf, sK[cur], sV[cur], st * BK, qpos, Nk, g, l16,
+                                                        p.scale_log2);
+        wait_stage();
+        __syncthreads();
+    }
+    float ltot[QT], z = 0.f;
 #pragma unroll
-    for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt][0]);
+    for (int qt = 0; qt < QT; ++qt) {
+        ltot[qt] = xg_sum(lsum[qt]);
+        z += 0.f * ltot[qt];
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt][qt]);
+    }
     float *part = nullptr, *ml = nullptr;
     if (it.shares > 1) {
-        part = batch_part<false>(p, it.slot, D);
-        ml = batch_ml<false>(p, it.slot, D);
+        part = batch_part<false, ROWS>(p, it.slot, D);
+        ml = batch_ml<false, ROWS>(p, it.slot, D);
     }
     const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
     if (lane == 0) flags[wave] = bad;
     __syncthreads();
     if (flags[0] | flags[1] | flags[2] | flags[3]) {
-        batch_plain<T, D, kBatchMany>(p, it, s_lo * BK, s_hi * BK, part, ml);
+        for (int i = 0; i < QT; ++i) batch_plain<T, D, ROWS>(p, it, 64 * i, s_lo * BK, s_hi * BK, part, ml);
         return;
     }
-    if (it.shares > 1) {
-        const int rl = wave * 16 + l16;
-        if (r < it.s.rows) {
 #pragma unroll
-            for (int i = 0; i < XT; ++i)
-                store4<float>(part + rl * D + batch_col<Pol>(i, g), batch_quad<Pol>(acc, i), 1.0f);
-            if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m[0], ltot);
+    for (int qt = 0; qt < QT; ++qt) {
+        const int r = rw + 16 * qt + l16, rl = r - r0;
+        const bool have = r < it.s.rows;
+        if (it.shares > 1) {
+            if (have) {
+#pragma unroll
+                for (int i = 0; i < XT; ++i)
+                    store4<float>(part + rl * D + batch_col<Pol>(i, g), batch_quad<Pol>(acc, i, qt), 1.0f);
+                if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m[qt], ltot[qt]);
+            }
+            continue;
         }
-        return;
-    }
-    const float inv = ltot > 0.f ? 1.0f / ltot : 0.f;
-    T *O = static_cast<T *>(p.o) + batch_elem(p, it, row, p.o_rs, D);
-    if constexpr (sizeof(T) == 2) {
+        const float inv = ltot[qt] > 0.f ? 1.0f / ltot[qt] : 0.f;
+        T *O = static_cast<T *>(p.o) + batch_elem(p, it, min(r, last_row), p.o_rs, D);
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int xt = 0; xt < XT; xt += 2)
-            store8_pair_bf16(O, 16 * xt, g, acc[xt][0], acc[xt + 1][0], inv, r < it.s.rows);
-    } else if (r < it.s.rows) {
+            for (int xt = 0; xt < XT; xt += 2)
+                store8_pair_bf16(O, 16 * xt, g, acc[xt][qt], acc[xt + 1][qt], inv, have);
+        } else if (have) {
 #pragma unroll
-        for (int i = 0; i < XT; ++i) store4<T>(O + batch_col<Pol>(i, g), batch_quad<Pol>(acc, i), inv);
+            for (int i = 0; i < XT; ++i) store4<T>(O + batch_col<Pol>(i, g), batch_quad<Pol>(acc, i, qt), inv);
+        }
+        if (p.lse != nullptr && have && g == 0)
+            p.lse[batch_lse(p, it, r)] = ltot[qt] > 0.f ? (m[qt] + fast_log2(ltot[qt])) * kLn2 : -INFINITY;
     }
-    if (p.lse != nullptr && r < it.s.rows && g == 0)
-        p.lse[batch_lse(p, it, r)] = ltot > 0.f ? (m[0] + fast_log2(ltot)) * kLn2 : -INFINITY;
 }
 
 // ---------------------------------------------------------------------- the join
@@ -586,19 +699,19 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
 // The shares of a split unit: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
 // D / 4 threads have a row, four elements each; where the unit has few rows
 // several such groups take turns over a row's shares and meet in LDS.
-template <class T, int D, bool FEW>
+template <class T, int D, bool FEW, int ROWS>
 __device__ __forceinline__ void batch_join_body(const BatchParams &p, int w) {
-    constexpr int C = D / 4, NG = 256 / C, ROWS = batch_rows<FEW>();
+    constexpr int C = D / 4, NG = 256 / C;
     __shared__ __attribute__((aligned(16))) f32x4 so[NG][C];
     BatchItem it;
-    if (!find_item<FEW, true>(p, w, it)) return;
+    if (!find_item<FEW, ROWS, true>(p, w, it)) return;
     const int tid = threadIdx.x, c = tid % C, grp = tid / C;
     const int nrows = min(ROWS, it.s.rows - it.unit * ROWS), S = it.shares;
     int together = 1;  // groups to a row
     while (together * 2 * nrows <= NG) together *= 2;
     const int turn = grp % together;
-    const float *part = batch_part<FEW>(p, it.slot, D);
-    const float *ml = batch_ml<FEW>(p, it.slot, D);
+    const float *part = batch_part<FEW, ROWS>(p, it.slot, D);
+    const float *ml = batch_ml<FEW, ROWS>(p, it.slot, D);
     const size_t pstep = (size_t)p.Hkv * ROWS * D, mstep = (size_t)p.Hkv * ROWS * 2;
     for (int r0 = 0; r0 < nrows; r0 += NG / together) {
         const int r = r0 + grp / together;
@@ -640,25 +753,24 @@ template <class T, int D>
 __device__ __forceinline__ void batch_join(const BatchParams &p, int few_groups) {
     const int w = blockIdx.x;
     if (w < few_groups) {
-        batch_join_body<T, D, true>(p, w);
+        batch_join_body<T, D, true, kBatchFew>(p, w);
     } else {
-        batch_join_body<T, D, false>(p, w - few_groups);
+        batch_join_body<T, D, false, batch_many_rows(sizeof(T) == 2)>(p, w - few_groups);
     }
 }
 
-#if defined(__HIP_DEVICE_COMPILE__)
 #define MXFA_BATCH(SUFFIX, POL, NW, WPS)                                                              \
     extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {  \
         batch_few_body<POL, NW>(p);                                                                   \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) { \
-        batch_many_body<POL>(p);                                                                      \
+        batch_many_body<POL, batch_tiles(sizeof(POL::T) == 2)>(p);                                                                     \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void mxfa_batch_##SUFFIX##_join(BatchParams p, int few_groups) { \
         batch_join<POL::T, POL::D>(p, few_groups);                                                    \
     }
-MXFA_BATCH(b64, PolBF16<64>, 8, 3)
-MXFA_BATCH(b128, PolBF16<128>, 4, 2)
+MXFA_BATCH(b64, PolRows<64>, 8, 3)
+MXFA_BATCH(b128, PolRows<128>, 4, 2)
 MXFA_BATCH(f64, PolF32, 4, 2)
 #undef MXFA_BATCH
 #endif
@@ -682,10 +794,10 @@ static bool batch_may_be_many(const BatchParams &p) {
 }
 
 // Units there can be: for the few-row form one per sequence and KV head; the
-// many-row form's hold 64 rows but for a sequence's last.
-static long long batch_units(const BatchParams &p, bool few) {
+// many-row form's are full but for a sequence's last.
+static long long batch_units(const BatchParams &p, bool few, int dtype_bf16) {
     if (few) return (long long)std::min(p.n_seq, p.n_tok) * p.Hkv;
-    return ((long long)p.n_tok * p.group / kBatchMany + std::min(p.n_seq, p.n_tok)) * p.Hkv;
+    return ((long long)p.n_tok * p.group / batch_many_rows(dtype_bf16) + std::min(p.n_seq, p.n_tok)) * p.Hkv;
 }
 
 size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
@@ -693,13 +805,13 @@ size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
     p.few_rows = batch_few_rows(p);
     size_t n = 0;
     if (p.few_rows > 0) n += batch_part_floats(batch_target(true, dtype_bf16, p.d), kBatchFew, p.d);
-    if (batch_may_be_many(p)) n += batch_part_floats(batch_target(false, dtype_bf16, p.d), kBatchMany, p.d);
+    if (batch_may_be_many(p)) n += batch_part_floats(batch_target(false, dtype_bf16, p.d), batch_many_rows(dtype_bf16), p.d);
     return n * sizeof(float);
 }
 
 long long batch_groups(const BatchParams &q, int dtype_bf16) {
-    return std::max(batch_units(q, true) + batch_target(true, dtype_bf16, q.d),
-                    batch_units(q, false) + batch_target(false, dtype_bf16, q.d));
+    return std::max(batch_units(q, true, dtype_bf16) + batch_target(true, dtype_bf16, q.d),
+                    batch_units(q, false, dtype_bf16) + batch_target(false, dtype_bf16, q.d));
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
@@ -712,19 +824,20 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     const bool few = p.few_rows > 0, many = batch_may_be_many(p);
     p.target[0] = batch_target(true, dtype_bf16, p.d);
     p.target[1] = batch_target(false, dtype_bf16, p.d);
+    for (int f = 0; f < 2; ++f) p.per_item[f] = 1.0f / (float)p.target[f];
     p.part[0] = static_cast<float *>(workspace);
     p.part[1] = p.part[0] + (few ? batch_part_floats(p.target[0], kBatchFew, p.d) : 0);
     void *args[] = {&p};
     hipError_t e = hipSuccess;
     if (many)
-        e = launch_kernel(id[1], dim3((unsigned)(batch_units(p, false) + p.target[1])), dim3(256), args, stream);
+        e = launch_kernel(id[1], dim3((unsigned)(batch_units(p, false, dtype_bf16) + p.target[1])), dim3(256), args, stream);
     if (e == hipSuccess && few)
-        e = launch_kernel(id[0], dim3((unsigned)(batch_units(p, true) + p.target[0])),
+        e = launch_kernel(id[0], dim3((unsigned)(batch_units(p, true, dtype_bf16) + p.target[0])),
                           dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
     if (e != hipSuccess) return e;
     // a split unit has two shares at least
-    int few_groups = few ? (int)std::min<long long>(batch_units(p, true), p.target[0]) : 0;
-    const int many_groups = many ? (int)std::min<long long>(batch_units(p, false), p.target[1]) : 0;
+    int few_groups = few ? (int)std::min<long long>(batch_units(p, true, dtype_bf16), p.target[0]) : 0;
+    const int many_groups = many ? (int)std::min<long long>(batch_units(p, false, dtype_bf16), p.target[1]) : 0;
     void *jargs[] = {&p, &few_groups};
     return launch_kernel(id[2], dim3(few_groups + many_groups), dim3(256), jargs, stream);
 }

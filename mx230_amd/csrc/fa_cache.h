@@ -49,6 +49,7 @@ struct BatchParams {
     // (0: none); per form (few, many) the items the work is cut into, about,
     // and the workspace's part of it
     int few_rows, target[2];
+    float per_item[2];  // 1 / target
     float *part[2];
 };
 

@@ -200,6 +200,18 @@ __device__ __forceinline__ float xg_sum_pairs(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Position of a lane's row of query tile qt: consecutive rows from the wave's
+// first one, or each lane's own (rows that share tokens, fa_batch.hip).
+__device__ __forceinline__ int row_pos(int qpos0, int qt, int l16) { return qpos0 + 16 * qt + l16; }
+template <int QT>
+struct RowPos {
+    int at[QT];
+};
+template <int QT>
+__device__ __forceinline__ int row_pos(const RowPos<QT> &p, int qt, int) {
+    return p.at[qt];
+}
+
 // Makes x opaque to the optimiser (an empty asm that "modifies" it), so a value
 // computed once before a loop is not recomputed inside it.
 template <class X>

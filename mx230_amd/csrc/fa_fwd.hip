@@ -52,11 +52,11 @@ struct FwdNothing {
     __device__ __forceinline__ void operator()() const {}
 };
 template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, bool EMPTY_ROWS = false,
-          class AfterK = FwdNothing, class BeforeV = FwdNothing>
+          class AfterK = FwdNothing, class BeforeV = FwdNothing, class Pos = int>
 __device__ __forceinline__ void fwd_stage(f32x4 (&acc)[Pol::D / 16][QT], float (&m)[QT], float (&lsum)[QT],
                                           const typename Pol::Frag (&qf)[QT][Pol::NC],
-                                          const typename Pol::T *sk, const typename Pol::T *sv, int k0, int qpos0,
-                                          int Nk, int g, int l16, float xmul, AfterK after_k = {},
+                                          const typename Pol::T *sk, const typename Pol::T *sv, int k0,
+                                          const Pos &qpos0, int Nk, int g, int l16, float xmul, AfterK after_k = {},
                                           BeforeV before_v = {}) {
     using Frag = typename Pol::Frag;
     constexpr int NC = Pol::NC, XT = Pol::D / 16;
@@ -81,7 +81,7 @@ __device__ __forceinline__ void fwd_stage(f32x4 (&acc)[Pol::D / 16][QT], float (
     after_k();
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        const int lim = fwd_mask_limit<Pol, CAUSAL>(qpos0 + 16 * qt + l16, k0, Nk, g);
+        const int lim = fwd_mask_limit<Pol, CAUSAL>(row_pos(qpos0, qt, l16), k0, Nk, g);
         float mx = -INFINITY;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
@@ -159,10 +159,10 @@ constexpr float kLazySum = 65536.0f;
 // Scores of one 64-key stage relative to m: s = K Q^T scale log2(e) - m, with
 // masked keys (MASK) at -inf: the accumulators start at -m / xmul and the
 // fp32 result is multiplied by xmul = scale log2(e).
-template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false>
+template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, class Pos = int>
 __device__ __forceinline__ void fwd_scores(f32x4 (&s)[2][2][QT], const float (&m)[QT],
                                            const typename Pol::Frag (&qf)[QT][Pol::NC], const typename Pol::T *sk,
-                                           int k0, int qpos0, int Nk, int g, int l16, float xmul) {
+                                           int k0, const Pos &qpos0, int Nk, int g, int l16, float xmul) {
     using Frag = typename Pol::Frag;
     constexpr int NC = Pol::NC;
     const float im = 1.0f / xmul;
@@ -192,7 +192,7 @@ __device__ __forceinline__ void fwd_scores(f32x4 (&s)[2][2][QT], const float (&m
     if constexpr (MASK) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            const int lim = fwd_mask_limit<Pol, CAUSAL>(qpos0 + 16 * qt + l16, k0, Nk, g);
+            const int lim = fwd_mask_limit<Pol, CAUSAL>(row_pos(qpos0, qt, l16), k0, Nk, g);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
@@ -229,11 +229,11 @@ __device__ __forceinline__ void fwd_exp_sum(f32x4 (&s)[2][2][QT], float (&l)[QT]
     }
 }
 
-template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false>
+template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, class Pos = int>
 __device__ __forceinline__ void fwd_stage_lazy(f32x4 (&acc)[Pol::D / 16][QT], float (&m)[QT], float (&lsum)[QT],
                                                const typename Pol::Frag (&qf)[QT][Pol::NC],
                                                const typename Pol::T *sk, const typename Pol::T *sv, int k0,
-                                               int qpos0, int Nk, int g, int l16, float xmul) {
+                                               const Pos &qpos0, int Nk, int g, int l16, float xmul) {
     constexpr int XT = Pol::D / 16;
     f32x4 s[2][2][QT];  // [block][t][qt]
     fwd_scores<Pol, QT, CAUSAL, MASK, PRIO>(s, m, qf, sk, k0, qpos0, Nk, g, l16, xmul);

@@ -757,7 +757,9 @@ int mxfa_check_batch(const mxfa_batch_shape *s) {
     if (s->dtype == MXFA_F32 && s->head_dim != 64) return MXFA_ERR_UNSUPPORTED;
     // rows of a KV head, and the work-groups of a launch, are counted in ints
     const long long group = s->n_head / s->n_kv_head;
-    if ((long long)s->n_tok * group > 0x7fffffffLL - 64) return MXFA_ERR_SHAPE;
+    if ((long long)s->n_tok * group > 0x7fffffffLL - 128) return MXFA_ERR_SHAPE;
+    // and the caches' rows in 32 bits
+    if ((long long)s->n_blocks * s->block_size > 0x80000000LL) return MXFA_ERR_SHAPE;
     const mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
     if (mxfa::batch_groups(p, s->dtype == MXFA_BF16) > 0x7fffffffLL / 512) return MXFA_ERR_SHAPE;
     return MXFA_OK;
