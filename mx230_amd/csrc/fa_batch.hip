@@ -29,20 +29,15 @@
 namespace mxfa {
 
 constexpr int kBatchFew = 16;  // rows of the few-row form's units
-// the fewest stages of a share, per form: shorter ones cost more in the join
-// than they save
-constexpr int kFewLeast = 4, kManyLeast = 4;
-
+constexpr int kJoinRows = 32;  // rows of a work-group of the join
 // Rows of the many-row form's units: 16 per wave and query tile.
 __host__ __device__ constexpr int batch_tiles(bool bf16) { return bf16 ? 2 : 1; }
 __host__ __device__ constexpr int batch_many_rows(bool bf16) { return 64 * batch_tiles(bf16); }
 
-// Slots of the workspace: the shares of split units. A unit of n stages is
-// split where n > quota, into ceil(n / quota) < 2 n / quota shares, and quota
-// >= all stages / target, so there are at most 2 target of them.
-__host__ __device__ constexpr long long batch_slots(int target) { return 2LL * target; }
-__host__ __device__ constexpr size_t batch_part_floats(int target, int rows, int d) {
-    return (size_t)batch_slots(target) * rows * (d + 2);
+// The workspace holds the shares of split units: `slots` of them, each ROWS rows
+// of D floats and their (max, sum) pairs.
+__host__ __device__ constexpr size_t batch_part_floats(long long slots, int rows, int d) {
+    return (size_t)slots * rows * (d + 2);
 }
 
 // The device code builds on the forward's stages (fa_fwd.hip, the same
@@ -219,18 +214,27 @@ __device__ __forceinline__ BatchSeq batch_seq(const BatchParams &p, int s) {
     return b;
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) x += __shfl_xor(x, k, 64);
+// Inclusive prefix over the wave, all 64 lanes active (rows of 16 by shifts, then
+// the rows' ends broadcast into the next row, and into the upper half).
+template <class X>
+__device__ __forceinline__ X wave_prefix(X x) {
+    auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                  decltype(rows)::value, 0xf, false);
+        x += __builtin_bit_cast(X, o);
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15, 31
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
     return x;
 }
-__device__ __forceinline__ int wave_prefix(int x, int lane) {  // inclusive
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const int o = __shfl_up(x, k, 64);
-        if (lane >= k) x += o;
-    }
-    return x;
+template <class X>
+__device__ __forceinline__ X wave_sum(X x) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_prefix(x)), 63));
 }
 
 struct BatchItem {
@@ -239,33 +243,65 @@ struct BatchItem {
     int slot;  // of share 0 (the join) or of this share, where shares > 1
 };
 
+__device__ __forceinline__ int batch_shares(int stages, unsigned quota) {
+    return (unsigned)stages > quota ? (int)(((unsigned)stages + quota - 1) / quota) : 1;
+}
+
 // Item `w` of a form (JOIN: split unit `w`), found by every wave for itself: a
-// lane per sequence, twice over them where there are more than 64. False past
+// lane per sequence, again over them where there are more than 64. False past
 // the last one. Items of a sequence: units (the last, heaviest one first) x
 // shares x KV heads, so that neighbouring work-groups, which the dispatcher
 // spreads over the XCDs, have the heads and an XCD's share of them the same
 // head's keys.
+//
+// The quota, the most stages of a share: where the units fit the work-groups
+// that are resident at once (p.resident), the least one by which their shares
+// still do, found by raising an even share's; else, or where that leaves the
+// longest share half as long again as an even one, shares of 1 / rounds of it,
+// which later rounds even out. It depends on lengths alone, so the join
+// finds the same one.
 template <bool FEW, int ROWS, bool JOIN>
 __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem &it) {
+    constexpr int F = FEW ? 0 : 1;
     const int lane = threadIdx.x & 63;
     BatchSeq b = batch_seq<FEW, ROWS>(p, lane);
-    // the sum of all stages in fp32, rounded up by more than its rounding
+    // sums of all sequences; the stages' in fp32, rounded up by more than its rounding
     float all = (float)b.units * (float)max(b.stages, 1);
+    float units = (float)b.units;
     for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
         const BatchSeq c = batch_seq<FEW, ROWS>(p, s0 + lane);
         all += (float)c.units * (float)max(c.stages, 1);
+        units += (float)c.units;
     }
-    all = wave_sum(all) * (float)p.Hkv;
-    const float even = fminf(all * p.per_item[FEW ? 0 : 1] * 1.001f + 1.0f, 1e9f);
-    const unsigned quota = max((unsigned)even, (unsigned)(FEW ? kFewLeast : kManyLeast));
+    all = fminf(wave_sum(all) * (float)p.Hkv * 1.001f, 1e18f);
+    units = wave_sum(units) * (float)p.Hkv;
+    const float resident = (float)p.resident[F], even = fminf(all * p.per_resident[F] + 1.0f, 1e9f);
+    unsigned quota = (unsigned)fmaxf(fminf(all * p.per_target[F] + 1.0f, 1e9f), (float)p.least[F]);
+    if (units <= resident) {
+        unsigned q = max((unsigned)even, (unsigned)p.least[F]);
+        const float most = fmaxf(1.5f * even + 1.0f, (float)p.least[F]);
+        for (int i = 0; i < 5 && (float)q <= most; ++i) {
+            int n = b.units * batch_shares(b.stages, q);
+            for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
+                const BatchSeq c = batch_seq<FEW, ROWS>(p, s0 + lane);
+                n += c.units * batch_shares(c.stages, q);
+            }
+            const float items = (float)wave_sum(n) * (float)p.Hkv;
+            if (items <= resident) {
+                quota = q;
+                break;
+            }
+            q = max(q + 1, (unsigned)((float)q * items * p.per_resident[F]));
+        }
+    }
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
         if (s0 > 0) b = batch_seq<FEW, ROWS>(p, s0 + lane);
-        const int shares = (unsigned)b.stages > quota ? (int)(((unsigned)b.stages + quota - 1) / quota) : 1;
+        const int shares = batch_shares(b.stages, quota);
         const int unit_items = b.units * p.Hkv;
         const int mine = shares > 1 ? unit_items * shares : 0;
         const int per = JOIN ? (shares > 1 ? unit_items : 0) : unit_items * shares;
-        const int upto = wave_prefix(per, lane), slots_upto = wave_prefix(mine, lane);
+        const int upto = wave_prefix(per), slots_upto = wave_prefix(mine);
         const unsigned long long at = __builtin_amdgcn_ballot_w64(before + upto > w);
         if (at != 0) {
             const int l = __builtin_ctzll(at);
@@ -285,13 +321,14 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
                 it.slot += per_unit * it.shares * heads + it.head;  // the unit's shares are `heads` apart
                 it.share = 0;
                 it.unit = it.s.units - 1 - (int)per_unit;
-            } else {
-                it.slot += i;
-                const unsigned u = per_unit / (unsigned)it.shares;
-                it.share = per_unit - u * it.shares;
-                it.unit = it.s.units - 1 - (int)u;
+                return it.slot + (it.shares - 1) * p.Hkv < p.slots[F];
             }
-            return true;
+            it.slot += i;
+            const unsigned u = per_unit / (unsigned)it.shares;
+            it.share = per_unit - u * it.shares;
+            it.unit = it.s.units - 1 - (int)u;
+            // (false only where cu_q says the same rows twice over)
+            return it.shares == 1 || it.slot < p.slots[F];
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         slots += __builtin_amdgcn_readlane(slots_upto, 63);
@@ -404,7 +441,7 @@ __device__ __forceinline__ float *batch_part(const BatchParams &p, int slot, int
 template <bool FEW, int ROWS>
 __device__ __forceinline__ float *batch_ml(const BatchParams &p, int slot, int d) {
     const int f = FEW ? 0 : 1;
-    return p.part[f] + (size_t)batch_slots(p.target[f]) * ROWS * d + (size_t)slot * ROWS * 2;
+    return p.part[f] + (size_t)p.slots[f] * ROWS * d + (size_t)slot * ROWS * 2;
 }
 
 // ------------------------------------------------------------------ the few rows
@@ -696,17 +733,20 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
 
 // ---------------------------------------------------------------------- the join
 
-// The shares of a split unit: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-// D / 4 threads have a row, four elements each; where the unit has few rows
-// several such groups take turns over a row's shares and meet in LDS.
+// The shares of a split unit: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
+// kJoinRows rows per work-group (part). D / 4 threads have a row, four elements
+// each; where there are few rows several such groups take turns over a row's
+// shares and meet in LDS.
 template <class T, int D, bool FEW, int ROWS>
-__device__ __forceinline__ void batch_join_body(const BatchParams &p, int w) {
+__device__ __forceinline__ void batch_join_body(const BatchParams &p, int w, int piece) {
     constexpr int C = D / 4, NG = 256 / C;
     __shared__ __attribute__((aligned(16))) f32x4 so[NG][C];
     BatchItem it;
     if (!find_item<FEW, ROWS, true>(p, w, it)) return;
     const int tid = threadIdx.x, c = tid % C, grp = tid / C;
-    const int nrows = min(ROWS, it.s.rows - it.unit * ROWS), S = it.shares;
+    const int first = piece * kJoinRows, end = min(min(first + kJoinRows, ROWS), it.s.rows - it.unit * ROWS);
+    const int nrows = end - first, S = it.shares;
+    if (nrows <= 0) return;
     int together = 1;  // groups to a row
     while (together * 2 * nrows <= NG) together *= 2;
     const int turn = grp % together;
@@ -714,8 +754,8 @@ __device__ __forceinline__ void batch_join_body(const BatchParams &p, int w) {
     const float *ml = batch_ml<FEW, ROWS>(p, it.slot, D);
     const size_t pstep = (size_t)p.Hkv * ROWS * D, mstep = (size_t)p.Hkv * ROWS * 2;
     for (int r0 = 0; r0 < nrows; r0 += NG / together) {
-        const int r = r0 + grp / together;
-        const bool have = r < nrows;
+        const bool have = r0 + grp / together < nrows;
+        const int r = first + r0 + grp / together;
         float M = -INFINITY, L = 0.f;
         f32x4 o = zero4();
         if (have) {
@@ -748,14 +788,16 @@ __device__ __forceinline__ void batch_join_body(const BatchParams &p, int w) {
     }
 }
 
-// Grid: the split units the few-row form may have, then the many-row form's.
+// Grid: the split units the few-row form may have, then the pieces of the
+// many-row form's.
 template <class T, int D>
 __device__ __forceinline__ void batch_join(const BatchParams &p, int few_groups) {
-    const int w = blockIdx.x;
-    if (w < few_groups) {
-        batch_join_body<T, D, true, kBatchFew>(p, w);
+    constexpr int ROWS = batch_many_rows(sizeof(T) == 2), PIECES = ROWS / kJoinRows;
+    const int w = (int)blockIdx.x - few_groups;
+    if (w < 0) {
+        batch_join_body<T, D, true, kBatchFew>(p, (int)blockIdx.x, 0);
     } else {
-        batch_join_body<T, D, false, batch_many_rows(sizeof(T) == 2)>(p, w - few_groups);
+        batch_join_body<T, D, false, ROWS>(p, w / PIECES, w % PIECES);
     }
 }
 
@@ -775,12 +817,13 @@ MXFA_BATCH(f64, PolF32, 4, 2)
 #undef MXFA_BATCH
 #endif
 
-// Items the work is cut into, about: the few-row form's work-groups have a CU
-// each, so that four rounds of them even out sequences of different lengths;
-// the many-row form's are resident two or three to a CU.
-static int batch_target(bool few, int dtype_bf16, int d) {
-    return few ? 1024 : 256 * (dtype_bf16 && d == 64 ? 3 : 2);
+// Work-groups resident at once: the few-row form's have a CU each, the many-row
+// form's share one in twos or threes.
+static int batch_resident(bool few, int dtype_bf16, int d) {
+    return few ? 256 : 256 * (dtype_bf16 && d == 64 ? 3 : 2);
 }
+// Rounds of them that longer work is cut into: the items' target.
+static int batch_rounds(bool few) { return few ? 4 : 2; }
 
 // Which forms a call launches, by what the host knows: the few-row form alone
 // where no sequence can have more rows; the many-row form alone where one
@@ -800,18 +843,51 @@ static long long batch_units(const BatchParams &p, bool few, int dtype_bf16) {
     return ((long long)p.n_tok * p.group / batch_many_rows(dtype_bf16) + std::min(p.n_seq, p.n_tok)) * p.Hkv;
 }
 
+// A form's sizes. A unit of n stages has ceil(n / quota) shares where n > quota,
+// and the quota is at least all stages / target: so all items are at most the
+// units + target, the shares of split units at most target + the split units,
+// and those at most target and the units.
+struct BatchForm {
+    int target, rows;
+    long long units, split, slots;
+};
+static BatchForm batch_form(const BatchParams &p, bool few, int dtype_bf16) {
+    BatchForm f;
+    f.target = batch_resident(few, dtype_bf16, p.d) * batch_rounds(few);
+    f.rows = few ? kBatchFew : batch_many_rows(dtype_bf16);
+    f.units = batch_units(p, few, dtype_bf16);
+    f.split = std::min<long long>(f.units, f.target);
+    // a table that holds no more positions than the least share splits nothing
+    if (((((long long)p.max_blocks << p.bs_shift) + 63) / 64) <= p.least[few ? 0 : 1]) f.split = 0;
+    f.slots = f.split > 0 ? f.target + f.split : 0;
+    return f;
+}
+
+// The least stages of a share: one for each of the few-row form's waves; 8 of the
+// many-row form's, below which the join costs more than the split saves.
+static void batch_plan(BatchParams *p, int dtype_bf16) {
+    p->few_rows = batch_few_rows(*p);
+    p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
+    p->least[1] = 8;
+}
+
 size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
     BatchParams p = q;
-    p.few_rows = batch_few_rows(p);
+    batch_plan(&p, dtype_bf16);
     size_t n = 0;
-    if (p.few_rows > 0) n += batch_part_floats(batch_target(true, dtype_bf16, p.d), kBatchFew, p.d);
-    if (batch_may_be_many(p)) n += batch_part_floats(batch_target(false, dtype_bf16, p.d), batch_many_rows(dtype_bf16), p.d);
-    return n * sizeof(float);
+    for (int i = 0; i < 2; ++i) {
+        if (i == 0 ? p.few_rows == 0 : !batch_may_be_many(p)) continue;
+        const BatchForm f = batch_form(p, i == 0, dtype_bf16);
+        n += batch_part_floats(f.slots, f.rows, p.d);
+    }
+    return std::max<size_t>(n * sizeof(float), 16);
 }
 
 long long batch_groups(const BatchParams &q, int dtype_bf16) {
-    return std::max(batch_units(q, true, dtype_bf16) + batch_target(true, dtype_bf16, q.d),
-                    batch_units(q, false, dtype_bf16) + batch_target(false, dtype_bf16, q.d));
+    BatchParams p = q;
+    batch_plan(&p, dtype_bf16);
+    const BatchForm a = batch_form(p, true, dtype_bf16), b = batch_form(p, false, dtype_bf16);
+    return std::max(a.units + a.target, b.units + b.target);
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
@@ -820,26 +896,30 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
         {k_mxfa_batch_b128_few, k_mxfa_batch_b128_many, k_mxfa_batch_b128_join},
         {k_mxfa_batch_f64_few, k_mxfa_batch_f64_many, k_mxfa_batch_f64_join}};
     const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
-    p.few_rows = batch_few_rows(p);
-    const bool few = p.few_rows > 0, many = batch_may_be_many(p);
-    p.target[0] = batch_target(true, dtype_bf16, p.d);
-    p.target[1] = batch_target(false, dtype_bf16, p.d);
-    for (int f = 0; f < 2; ++f) p.per_item[f] = 1.0f / (float)p.target[f];
-    p.part[0] = static_cast<float *>(workspace);
-    p.part[1] = p.part[0] + (few ? batch_part_floats(p.target[0], kBatchFew, p.d) : 0);
+    batch_plan(&p, dtype_bf16);
+    float *next = static_cast<float *>(workspace);
+    unsigned groups[2] = {0, 0};
+    int joins[2] = {0, 0};
+    for (int i = 0; i < 2; ++i) {
+        if (i == 0 ? p.few_rows == 0 : !batch_may_be_many(p)) continue;
+        const BatchForm f = batch_form(p, i == 0, dtype_bf16);
+        p.resident[i] = batch_resident(i == 0, dtype_bf16, p.d);
+        p.per_resident[i] = 1.0f / (float)p.resident[i];
+        p.per_target[i] = 1.0f / (float)f.target;
+        p.slots[i] = (int)f.slots;
+        p.part[i] = next;
+        next += batch_part_floats(f.slots, f.rows, p.d);
+        groups[i] = (unsigned)(f.units + f.target);
+        joins[i] = (int)f.split * (i == 0 ? 1 : f.rows / kJoinRows);
+    }
     void *args[] = {&p};
     hipError_t e = hipSuccess;
-    if (many)
-        e = launch_kernel(id[1], dim3((unsigned)(batch_units(p, false, dtype_bf16) + p.target[1])), dim3(256), args, stream);
-    if (e == hipSuccess && few)
-        e = launch_kernel(id[0], dim3((unsigned)(batch_units(p, true, dtype_bf16) + p.target[0])),
-                          dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
-    if (e != hipSuccess) return e;
-    // a split unit has two shares at least
-    int few_groups = few ? (int)std::min<long long>(batch_units(p, true, dtype_bf16), p.target[0]) : 0;
-    const int many_groups = many ? (int)std::min<long long>(batch_units(p, false, dtype_bf16), p.target[1]) : 0;
-    void *jargs[] = {&p, &few_groups};
-    return launch_kernel(id[2], dim3(few_groups + many_groups), dim3(256), jargs, stream);
+    if (groups[1] > 0) e = launch_kernel(id[1], dim3(groups[1]), dim3(256), args, stream);
+    if (e == hipSuccess && groups[0] > 0)
+        e = launch_kernel(id[0], dim3(groups[0]), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+    if (e != hipSuccess || joins[0] + joins[1] == 0) return e;
+    void *jargs[] = {&p, &joins[0]};
+    return launch_kernel(id[2], dim3(joins[0] + joins[1]), dim3(256), jargs, stream);
 }
 
 }  // namespace mxfa

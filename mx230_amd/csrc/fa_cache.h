@@ -44,12 +44,13 @@ struct BatchParams {
     int dim, interleaved;
     float factor;
     int hpt;  // heads per thread
-    // attention (fa_batch.hip): the sequences whose rows (new tokens x query
-    // heads of a KV head) the few-row kernel takes, at most few_rows of them
-    // (0: none); per form (few, many) the items the work is cut into, about,
-    // and the workspace's part of it
-    int few_rows, target[2];
-    float per_item[2];  // 1 / target
+    // attention (fa_batch.hip): the most rows (new tokens x query heads of a KV
+    // head) of a sequence that the few-row form takes (0: it takes none); per
+    // form (few, many) the work-groups resident at once, the least stages of a
+    // share, 1 / resident and 1 / the items the work is cut into at most, and the
+    // shares' slots of the workspace
+    int few_rows, resident[2], least[2], slots[2];
+    float per_resident[2], per_target[2];
     float *part[2];
 };
 

@@ -758,6 +758,8 @@ int mxfa_check_batch(const mxfa_batch_shape *s) {
     // rows of a KV head, and the work-groups of a launch, are counted in ints
     const long long group = s->n_head / s->n_kv_head;
     if ((long long)s->n_tok * group > 0x7fffffffLL - 128) return MXFA_ERR_SHAPE;
+    // (also where cu_q gives every sequence all rows)
+    if ((double)s->n_seq * ((double)s->n_tok * group / 64 + 1) * s->n_kv_head > 1073741824.0) return MXFA_ERR_SHAPE;
     // and the caches' rows in 32 bits
     if ((long long)s->n_blocks * s->block_size > 0x80000000LL) return MXFA_ERR_SHAPE;
     const mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);

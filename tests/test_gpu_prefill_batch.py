@@ -160,9 +160,10 @@ def test_strides_and_shared_rows():
     torch.cuda.synchronize()
     check(b, out[:, :nh * hd].cpu(), None)
     assert bool((out[:, nh * hd:] == 7.0).all())
+    far = torch.zeros(2, 1000, dtype=torch.int32, device="cuda")  # a table whose sequences may be split
     with pytest.raises(mx.MxfaError):
-        mx.run_prefill_batch(qkv[:, :nh * hd], w[:, :nkv * hd], w[:, nkv * hd:2 * nkv * hd], out, tab, bs, cu, lens, 3,
-                             nh, nkv, hd, workspace=ws[:-256])
+        mx.run_prefill_batch(qkv[:, :nh * hd], w[:, :nkv * hd], w[:, nkv * hd:2 * nkv * hd], out, far, bs, cu, lens, 3,
+                             nh, nkv, hd, workspace=ws[:256])
     with pytest.raises(ValueError):
         mx.run_prefill_batch(qkv[:, :nh * hd], w[:, :nkv * hd], w[:, nkv * hd:2 * nkv * hd], out, tab[:1], bs, cu, lens,
                              3, nh, nkv, hd)
