@@ -225,7 +225,7 @@ class _NoBinding:
     def _other(*args):
         return NotImplemented
     attention_fwd = attention_bwd = prefill = _other
-    rotary = cache_append = prefill_batch = pages_free = pages_fork = pages_compact = pages_copy = _other
+    rotary = rotary_embedding = cache_append = prefill_batch = pages_free = pages_fork = pages_compact = pages_copy = _other
 
 
 def _calls():

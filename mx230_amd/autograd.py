@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from . import attention_bwd, attention_fwd, run_rotary
+from . import _calls, attention_bwd, attention_fwd, run_rotary
 
 
 class FlashAttentionFunction(torch.autograd.Function):
@@ -54,33 +54,36 @@ def _rows16(x):
 
 
 class RotaryFunction(torch.autograd.Function):
-    """Q and K with rotary positions; the gradient is the transposed rotation."""
+    """Q and K with rotary positions; the gradient is the transposed rotation,
+    differentiable itself (the binding's C++ node in Python, for the calls it
+    leaves)."""
 
     @staticmethod
-    def forward(ctx, q, k, frequencies, positions, pos0: int, interleaved: bool, factor: float):
+    def forward(ctx, q, k, frequencies, positions, pos0: int, interleaved: bool, factor: float, inverse: bool):
         ctx.save_for_backward(frequencies, positions)
-        ctx.args = pos0, interleaved, factor
+        ctx.args = pos0, interleaved, factor, inverse
         q, k = _rows16(q), _rows16(k)
         qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
-        run_rotary(q, k, qo, ko, frequencies, positions, pos0, interleaved, factor)
+        run_rotary(q, k, qo, ko, frequencies, positions, pos0, interleaved, factor, inverse)
         return qo, ko
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         frequencies, positions = ctx.saved_tensors
-        pos0, interleaved, factor = ctx.args
-        dq, dk = _rows16(dq), _rows16(dk)
-        gq, gk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (dq, dk))
-        run_rotary(dq, dk, gq, gk, frequencies, positions, pos0, interleaved, factor, inverse=True)
-        return gq, gk, None, None, None, None, None
+        pos0, interleaved, factor, inverse = ctx.args
+        gq, gk = RotaryFunction.apply(dq, dk, frequencies, positions, pos0, interleaved, factor, not inverse)
+        return gq, gk, None, None, None, None, None, None
 
 
 def rotary_embedding(q, k, frequencies, positions=None, pos0: int = 0, interleaved: bool = False, factor: float = 1.0):
     """Differentiable rotary positions of Q and K [B, H, N, d] (any strides; the
-    results are contiguous), as :func:`mx230_amd.run_rotary` takes them. The
-    positions and frequencies must stay as they are until the backward has run."""
-    return RotaryFunction.apply(q, k, frequencies, positions, pos0, interleaved, factor)
+    results are contiguous), as :func:`mx230_amd.run_rotary` takes them; no
+    gradient reaches the frequencies. Positions and frequencies must stay as
+    they are until the backward has run."""
+    out = _calls().rotary_embedding(q, k, frequencies, positions, pos0, interleaved, factor)
+    if out is not NotImplemented:
+        return out
+    return RotaryFunction.apply(q, k, frequencies, positions, pos0, interleaved, factor, False)
 
 
 class CausalSelfAttention(torch.nn.Module):

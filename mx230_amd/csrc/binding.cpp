@@ -11,9 +11,11 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <optional>
 
 #include "../../include/mxfa.h"
 
@@ -257,54 +259,136 @@ bool heads(const at::Tensor *t, at::ScalarType type, int64_t (&n)[4], long long 
     return n[3] == 1 || t->stride(-1) == 1;
 }
 
+// The shape of a rotary call over checked tensors (k and ko null: Q alone).
+struct RotaryArgs {
+    const at::Tensor *q, *k, *qo, *ko, *f, *pos;
+    bool shape(mxfa_rotary_shape *s) const {
+        int64_t nq[4], nk[4], no[4];
+        long long sq[3], sk[3] = {0, 0, 0}, so[3], sko[3] = {0, 0, 0};
+        if (!q || !is_mxfa_type(*q) || !heads(q, q->scalar_type(), nq, sq) || !heads(qo, q->scalar_type(), no, so) ||
+            !same(nq, no))
+            return false;
+        if (k != nullptr && (!heads(k, q->scalar_type(), nk, sk) || !heads(ko, q->scalar_type(), no, sko) ||
+                             !same(nk, no) || nk[0] != nq[0] || nk[2] != nq[2] || nk[3] != nq[3]))
+            return false;
+        if (!vec(f, at::kDouble, 1) || 2 * f->numel() > nq[3]) return false;
+        if (pos != nullptr) {
+            if (!here(pos) || pos->scalar_type() != at::kInt || pos->dim() < 1 || pos->dim() > 2 ||
+                pos->size(-1) != nq[2] || (nq[2] > 1 && pos->stride(-1) != 1) ||
+                (pos->dim() == 2 && pos->size(0) != nq[0]))
+                return false;
+            s->pos_bs = pos->dim() == 2 ? pos->stride(0) : 0;
+        }
+        s->B = (int)nq[0];
+        s->Hq = (int)nq[1];
+        s->Hkv = k != nullptr ? (int)nk[1] : 0;
+        s->N = (int)nq[2];
+        s->head_dim = (int)nq[3];
+        s->rotary_dim = 2 * (int)f->numel();
+        s->dtype = q->scalar_type() == at::kBFloat16 ? MXFA_BF16 : MXFA_F32;
+        s->q_bs = sq[0], s->q_hs = sq[1], s->q_ts = sq[2];
+        s->k_bs = sk[0], s->k_hs = sk[1], s->k_ts = sk[2];
+        s->qo_bs = so[0], s->qo_hs = so[1], s->qo_ts = so[2];
+        s->ko_bs = sko[0], s->ko_hs = sko[1], s->ko_ts = sko[2];
+        return true;
+    }
+    int run(const mxfa_rotary_shape &s) const {
+        return abi.rotary(&s, q->data_ptr(), k ? k->data_ptr() : nullptr, qo->data_ptr(), ko ? ko->data_ptr() : nullptr,
+                          pos ? ints(pos) : nullptr, static_cast<const double *>(f->data_ptr()), current_stream());
+    }
+};
+
 // rotary(q, k, q_out, k_out, frequencies, positions, pos0, interleaved, factor, inverse): the status
 PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 10 || abi.rotary == nullptr) return other();
     return guarded([&]() -> PyObject * {
         const bool two = a[1] != Py_None, given = a[5] != Py_None;
-        const at::Tensor *q = plain(a[0]), *k = two ? plain(a[1]) : nullptr, *qo = plain(a[2]),
-                         *ko = two ? plain(a[3]) : nullptr, *f = plain(a[4]), *pos = given ? plain(a[5]) : nullptr;
-        int64_t nq[4], nk[4], no[4];
+        const RotaryArgs r{plain(a[0]), two ? plain(a[1]) : nullptr, plain(a[2]), two ? plain(a[3]) : nullptr,
+                           plain(a[4]), given ? plain(a[5]) : nullptr};
         mxfa_rotary_shape s{};
-        long long sq[3], sk[3] = {0, 0, 0}, so[3], sko[3] = {0, 0, 0};
         double factor;
-        if (!q || !is_mxfa_type(*q) || !heads(q, q->scalar_type(), nq, sq) || !heads(qo, q->scalar_type(), no, so) ||
-            !same(nq, no) || (!two && a[3] != Py_None))
-            return other();
-        if (two && (!heads(k, q->scalar_type(), nk, sk) || !heads(ko, q->scalar_type(), no, sko) || !same(nk, no) ||
-                    nk[0] != nq[0] || nk[2] != nq[2] || nk[3] != nq[3]))
-            return other();
-        if (!vec(f, at::kDouble, 1) || 2 * f->numel() > nq[3] || !integer(a[6], &s.pos0) ||
+        if ((two && !r.k) || (!two && a[3] != Py_None) || (given && !r.pos) || !r.shape(&s) || !integer(a[6], &s.pos0) ||
             !flag(a[7], &s.interleaved) || !number(a[8], &factor) || !flag(a[9], &s.inverse))
             return other();
-        if (given) {
-            if (!here(pos) || pos->scalar_type() != at::kInt || pos->dim() < 1 || pos->dim() > 2 ||
-                pos->size(-1) != nq[2] || (nq[2] > 1 && pos->stride(-1) != 1) ||
-                (pos->dim() == 2 && pos->size(0) != nq[0]))
-                return other();
-            s.pos_bs = pos->dim() == 2 ? pos->stride(0) : 0;
-        }
-        s.B = (int)nq[0];
-        s.Hq = (int)nq[1];
-        s.Hkv = two ? (int)nk[1] : 0;
-        s.N = (int)nq[2];
-        s.head_dim = (int)nq[3];
-        s.rotary_dim = 2 * (int)f->numel();
-        s.dtype = q->scalar_type() == at::kBFloat16 ? MXFA_BF16 : MXFA_F32;
         s.factor = (float)factor;
-        s.q_bs = sq[0], s.q_hs = sq[1], s.q_ts = sq[2];
-        s.k_bs = sk[0], s.k_hs = sk[1], s.k_ts = sk[2];
-        s.qo_bs = so[0], s.qo_hs = so[1], s.qo_ts = so[2];
-        s.ko_bs = sko[0], s.ko_hs = sko[1], s.ko_ts = sko[2];
-        const void *qp = q->data_ptr(), *kp = two ? k->data_ptr() : nullptr;
-        void *qop = qo->data_ptr(), *kop = two ? ko->data_ptr() : nullptr, *stream = current_stream();
-        const int *pp = given ? ints(pos) : nullptr;
-        const double *fp = static_cast<const double *>(f->data_ptr());
         int rc;
         Py_BEGIN_ALLOW_THREADS;
-        rc = abi.rotary(&s, qp, kp, qop, kop, pp, fp, stream);
+        rc = r.run(s);
         Py_END_ALLOW_THREADS;
         return status(rc);
+    });
+}
+
+// Rows as the kernels take them: contiguous, starting on 16 bytes.
+at::Tensor rows16(const at::Tensor &x) {
+    const int64_t es = (int64_t)x.element_size();
+    bool good = (x.size(-1) < 2 || x.stride(-1) == 1) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) good = good && (x.size(i) < 2 || x.stride(i) * es % 16 == 0);
+    return good ? x : x.contiguous();
+}
+
+// The differentiable rotation (autograd.rotary_embedding): its gradient is the
+// transposed rotation of the outputs' gradients, itself such a node where a
+// graph of it is asked for.
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q0,
+                                                  const at::Tensor &k0, const at::Tensor &f,
+                                                  const std::optional<at::Tensor> &pos,
+                                                  int64_t pos0, bool interleaved, double factor, bool inverse) {
+        ctx->save_for_backward({f, pos ? *pos : at::Tensor()});
+        ctx->saved_data["pos0"] = pos0;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["factor"] = factor;
+        ctx->saved_data["inverse"] = inverse;
+        const at::Tensor q = rows16(q0), k = rows16(k0);
+        at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+        const RotaryArgs r{&q, &k, &qo, &ko, &f, pos ? &*pos : nullptr};
+        mxfa_rotary_shape s{};
+        TORCH_CHECK_VALUE(r.shape(&s), "rotary_embedding: tensors that do not fit together or are on another device");
+        s.pos0 = (int)pos0;
+        s.interleaved = interleaved;
+        s.factor = (float)factor;
+        s.inverse = inverse;
+        const int rc = r.run(s);
+        TORCH_CHECK(rc == 0, "rotary_embedding: mxfa_run_rotary returned ", rc);
+        return {qo, ko};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                   torch::autograd::variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        std::optional<at::Tensor> pos;
+        if (saved[1].defined()) pos = saved[1];
+        auto out = apply(g[0], g[1], saved[0], pos, ctx->saved_data["pos0"].toInt(),
+                         ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(),
+                         !ctx->saved_data["inverse"].toBool());
+        const at::Tensor none;
+        return {out[0], out[1], none, none, none, none, none, none};
+    }
+};
+
+// rotary_embedding(q, k, frequencies, positions or None, pos0, interleaved, factor) -> (q, k) turned
+PyObject *rotary_embedding(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 7 || abi.rotary == nullptr) return other();
+    return guarded([&]() -> PyObject * {
+        const bool given = a[3] != Py_None;
+        const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *f = plain(a[2]), *pos = given ? plain(a[3]) : nullptr;
+        int pos0, interleaved;
+        double factor;
+        // (strides are put right in forward)
+        if (!q || !k || !f || (given && !pos) || f->requires_grad() || !is_mxfa_type(*q) || q->dim() != 4 ||
+            k->dim() != 4 || q->numel() == 0 || k->numel() == 0 || !integer(a[4], &pos0) || !flag(a[5], &interleaved) ||
+            !number(a[6], &factor))
+            return other();
+        const at::Tensor &qq = *q, &kk = *k;
+        if (!here(q) || !here(k) || kk.scalar_type() != qq.scalar_type() || qq.size(0) != kk.size(0) ||
+            qq.size(2) != kk.size(2) || qq.size(3) != kk.size(3) || !vec(f, at::kDouble, 1) ||
+            2 * f->numel() > qq.size(3) || qq.size(3) % 8 != 0 || qq.size(3) > 256 ||
+            pos0 + qq.size(2) > INT32_MAX)
+            return other();
+        std::optional<at::Tensor> at_pos;
+        if (given) at_pos = *pos;
+        auto out = RotaryNode::apply(qq, kk, *f, at_pos, (int64_t)pos0, interleaved != 0, factor, false);
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])));
     });
 }
 
@@ -536,7 +620,8 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define MXFA_METHOD(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MXFA_METHOD(bind), MXFA_METHOD(attention_fwd), MXFA_METHOD(attention_bwd),
-                         MXFA_METHOD(prefill), MXFA_METHOD(rotary), MXFA_METHOD(cache_append),
+                         MXFA_METHOD(prefill), MXFA_METHOD(rotary), MXFA_METHOD(rotary_embedding),
+                         MXFA_METHOD(cache_append),
                          MXFA_METHOD(prefill_batch), MXFA_METHOD(pages_free), MXFA_METHOD(pages_fork),
                          MXFA_METHOD(pages_compact), MXFA_METHOD(pages_copy), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

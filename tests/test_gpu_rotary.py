@@ -159,6 +159,40 @@ def test_gradient(interleaved):
     assert dk is None or not dk.any()
 
 
+def test_second_gradient_and_the_python_node(monkeypatch):
+    """The rotation is linear, so the gradient of its gradient is the rotation again;
+    the Python node gives the C++ one's bits, gradients included."""
+    from mx230_amd import autograd
+    g = torch.Generator().manual_seed(16)
+    f, _ = mx.rotary_frequencies(64)
+    q, k = (torch.randn(1, h, 9, 64, generator=g).cuda().requires_grad_(True) for h in (3, 1))
+    dy = [torch.randn(x.shape, generator=g).cuda().requires_grad_(True) for x in (q, k)]
+    t = [torch.randn(x.shape, generator=g).cuda() for x in (q, k)]
+
+    def go():
+        y = autograd.rotary_embedding(q, k, f, pos0=7, factor=1.5)
+        dx = torch.autograd.grad(y, (q, k), dy, create_graph=True)
+        return (*y, *dx, *torch.autograd.grad(dx, dy, t))
+    native = go()
+    _check(native[4].detach(), t[0], torch.arange(7, 16), f, factor=1.5)
+    monkeypatch.setattr(autograd, "_calls", lambda: mx._NoBinding)
+    for a, b in zip(native, go()):
+        assert torch.equal(a, b)
+    # what the C++ node leaves: the error is the package's
+    monkeypatch.undo()
+    z = torch.zeros(1, 1, 2, 68, device="cuda")
+    with pytest.raises(mx.MxfaError):
+        autograd.rotary_embedding(z, z, f)
+    with pytest.raises(ValueError):
+        autograd.rotary_embedding(q, k, f, positions=torch.zeros(4, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError):
+        autograd.rotary_embedding(q, k[:, :, :5], f)
+    # rows that are not on 16 bytes are copied
+    odd = torch.randn(1, 3, 9, 65, generator=g).cuda()[..., 1:]
+    y = autograd.rotary_embedding(odd, k, f)[0]
+    _check(y, odd, torch.arange(9), f)
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 def test_attention_block(bf16):
     """CausalSelfAttention with rotary positions against the same block made of
