@@ -1037,7 +1037,8 @@ def prefill_batch_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head: in
                                   bf16: bool = True) -> int:
     """mxfa_prefill_batch_workspace_bytes: what run_prefill_batch needs for such a
     batch, whatever its lengths (0 for one it does not take)."""
-    w, entries = n_head * head_dim, 1 << 28
+    # (a table of any width: at 2^20 positions every form has all its work-groups)
+    w, entries = n_head * head_dim, 1 << 20
     sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w,
                         n_kv_head * head_dim, w, MXFA_BF16 if bf16 else MXFA_F32, 0.0)
     return int(load_library().mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh)))

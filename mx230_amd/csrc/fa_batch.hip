@@ -19,26 +19,13 @@
 // items, gives each less than the unit has; its shares' unnormalised outputs
 // are then joined by a second launch, in a fixed order.
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
-#include "fa_cache.h"
+#include "fa_batch_items.h"
 #include "fa_device.h"
 #include "fa_launch.h"
 
 namespace mxfa {
-
-constexpr int kBatchFew = 16;  // rows of the few-row form's units
-constexpr int kJoinRows = 32;  // rows of a work-group of the join
-// Rows of the many-row form's units: 16 per wave and query tile.
-__host__ __device__ constexpr int batch_tiles(bool bf16) { return bf16 ? 2 : 1; }
-__host__ __device__ constexpr int batch_many_rows(bool bf16) { return 64 * batch_tiles(bf16); }
-
-// The workspace holds the shares of split units: `slots` of them, each ROWS rows
-// of D floats and their (max, sum) pairs.
-__host__ __device__ constexpr size_t batch_part_floats(long long slots, int rows, int d) {
-    return (size_t)slots * rows * (d + 2);
-}
 
 // The device code builds on the forward's stages (fa_fwd.hip, the same
 // translation unit in the code object).
@@ -164,55 +151,29 @@ struct BatchRows {
 };
 
 // The loads of one 64-key tile by NT threads: load k fills 16-byte positions k NT
-// + tid, whole rows of the cache; row_of(r) is the cache row of the tile's row r.
+// + tid, whole rows of the cache; off holds the loads' byte offsets in the cache
+// (row_of(r): the cache row of the tile's row r).
 template <class Pol, int NT>
 struct BatchStage {
     static constexpr int CPR = Pol::D / Pol::EPC, LOADS = 64 * CPR / NT;
+    unsigned long long off[LOADS];
     template <class RowOf>
-    __device__ static __forceinline__ void load(typename Pol::T *tile, const typename Pol::T *X, int tid, int wave,
-                                                unsigned stride_bytes, RowOf row_of) {
-        const uint32_t base = lds_addr(tile) + wave * 64 * 16;
+    __device__ __forceinline__ void rows(int tid, unsigned stride_bytes, RowOf row_of) {
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) {
             int row, c;
             Pol::chunk_at(k * NT + tid, row, c);
-            lds_dma16(base + k * NT * 16, reinterpret_cast<const char *>(X) +
-                                              (unsigned long long)row_of(row) * stride_bytes + 16 * c);
+            off[k] = (unsigned long long)row_of(row) * stride_bytes + 16 * c;
         }
+    }
+    __device__ __forceinline__ void load(typename Pol::T *tile, const typename Pol::T *X, int wave) const {
+        const uint32_t base = lds_addr(tile) + wave * 64 * 16;
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) lds_dma16(base + k * NT * 16, reinterpret_cast<const char *>(X) + off[k]);
     }
 };
 
 // -------------------------------------------------------------------- the items
-
-// What a sequence brings to a form.
-struct BatchSeq {
-    int q0;      // its first row of q
-    int pos;     // position of that row's token
-    int rows;    // new tokens x query heads per KV head (0: none for this form)
-    int keys;    // positions that its last token sees
-    int units, stages;
-};
-
-template <bool FEW, int ROWS>
-__device__ __forceinline__ BatchSeq batch_seq(const BatchParams &p, int s) {
-    BatchSeq b{0, 0, 0, 0, 0, 0};
-    if (s >= p.n_seq) return b;
-    const int c0 = p.cu_q[s], c1 = p.cu_q[s + 1], len = p.lens[s];
-    b.q0 = min(max(c0, 0), p.n_tok);
-    const int count = min(min(c1, p.n_tok) - b.q0, p.max_q);
-    // positions stay within int with a stage to spare, whatever the arrays hold
-    const long long cap = min((long long)p.max_blocks << p.bs_shift, (long long)INT_MAX - 256);
-    const long long pos = (long long)len - ((long long)c1 - b.q0);
-    b.pos = (int)min(max(pos, -(1LL << 30)), cap);
-    const long long rows = (long long)max(count, 0) * p.group;
-    const bool mine = FEW ? rows <= p.few_rows : rows > p.few_rows;
-    b.rows = mine ? (int)rows : 0;
-    b.keys = (int)min(min((long long)b.pos + max(count, 0), (long long)len), cap);
-    b.keys = max(b.keys, 0);
-    b.units = (b.rows + ROWS - 1) / ROWS;
-    b.stages = (b.keys + 63) / 64;
-    return b;
-}
 
 // Inclusive prefix over the wave, all 64 lanes active (rows of 16 by shifts, then
 // the rows' ends broadcast into the next row, and into the upper half).
@@ -237,98 +198,43 @@ __device__ __forceinline__ X wave_sum(X x) {
     return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_prefix(x)), 63));
 }
 
-struct BatchItem {
-    BatchSeq s;
-    int seq, head, unit, share, shares;
-    int slot;  // of share 0 (the join) or of this share, where shares > 1
-};
-
-__device__ __forceinline__ int batch_shares(int stages, unsigned quota) {
-    return (unsigned)stages > quota ? (int)(((unsigned)stages + quota - 1) / quota) : 1;
+__device__ __forceinline__ BatchSeq seq_of_lane(const BatchSeq &b, int l) {
+    auto of = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, l); };
+    return BatchSeq{of(b.q0), of(b.pos), of(b.rows), of(b.keys), of(b.units), of(b.stages)};
 }
 
-// Item `w` of a form (JOIN: split unit `w`), found by every wave for itself: a
-// lane per sequence, again over them where there are more than 64. False past
-// the last one. Items of a sequence: units (the last, heaviest one first) x
-// shares x KV heads, so that neighbouring work-groups, which the dispatcher
-// spreads over the XCDs, have the heads and an XCD's share of them the same
-// head's keys.
-//
-// The quota, the most stages of a share: where the units fit the work-groups
-// that are resident at once (p.resident), the least one by which their shares
-// still do, found by raising an even share's; else, or where that leaves the
-// longest share half as long again as an even one, shares of 1 / rounds of it,
-// which later rounds even out. It depends on lengths alone, so the join
-// finds the same one.
-template <bool FEW, int ROWS, bool JOIN>
+// Item `w` of the many-row form (JOIN: split unit `w`), found by every wave for
+// itself: a lane per sequence, again over them where there are more than 64
+// (the rules: fa_batch_items.h). False past the last one.
+template <int ROWS, bool JOIN>
 __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem &it) {
-    constexpr int F = FEW ? 0 : 1;
     const int lane = threadIdx.x & 63;
-    BatchSeq b = batch_seq<FEW, ROWS>(p, lane);
-    // sums of all sequences; the stages' in fp32, rounded up by more than its rounding
-    float all = (float)b.units * (float)max(b.stages, 1);
-    float units = (float)b.units;
+    BatchSeq b = batch_seq<false, ROWS>(p, lane);
+    float all = seq_stages<ROWS>(p, b), units = (float)b.units;
     for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
-        const BatchSeq c = batch_seq<FEW, ROWS>(p, s0 + lane);
-        all += (float)c.units * (float)max(c.stages, 1);
+        const BatchSeq c = batch_seq<false, ROWS>(p, s0 + lane);
+        all += seq_stages<ROWS>(p, c);
         units += (float)c.units;
     }
-    all = fminf(wave_sum(all) * (float)p.Hkv * 1.001f, 1e18f);
-    units = wave_sum(units) * (float)p.Hkv;
-    const float resident = (float)p.resident[F], even = fminf(all * p.per_resident[F] + 1.0f, 1e9f);
-    unsigned quota = (unsigned)fmaxf(fminf(all * p.per_target[F] + 1.0f, 1e9f), (float)p.least[F]);
-    if (units <= resident) {
-        unsigned q = max((unsigned)even, (unsigned)p.least[F]);
-        const float most = fmaxf(1.5f * even + 1.0f, (float)p.least[F]);
-        for (int i = 0; i < 5 && (float)q <= most; ++i) {
-            int n = b.units * batch_shares(b.stages, q);
-            for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
-                const BatchSeq c = batch_seq<FEW, ROWS>(p, s0 + lane);
-                n += c.units * batch_shares(c.stages, q);
-            }
-            const float items = (float)wave_sum(n) * (float)p.Hkv;
-            if (items <= resident) {
-                quota = q;
-                break;
-            }
-            q = max(q + 1, (unsigned)((float)q * items * p.per_resident[F]));
-        }
-    }
+    const unsigned quota = batch_quota(p, wave_sum(all), wave_sum(units), [&](unsigned q) __attribute__((always_inline)) {
+        int n = seq_items<ROWS>(p, b, q).items;
+        for (int s0 = 64; s0 < p.n_seq; s0 += 64) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s0 + lane), q).items;
+        return (float)wave_sum(n);
+    });
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-        if (s0 > 0) b = batch_seq<FEW, ROWS>(p, s0 + lane);
-        const int shares = batch_shares(b.stages, quota);
-        const int unit_items = b.units * p.Hkv;
-        const int mine = shares > 1 ? unit_items * shares : 0;
-        const int per = JOIN ? (shares > 1 ? unit_items : 0) : unit_items * shares;
-        const int upto = wave_prefix(per), slots_upto = wave_prefix(mine);
+        if (s0 > 0) b = batch_seq<false, ROWS>(p, s0 + lane);
+        const SeqItems n = seq_items<ROWS>(p, b, quota);
+        const int per = JOIN ? n.split : n.items;
+        const int upto = wave_prefix(per), slots_upto = wave_prefix(n.slots);
         const unsigned long long at = __builtin_amdgcn_ballot_w64(before + upto > w);
         if (at != 0) {
             const int l = __builtin_ctzll(at);
+            auto of = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, l); };
             it.seq = s0 + l;
-            it.s.q0 = __builtin_amdgcn_readlane(b.q0, l);
-            it.s.pos = __builtin_amdgcn_readlane(b.pos, l);
-            it.s.rows = __builtin_amdgcn_readlane(b.rows, l);
-            it.s.keys = __builtin_amdgcn_readlane(b.keys, l);
-            it.s.units = __builtin_amdgcn_readlane(b.units, l);
-            it.s.stages = __builtin_amdgcn_readlane(b.stages, l);
-            it.shares = __builtin_amdgcn_readlane(shares, l);
-            unsigned i = w - before - __builtin_amdgcn_readlane(upto - per, l);
-            it.slot = slots + __builtin_amdgcn_readlane(slots_upto - mine, l);
-            const unsigned heads = p.Hkv, per_unit = i / heads;
-            it.head = i - per_unit * heads;
-            if (JOIN) {
-                it.slot += per_unit * it.shares * heads + it.head;  // the unit's shares are `heads` apart
-                it.share = 0;
-                it.unit = it.s.units - 1 - (int)per_unit;
-                return it.slot + (it.shares - 1) * p.Hkv < p.slots[F];
-            }
-            it.slot += i;
-            const unsigned u = per_unit / (unsigned)it.shares;
-            it.share = per_unit - u * it.shares;
-            it.unit = it.s.units - 1 - (int)u;
-            // (false only where cu_q says the same rows twice over)
-            return it.shares == 1 || it.slot < p.slots[F];
+            it.s = seq_of_lane(b, l);
+            const SeqItems m{of(n.whole), of(n.shares), of(n.split), of(n.slots), of(n.items)};
+            return batch_item<JOIN>(p, m, slots + of(slots_upto - n.slots), w - before - of(upto - per), it);
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         slots += __builtin_amdgcn_readlane(slots_upto, 63);
@@ -336,15 +242,29 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
     return false;
 }
 
-// The share's stages of the unit's n.
-__device__ __forceinline__ void share_stages(const BatchItem &it, int n, int &lo, int &hi) {
-    // n < 2^25 stages and at most 2^11 shares: the products pass 32 bits
-    if (it.shares == 1) {
-        lo = 0;
-        hi = n;
-    } else {
-        lo = (int)((unsigned long long)(unsigned)it.share * (unsigned)n / (unsigned)it.shares);
-        hi = (int)((unsigned long long)(unsigned)(it.share + 1) * (unsigned)n / (unsigned)it.shares);
+// The length of the few-row form's line.
+__device__ __forceinline__ unsigned few_line(const BatchParams &p) {
+    unsigned all = 0;
+    for (int s0 = 0; s0 < p.n_seq; s0 += 64) all += few_weight(batch_seq<true, kBatchFew>(p, s0 + (threadIdx.x & 63)));
+    return wave_sum(all);
+}
+
+// f(sequence's number, BatchSeq, its begin and end on the line) for the sequences
+// from position x of the line on, until f returns true.
+template <class F>
+__device__ __forceinline__ void few_walk(const BatchParams &p, unsigned x, F f) {
+    const int lane = threadIdx.x & 63;
+    unsigned before = 0;
+    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
+        const BatchSeq b = batch_seq<true, kBatchFew>(p, s0 + lane);
+        const unsigned w = few_weight(b), upto = before + wave_prefix(w);
+        unsigned long long left = __builtin_amdgcn_ballot_w64(w > 0 && upto > x);
+        for (; left != 0; left &= left - 1) {
+            const int l = __builtin_ctzll(left);
+            const unsigned u1 = __builtin_amdgcn_readlane(upto, l);
+            if (f(s0 + l, seq_of_lane(b, l), u1 - __builtin_amdgcn_readlane(w, l), u1)) return;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
 }
 
@@ -383,7 +303,7 @@ __device__ __forceinline__ f32x4 batch_quad(const f32x4 (&acc)[XT][QT], int i, i
 // altogether: taken where a value was not finite, since in the matrix products
 // an infinity or NaN in the V of a key that a row does not see reaches it as 0
 // x inf. 4 threads per row, rows from row0 of the unit. A row's running (max, sum) and output go where
-// the form's would: to the workspace slot, or finished.
+// the form's would: to the workspace slot, or (part null) finished.
 template <class T, int D, int ROWS>
 __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchItem &it, int row0, int key0, int key1,
                                             float *part, float *ml) {
@@ -424,25 +344,25 @@ __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchIte
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
         const f32x4 o{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-        if (it.shares > 1) {
+        if (part != nullptr) {
             store4<float>(part + (size_t)rl * D + c + e, o, 1.0f);
         } else {
             batch_store<T>(p, it, r, D, c + e, o, m, l);
         }
     }
-    if (it.shares > 1 && c == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m, l);
+    if (part != nullptr && c == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m, l);
 }
 
-// The workspace of an item's share: ROWS rows of D floats, and their (max, sum).
-template <bool FEW, int ROWS>
-__device__ __forceinline__ float *batch_part(const BatchParams &p, int slot, int d) {
-    return p.part[FEW ? 0 : 1] + (size_t)slot * ROWS * d;
+// A slot of a form's workspace: ROWS rows of D floats, and their (max, sum).
+template <int ROWS>
+__device__ __forceinline__ float *batch_part(float *part, int slot, int d) {
+    return part + (size_t)slot * ROWS * d;
 }
-template <bool FEW, int ROWS>
-__device__ __forceinline__ float *batch_ml(const BatchParams &p, int slot, int d) {
-    const int f = FEW ? 0 : 1;
-    return p.part[f] + (size_t)p.slots[f] * ROWS * d + (size_t)slot * ROWS * 2;
+template <int ROWS>
+__device__ __forceinline__ float *batch_ml(float *part, int slots, int slot, int d) {
+    return part + (size_t)slots * ROWS * d + (size_t)slot * ROWS * 2;
 }
+__device__ __forceinline__ int few_slots(const BatchParams &p) { return 2 * p.few_groups * p.Hkv; }
 
 // ------------------------------------------------------------------ the few rows
 
@@ -459,29 +379,25 @@ union BatchFewSmem {
     } merge;
 };
 
-// Each of the NW waves takes every NW-th stage of the share, staged into its
-// own tiles with no barrier; the waves' maxima, sums and O meet in LDS. The
-// stage's blocks come through LDS too, two stages ahead: as loads into
-// registers the compiler would wait for them with vmcnt(0), and with them for
-// every staging load in flight.
+// One piece of a sequence: each of the NW waves takes every NW-th of its stages
+// [s_lo, s_hi), staged into its own tiles with no barrier; the waves' maxima,
+// sums and O meet in LDS. The stage's blocks come through LDS too, two stages
+// ahead: as loads into registers the compiler would wait for them with
+// vmcnt(0), and with them for every staging load in flight.
 template <class Pol, int NW>
-__device__ __forceinline__ void batch_few_body(const BatchParams &p) {
+__device__ __forceinline__ void batch_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
+                                                BatchFewSmem<Pol, NW> &sm) {
     using T = typename Pol::T;
     using Stage = BatchStage<Pol, 64>;
     constexpr int D = Pol::D, XT = D / 16, ROWS = kBatchFew, NL = Stage::LOADS;
-    __shared__ __attribute__((aligned(16))) BatchFewSmem<Pol, NW> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
-    BatchItem it;
-    if (!find_item<true, ROWS, false>(p, blockIdx.x, it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
     const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, it.s.keys, (unsigned)(p.n_blocks - 1)};
     const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
     T *sk = sm.t.k[wave], *sv = sm.t.v[wave];
     const int Nk = it.s.keys;
-    int s_lo, s_hi;
-    share_stages(it, it.s.stages, s_lo, s_hi);
 
     // stage `st` is the wave's n-th: its blocks in buffer n & 1
     auto fetch = [&](int st, int n) __attribute__((always_inline)) {
@@ -489,8 +405,9 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
     };
     auto load = [&](T *tile, const T *X, int st, int n) __attribute__((always_inline)) {
         const int *blk = sm.t.blk[wave][n & 1];
-        Stage::load(tile, X, lane, 0, stride,
-                    [&](int r) __attribute__((always_inline)) { return rows.row(blk[r], st * 64 + r); });
+        Stage stage;
+        stage.rows(lane, stride, [&](int r) __attribute__((always_inline)) { return rows.row(blk[r], st * 64 + r); });
+        stage.load(tile, X, 0);
     };
     int st = s_lo + wave, n = 0;
     if (st < s_hi) fetch(st, 0);
@@ -550,9 +467,9 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
     if (g == 0) *reinterpret_cast<float2 *>(sm.merge.ml[wave][l16]) = make_float2(m[0], lw);
     __syncthreads();
     float *part = nullptr, *ml = nullptr;
-    if (it.shares > 1) {
-        part = batch_part<true, ROWS>(p, it.slot, D);
-        ml = batch_ml<true, ROWS>(p, it.slot, D);
+    if (slot >= 0) {
+        part = batch_part<ROWS>(p.part[0], slot, D);
+        ml = batch_ml<ROWS>(p.part[0], few_slots(p), slot, D);
     }
     if (sm.merge.bad) {
         if (tid < 4 * ROWS) batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
@@ -571,13 +488,36 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
             L += x * sm.merge.ml[w][r][1];
             o += *reinterpret_cast<const f32x4 *>(&sm.merge.acc[w][r][c]) * x;
         }
-        if (it.shares > 1) {
+        if (part != nullptr) {
             store4<float>(part + r * D + c, o, 1.0f);
             if (c == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(M, L);
         } else {
             batch_store<T>(p, it, r, D, c, o, M, L);
         }
     }
+}
+
+// Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line.
+template <class Pol, int NW>
+__device__ __forceinline__ void batch_few_body(const BatchParams &p) {
+    __shared__ __attribute__((aligned(16))) BatchFewSmem<Pol, NW> sm;
+    const int g = blockIdx.x;
+    const unsigned all = few_line(p), run = few_run(p, all);
+    unsigned x = (unsigned)(g / p.Hkv) * run;
+    const unsigned x1 = min(x + run, all);
+    if (x >= x1) return;
+    BatchItem it;
+    it.head = g % p.Hkv;
+    it.unit = 0;
+    few_walk(p, x, [&](int seq, const BatchSeq &s, unsigned u0, unsigned u1) __attribute__((always_inline)) {
+        it.seq = seq;
+        it.s = s;
+        const FewPiece f = few_piece(x, x1, u0, u1, g);
+        batch_few_piece<Pol, NW>(p, it, f.lo, f.hi, f.slot, sm);
+        x = f.end;
+        if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
+        return x >= x1;
+    });
 }
 
 // ----------------------------------------------------------------- the many rows
@@ -596,7 +536,9 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    if (!find_item<false, ROWS, false>(p, blockIdx.x, it)) return;
+    // neighbours in eights (the XCDs) stay together
+    const int w = cu_order_wg((int)blockIdx.x >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + ((int)blockIdx.x & 7);
+    if (!find_item<ROWS, false>(p, w, it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
 
     const int r0 = it.unit * ROWS, rw = r0 + wave * 16 * QT;  // the unit's and the wave's first row
@@ -635,9 +577,10 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
     auto fetch = [&](int st) __attribute__((always_inline)) { blk = rows.table[rows.block_at(st * BK + lane)]; };
     auto stage_next = [&](T *sk, T *sv, int st) __attribute__((always_inline)) {
         const unsigned mine = rows.row(blk, st * BK + lane);
-        auto row_of = [&](int r) __attribute__((always_inline)) { return (unsigned)__shfl((int)mine, r, 64); };
-        Stage::load(sk, K, tid, wave, stride, row_of);
-        Stage::load(sv, V, tid, wave, stride, row_of);
+        Stage stage;
+        stage.rows(tid, stride, [&](int r) __attribute__((always_inline)) { return (unsigned)__shfl((int)mine, r, 64); });
+        stage.load(sk, K, wave);
+        stage.load(sv, V, wave);
         if (st + 1 < s_hi) fetch(st + 1);
     };
     if (s_lo < s_hi) {
@@ -693,8 +636,8 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
     }
     float *part = nullptr, *ml = nullptr;
     if (it.shares > 1) {
-        part = batch_part<false, ROWS>(p, it.slot, D);
-        ml = batch_ml<false, ROWS>(p, it.slot, D);
+        part = batch_part<ROWS>(p.part[1], it.slot, D);
+        ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
     }
     const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
     if (lane == 0) flags[wave] = bad;
@@ -733,46 +676,42 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
 
 // ---------------------------------------------------------------------- the join
 
-// The shares of a split unit: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
-// kJoinRows rows per work-group (part). D / 4 threads have a row, four elements
-// each; where there are few rows several such groups take turns over a row's
-// shares and meet in LDS.
-template <class T, int D, bool FEW, int ROWS>
-__device__ __forceinline__ void batch_join_body(const BatchParams &p, int w, int piece) {
+// The parts of a unit's rows [first, end): o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s
+// - M) l_s, part s being slot at(s) of the workspace. D / 4 threads have a row,
+// four elements each; where there are few rows several such groups take turns
+// over a row's parts and meet in LDS.
+template <class T, int D, int ROWS, class At>
+__device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int first, int end, int S,
+                                                float *parts, int slots, At at) {
     constexpr int C = D / 4, NG = 256 / C;
     __shared__ __attribute__((aligned(16))) f32x4 so[NG][C];
-    BatchItem it;
-    if (!find_item<FEW, ROWS, true>(p, w, it)) return;
-    const int tid = threadIdx.x, c = tid % C, grp = tid / C;
-    const int first = piece * kJoinRows, end = min(min(first + kJoinRows, ROWS), it.s.rows - it.unit * ROWS);
-    const int nrows = end - first, S = it.shares;
-    if (nrows <= 0) return;
+    const int tid = threadIdx.x, c = tid % C, grp = tid / C, nrows = end - first;
     int together = 1;  // groups to a row
     while (together * 2 * nrows <= NG) together *= 2;
     const int turn = grp % together;
-    const float *part = batch_part<FEW, ROWS>(p, it.slot, D);
-    const float *ml = batch_ml<FEW, ROWS>(p, it.slot, D);
-    const size_t pstep = (size_t)p.Hkv * ROWS * D, mstep = (size_t)p.Hkv * ROWS * 2;
+    auto ml = [&](int s, int r) __attribute__((always_inline)) {
+        return *reinterpret_cast<const float2 *>(batch_ml<ROWS>(parts, slots, at(s), D) + 2 * r);
+    };
     for (int r0 = 0; r0 < nrows; r0 += NG / together) {
         const bool have = r0 + grp / together < nrows;
         const int r = first + r0 + grp / together;
         float M = -INFINITY, L = 0.f;
         f32x4 o = zero4();
         if (have) {
-            for (int s = c; s < S; s += C) M = fmaxf(M, ml[s * mstep + 2 * r]);
+            for (int s = c; s < S; s += C) M = fmaxf(M, ml(s, r).x);
         }
 #pragma unroll
         for (int k = C / 2; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
         const float mref = M == -INFINITY ? 0.f : M;
         if (have) {
             for (int s = c; s < S; s += C) {
-                const float2 v = *reinterpret_cast<const float2 *>(ml + s * mstep + 2 * r);
+                const float2 v = ml(s, r);
                 L += fast_exp2(v.x - mref) * v.y;
             }
 #pragma unroll 4
             for (int s = turn; s < S; s += together)
-                o += *reinterpret_cast<const f32x4 *>(part + s * pstep + r * D + 4 * c) *
-                     fast_exp2(ml[s * mstep + 2 * r] - mref);
+                o += *reinterpret_cast<const f32x4 *>(batch_part<ROWS>(parts, at(s), D) + r * D + 4 * c) *
+                     fast_exp2(ml(s, r).x - mref);
         }
 #pragma unroll
         for (int k = C / 2; k > 0; k >>= 1) L += __shfl_xor(L, k, 64);
@@ -788,17 +727,37 @@ __device__ __forceinline__ void batch_join_body(const BatchParams &p, int w, int
     }
 }
 
-// Grid: the split units the few-row form may have, then the pieces of the
-// many-row form's.
+// Grid: the cuts of the few-row form's lines, then the pieces of the split units
+// that the many-row form may have, kJoinRows rows each.
 template <class T, int D>
-__device__ __forceinline__ void batch_join(const BatchParams &p, int few_groups) {
+__device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
     constexpr int ROWS = batch_many_rows(sizeof(T) == 2), PIECES = ROWS / kJoinRows;
-    const int w = (int)blockIdx.x - few_groups;
-    if (w < 0) {
-        batch_join_body<T, D, true, kBatchFew>(p, (int)blockIdx.x, 0);
-    } else {
-        batch_join_body<T, D, false, ROWS>(p, w / PIECES, w % PIECES);
+    BatchItem it;
+    if ((int)blockIdx.x < few_cuts) {
+        // the cut at the end of run `cut`; the first cut through a sequence joins it
+        const int cut = (int)blockIdx.x / p.Hkv, heads = p.Hkv;
+        it.head = (int)blockIdx.x % p.Hkv;
+        it.unit = 0;
+        const unsigned all = few_line(p), run = few_run(p, all), x = (unsigned)(cut + 1) * run;
+        if (x >= all) return;
+        few_walk(p, x, [&](int seq, const BatchSeq &s, unsigned u0, unsigned u1) __attribute__((always_inline)) {
+            if (u0 >= x || u0 / run != (unsigned)cut) return true;
+            it.seq = seq;
+            it.s = s;
+            const int head = it.head, S = (int)((u1 - 1) / run) - cut + 1;
+            batch_join_rows<T, D, kBatchFew>(p, it, 0, s.rows, S, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
+                return i == 0 ? few_first_slot(cut, heads, head) : few_next_slot(cut, heads, head) + 2 * heads * (i - 1);
+            });
+            return true;
+        });
+        return;
     }
+    const int w = (int)blockIdx.x - few_cuts;
+    if (!find_item<ROWS, true>(p, w / PIECES, it)) return;
+    const int first = w % PIECES * kJoinRows, end = min(first + kJoinRows, it.s.rows - it.unit * ROWS);
+    if (first >= end) return;
+    batch_join_rows<T, D, ROWS>(p, it, first, end, it.shares, p.part[1], p.slots,
+                                [&](int i) __attribute__((always_inline)) { return it.slot + i * p.Hkv; });
 }
 
 #define MXFA_BATCH(SUFFIX, POL, NW, WPS)                                                              \
@@ -817,77 +776,27 @@ MXFA_BATCH(f64, PolF32, 4, 2)
 #undef MXFA_BATCH
 #endif
 
-// Work-groups resident at once: the few-row form's have a CU each, the many-row
-// form's share one in twos or threes.
-static int batch_resident(bool few, int dtype_bf16, int d) {
-    return few ? 256 : 256 * (dtype_bf16 && d == 64 ? 3 : 2);
-}
-// Rounds of them that longer work is cut into: the items' target.
-static int batch_rounds(bool few) { return few ? 4 : 2; }
-
-// Which forms a call launches, by what the host knows: the few-row form alone
-// where no sequence can have more rows; the many-row form alone where one
-// sequence has the rows; else both, each taking its own sequences.
-static int batch_few_rows(const BatchParams &p) {
-    const bool may_exceed = (long long)p.max_q * p.group > kBatchFew;
-    return may_exceed && p.n_seq == 1 ? 0 : kBatchFew;
-}
-static bool batch_may_be_many(const BatchParams &p) {
-    return (long long)std::min(p.max_q, p.n_tok) * p.group > kBatchFew || p.few_rows == 0;
-}
-
-// Units there can be: for the few-row form one per sequence and KV head; the
-// many-row form's are full but for a sequence's last.
-static long long batch_units(const BatchParams &p, bool few, int dtype_bf16) {
-    if (few) return (long long)std::min(p.n_seq, p.n_tok) * p.Hkv;
-    return ((long long)p.n_tok * p.group / batch_many_rows(dtype_bf16) + std::min(p.n_seq, p.n_tok)) * p.Hkv;
-}
-
-// A form's sizes. A unit of n stages has ceil(n / quota) shares where n > quota,
-// and the quota is at least all stages / target: so all items are at most the
-// units + target, the shares of split units at most target + the split units,
-// and those at most target and the units.
-struct BatchForm {
-    int target, rows;
-    long long units, split, slots;
-};
-static BatchForm batch_form(const BatchParams &p, bool few, int dtype_bf16) {
-    BatchForm f;
-    f.target = batch_resident(few, dtype_bf16, p.d) * batch_rounds(few);
-    f.rows = few ? kBatchFew : batch_many_rows(dtype_bf16);
-    f.units = batch_units(p, few, dtype_bf16);
-    f.split = std::min<long long>(f.units, f.target);
-    // a table that holds no more positions than the least share splits nothing
-    if (((((long long)p.max_blocks << p.bs_shift) + 63) / 64) <= p.least[few ? 0 : 1]) f.split = 0;
-    f.slots = f.split > 0 ? f.target + f.split : 0;
-    return f;
-}
-
-// The least stages of a share: one for each of the few-row form's waves; 8 of the
-// many-row form's, below which the join costs more than the split saves.
-static void batch_plan(BatchParams *p, int dtype_bf16) {
-    p->few_rows = batch_few_rows(*p);
-    p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
-    p->least[1] = 8;
+// The forms of a call; groups = 0: not launched.
+static void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2]) {
+    batch_plan(p, dtype_bf16);
+    f[0] = f[1] = BatchForm{0, 0, 0, 0};
+    if (p->few_rows > 0) f[0] = batch_few_form(p);
+    if (batch_may_be_many(*p)) f[1] = batch_many_form(p, dtype_bf16);
 }
 
 size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
     BatchParams p = q;
-    batch_plan(&p, dtype_bf16);
+    BatchForm f[2];
+    batch_forms(&p, dtype_bf16, f);
     size_t n = 0;
-    for (int i = 0; i < 2; ++i) {
-        if (i == 0 ? p.few_rows == 0 : !batch_may_be_many(p)) continue;
-        const BatchForm f = batch_form(p, i == 0, dtype_bf16);
-        n += batch_part_floats(f.slots, f.rows, p.d);
-    }
+    for (const BatchForm &x : f) n += batch_part_floats(x.slots, x.rows, p.d);
     return std::max<size_t>(n * sizeof(float), 16);
 }
 
 long long batch_groups(const BatchParams &q, int dtype_bf16) {
     BatchParams p = q;
     batch_plan(&p, dtype_bf16);
-    const BatchForm a = batch_form(p, true, dtype_bf16), b = batch_form(p, false, dtype_bf16);
-    return std::max(a.units + a.target, b.units + b.target);
+    return std::max(batch_few_form(&p).groups, batch_many_form(&p, dtype_bf16).groups);
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
@@ -896,30 +805,20 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
         {k_mxfa_batch_b128_few, k_mxfa_batch_b128_many, k_mxfa_batch_b128_join},
         {k_mxfa_batch_f64_few, k_mxfa_batch_f64_many, k_mxfa_batch_f64_join}};
     const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
-    batch_plan(&p, dtype_bf16);
-    float *next = static_cast<float *>(workspace);
-    unsigned groups[2] = {0, 0};
-    int joins[2] = {0, 0};
-    for (int i = 0; i < 2; ++i) {
-        if (i == 0 ? p.few_rows == 0 : !batch_may_be_many(p)) continue;
-        const BatchForm f = batch_form(p, i == 0, dtype_bf16);
-        p.resident[i] = batch_resident(i == 0, dtype_bf16, p.d);
-        p.per_resident[i] = 1.0f / (float)p.resident[i];
-        p.per_target[i] = 1.0f / (float)f.target;
-        p.slots[i] = (int)f.slots;
-        p.part[i] = next;
-        next += batch_part_floats(f.slots, f.rows, p.d);
-        groups[i] = (unsigned)(f.units + f.target);
-        joins[i] = (int)f.split * (i == 0 ? 1 : f.rows / kJoinRows);
-    }
+    BatchForm f[2];
+    batch_forms(&p, dtype_bf16, f);
+    p.part[0] = static_cast<float *>(workspace);
+    p.part[1] = p.part[0] + batch_part_floats(f[0].slots, f[0].rows, p.d);
     void *args[] = {&p};
     hipError_t e = hipSuccess;
-    if (groups[1] > 0) e = launch_kernel(id[1], dim3(groups[1]), dim3(256), args, stream);
-    if (e == hipSuccess && groups[0] > 0)
-        e = launch_kernel(id[0], dim3(groups[0]), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
-    if (e != hipSuccess || joins[0] + joins[1] == 0) return e;
-    void *jargs[] = {&p, &joins[0]};
-    return launch_kernel(id[2], dim3(joins[0] + joins[1]), dim3(256), jargs, stream);
+    if (f[1].groups > 0) e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(256), args, stream);
+    if (e == hipSuccess && f[0].groups > 0)
+        e = launch_kernel(id[0], dim3((unsigned)f[0].groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+    int cuts = (int)f[0].joins;
+    const unsigned joins = (unsigned)(cuts + f[1].joins * (f[1].rows / kJoinRows));
+    if (e != hipSuccess || joins == 0) return e;
+    void *jargs[] = {&p, &cuts};
+    return launch_kernel(id[2], dim3(joins), dim3(256), jargs, stream);
 }
 
 }  // namespace mxfa

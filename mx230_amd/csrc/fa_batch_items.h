@@ -1,0 +1,282 @@
+// The work of the attention over a batch (fa_batch.hip): which rows and keys each
+// work-group takes. Plain arithmetic on the batch's lengths, used by the kernels
+// and by the launcher, and compiled for the host by its tests.
+#pragma once
+
+#include <limits.h>
+
+#include <algorithm>
+
+#include "fa_cache.h"
+
+namespace mxfa {
+
+constexpr int kBatchFew = 16;  // rows of the few-row form's units
+constexpr int kCusPerXcd = 32;  // of 8 XCDs
+constexpr int kJoinRows = 32;  // rows of a work-group of the join
+// Rows of the many-row form's units: 16 per wave and query tile.
+__host__ __device__ constexpr int batch_tiles(bool bf16) { return bf16 ? 2 : 1; }
+__host__ __device__ constexpr int batch_many_rows(bool bf16) { return 64 * batch_tiles(bf16); }
+
+// The workspace holds the shares of split units: `slots` of them, each ROWS rows
+// of D floats and their (max, sum) pairs.
+__host__ __device__ constexpr size_t batch_part_floats(long long slots, int rows, int d) {
+    return (size_t)slots * rows * (d + 2);
+}
+
+template <class X>
+__host__ __device__ inline X less_of(X a, X b) {
+    return a < b ? a : b;
+}
+template <class X>
+__host__ __device__ inline X more_of(X a, X b) {
+    return a < b ? b : a;
+}
+
+// What a sequence brings to a form.
+struct BatchSeq {
+    int q0;      // its first row of q
+    int pos;     // position of that row's token
+    int rows;    // new tokens x query heads per KV head (0: none for this form)
+    int keys;    // positions that its last token sees
+    int units, stages;  // units, and stages of the last one, which has the most
+};
+
+template <bool FEW, int ROWS>  // (FEW: ROWS = kBatchFew, one unit)
+__host__ __device__ inline BatchSeq batch_seq(const BatchParams &p, int s) {
+    BatchSeq b{0, 0, 0, 0, 0, 0};
+    if (s >= p.n_seq) return b;
+    const int c0 = p.cu_q[s], c1 = p.cu_q[s + 1], len = p.lens[s];
+    b.q0 = less_of(more_of(c0, 0), p.n_tok);
+    const int count = less_of(less_of(more_of(c1, b.q0), p.n_tok) - b.q0, p.max_q);
+    const long long rows = (long long)count * p.group;
+    const bool mine = FEW ? rows <= p.few_rows : rows > p.few_rows;
+    if (!mine || count == 0) return b;
+    b.rows = (int)rows;
+    // positions stay within int with a stage to spare, whatever the arrays hold
+    const long long cap = less_of((long long)p.max_blocks << p.bs_shift, (long long)INT_MAX - 256);
+    const long long pos = (long long)len - ((long long)c1 - b.q0);
+    b.pos = (int)less_of(more_of(pos, -(1LL << 30)), cap);
+    b.keys = (int)more_of(less_of(less_of((long long)b.pos + count, (long long)len), cap), 0LL);
+    b.units = (int)((rows + ROWS - 1) / ROWS);
+    b.stages = (b.keys + 63) / 64;
+    return b;
+}
+
+// ---- the few-row form. The sequences' stages, and one more for each sequence,
+// lie on a line in their order (the extra one first: it stands for what a
+// piece costs besides its stages, and gives a sequence without keys a place). A
+// KV head's p.few_groups work-groups cut the line into equal runs, so all have
+// the same work; a sequence that a cut goes through is in pieces, which the
+// join puts together. A work-group has two slots of the workspace: one for a
+// piece that its run ends in, one for a piece that its run begins in or is in.
+__host__ __device__ inline unsigned few_weight(const BatchSeq &b) { return b.rows > 0 ? (unsigned)b.stages + 1u : 0u; }
+// The run of each work-group, of a line of `all`.
+__host__ __device__ inline unsigned few_run(const BatchParams &p, unsigned all) {
+    return more_of((all + (unsigned)p.few_groups - 1) / (unsigned)p.few_groups, (unsigned)p.least[0]);
+}
+struct FewPiece {
+    int lo, hi;   // stages
+    int slot;     // -1: all of the sequence's stages, finished in place
+    unsigned end; // where the next piece begins
+};
+// The piece of the sequence at [u0, u1) of the line that work-group g (of all KV
+// heads') has from x on, its run ending at x1.
+__host__ __device__ inline FewPiece few_piece(unsigned x, unsigned x1, unsigned u0, unsigned u1, int g) {
+    FewPiece f;
+    f.end = less_of(x1, u1);
+    f.lo = (int)(x > u0 ? x - u0 - 1 : 0);
+    f.hi = (int)(f.end - u0 - 1);
+    f.slot = x > u0 ? 2 * g : f.end < u1 ? 2 * g + 1 : -1;
+    return f;
+}
+// The slots of a sequence's pieces, by the run it begins in: the first piece's
+// and then one each 2 Hkv on from the second's.
+__host__ __device__ inline int few_first_slot(int run, int heads, int head) { return 2 * (run * heads + head) + 1; }
+__host__ __device__ inline int few_next_slot(int run, int heads, int head) { return 2 * ((run + 1) * heads + head); }
+
+// ---- the many-row form.
+
+// About the stages of all its units: those of the first and of the last one
+// each count for half of them.
+template <int ROWS>
+__host__ __device__ inline float seq_stages(const BatchParams &p, const BatchSeq &b) {
+    const int last = more_of(b.stages, 1);
+    const int tokens = (int)((unsigned)less_of(ROWS, b.rows) / (unsigned)p.group);
+    const int first = less_of(more_of((b.pos + tokens + 63) / 64, 1), last);
+    return (float)b.units * 0.5f * (float)(first + last);
+}
+
+// A sequence's items at a quota, the most stages of a share: its first `whole`
+// units are whole items, the others are cut into `shares` each. Counts over all
+// KV heads: `split` units that are cut, their `slots` shares, and all items.
+struct SeqItems {
+    int whole, shares, split, slots, items;
+};
+template <int ROWS>
+__host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchSeq &b, unsigned quota) {
+    SeqItems n{b.units, 1, 0, 0, 0};
+    if (b.units > 0 && (unsigned)b.stages > quota) {
+        n.shares = (int)(((unsigned)b.stages + quota - 1) / quota);
+        // unit u ends with row (u + 1) ROWS - 1, which sees more than 64 quota
+        // positions from row t group on, t = 64 quota - pos; the last one does
+        const long long t = 64LL * quota - b.pos;
+        n.whole = t <= 0 ? 0 : (int)less_of((unsigned long long)t * (unsigned)p.group / ROWS, (unsigned long long)(b.units - 1));
+    }
+    n.split = (b.units - n.whole) * p.Hkv;
+    n.slots = n.split * n.shares;
+    n.items = n.whole * p.Hkv + n.slots;
+    return n;
+}
+
+// The quota, from the sums of seq_stages and of the units over the sequences (of
+// one KV head) and the count of all items at a quota. Where the units fit the
+// work-groups that are resident at once (p.resident), it is about the least one
+// by which their shares still do, found by raising an even share's (INT_MAX,
+// no split, where that takes too long); else one and a half even shares. It
+// depends on lengths alone, so the join finds the same one.
+constexpr float kManySplit = 1.5f;
+template <class Count>
+__host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, Count count) {
+    all = less_of(all * (float)p.Hkv * 1.001f, 1e18f);  // (more than its rounding)
+    const float resident = (float)p.resident, even = less_of(all * p.per_resident + 1.0f, 1e9f);
+    const float least = (float)p.least[1];
+    if (units * (float)p.Hkv > resident) return (unsigned)more_of(kManySplit * even, least);
+    unsigned q = (unsigned)more_of(even, least);
+    for (int i = 0; i < 8; ++i) {
+        const float items = count(q);
+        if (items <= resident) return q;
+        q = more_of(q + 1, (unsigned)((float)q * items * p.per_resident));
+    }
+    return INT_MAX;
+}
+
+struct BatchItem {
+    BatchSeq s;
+    int seq, head, unit, share, shares;
+    int slot;  // of share 0 (the join) or of this share, where shares > 1
+};
+
+// Item i of a sequence (JOIN: its i-th split unit) whose shares' slots begin at
+// `slot`. Items: the split units (the last, heaviest one first) x shares x KV
+// heads, then the whole ones x KV heads, so that neighbouring work-groups, which
+// the dispatcher spreads over the XCDs, have the heads and an XCD's share of
+// them the same head's keys. False where the share has no slot, which only a
+// cu_q that gives rows to several sequences can bring about.
+template <bool JOIN>
+__host__ __device__ inline bool batch_item(const BatchParams &p, const SeqItems &n, int slot, int item, BatchItem &it) {
+    const unsigned heads = p.Hkv;
+    unsigned i = item;
+    it.share = 0;
+    it.shares = n.shares;
+    it.slot = slot;
+    if (!JOIN && i >= (unsigned)n.slots) {
+        i -= n.slots;
+        it.shares = 1;
+        it.unit = n.whole - 1 - (int)(i / heads);
+        it.head = i % heads;
+        return true;
+    }
+    const unsigned per_unit = i / heads;
+    it.head = i - per_unit * heads;
+    if (JOIN) {
+        it.slot += per_unit * n.shares * heads + it.head;  // the unit's shares are `heads` apart
+        it.unit = it.s.units - 1 - (int)per_unit;
+        return it.slot + (n.shares - 1) * p.Hkv < p.slots;
+    }
+    const unsigned u = per_unit / (unsigned)n.shares;
+    it.share = per_unit - u * n.shares;
+    it.unit = it.s.units - 1 - (int)u;
+    it.slot += item;
+    return it.slot < p.slots;
+}
+
+// The share's stages of the unit's n.
+__host__ __device__ inline void share_stages(const BatchItem &it, int n, int &lo, int &hi) {
+    // n < 2^25 stages and at most 2^11 shares: the products pass 32 bits
+    if (it.shares == 1) {
+        lo = 0;
+        hi = n;
+    } else {
+        lo = (int)((unsigned long long)(unsigned)it.share * (unsigned)n / (unsigned)it.shares);
+        hi = (int)((unsigned long long)(unsigned)(it.share + 1) * (unsigned)n / (unsigned)it.shares);
+    }
+}
+
+// ---- the launcher's side
+
+// Work-groups resident at once: the few-row form's have a CU each, the many-row
+// form's share one in twos or threes.
+constexpr int kBatchCus = 256;
+inline int batch_resident(int dtype_bf16, int d) { return kBatchCus * (dtype_bf16 && d == 64 ? 3 : 2); }
+
+// Which forms a call launches, by what the host knows: the few-row form alone
+// where no sequence can have more rows; the many-row form alone where one
+// sequence has the rows; else both, each taking its own sequences.
+inline int batch_few_rows(const BatchParams &p) {
+    const bool may_exceed = (long long)p.max_q * p.group > kBatchFew;
+    return may_exceed && p.n_seq == 1 ? 0 : kBatchFew;
+}
+inline bool batch_may_be_many(const BatchParams &p) {
+    return (long long)less_of(p.max_q, p.n_tok) * p.group > kBatchFew || p.few_rows == 0;
+}
+
+// Stages that a sequence has at most, by its table.
+inline long long batch_most_stages(const BatchParams &p) { return (((long long)p.max_blocks << p.bs_shift) + 63) / 64; }
+
+// A form's launch: its work-groups and the join's, and the workspace's slots.
+struct BatchForm {
+    int rows;
+    long long groups, joins, slots;
+};
+
+// Few rows: a CU's work-group for each run of the line, at least one per KV head;
+// no more than give each `least` stages of the longest line there can be.
+inline BatchForm batch_few_form(BatchParams *p) {
+    const long long line = less_of(p->n_seq, p->n_tok) * (batch_most_stages(*p) + 1);
+    const long long each = more_of(kBatchCus / p->Hkv, 1);
+    p->few_groups = (int)less_of(each, (line + p->least[0] - 1) / p->least[0]);
+    BatchForm f;
+    f.rows = kBatchFew;
+    f.groups = (long long)p->few_groups * p->Hkv;
+    // a cut between each two runs
+    f.joins = p->few_groups > 1 ? f.groups - p->Hkv : 0;
+    f.slots = f.joins > 0 ? 2 * f.groups : 0;
+    return f;
+}
+
+// Many rows. The units are full but for a sequence's last. Where they fit the
+// resident work-groups, so do all items, the shares of split units among them.
+// Else the quota is at least one and a half even shares, and find_item's sum of
+// stages at least half of units x the last one's in each sequence: then the
+// shares of split units, ceil(last one's / quota) each, are at most 4/3 of the
+// resident + the split units, those at most 4/3 of the resident and the units.
+inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
+    BatchForm f;
+    f.rows = batch_many_rows(dtype_bf16);
+    p->resident = batch_resident(dtype_bf16, p->d);
+    p->per_resident = 1.0f / (float)p->resident;
+    const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
+    const long long more = (long long)p->resident * 4 / 3 + 1;
+    if (batch_most_stages(*p) <= p->least[1]) {  // nothing to split
+        f.groups = units;
+        f.joins = f.slots = 0;
+    } else {
+        f.groups = units <= p->resident ? p->resident : units + more;
+        const long long split = units <= p->resident ? less_of(units, (long long)p->resident / 2) : less_of(units, more);
+        f.slots = units <= p->resident ? p->resident : more + split;
+        f.joins = split;
+    }
+    p->slots = (int)f.slots;
+    return f;
+}
+
+// The least stages of a share or run: one for each of the few-row form's waves; 8
+// of the many-row form's, below which the join costs more than the split saves.
+inline void batch_plan(BatchParams *p, int dtype_bf16) {
+    p->few_rows = batch_few_rows(*p);
+    p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
+    p->least[1] = 8;
+}
+
+}  // namespace mxfa

@@ -44,13 +44,13 @@ struct BatchParams {
     int dim, interleaved;
     float factor;
     int hpt;  // heads per thread
-    // attention (fa_batch.hip): the most rows (new tokens x query heads of a KV
-    // head) of a sequence that the few-row form takes (0: it takes none); per
-    // form (few, many) the work-groups resident at once, the least stages of a
-    // share, 1 / resident and 1 / the items the work is cut into at most, and the
-    // shares' slots of the workspace
-    int few_rows, resident[2], least[2], slots[2];
-    float per_resident[2], per_target[2];
+    // attention (fa_batch_items.h): the most rows (new tokens x query heads of a
+    // KV head) of a sequence that the few-row form takes (0: it takes none) and
+    // its work-groups per KV head; per form (few, many) the least stages of a run
+    // or share; the many-row form's work-groups resident at once, 1 / that, and
+    // the slots of its shares; the forms' parts of the workspace
+    int few_rows, few_groups, least[2], resident, slots;
+    float per_resident;
     float *part[2];
 };
 

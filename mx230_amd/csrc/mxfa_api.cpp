@@ -760,7 +760,8 @@ int mxfa_check_batch(const mxfa_batch_shape *s) {
     if ((long long)s->n_tok * group > 0x7fffffffLL - 128) return MXFA_ERR_SHAPE;
     // (also where cu_q gives every sequence all rows)
     if ((double)s->n_seq * ((double)s->n_tok * group / 64 + 1) * s->n_kv_head > 1073741824.0) return MXFA_ERR_SHAPE;
-    // and the caches' rows in 32 bits
+    // the stages of all sequences, and the caches' rows, in 32 bits
+    if (((double)s->max_blocks * s->block_size / 64 + 2) * s->n_seq > 2147483648.0) return MXFA_ERR_SHAPE;
     if ((long long)s->n_blocks * s->block_size > 0x80000000LL) return MXFA_ERR_SHAPE;
     const mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
     if (mxfa::batch_groups(p, s->dtype == MXFA_BF16) > 0x7fffffffLL / 512) return MXFA_ERR_SHAPE;

@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 
@@ -218,3 +220,16 @@ def test_binding_leaves_other_calls():
         assert getattr(c, name)(*[z] * n) is NotImplemented
         assert getattr(c, name)() is NotImplemented
         assert getattr(c, name)(*[None] * n) is NotImplemented
+
+
+@pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc"), reason="hipcc is not installed")
+def test_batch_items():
+    """The items of the attention over a batch (fa_batch_items.h) on the host, with
+    sanitizers: they cover every row and stage once, their workspace slots are
+    theirs alone, and nothing lies outside the buffers, whatever the arrays hold."""
+    here = os.path.join(os.path.dirname(os.path.abspath(__file__)), "sanitize")
+    subprocess.run(["make", "-s", "-j8", "-C", here], check=True)
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=1", UBSAN_OPTIONS="print_stacktrace=1")
+    r = subprocess.run([os.path.join(here, "_build", "items_selftest")], capture_output=True, text=True, env=env,
+                       timeout=300)
+    assert r.returncode == 0 and "all checks passed" in r.stdout, r.stderr[-2000:]
