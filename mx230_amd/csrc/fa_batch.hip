@@ -384,7 +384,7 @@ union BatchFewSmem {
 // sums and O meet in LDS. The stage's blocks come through LDS too, two stages
 // ahead: as loads into registers the compiler would wait for them with
 // vmcnt(0), and with them for every staging load in flight.
-template <class Pol, int NW>
+template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
                                                 BatchFewSmem<Pol, NW> &sm) {
     using T = typename Pol::T;
@@ -396,20 +396,22 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
     const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, it.s.keys, (unsigned)(p.n_blocks - 1)};
     const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
-    T *sk = sm.t.k[wave], *sv = sm.t.v[wave];
+    // waves past the NW that have tiles only take part in the join
+    const int own = NW * 64 < THREADS ? min(wave, NW - 1) : wave;
+    T *sk = sm.t.k[own], *sv = sm.t.v[own];
     const int Nk = it.s.keys;
 
     // stage `st` is the wave's n-th: its blocks in buffer n & 1
     auto fetch = [&](int st, int n) __attribute__((always_inline)) {
-        lds_dma4(lds_addr(sm.t.blk[wave][n & 1]), rows.table + rows.block_at(st * 64 + lane));
+        lds_dma4(lds_addr(sm.t.blk[own][n & 1]), rows.table + rows.block_at(st * 64 + lane));
     };
     auto load = [&](T *tile, const T *X, int st, int n) __attribute__((always_inline)) {
-        const int *blk = sm.t.blk[wave][n & 1];
+        const int *blk = sm.t.blk[own][n & 1];
         Stage stage;
         stage.rows(lane, stride, [&](int r) __attribute__((always_inline)) { return rows.row(blk[r], st * 64 + r); });
         stage.load(tile, X, 0);
     };
-    int st = s_lo + wave, n = 0;
+    int st = wave < NW ? s_lo + wave : s_hi, n = 0;
     if (st < s_hi) fetch(st, 0);
     const int row = min(l16, it.s.rows - 1);
     const int qpos = it.s.pos + row / p.group;
@@ -461,10 +463,12 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
     if (tid == 0) sm.merge.bad = 0;
     __syncthreads();
     if (bad && lane == 0) sm.merge.bad = 1;
+    if (wave < NW) {
 #pragma unroll
-    for (int i = 0; i < XT; ++i)
-        *reinterpret_cast<f32x4 *>(&sm.merge.acc[wave][l16][batch_col<Pol>(i, g)]) = batch_quad<Pol>(acc, i, 0);
-    if (g == 0) *reinterpret_cast<float2 *>(sm.merge.ml[wave][l16]) = make_float2(m[0], lw);
+        for (int i = 0; i < XT; ++i)
+            *reinterpret_cast<f32x4 *>(&sm.merge.acc[own][l16][batch_col<Pol>(i, g)]) = batch_quad<Pol>(acc, i, 0);
+        if (g == 0) *reinterpret_cast<float2 *>(sm.merge.ml[own][l16]) = make_float2(m[0], lw);
+    }
     __syncthreads();
     float *part = nullptr, *ml = nullptr;
     if (slot >= 0) {
@@ -475,7 +479,7 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
         if (tid < 4 * ROWS) batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
         return;
     }
-    for (int i = tid; i < it.s.rows * (D / 4); i += 64 * NW) {
+    for (int i = tid; i < it.s.rows * (D / 4); i += THREADS) {
         const int r = i / (D / 4), c = 4 * (i % (D / 4));
         float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -498,10 +502,8 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
 }
 
 // Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line.
-template <class Pol, int NW>
-__device__ __forceinline__ void batch_few_body(const BatchParams &p) {
-    __shared__ __attribute__((aligned(16))) BatchFewSmem<Pol, NW> sm;
-    const int g = blockIdx.x;
+template <class Pol, int NW, int THREADS>
+__device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
     const unsigned all = few_line(p), run = few_run(p, all);
     unsigned x = (unsigned)(g / p.Hkv) * run;
     const unsigned x1 = min(x + run, all);
@@ -513,7 +515,7 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
         it.seq = seq;
         it.s = s;
         const FewPiece f = few_piece(x, x1, u0, u1, g);
-        batch_few_piece<Pol, NW>(p, it, f.lo, f.hi, f.slot, sm);
+        batch_few_piece<Pol, NW, THREADS>(p, it, f.lo, f.hi, f.slot, sm);
         x = f.end;
         if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
         return x >= x1;
@@ -522,22 +524,27 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p) {
 
 // ----------------------------------------------------------------- the many rows
 
+template <class Pol>
+struct BatchManySmem {
+    typename Pol::T k[2][Pol::ROWS * Pol::D], v[2][Pol::ROWS * Pol::D];
+    int bad[4];
+};
+
 template <class Pol, int QT>
-__device__ __forceinline__ void batch_many_body(const BatchParams &p) {
+__device__ __forceinline__ void batch_many_body(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
     using T = typename Pol::T;
     using Stage = BatchStage<Pol, 256>;
     constexpr int D = Pol::D, XT = D / 16, BK = Pol::ROWS, ROWS = 64 * QT;
     constexpr bool kLazy = sizeof(T) == 2;  // fp32 scores are summed from zero
     constexpr bool kPrio = sizeof(T) == 2;
-    __shared__ __attribute__((aligned(16))) T sK[2][BK * D];
-    __shared__ __attribute__((aligned(16))) T sV[2][BK * D];
-    __shared__ int flags[4];
+    auto &sK = sm.k;
+    auto &sV = sm.v;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
     // neighbours in eights (the XCDs) stay together
-    const int w = cu_order_wg((int)blockIdx.x >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + ((int)blockIdx.x & 7);
+    const int w = cu_order_wg(block >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + (block & 7);
     if (!find_item<ROWS, false>(p, w, it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
 
@@ -640,9 +647,9 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p) {
         ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
     }
     const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
-    if (lane == 0) flags[wave] = bad;
+    if (lane == 0) sm.bad[wave] = bad;
     __syncthreads();
-    if (flags[0] | flags[1] | flags[2] | flags[3]) {
+    if (sm.bad[0] | sm.bad[1] | sm.bad[2] | sm.bad[3]) {
         for (int i = 0; i < QT; ++i) batch_plain<T, D, ROWS>(p, it, 64 * i, s_lo * BK, s_hi * BK, part, ml);
         return;
     }
@@ -760,19 +767,41 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
                                 [&](int i) __attribute__((always_inline)) { return it.slot + i * p.Hkv; });
 }
 
-#define MXFA_BATCH(SUFFIX, POL, NW, WPS)                                                              \
+// Both forms in one launch: the few-row form's work-groups first, each wave's
+// tiles a quarter of its work-group's (bf16, d = 64) or half of it, so that LDS
+// holds as many of them as of the many-row form's: their reads and its matrix
+// products then share the CUs.
+template <class Pol, int NW, int QT>
+__device__ __forceinline__ void batch_both_body(const BatchParams &p, int few_groups) {
+    __shared__ __attribute__((aligned(16))) union {
+        BatchFewSmem<Pol, NW> few;
+        BatchManySmem<Pol> many;
+    } sm;
+    if ((int)blockIdx.x < few_groups) {
+        batch_few_body<Pol, NW, 256>(p, blockIdx.x, sm.few);
+    } else {
+        batch_many_body<Pol, QT>(p, (int)blockIdx.x - few_groups, sm.many);
+    }
+}
+
+#define MXFA_BATCH(SUFFIX, POL, NW, WPS, BOTH_NW)                                                     \
     extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {  \
-        batch_few_body<POL, NW>(p);                                                                   \
+        __shared__ __attribute__((aligned(16))) BatchFewSmem<POL, NW> sm;                             \
+        batch_few_body<POL, NW, 64 * NW>(p, blockIdx.x, sm);                                          \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) { \
-        batch_many_body<POL, batch_tiles(sizeof(POL::T) == 2)>(p);                                                                     \
+        __shared__ __attribute__((aligned(16))) BatchManySmem<POL> sm;                                \
+        batch_many_body<POL, batch_tiles(sizeof(POL::T) == 2)>(p, blockIdx.x, sm);                    \
+    }                                                                                                 \
+    extern "C" __global__ __launch_bounds__(256, 2) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
+        batch_both_body<POL, BOTH_NW, batch_tiles(sizeof(POL::T) == 2)>(p, few_groups);               \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void mxfa_batch_##SUFFIX##_join(BatchParams p, int few_groups) { \
         batch_join<POL::T, POL::D>(p, few_groups);                                                    \
     }
-MXFA_BATCH(b64, PolRows<64>, 8, 3)
-MXFA_BATCH(b128, PolRows<128>, 4, 2)
-MXFA_BATCH(f64, PolF32, 4, 2)
+MXFA_BATCH(b64, PolRows<64>, 8, 3, 4)
+MXFA_BATCH(b128, PolRows<128>, 4, 2, 2)
+MXFA_BATCH(f64, PolF32, 4, 2, 2)
 #undef MXFA_BATCH
 #endif
 
@@ -800,20 +829,25 @@ long long batch_groups(const BatchParams &q, int dtype_bf16) {
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
-    static constexpr KernelId ids[3][3] = {
-        {k_mxfa_batch_b64_few, k_mxfa_batch_b64_many, k_mxfa_batch_b64_join},
-        {k_mxfa_batch_b128_few, k_mxfa_batch_b128_many, k_mxfa_batch_b128_join},
-        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_many, k_mxfa_batch_f64_join}};
+    static constexpr KernelId ids[3][4] = {
+        {k_mxfa_batch_b64_few, k_mxfa_batch_b64_many, k_mxfa_batch_b64_join, k_mxfa_batch_b64_both},
+        {k_mxfa_batch_b128_few, k_mxfa_batch_b128_many, k_mxfa_batch_b128_join, k_mxfa_batch_b128_both},
+        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_many, k_mxfa_batch_f64_join, k_mxfa_batch_f64_both}};
     const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
     BatchForm f[2];
     batch_forms(&p, dtype_bf16, f);
     p.part[0] = static_cast<float *>(workspace);
     p.part[1] = p.part[0] + batch_part_floats(f[0].slots, f[0].rows, p.d);
-    void *args[] = {&p};
-    hipError_t e = hipSuccess;
-    if (f[1].groups > 0) e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(256), args, stream);
-    if (e == hipSuccess && f[0].groups > 0)
-        e = launch_kernel(id[0], dim3((unsigned)f[0].groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+    hipError_t e;
+    int few_groups = (int)f[0].groups;
+    void *args[] = {&p, &few_groups};
+    if (f[1].groups == 0) {
+        e = launch_kernel(id[0], dim3(few_groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+    } else if (few_groups == 0) {
+        e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(256), args, stream);
+    } else {
+        e = launch_kernel(id[3], dim3((unsigned)(few_groups + f[1].groups)), dim3(256), args, stream);
+    }
     int cuts = (int)f[0].joins;
     const unsigned joins = (unsigned)(cuts + f[1].joins * (f[1].rows / kJoinRows));
     if (e != hipSuccess || joins == 0) return e;

@@ -208,7 +208,8 @@ __host__ __device__ inline void share_stages(const BatchItem &it, int n, int &lo
 // Work-groups resident at once: the few-row form's have a CU each, the many-row
 // form's share one in twos or threes.
 constexpr int kBatchCus = 256;
-inline int batch_resident(int dtype_bf16, int d) { return kBatchCus * (dtype_bf16 && d == 64 ? 3 : 2); }
+// (two where they share a launch with the few-row form's)
+inline int batch_resident(int dtype_bf16, int d, bool both) { return kBatchCus * (dtype_bf16 && d == 64 && !both ? 3 : 2); }
 
 // Which forms a call launches, by what the host knows: the few-row form alone
 // where no sequence can have more rows; the many-row form alone where one
@@ -254,7 +255,7 @@ inline BatchForm batch_few_form(BatchParams *p) {
 inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     BatchForm f;
     f.rows = batch_many_rows(dtype_bf16);
-    p->resident = batch_resident(dtype_bf16, p->d);
+    p->resident = batch_resident(dtype_bf16, p->d, p->few_rows > 0);
     p->per_resident = 1.0f / (float)p->resident;
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;

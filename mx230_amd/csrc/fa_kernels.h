@@ -44,9 +44,9 @@
     /* naive baselines (fa_naive.hip) */                                                      \
     X(mxfa_naive_scores) X(mxfa_naive_softmax) X(mxfa_naive_av) X(mxfa_naive_bwd)            \
     /* attention of a batch over a paged cache (fa_batch.hip) */                              \
-    X(mxfa_batch_b64_few) X(mxfa_batch_b64_many) X(mxfa_batch_b64_join)                       \
-    X(mxfa_batch_b128_few) X(mxfa_batch_b128_many) X(mxfa_batch_b128_join)                    \
-    X(mxfa_batch_f64_few) X(mxfa_batch_f64_many) X(mxfa_batch_f64_join)                       \
+    X(mxfa_batch_b64_few) X(mxfa_batch_b64_many) X(mxfa_batch_b64_join) X(mxfa_batch_b64_both)                       \
+    X(mxfa_batch_b128_few) X(mxfa_batch_b128_many) X(mxfa_batch_b128_join) X(mxfa_batch_b128_both)                    \
+    X(mxfa_batch_f64_few) X(mxfa_batch_f64_many) X(mxfa_batch_f64_join) X(mxfa_batch_f64_both)                       \
     /* rotary positions and the cache append (fa_rotary.hip): 16-byte, 8-byte, single-element chunks */ \
     X(mxfa_rotary_b) X(mxfa_rotary_b4) X(mxfa_rotary_b1) X(mxfa_rotary_f) X(mxfa_rotary_f1)   \
     X(mxfa_append_b) X(mxfa_append_b4) X(mxfa_append_b1) X(mxfa_append_f) X(mxfa_append_f1)   \
