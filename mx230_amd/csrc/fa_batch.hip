@@ -34,7 +34,7 @@ namespace mxfa {
 // ------------------------------------------------- fp32 on its own instructions
 
 // fp32 inputs (d = 64) on v_mfma_f32_16x16x4_f32, in the policy form of
-// fwd_stage. LDS rows of 256 bytes hold their 16-byte chunk c at c ^ (row & 15),
+// fwd_stage, for the few-row form, which the reads bound. LDS rows of 256 bytes hold their 16-byte chunk c at c ^ (row & 15),
 // so the 16 rows of a score operand and the 16 chunks of a V row both cover
 // all banks. Score k-steps: MFMA (c, e) takes element 16c + 4g + e of lane
 // group g. In the chained product a lane reads 4 columns of a V row at once, so
@@ -524,6 +524,13 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
 
 // ----------------------------------------------------------------- the many rows
 
+// The item of the many-row form's work-group `block`, in the order by which a CU's
+// resident ones have long and short units (cu_order_wg); neighbours in eights
+// (the XCDs) stay together.
+__device__ __forceinline__ int batch_order(const BatchParams &p, int block) {
+    return cu_order_wg(block >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + (block & 7);
+}
+
 template <class Pol>
 struct BatchManySmem {
     typename Pol::T k[2][Pol::ROWS * Pol::D], v[2][Pol::ROWS * Pol::D];
@@ -535,17 +542,14 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
     using T = typename Pol::T;
     using Stage = BatchStage<Pol, 256>;
     constexpr int D = Pol::D, XT = D / 16, BK = Pol::ROWS, ROWS = 64 * QT;
-    constexpr bool kLazy = sizeof(T) == 2;  // fp32 scores are summed from zero
-    constexpr bool kPrio = sizeof(T) == 2;
+    constexpr bool kPrio = true;
     auto &sK = sm.k;
     auto &sV = sm.v;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    // neighbours in eights (the XCDs) stay together
-    const int w = cu_order_wg(block >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + (block & 7);
-    if (!find_item<ROWS, false>(p, w, it)) return;
+    if (!find_item<ROWS, false>(p, batch_order(p, block), it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
 
     const int r0 = it.unit * ROWS, rw = r0 + wave * 16 * QT;  // the unit's and the wave's first row
@@ -604,7 +608,7 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
         constexpr int B = decltype(buf)::value;
         if (st + 1 < s_hi) stage_next(sK[B ^ 1], sV[B ^ 1], st + 1);
         if (some) {
-            if constexpr (decltype(first)::value || !kLazy) {
+            if constexpr (decltype(first)::value) {
                 fwd_stage<Pol, QT, true, false, kPrio>(acc, m, lsum, qf, sK[B], sV[B], st * BK, qpos, Nk, g, l16,
                                                        p.scale_log2);
             } else {
@@ -668,17 +672,209 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
         }
         const float inv = ltot[qt] > 0.f ? 1.0f / ltot[qt] : 0.f;
         T *O = static_cast<T *>(p.o) + batch_elem(p, it, min(r, last_row), p.o_rs, D);
-        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int xt = 0; xt < XT; xt += 2)
-                store8_pair_bf16(O, 16 * xt, g, acc[xt][qt], acc[xt + 1][qt], inv, have);
-        } else if (have) {
-#pragma unroll
-            for (int i = 0; i < XT; ++i) store4<T>(O + batch_col<Pol>(i, g), batch_quad<Pol>(acc, i, qt), inv);
-        }
+        for (int xt = 0; xt < XT; xt += 2)
+            store8_pair_bf16(O, 16 * xt, g, acc[xt][qt], acc[xt + 1][qt], inv, have);
         if (p.lse != nullptr && have && g == 0)
             p.lse[batch_lse(p, it, r)] = ltot[qt] > 0.f ? (m[qt] + fast_log2(ltot[qt])) * kLn2 : -INFINITY;
     }
+}
+
+// The same for fp32 (d = 64, 64 rows) with its products in bf16 parts (Split3): K
+// and V pass through registers, loaded one stage ahead, and are split once per
+// work-group into one LDS buffer; three work-groups per CU. Scores and a
+// stage's part of O are summed from zero; operands that the parts cannot hold
+// (kPartMin, infinities) flag the unit, whose rows are then run in plain
+// arithmetic. On v_mfma_f32_16x16x4_f32 2000 tokens of 14/2 heads after 2096 took
+// 235 us (94 TFLOP/s).
+__device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block, FwdSplitSmem &sm) {
+    constexpr int D = 64, XT = 4, BK = 64, NT = 256, ROWS = batch_many_rows(false);
+    using PL = PolBF16<64>;  // the parts' layout
+    using Stage = SplitStage<NT>;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    BatchItem it;
+    if (!find_item<ROWS, false>(p, batch_order(p, block), it)) return;
+    const float *K = static_cast<const float *>(p.k) + it.head * D, *V = static_cast<const float *>(p.v) + it.head * D;
+
+    const int r0 = it.unit * ROWS, rw = r0 + wave * 16, r = rw + l16;
+    const int last_row = it.s.rows - 1, row = min(r, last_row);
+    const int qpos = it.s.pos + row / p.group;
+    const int pos_lo = it.s.pos + r0 / p.group;
+    const int pos_hi = it.s.pos + min(r0 + ROWS - 1, last_row) / p.group;
+    const int pos_w = it.s.pos + min(rw + 15, last_row) / p.group;
+    const int Nk = min(it.s.keys, max(pos_hi + 1, 0)), n = (Nk + BK - 1) / BK;
+    const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, Nk, (unsigned)(p.n_blocks - 1)};
+    int s_lo, s_hi;
+    share_stages(it, n, s_lo, s_hi);
+
+    // this thread's chunks of a tile: row and first column
+    int srow[Stage::NK], scol[Stage::NK];
+#pragma unroll
+    for (int k = 0; k < Stage::NK; ++k) {
+        PL::chunk_at(k * NT + tid, srow[k], scol[k]);
+        scol[k] *= 8;
+    }
+    int blk = 0;  // of the lane's row of the stage to be loaded next
+    auto fetch = [&](int st) __attribute__((always_inline)) { blk = rows.table[rows.block_at(st * BK + lane)]; };
+    Stage xk, xv;
+    auto load = [&](int st) __attribute__((always_inline)) {
+        const unsigned mine = rows.row(blk, st * BK + lane);
+#pragma unroll
+        for (int k = 0; k < Stage::NK; ++k) {
+            const unsigned at = (unsigned)__shfl((int)mine, srow[k], 64);
+            const size_t off = (size_t)at * (size_t)p.kv_rs + scol[k];
+            xk.load(k, K + off);
+            xv.load(k, V + off);
+        }
+        if (st + 1 < s_hi) fetch(st + 1);
+    };
+    if (s_lo < s_hi) {
+        fetch(s_lo);
+        load(s_lo);
+    }
+    Split3 qf[1][2];
+    const bool low = split_row(qf[0], static_cast<const float *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g,
+                               p.scale_log2 * kPartDown, r <= last_row);
+    f32x4 acc[XT][1];
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) acc[xt][0] = zero4();
+    float m = -INFINITY, lsum = 0.f;
+
+    // One stage: the share's first, or m raised only where a lane's sum of p
+    // passes kLazySum. A row that sees no key of the first stage keeps m = -inf,
+    // and sees none of the later ones.
+    auto compute = [&](auto first, bool edge, int k0) __attribute__((always_inline)) {
+        constexpr bool FIRST = decltype(first)::value;
+        f32x4 s[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Split3 a[1][2];
+                f32x4 c[1][1] = {{zero4()}};
+                sm.k.row_frags(a[0], 32 * u + PL::arow(t, l16), g);
+                mma_split_tiles<2, 1, 1>(c, a, qf);
+                s[u][t] = c[0][0];
+            }
+        }
+        if (edge) {
+            const int lim = min(qpos, Nk - 1) - k0 - PL::bidx(0, g, 0);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (32 * u + PL::bidx(t, 0, e) > lim) s[u][t][e] = -INFINITY;
+                    }
+                }
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : m;  // what p is relative to
+        f32x4 pv[2][2];
+        auto exps = [&](float sub) __attribute__((always_inline)) {
+            float ls = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = fast_exp2(s[u][t][e] - sub);
+                        pv[u][t][e] = x;
+                        ls += x;
+                    }
+                }
+            }
+            return ls;
+        };
+        auto raise = [&]() __attribute__((always_inline)) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[u][t][e]);
+                }
+            }
+            mx = fmaxf(xg_max(mx), m);
+            const float to = mx == -INFINITY ? 0.f : mx;
+            if constexpr (!FIRST) {
+                const float corr = fast_exp2(base - to);
+                lsum *= corr;
+#pragma unroll
+                for (int xt = 0; xt < XT; ++xt) acc[xt][0] *= corr;
+            }
+            m = mx;
+            lsum += exps(to);
+        };
+        if constexpr (FIRST) {
+            raise();
+        } else {
+            const float ls = exps(base);
+            if (__builtin_amdgcn_ballot_w64(ls > kLazySum) != 0) {
+                raise();
+            } else {
+                lsum += ls;
+            }
+        }
+        const Split3 pf[2][1] = {{split3(pv[0][0], pv[0][1])}, {split3(pv[1][0], pv[1][1])}};
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) {
+            f32x4 c = zero4();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Split3 a[1] = {sm.v.chain_a(16 * xt, 32 * u, g, l16)};
+                c = mma_split<1>(a, pf[u], c);
+            }
+            acc[xt][0] += c;
+        }
+    };
+    // stages before `whole` hold no key that a row of the unit does not see
+    const int whole = min(s_hi, min(Nk, pos_lo + 1) / BK);
+    auto stage = [&](auto first, int st) __attribute__((always_inline)) {
+        if (st > s_lo) barrier_lds();  // every wave is done with the stage before
+        xk.write(sm.k, tid);
+        xv.write(sm.v, tid);
+        if (st + 1 < s_hi) load(st + 1);
+        barrier_lds();
+        if (rw <= last_row && st * BK <= pos_w) compute(first, st >= whole, st * BK);
+    };
+    if (s_lo < s_hi) stage(std::true_type{}, s_lo);
+    for (int st = s_lo + 1; st < s_hi; ++st) stage(std::false_type{}, st);
+    const float ltot = xg_sum(lsum);
+    float z = 0.f * ltot;
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt][0]);
+    // a row that sees keys of the share, all of whose scores overflowed to -inf
+    if (rw <= last_row && m == -INFINITY && s_lo < s_hi && s_lo * BK <= qpos) z = NAN;
+    if (low) z = NAN;
+    float *part = nullptr, *ml = nullptr;
+    if (it.shares > 1) {
+        part = batch_part<ROWS>(p.part[1], it.slot, D);
+        ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
+    }
+    if (any_nonfinite<4>(z, sm.flags, wave, lane)) {
+        batch_plain<float, D, ROWS>(p, it, 0, s_lo * BK, s_hi * BK, part, ml);
+        return;
+    }
+    if (r > last_row) return;
+    if (part != nullptr) {
+        const int rl = r - r0;
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) store4<float>(part + rl * D + 16 * xt + 4 * g, acc[xt][0], kPartDown);
+        if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m, ltot);
+        return;
+    }
+    const float inv = ltot > 0.f ? kPartDown / ltot : 0.f;
+    float *O = static_cast<float *>(p.o) + batch_elem(p, it, r, p.o_rs, D);
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) store4<float>(O + 16 * xt + 4 * g, acc[xt][0], inv);
+    if (p.lse != nullptr && g == 0)
+        p.lse[batch_lse(p, it, r)] = ltot > 0.f ? (m + fast_log2(ltot)) * kLn2 : -INFINITY;
 }
 
 // ---------------------------------------------------------------------- the join
@@ -771,37 +967,46 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
 // tiles a quarter of its work-group's (bf16, d = 64) or half of it, so that LDS
 // holds as many of them as of the many-row form's: their reads and its matrix
 // products then share the CUs.
-template <class Pol, int NW, int QT>
+__device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<PolRows<64>> &sm) {
+    batch_many_body<PolRows<64>, 2>(p, block, sm);
+}
+__device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<PolRows<128>> &sm) {
+    batch_many_body<PolRows<128>, 2>(p, block, sm);
+}
+__device__ __forceinline__ void batch_many(const BatchParams &p, int block, FwdSplitSmem &sm) {
+    batch_many_parts(p, block, sm);
+}
+template <class Pol, class Many, int NW>
 __device__ __forceinline__ void batch_both_body(const BatchParams &p, int few_groups) {
     __shared__ __attribute__((aligned(16))) union {
         BatchFewSmem<Pol, NW> few;
-        BatchManySmem<Pol> many;
+        Many many;
     } sm;
     if ((int)blockIdx.x < few_groups) {
         batch_few_body<Pol, NW, 256>(p, blockIdx.x, sm.few);
     } else {
-        batch_many_body<Pol, QT>(p, (int)blockIdx.x - few_groups, sm.many);
+        batch_many(p, (int)blockIdx.x - few_groups, sm.many);
     }
 }
 
-#define MXFA_BATCH(SUFFIX, POL, NW, WPS, BOTH_NW)                                                     \
+#define MXFA_BATCH(SUFFIX, POL, MANY, NW, WPS, BOTH_NW)                                               \
     extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {  \
         __shared__ __attribute__((aligned(16))) BatchFewSmem<POL, NW> sm;                             \
         batch_few_body<POL, NW, 64 * NW>(p, blockIdx.x, sm);                                          \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) { \
-        __shared__ __attribute__((aligned(16))) BatchManySmem<POL> sm;                                \
-        batch_many_body<POL, batch_tiles(sizeof(POL::T) == 2)>(p, blockIdx.x, sm);                    \
+        __shared__ __attribute__((aligned(16))) MANY sm;                                              \
+        batch_many(p, blockIdx.x, sm);                                                                \
     }                                                                                                 \
-    extern "C" __global__ __launch_bounds__(256, 2) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
-        batch_both_body<POL, BOTH_NW, batch_tiles(sizeof(POL::T) == 2)>(p, few_groups);               \
+    extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
+        batch_both_body<POL, MANY, BOTH_NW>(p, few_groups);                                           \
     }                                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void mxfa_batch_##SUFFIX##_join(BatchParams p, int few_groups) { \
         batch_join<POL::T, POL::D>(p, few_groups);                                                    \
     }
-MXFA_BATCH(b64, PolRows<64>, 8, 3, 4)
-MXFA_BATCH(b128, PolRows<128>, 4, 2, 2)
-MXFA_BATCH(f64, PolF32, 4, 2, 2)
+MXFA_BATCH(b64, PolRows<64>, BatchManySmem<PolRows<64>>, 8, 3, 3)
+MXFA_BATCH(b128, PolRows<128>, BatchManySmem<PolRows<128>>, 4, 2, 2)
+MXFA_BATCH(f64, PolF32, FwdSplitSmem, 4, 3, 1)
 #undef MXFA_BATCH
 #endif
 

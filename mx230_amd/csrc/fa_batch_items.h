@@ -208,8 +208,7 @@ __host__ __device__ inline void share_stages(const BatchItem &it, int n, int &lo
 // Work-groups resident at once: the few-row form's have a CU each, the many-row
 // form's share one in twos or threes.
 constexpr int kBatchCus = 256;
-// (two where they share a launch with the few-row form's)
-inline int batch_resident(int dtype_bf16, int d, bool both) { return kBatchCus * (dtype_bf16 && d == 64 && !both ? 3 : 2); }
+inline int batch_resident(int d) { return d == 64 ? 3 * kBatchCus : 2 * kBatchCus; }
 
 // Which forms a call launches, by what the host knows: the few-row form alone
 // where no sequence can have more rows; the many-row form alone where one
@@ -255,7 +254,16 @@ inline BatchForm batch_few_form(BatchParams *p) {
 inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     BatchForm f;
     f.rows = batch_many_rows(dtype_bf16);
-    p->resident = batch_resident(dtype_bf16, p->d, p->few_rows > 0);
+    p->resident = batch_resident(p->d);
+    // Beside the few-row form's work-groups a CU holds two of these. The host
+    // knows how many sequences can be of few rows: the others have max_q tokens at
+    // most. us, 14/2 heads, d = 64: 4 chunks and 28 tokens 57.6 (61 by three a CU);
+    // 8 chunks 84 by three (104 by two)
+    if (p->few_rows > 0) {
+        const long long few_tok = p->few_rows / p->group;
+        const long long chunks = more_of((long long)p->n_tok - p->n_seq * few_tok, 0LL) / p->max_q;
+        if (2 * chunks < p->n_seq) p->resident = 2 * kBatchCus;
+    }
     p->per_resident = 1.0f / (float)p->resident;
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;
