@@ -680,15 +680,14 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
     }
 }
 
-// The same for fp32 (d = 64, 64 rows) with its products in bf16 parts (Split3): K
-// and V pass through registers, loaded one stage ahead, and are split once per
-// work-group into one LDS buffer; three work-groups per CU. Scores and a
-// stage's part of O are summed from zero; operands that the parts cannot hold
-// (kPartMin, infinities) flag the unit, whose rows are then run in plain
-// arithmetic. On v_mfma_f32_16x16x4_f32 2000 tokens of 14/2 heads after 2096 took
-// 235 us (94 TFLOP/s).
+// The same for fp32 (d = 64), 16 rows per wave of 8, with its products in bf16 parts
+// (Split3): K and V pass through registers, loaded one stage ahead, and are
+// split once per work-group into one LDS buffer; two work-groups per CU. Operands
+// that the parts cannot hold (kPartMin, infinities) flag the unit, whose rows
+// are then run in plain arithmetic. 2000 tokens of 14/2 heads after 2096, us: on
+// v_mfma_f32_16x16x4_f32 235, parts with 4 waves and 64 rows 203.
 __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block, FwdSplitSmem &sm) {
-    constexpr int D = 64, XT = 4, BK = 64, NT = 256, ROWS = batch_many_rows(false);
+    constexpr int D = 64, XT = 4, BK = 64, NW = kBatchF32Waves, NT = 64 * NW, ROWS = batch_many_rows(false);
     using PL = PolBF16<64>;  // the parts' layout
     using Stage = SplitStage<NT>;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -821,16 +820,14 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
                 lsum += ls;
             }
         }
-        const Split3 pf[2][1] = {{split3(pv[0][0], pv[0][1])}, {split3(pv[1][0], pv[1][1])}};
 #pragma unroll
-        for (int xt = 0; xt < XT; ++xt) {
-            f32x4 c = zero4();
+        for (int u = 0; u < 2; ++u) {
+            const Split3 pf[1] = {split3(pv[u][0], pv[u][1])};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int xt = 0; xt < XT; ++xt) {
                 const Split3 a[1] = {sm.v.chain_a(16 * xt, 32 * u, g, l16)};
-                c = mma_split<1>(a, pf[u], c);
+                acc[xt][0] = mma_split<1>(a, pf, acc[xt][0]);
             }
-            acc[xt][0] += c;
         }
     };
     // stages before `whole` hold no key that a row of the unit does not see
@@ -857,7 +854,7 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
         part = batch_part<ROWS>(p.part[1], it.slot, D);
         ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
     }
-    if (any_nonfinite<4>(z, sm.flags, wave, lane)) {
+    if (any_nonfinite<NW>(z, sm.flags, wave, lane)) {
         batch_plain<float, D, ROWS>(p, it, 0, s_lo * BK, s_hi * BK, part, ml);
         return;
     }
@@ -880,44 +877,69 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
 // ---------------------------------------------------------------------- the join
 
 // The parts of a unit's rows [first, end): o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s
-// - M) l_s, part s being slot at(s) of the workspace. D / 4 threads have a row,
-// four elements each; where there are few rows several such groups take turns
-// over a row's parts and meet in LDS.
+// - M) l_s, part s being slot at(s) of the workspace, 128 parts at a time. A
+// group of D / 4 threads, four elements each, has a row; where there are few
+// rows several groups take turns over its parts and meet in LDS. Bound by
+// latency: the (max, sum) pairs of all parts are one round of loads, and eight
+// parts of a thread's turn another.
 template <class T, int D, int ROWS, class At>
 __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int first, int end, int S,
                                                 float *parts, int slots, At at) {
-    constexpr int C = D / 4, NG = 256 / C;
+    constexpr int C = D / 4, NG = 256 / C, PARTS = 128, EACH = PARTS / C;
     __shared__ __attribute__((aligned(16))) f32x4 so[NG][C];
+    __shared__ float weights[NG][PARTS];
     const int tid = threadIdx.x, c = tid % C, grp = tid / C, nrows = end - first;
     int together = 1;  // groups to a row
     while (together * 2 * nrows <= NG) together *= 2;
     const int turn = grp % together;
-    auto ml = [&](int s, int r) __attribute__((always_inline)) {
-        return *reinterpret_cast<const float2 *>(batch_ml<ROWS>(parts, slots, at(s), D) + 2 * r);
-    };
     for (int r0 = 0; r0 < nrows; r0 += NG / together) {
         const bool have = r0 + grp / together < nrows;
-        const int r = first + r0 + grp / together;
+        const int r = have ? first + r0 + grp / together : first;  // (others repeat a row and store nothing)
         float M = -INFINITY, L = 0.f;
         f32x4 o = zero4();
-        if (have) {
-            for (int s = c; s < S; s += C) M = fmaxf(M, ml(s, r).x);
-        }
+        for (int s0 = 0; s0 < S; s0 += PARTS) {
+            const int n = min(PARTS, S - s0);
+            float2 v[EACH];
 #pragma unroll
-        for (int k = C / 2; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
-        const float mref = M == -INFINITY ? 0.f : M;
-        if (have) {
-            for (int s = c; s < S; s += C) {
-                const float2 v = ml(s, r);
-                L += fast_exp2(v.x - mref) * v.y;
+            for (int i = 0; i < EACH; ++i) {
+                v[i] = make_float2(-INFINITY, 0.f);
+                if (i * C + c < n)
+                    v[i] = *reinterpret_cast<const float2 *>(batch_ml<ROWS>(parts, slots, at(s0 + i * C + c), D) + 2 * r);
             }
-#pragma unroll 4
-            for (int s = turn; s < S; s += together)
-                o += *reinterpret_cast<const f32x4 *>(batch_part<ROWS>(parts, at(s), D) + r * D + 4 * c) *
-                     fast_exp2(ml(s, r).x - mref);
-        }
+            float mx = M;
 #pragma unroll
-        for (int k = C / 2; k > 0; k >>= 1) L += __shfl_xor(L, k, 64);
+            for (int i = 0; i < EACH; ++i) mx = fmaxf(mx, v[i].x);
+#pragma unroll
+            for (int k = C / 2; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
+            const float mref = mx == -INFINITY ? 0.f : mx, corr = fast_exp2(M - mref);
+            M = mx;
+            L *= corr;
+            o *= corr;
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const float w = fast_exp2(v[i].x - mref);
+                l += w * v[i].y;
+                weights[grp][i * C + c] = w;  // read by the group's own lanes of the wave
+            }
+#pragma unroll
+            for (int k = C / 2; k > 0; k >>= 1) l += __shfl_xor(l, k, 64);
+            L += l;
+            wait_lds();
+            for (int s = turn; s < n; s += 8 * together) {
+                f32x4 x[8];
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = min(s + i * together, n - 1);
+                    w[i] = s + i * together < n ? weights[grp][j] : 0.f;
+                    x[i] = *reinterpret_cast<const f32x4 *>(batch_part<ROWS>(parts, at(s0 + j), D) + r * D + 4 * c);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o += x[i] * w[i];
+            }
+            wait_lds();
+        }
         if (together > 1) {
             __syncthreads();
             so[grp][c] = o;
@@ -934,12 +956,13 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
 // that the many-row form may have, kJoinRows rows each.
 template <class T, int D>
 __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
-    constexpr int ROWS = batch_many_rows(sizeof(T) == 2), PIECES = ROWS / kJoinRows;
+    constexpr int ROWS = batch_many_rows(sizeof(T) == 2), JOIN = join_rows(D), PIECES = ROWS / JOIN;
     BatchItem it;
     if ((int)blockIdx.x < few_cuts) {
         // the cut at the end of run `cut`; the first cut through a sequence joins it
-        const int cut = (int)blockIdx.x / p.Hkv, heads = p.Hkv;
-        it.head = (int)blockIdx.x % p.Hkv;
+        const int heads = p.Hkv, j = (int)blockIdx.x / kFewJoins, first = (int)blockIdx.x % kFewJoins * (kBatchFew / kFewJoins);
+        const int cut = j / heads;
+        it.head = j % heads;
         it.unit = 0;
         const unsigned all = few_line(p), run = few_run(p, all), x = (unsigned)(cut + 1) * run;
         if (x >= all) return;
@@ -947,8 +970,9 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
             if (u0 >= x || u0 / run != (unsigned)cut) return true;
             it.seq = seq;
             it.s = s;
-            const int head = it.head, S = (int)((u1 - 1) / run) - cut + 1;
-            batch_join_rows<T, D, kBatchFew>(p, it, 0, s.rows, S, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
+            const int head = it.head, S = (int)((u1 - 1) / run) - cut + 1, end = min(first + kBatchFew / kFewJoins, s.rows);
+            if (first >= end) return true;
+            batch_join_rows<T, D, kBatchFew>(p, it, first, end, S, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
                 return i == 0 ? few_first_slot(cut, heads, head) : few_next_slot(cut, heads, head) + 2 * heads * (i - 1);
             });
             return true;
@@ -957,7 +981,7 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
     }
     const int w = (int)blockIdx.x - few_cuts;
     if (!find_item<ROWS, true>(p, w / PIECES, it)) return;
-    const int first = w % PIECES * kJoinRows, end = min(first + kJoinRows, it.s.rows - it.unit * ROWS);
+    const int first = w % PIECES * JOIN, end = min(first + JOIN, it.s.rows - it.unit * ROWS);
     if (first >= end) return;
     batch_join_rows<T, D, ROWS>(p, it, first, end, it.shares, p.part[1], p.slots,
                                 [&](int i) __attribute__((always_inline)) { return it.slot + i * p.Hkv; });
@@ -976,37 +1000,37 @@ __device__ __forceinline__ void batch_many(const BatchParams &p, int block, Batc
 __device__ __forceinline__ void batch_many(const BatchParams &p, int block, FwdSplitSmem &sm) {
     batch_many_parts(p, block, sm);
 }
-template <class Pol, class Many, int NW>
+template <class Pol, class Many, int NW, int THREADS>
 __device__ __forceinline__ void batch_both_body(const BatchParams &p, int few_groups) {
     __shared__ __attribute__((aligned(16))) union {
         BatchFewSmem<Pol, NW> few;
         Many many;
     } sm;
     if ((int)blockIdx.x < few_groups) {
-        batch_few_body<Pol, NW, 256>(p, blockIdx.x, sm.few);
+        batch_few_body<Pol, NW, THREADS>(p, blockIdx.x, sm.few);
     } else {
         batch_many(p, (int)blockIdx.x - few_groups, sm.many);
     }
 }
 
-#define MXFA_BATCH(SUFFIX, POL, MANY, NW, WPS, BOTH_NW)                                               \
-    extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {  \
-        __shared__ __attribute__((aligned(16))) BatchFewSmem<POL, NW> sm;                             \
-        batch_few_body<POL, NW, 64 * NW>(p, blockIdx.x, sm);                                          \
-    }                                                                                                 \
-    extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) { \
-        __shared__ __attribute__((aligned(16))) MANY sm;                                              \
-        batch_many(p, blockIdx.x, sm);                                                                \
-    }                                                                                                 \
-    extern "C" __global__ __launch_bounds__(256, WPS) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
-        batch_both_body<POL, MANY, BOTH_NW>(p, few_groups);                                           \
-    }                                                                                                 \
+#define MXFA_BATCH(SUFFIX, POL, MANY, THREADS, WPS, NW, BOTH_NW)                                             \
+    extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {         \
+        __shared__ __attribute__((aligned(16))) BatchFewSmem<POL, NW> sm;                                    \
+        batch_few_body<POL, NW, 64 * NW>(p, blockIdx.x, sm);                                                 \
+    }                                                                                                        \
+    extern "C" __global__ __launch_bounds__(THREADS, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) {   \
+        __shared__ __attribute__((aligned(16))) MANY sm;                                                     \
+        batch_many(p, blockIdx.x, sm);                                                                       \
+    }                                                                                                        \
+    extern "C" __global__ __launch_bounds__(THREADS, WPS) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
+        batch_both_body<POL, MANY, BOTH_NW, THREADS>(p, few_groups);                                         \
+    }                                                                                                        \
     extern "C" __global__ __launch_bounds__(256) void mxfa_batch_##SUFFIX##_join(BatchParams p, int few_groups) { \
-        batch_join<POL::T, POL::D>(p, few_groups);                                                    \
+        batch_join<POL::T, POL::D>(p, few_groups);                                                           \
     }
-MXFA_BATCH(b64, PolRows<64>, BatchManySmem<PolRows<64>>, 8, 3, 3)
-MXFA_BATCH(b128, PolRows<128>, BatchManySmem<PolRows<128>>, 4, 2, 2)
-MXFA_BATCH(f64, PolF32, FwdSplitSmem, 4, 3, 1)
+MXFA_BATCH(b64, PolRows<64>, BatchManySmem<PolRows<64>>, 256, 3, 8, 3)
+MXFA_BATCH(b128, PolRows<128>, BatchManySmem<PolRows<128>>, 256, 2, 4, 2)
+MXFA_BATCH(f64, PolF32, FwdSplitSmem, 64 * kBatchF32Waves, 4, 4, 2)
 #undef MXFA_BATCH
 #endif
 
@@ -1043,18 +1067,19 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     batch_forms(&p, dtype_bf16, f);
     p.part[0] = static_cast<float *>(workspace);
     p.part[1] = p.part[0] + batch_part_floats(f[0].slots, f[0].rows, p.d);
+    const int threads = dtype_bf16 ? 256 : 64 * kBatchF32Waves;
     hipError_t e;
     int few_groups = (int)f[0].groups;
     void *args[] = {&p, &few_groups};
     if (f[1].groups == 0) {
         e = launch_kernel(id[0], dim3(few_groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
     } else if (few_groups == 0) {
-        e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(256), args, stream);
+        e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
     } else {
-        e = launch_kernel(id[3], dim3((unsigned)(few_groups + f[1].groups)), dim3(256), args, stream);
+        e = launch_kernel(id[3], dim3((unsigned)(few_groups + f[1].groups)), dim3(threads), args, stream);
     }
-    int cuts = (int)f[0].joins;
-    const unsigned joins = (unsigned)(cuts + f[1].joins * (f[1].rows / kJoinRows));
+    int cuts = (int)f[0].joins * kFewJoins;
+    const unsigned joins = (unsigned)(cuts + f[1].joins * (f[1].rows / join_rows(p.d)));
     if (e != hipSuccess || joins == 0) return e;
     void *jargs[] = {&p, &cuts};
     return launch_kernel(id[2], dim3(joins), dim3(256), jargs, stream);

@@ -13,10 +13,14 @@ namespace mxfa {
 
 constexpr int kBatchFew = 16;  // rows of the few-row form's units
 constexpr int kCusPerXcd = 32;  // of 8 XCDs
-constexpr int kJoinRows = 32;  // rows of a work-group of the join
-// Rows of the many-row form's units: 16 per wave and query tile.
-__host__ __device__ constexpr int batch_tiles(bool bf16) { return bf16 ? 2 : 1; }
-__host__ __device__ constexpr int batch_many_rows(bool bf16) { return 64 * batch_tiles(bf16); }
+// Rows of a work-group of the join: as many of the many-row form's as it has
+// groups of D / 4 threads; a quarter of the few-row form's, whose sequences may be
+// in a hundred pieces.
+__host__ __device__ constexpr int join_rows(int d) { return 1024 / d; }
+constexpr int kFewJoins = 4;
+// Rows of the many-row form's units: 4 waves of 2 query tiles (bf16), 8 of one.
+constexpr int kBatchF32Waves = 8;
+__host__ __device__ constexpr int batch_many_rows(bool bf16) { return bf16 ? 128 : 16 * kBatchF32Waves; }
 
 // The workspace holds the shares of split units: `slots` of them, each ROWS rows
 // of D floats and their (max, sum) pairs.
@@ -110,17 +114,23 @@ __host__ __device__ inline float seq_stages(const BatchParams &p, const BatchSeq
 // A sequence's items at a quota, the most stages of a share: its first `whole`
 // units are whole items, the others are cut into `shares` each. Counts over all
 // KV heads: `split` units that are cut, their `slots` shares, and all items.
+//
+// Units of up to kManyWhole stages are not cut: the join's launch costs about as
+// much as half of their time (1000 tokens of 14/2 heads, d = 64, 16 stages at most:
+// 12 us whole, 20 in shares of 8).
+constexpr unsigned kManyWhole = 16;
 struct SeqItems {
     int whole, shares, split, slots, items;
 };
 template <int ROWS>
 __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchSeq &b, unsigned quota) {
     SeqItems n{b.units, 1, 0, 0, 0};
-    if (b.units > 0 && (unsigned)b.stages > quota) {
+    const unsigned most = more_of(quota, kManyWhole);
+    if (b.units > 0 && (unsigned)b.stages > most) {
         n.shares = (int)(((unsigned)b.stages + quota - 1) / quota);
-        // unit u ends with row (u + 1) ROWS - 1, which sees more than 64 quota
-        // positions from row t group on, t = 64 quota - pos; the last one does
-        const long long t = 64LL * quota - b.pos;
+        // unit u ends with row (u + 1) ROWS - 1, which sees more than 64 most
+        // positions from row t group on, t = 64 most - pos; the last one does
+        const long long t = 64LL * most - b.pos;
         n.whole = t <= 0 ? 0 : (int)less_of((unsigned long long)t * (unsigned)p.group / ROWS, (unsigned long long)(b.units - 1));
     }
     n.split = (b.units - n.whole) * p.Hkv;
@@ -208,7 +218,7 @@ __host__ __device__ inline void share_stages(const BatchItem &it, int n, int &lo
 // Work-groups resident at once: the few-row form's have a CU each, the many-row
 // form's share one in twos or threes.
 constexpr int kBatchCus = 256;
-inline int batch_resident(int d) { return d == 64 ? 3 * kBatchCus : 2 * kBatchCus; }
+inline int batch_resident(int dtype_bf16, int d) { return dtype_bf16 && d == 64 ? 3 * kBatchCus : 2 * kBatchCus; }
 
 // Which forms a call launches, by what the host knows: the few-row form alone
 // where no sequence can have more rows; the many-row form alone where one
@@ -254,7 +264,7 @@ inline BatchForm batch_few_form(BatchParams *p) {
 inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     BatchForm f;
     f.rows = batch_many_rows(dtype_bf16);
-    p->resident = batch_resident(p->d);
+    p->resident = batch_resident(dtype_bf16, p->d);
     // Beside the few-row form's work-groups a CU holds two of these. The host
     // knows how many sequences can be of few rows: the others have max_q tokens at
     // most. us, 14/2 heads, d = 64: 4 chunks and 28 tokens 57.6 (61 by three a CU);
@@ -267,7 +277,7 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     p->per_resident = 1.0f / (float)p->resident;
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;
-    if (batch_most_stages(*p) <= p->least[1]) {  // nothing to split
+    if (batch_most_stages(*p) <= kManyWhole) {  // nothing to split
         f.groups = units;
         f.joins = f.slots = 0;
     } else {
@@ -280,12 +290,12 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     return f;
 }
 
-// The least stages of a share or run: one for each of the few-row form's waves; 8
-// of the many-row form's, below which the join costs more than the split saves.
+// The least stages of a share or run: one for each of the few-row form's waves; 4
+// of the many-row form's.
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
     p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
-    p->least[1] = 8;
+    p->least[1] = 4;
 }
 
 }  // namespace mxfa
