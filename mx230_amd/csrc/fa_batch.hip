@@ -203,10 +203,11 @@ __device__ __forceinline__ BatchSeq seq_of_lane(const BatchSeq &b, int l) {
     return BatchSeq{of(b.q0), of(b.pos), of(b.rows), of(b.keys), of(b.units), of(b.stages)};
 }
 
-// Item `w` of the many-row form (JOIN: split unit `w`), found by every wave for
-// itself: a lane per sequence, again over them where there are more than 64
-// (the rules: fa_batch_items.h). False past the last one.
-template <int ROWS, bool JOIN>
+// Item `w` of the many-row form, found by every wave for itself: a lane per
+// sequence, again over them where there are more than 64 (the rules:
+// fa_batch_items.h). False past the last one. The work-group of item 0 also
+// notes the count of split units for the join.
+template <int ROWS>
 __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem &it) {
     const int lane = threadIdx.x & 63;
     BatchSeq b = batch_seq<false, ROWS>(p, lane);
@@ -221,12 +222,17 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
         for (int s0 = 64; s0 < p.n_seq; s0 += 64) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s0 + lane), q).items;
         return (float)wave_sum(n);
     });
-    int before = 0, slots = 0;
+    if (w == 0 && p.splits > 0) {
+        int n = seq_items<ROWS>(p, b, quota).split;
+        for (int s0 = 64; s0 < p.n_seq; s0 += 64) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s0 + lane), quota).split;
+        n = wave_sum(n);
+        if (threadIdx.x == 0) p.notes[1][0] = n;
+    }
+    int before = 0, slots = 0, splits = 0;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
         if (s0 > 0) b = batch_seq<false, ROWS>(p, s0 + lane);
         const SeqItems n = seq_items<ROWS>(p, b, quota);
-        const int per = JOIN ? n.split : n.items;
-        const int upto = wave_prefix(per), slots_upto = wave_prefix(n.slots);
+        const int upto = wave_prefix(n.items), slots_upto = wave_prefix(n.slots), splits_upto = wave_prefix(n.split);
         const unsigned long long at = __builtin_amdgcn_ballot_w64(before + upto > w);
         if (at != 0) {
             const int l = __builtin_ctzll(at);
@@ -234,10 +240,17 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
             it.seq = s0 + l;
             it.s = seq_of_lane(b, l);
             const SeqItems m{of(n.whole), of(n.shares), of(n.split), of(n.slots), of(n.items)};
-            return batch_item<JOIN>(p, m, slots + of(slots_upto - n.slots), w - before - of(upto - per), it);
+            if (!batch_item(p, m, slots + of(slots_upto - n.slots), splits + of(splits_upto - n.split),
+                            w - before - of(upto - n.items), it))
+                return false;
+            if (it.shares > 1 && it.share == 0 && it.split < p.splits && threadIdx.x == 0)
+                reinterpret_cast<ManyNote *>(p.notes[1])[1 + it.split] =
+                    ManyNote{it.shares, it.slot, it.s.q0, it.s.rows, it.unit, it.head, {0, 0}};
+            return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
         slots += __builtin_amdgcn_readlane(slots_upto, 63);
+        splits += __builtin_amdgcn_readlane(splits_upto, 63);
     }
     return false;
 }
@@ -507,7 +520,11 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
     const unsigned all = few_line(p), run = few_run(p, all);
     unsigned x = (unsigned)(g / p.Hkv) * run;
     const unsigned x1 = min(x + run, all);
-    if (x >= x1) return;
+    // what the join of a sequence that the run ends in reads
+    auto note = [&](const FewNote &n) __attribute__((always_inline)) {
+        if (threadIdx.x == 0 && p.few_groups > 1) reinterpret_cast<FewNote *>(p.notes[0])[g] = n;
+    };
+    if (x >= x1) return note(FewNote{0, 0, 0, 0});
     BatchItem it;
     it.head = g % p.Hkv;
     it.unit = 0;
@@ -515,6 +532,7 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
         it.seq = seq;
         it.s = s;
         const FewPiece f = few_piece(x, x1, u0, u1, g);
+        if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, s.q0, s.rows, 0});
         batch_few_piece<Pol, NW, THREADS>(p, it, f.lo, f.hi, f.slot, sm);
         x = f.end;
         if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
@@ -549,7 +567,7 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    if (!find_item<ROWS, false>(p, batch_order(p, block), it)) return;
+    if (!find_item<ROWS>(p, batch_order(p, block), it)) return;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
 
     const int r0 = it.unit * ROWS, rw = r0 + wave * 16 * QT;  // the unit's and the wave's first row
@@ -694,7 +712,7 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     BatchItem it;
-    if (!find_item<ROWS, false>(p, batch_order(p, block), it)) return;
+    if (!find_item<ROWS>(p, batch_order(p, block), it)) return;
     const float *K = static_cast<const float *>(p.k) + it.head * D, *V = static_cast<const float *>(p.v) + it.head * D;
 
     const int r0 = it.unit * ROWS, rw = r0 + wave * 16, r = rw + l16;
@@ -952,39 +970,38 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
     }
 }
 
-// Grid: the cuts of the few-row form's lines, then the pieces of the split units
-// that the many-row form may have, kJoinRows rows each.
+// Grid: the cuts of the few-row form's lines (the work-groups but the last run's),
+// then the pieces of the split units that the many-row form may have.
 template <class T, int D>
 __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
     constexpr int ROWS = batch_many_rows(sizeof(T) == 2), JOIN = join_rows(D), PIECES = ROWS / JOIN;
     BatchItem it;
     if ((int)blockIdx.x < few_cuts) {
-        // the cut at the end of run `cut`; the first cut through a sequence joins it
-        const int heads = p.Hkv, j = (int)blockIdx.x / kFewJoins, first = (int)blockIdx.x % kFewJoins * (kBatchFew / kFewJoins);
-        const int cut = j / heads;
-        it.head = j % heads;
+        // the cut at the end of work-group g's run
+        const int heads = p.Hkv, g = (int)blockIdx.x / kFewJoins, first = (int)blockIdx.x % kFewJoins * (kBatchFew / kFewJoins);
+        const FewNote n = reinterpret_cast<const FewNote *>(p.notes[0])[g];
+        const int end = min(first + kBatchFew / kFewJoins, n.rows);
+        if (n.parts < 2 || first >= end) return;
+        const int run = g / heads, head = g - run * heads;
+        it.head = head;
         it.unit = 0;
-        const unsigned all = few_line(p), run = few_run(p, all), x = (unsigned)(cut + 1) * run;
-        if (x >= all) return;
-        few_walk(p, x, [&](int seq, const BatchSeq &s, unsigned u0, unsigned u1) __attribute__((always_inline)) {
-            if (u0 >= x || u0 / run != (unsigned)cut) return true;
-            it.seq = seq;
-            it.s = s;
-            const int head = it.head, S = (int)((u1 - 1) / run) - cut + 1, end = min(first + kBatchFew / kFewJoins, s.rows);
-            if (first >= end) return true;
-            batch_join_rows<T, D, kBatchFew>(p, it, first, end, S, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
-                return i == 0 ? few_first_slot(cut, heads, head) : few_next_slot(cut, heads, head) + 2 * heads * (i - 1);
-            });
-            return true;
+        it.s.q0 = n.q0;
+        batch_join_rows<T, D, kBatchFew>(p, it, first, end, n.parts, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
+            return i == 0 ? few_first_slot(run, heads, head) : few_next_slot(run, heads, head) + 2 * heads * (i - 1);
         });
         return;
     }
-    const int w = (int)blockIdx.x - few_cuts;
-    if (!find_item<ROWS, true>(p, w / PIECES, it)) return;
-    const int first = w % PIECES * JOIN, end = min(first + JOIN, it.s.rows - it.unit * ROWS);
+    const int w = (int)blockIdx.x - few_cuts, unit = w / PIECES;
+    const int count = p.notes[1][0];
+    const ManyNote n = reinterpret_cast<const ManyNote *>(p.notes[1])[1 + unit];
+    if (unit >= count || !note_holds(p, n, ROWS)) return;
+    const int first = w % PIECES * JOIN, end = min(first + JOIN, n.rows - n.unit * ROWS);
     if (first >= end) return;
-    batch_join_rows<T, D, ROWS>(p, it, first, end, it.shares, p.part[1], p.slots,
-                                [&](int i) __attribute__((always_inline)) { return it.slot + i * p.Hkv; });
+    it.head = n.head;
+    it.unit = n.unit;
+    it.s.q0 = n.q0;
+    batch_join_rows<T, D, ROWS>(p, it, first, end, n.shares, p.part[1], p.slots,
+                                [&](int i) __attribute__((always_inline)) { return n.slot + i * p.Hkv; });
 }
 
 // Both forms in one launch: the few-row form's work-groups first, each wave's
@@ -1037,7 +1054,7 @@ MXFA_BATCH(f64, PolF32, FwdSplitSmem, 64 * kBatchF32Waves, 4, 4, 2)
 // The forms of a call; groups = 0: not launched.
 static void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2]) {
     batch_plan(p, dtype_bf16);
-    f[0] = f[1] = BatchForm{0, 0, 0, 0};
+    f[0] = f[1] = BatchForm{0, 0, 0, 0, 0};
     if (p->few_rows > 0) f[0] = batch_few_form(p);
     if (batch_may_be_many(*p)) f[1] = batch_many_form(p, dtype_bf16);
 }
@@ -1047,7 +1064,7 @@ size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
     BatchForm f[2];
     batch_forms(&p, dtype_bf16, f);
     size_t n = 0;
-    for (const BatchForm &x : f) n += batch_part_floats(x.slots, x.rows, p.d);
+    for (const BatchForm &x : f) n += batch_slot_floats(x.slots, x.rows, p.d) + (size_t)x.notes;
     return std::max<size_t>(n * sizeof(float), 16);
 }
 
@@ -1065,8 +1082,13 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
     BatchForm f[2];
     batch_forms(&p, dtype_bf16, f);
-    p.part[0] = static_cast<float *>(workspace);
-    p.part[1] = p.part[0] + batch_part_floats(f[0].slots, f[0].rows, p.d);
+    float *next = static_cast<float *>(workspace);
+    for (int i = 0; i < 2; ++i) {  // (notes of 16 and 32 bytes, slots of a multiple of that)
+        p.part[i] = next;
+        next += batch_slot_floats(f[i].slots, f[i].rows, p.d);
+        p.notes[i] = reinterpret_cast<int *>(next);
+        next += f[i].notes;
+    }
     const int threads = dtype_bf16 ? 256 : 64 * kBatchF32Waves;
     hipError_t e;
     int few_groups = (int)f[0].groups;

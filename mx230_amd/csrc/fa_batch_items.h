@@ -23,10 +23,19 @@ constexpr int kBatchF32Waves = 8;
 __host__ __device__ constexpr int batch_many_rows(bool bf16) { return bf16 ? 128 : 16 * kBatchF32Waves; }
 
 // The workspace holds the shares of split units: `slots` of them, each ROWS rows
-// of D floats and their (max, sum) pairs.
-__host__ __device__ constexpr size_t batch_part_floats(long long slots, int rows, int d) {
+// of D floats and their (max, sum) pairs; then what the join reads about them,
+// `notes` ints.
+__host__ __device__ constexpr size_t batch_slot_floats(long long slots, int rows, int d) {
     return (size_t)slots * rows * (d + 2);
 }
+// The join's notes. Few rows: per work-group the pieces of the sequence that its
+// run ends in (0: none) and its rows. Many rows: the count of split units, then each.
+struct FewNote {
+    int parts, q0, rows, unused;
+};
+struct ManyNote {
+    int shares, slot, q0, rows, unit, head, unused[2];
+};
 
 template <class X>
 __host__ __device__ inline X less_of(X a, X b) {
@@ -94,6 +103,10 @@ __host__ __device__ inline FewPiece few_piece(unsigned x, unsigned x1, unsigned 
     f.slot = x > u0 ? 2 * g : f.end < u1 ? 2 * g + 1 : -1;
     return f;
 }
+// The pieces of the sequence at [u0, u1).
+__host__ __device__ inline int few_parts(unsigned run, unsigned u0, unsigned u1) {
+    return (int)((u1 - 1) / run - u0 / run) + 1;
+}
 // The slots of a sequence's pieces, by the run it begins in: the first piece's
 // and then one each 2 Hkv on from the second's.
 __host__ __device__ inline int few_first_slot(int run, int heads, int head) { return 2 * (run * heads + head) + 1; }
@@ -144,7 +157,7 @@ __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchS
 // work-groups that are resident at once (p.resident), it is about the least one
 // by which their shares still do, found by raising an even share's (INT_MAX,
 // no split, where that takes too long); else one and a half even shares. It
-// depends on lengths alone, so the join finds the same one.
+// depends on lengths alone.
 constexpr float kManySplit = 1.5f;
 template <class Count>
 __host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, Count count) {
@@ -164,23 +177,24 @@ __host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all,
 struct BatchItem {
     BatchSeq s;
     int seq, head, unit, share, shares;
-    int slot;  // of share 0 (the join) or of this share, where shares > 1
+    int slot;   // of this share, where shares > 1
+    int split;  // the unit's number among the split ones
 };
 
-// Item i of a sequence (JOIN: its i-th split unit) whose shares' slots begin at
-// `slot`. Items: the split units (the last, heaviest one first) x shares x KV
+// Item i of a sequence whose shares' slots begin at `slot` and split units at
+// `split`. Items: the split units (the last, heaviest one first) x shares x KV
 // heads, then the whole ones x KV heads, so that neighbouring work-groups, which
 // the dispatcher spreads over the XCDs, have the heads and an XCD's share of
 // them the same head's keys. False where the share has no slot, which only a
 // cu_q that gives rows to several sequences can bring about.
-template <bool JOIN>
-__host__ __device__ inline bool batch_item(const BatchParams &p, const SeqItems &n, int slot, int item, BatchItem &it) {
+__host__ __device__ inline bool batch_item(const BatchParams &p, const SeqItems &n, int slot, int split, int item,
+                                           BatchItem &it) {
     const unsigned heads = p.Hkv;
     unsigned i = item;
-    it.share = 0;
+    it.share = it.split = 0;
     it.shares = n.shares;
-    it.slot = slot;
-    if (!JOIN && i >= (unsigned)n.slots) {
+    it.slot = slot + item;
+    if (i >= (unsigned)n.slots) {
         i -= n.slots;
         it.shares = 1;
         it.unit = n.whole - 1 - (int)(i / heads);
@@ -189,16 +203,19 @@ __host__ __device__ inline bool batch_item(const BatchParams &p, const SeqItems 
     }
     const unsigned per_unit = i / heads;
     it.head = i - per_unit * heads;
-    if (JOIN) {
-        it.slot += per_unit * n.shares * heads + it.head;  // the unit's shares are `heads` apart
-        it.unit = it.s.units - 1 - (int)per_unit;
-        return it.slot + (n.shares - 1) * p.Hkv < p.slots;
-    }
     const unsigned u = per_unit / (unsigned)n.shares;
     it.share = per_unit - u * n.shares;
     it.unit = it.s.units - 1 - (int)u;
-    it.slot += item;
+    it.split = split + (int)(u * heads) + it.head;
     return it.slot < p.slots;
+}
+
+// Whether a note of the join is one that find_item's items write (whatever the
+// workspace holds where none was written).
+__host__ __device__ inline bool note_holds(const BatchParams &p, const ManyNote &n, int ROWS) {
+    return n.shares > 1 && n.slot >= 0 && (long long)n.slot + (long long)(n.shares - 1) * p.Hkv < p.slots && n.q0 >= 0 &&
+           n.rows > 0 && n.q0 + (long long)(n.rows - 1) / p.group < p.n_tok && n.unit >= 0 &&
+           (long long)n.unit * ROWS < n.rows && n.head >= 0 && n.head < p.Hkv;
 }
 
 // The share's stages of the unit's n.
@@ -237,7 +254,7 @@ inline long long batch_most_stages(const BatchParams &p) { return (((long long)p
 // A form's launch: its work-groups and the join's, and the workspace's slots.
 struct BatchForm {
     int rows;
-    long long groups, joins, slots;
+    long long groups, joins, slots, notes;
 };
 
 // Few rows: a CU's work-group for each run of the line, at least one per KV head;
@@ -252,6 +269,7 @@ inline BatchForm batch_few_form(BatchParams *p) {
     // a cut between each two runs
     f.joins = p->few_groups > 1 ? f.groups - p->Hkv : 0;
     f.slots = f.joins > 0 ? 2 * f.groups : 0;
+    f.notes = f.joins > 0 ? f.groups * (long long)(sizeof(FewNote) / sizeof(int)) : 0;
     return f;
 }
 
@@ -287,6 +305,8 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
         f.joins = split;
     }
     p->slots = (int)f.slots;
+    p->splits = (int)f.joins;
+    f.notes = f.joins > 0 ? (f.joins + 1) * (long long)(sizeof(ManyNote) / sizeof(int)) : 0;
     return f;
 }
 

@@ -48,10 +48,12 @@ struct BatchParams {
     // KV head) of a sequence that the few-row form takes (0: it takes none) and
     // its work-groups per KV head; per form (few, many) the least stages of a run
     // or share; the many-row form's work-groups resident at once, 1 / that, and
-    // the slots of its shares; the forms' parts of the workspace
-    int few_rows, few_groups, least[2], resident, slots;
+    // the slots of its shares and the split units there can be; the forms' parts of
+    // the workspace
+    int few_rows, few_groups, least[2], resident, slots, splits;
     float per_resident;
     float *part[2];
+    int *notes[2];
 };
 
 struct PagesParams {

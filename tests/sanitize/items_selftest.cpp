@@ -35,9 +35,10 @@ static int g_fail = 0;
         }                                                             \
     } while (0)
 
-// find_item of the kernels with a loop in the place of a wave.
-template <int ROWS, bool JOIN>
-static bool find(const BatchParams &p, int w, BatchItem &it) {
+// find_item of the kernels with a loop in the place of a wave, and the count of
+// split units.
+template <int ROWS>
+static bool find(const BatchParams &p, int w, BatchItem &it, int *total = nullptr) {
     float all = 0, units = 0;
     for (int s = 0; s < p.n_seq; ++s) {
         const BatchSeq b = batch_seq<false, ROWS>(p, s);
@@ -49,20 +50,23 @@ static bool find(const BatchParams &p, int w, BatchItem &it) {
         for (int s = 0; s < p.n_seq; ++s) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s), q).items;
         return (float)n;
     });
-    int before = 0, slots = 0;
+    int before = 0, slots = 0, splits = 0;
+    bool found = false;
     for (int s = 0; s < p.n_seq; ++s) {
         const BatchSeq b = batch_seq<false, ROWS>(p, s);
         const SeqItems n = seq_items<ROWS>(p, b, quota);
-        const int per = JOIN ? n.split : n.items;
-        if (w < before + per) {
+        if (w >= before && w < before + n.items) {
             it.seq = s;
             it.s = b;
-            return batch_item<JOIN>(p, n, slots, w - before, it);
+            found = batch_item(p, n, slots, splits, w - before, it);
+            if (total == nullptr) return found;
         }
-        before += per;
+        before += n.items;
         slots += n.slots;
+        splits += n.split;
     }
-    return false;
+    if (total != nullptr) *total = splits;
+    return found;
 }
 
 static void check_bounds(const BatchParams &p, const BatchForm &f, const BatchItem &it) {
@@ -87,7 +91,7 @@ static void check_many(BatchParams p, int bf16, bool sound) {
     const long long step = sound ? 1 : std::max(1LL, groups / 400);
     for (long long w = 0; w < groups; w += step) {
         BatchItem it{};
-        if (!find<ROWS, false>(p, (int)w, it)) {
+        if (!find<ROWS>(p, (int)w, it)) {
             if (sound) break;
             continue;
         }
@@ -101,26 +105,39 @@ static void check_many(BatchParams p, int bf16, bool sound) {
     }
     const long long joins = f.joins;
     if (!sound) {
-        for (long long w = 0; w < joins; w += std::max(1LL, joins / 200)) {
-            BatchItem it{};
-            if (!find<ROWS, true>(p, (int)w, it)) continue;
-            check_bounds(p, f, it);
-            CHECK(it.slot + (it.shares - 1) * p.Hkv < f.slots, "last slot of %d + %d", it.slot, it.shares);
+        // what a note may hold is checked before it is used
+        std::mt19937 r(3);
+        for (int i = 0; i < 2000; ++i) {
+            ManyNote n;
+            for (int *x = &n.shares; x < &n.shares + 8; ++x) {
+                const int k = (int)(r() % 4);
+                *x = k == 0 ? (int)r() : k == 1 ? (int)(r() % 300) : k == 2 ? 0 : INT_MAX;
+            }
+            if (!note_holds(p, n, f.rows)) continue;
+            CHECK(n.slot >= 0 && n.slot + (n.shares - 1LL) * p.Hkv < f.slots, "slots %d + %d", n.slot, n.shares);
+            CHECK(n.q0 >= 0 && n.q0 + (long long)(n.rows - 1) / p.group < p.n_tok, "rows %d from %d", n.rows, n.q0);
         }
         return;
     }
     BatchItem past{};
-    CHECK(!(find<ROWS, false>(p, (int)groups, past)), "more items than work-groups (%lld)", groups);
+    CHECK(!(find<ROWS>(p, (int)groups, past)), "more items than work-groups (%lld)", groups);
     size_t want = 0, split = 0;
     for (int s = 0; s < p.n_seq; ++s) want += (size_t)batch_seq<false, ROWS>(p, s).units * p.Hkv;
     CHECK(units.size() == want, "%zu units of %zu", units.size(), want);
-    std::map<int, BatchItem> joined;
-    for (long long w = 0;; ++w) {
-        BatchItem it{};
-        if (!find<ROWS, true>(p, (int)w, it)) break;
-        CHECK(w < joins, "more split units than work-groups (%lld)", joins);
-        joined[it.slot] = it;
+    int total = 0;
+    find<ROWS>(p, 0, past, &total);
+    CHECK(total <= joins, "%d split units, %lld joins", total, joins);
+    std::map<int, BatchItem> joined;  // by number: what share 0 notes
+    for (auto &[key, v] : units) {
+        for (auto &x : v) {
+            if (x.shares < 2 || x.share != 0) continue;
+            CHECK(x.split >= 0 && x.split < total, "split unit %d of %d", x.split, total);
+            CHECK(joined.emplace(x.split, x).second, "split unit %d twice", x.split);
+            const ManyNote n{x.shares, x.slot, x.s.q0, x.s.rows, x.unit, x.head, {0, 0}};
+            CHECK(note_holds(p, n, f.rows), "the note of split unit %d", x.split);
+        }
     }
+    CHECK((int)joined.size() == total, "%zu joins for %d split units", joined.size(), total);
     for (auto &[key, v] : units) {
         const BatchItem &a = v[0];
         CHECK((int)v.size() == a.shares, "%zu of %d shares", v.size(), a.shares);
@@ -138,9 +155,6 @@ static void check_many(BatchParams p, int bf16, bool sound) {
             end = hi;
             if (a.shares > 1 && i == 0) {
                 ++split;
-                auto j = joined.find(s->slot);
-                CHECK(j != joined.end() && j->second.unit == a.unit && j->second.head == a.head &&
-                          j->second.seq == a.seq && j->second.shares == a.shares, "the join of slot %d", s->slot);
             }
         }
         CHECK(end == a.s.stages, "stages to %d of %d", end, a.s.stages);
@@ -197,11 +211,12 @@ static void check_few(BatchParams p, bool sound) {
     for (int j = 0; j < f.joins; ++j) {
         const int cut = j / p.Hkv, head = j % p.Hkv;
         const unsigned long long x = (unsigned long long)(cut + 1) * run;
+        // the note of work-group j: the sequence its run ends in, if it begins there
         if (x >= all) continue;
         int s = 0;
         while (u[s + 1] <= x) ++s;
         if (u[s] >= x || u[s] / run != (unsigned)cut) continue;
-        const int S = (int)((u[s + 1] - 1) / run) - cut + 1;
+        const int S = few_parts(run, u[s], u[s + 1]);
         ++joined[{s, head}];
         const auto &v = pieces[{s, head}];
         CHECK((int)v.size() == S, "%zu pieces, the join reads %d", v.size(), S);
