@@ -127,23 +127,17 @@ __host__ __device__ inline float seq_stages(const BatchParams &p, const BatchSeq
 // A sequence's items at a quota, the most stages of a share: its first `whole`
 // units are whole items, the others are cut into `shares` each. Counts over all
 // KV heads: `split` units that are cut, their `slots` shares, and all items.
-//
-// Units of up to kManyWhole stages are not cut: the join's launch costs about as
-// much as half of their time (1000 tokens of 14/2 heads, d = 64, 16 stages at most:
-// 12 us whole, 20 in shares of 8).
-constexpr unsigned kManyWhole = 16;
 struct SeqItems {
     int whole, shares, split, slots, items;
 };
 template <int ROWS>
 __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchSeq &b, unsigned quota) {
     SeqItems n{b.units, 1, 0, 0, 0};
-    const unsigned most = more_of(quota, kManyWhole);
-    if (b.units > 0 && (unsigned)b.stages > most) {
+    if (b.units > 0 && (unsigned)b.stages > quota) {
         n.shares = (int)(((unsigned)b.stages + quota - 1) / quota);
-        // unit u ends with row (u + 1) ROWS - 1, which sees more than 64 most
-        // positions from row t group on, t = 64 most - pos; the last one does
-        const long long t = 64LL * most - b.pos;
+        // unit u ends with row (u + 1) ROWS - 1, which sees more than 64 quota
+        // positions from row t group on, t = 64 quota - pos; the last one does
+        const long long t = 64LL * quota - b.pos;
         n.whole = t <= 0 ? 0 : (int)less_of((unsigned long long)t * (unsigned)p.group / ROWS, (unsigned long long)(b.units - 1));
     }
     n.split = (b.units - n.whole) * p.Hkv;
@@ -153,14 +147,18 @@ __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchS
 }
 
 // The quota, from the sums of seq_stages and of the units over the sequences (of
-// one KV head) and the count of all items at a quota. Where the units fit the
+// one KV head), whether any has more than p.whole stages, and the count of all items
+// at a quota. Without one nothing is split: that takes about the join's time, or
+// less (bf16, 1000 tokens of 14/2 heads: 12 us whole, 20 in shares of 8 stages).
+// Where the units fit the
 // work-groups that are resident at once (p.resident), it is about the least one
 // by which their shares still do, found by raising an even share's (INT_MAX,
 // no split, where that takes too long); else one and a half even shares. It
 // depends on lengths alone.
 constexpr float kManySplit = 1.5f;
 template <class Count>
-__host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, Count count) {
+__host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, bool any_long, Count count) {
+    if (!any_long) return INT_MAX;
     all = less_of(all * (float)p.Hkv * 1.001f, 1e18f);  // (more than its rounding)
     const float resident = (float)p.resident, even = less_of(all * p.per_resident + 1.0f, 1e9f);
     const float least = (float)p.least[1];
@@ -295,7 +293,7 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     p->per_resident = 1.0f / (float)p->resident;
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;
-    if (batch_most_stages(*p) <= kManyWhole) {  // nothing to split
+    if (batch_most_stages(*p) <= p->whole) {  // nothing to split
         f.groups = units;
         f.joins = f.slots = 0;
     } else {
@@ -311,11 +309,13 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
 }
 
 // The least stages of a share or run: one for each of the few-row form's waves; 4
-// of the many-row form's.
+// of the many-row form's, whose units all stay whole if none has more than
+// p.whole (a stage takes 0.6 us in bf16, 2.5 in fp32, and the join 5).
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
     p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
     p->least[1] = 4;
+    p->whole = dtype_bf16 ? 16 : 4;
 }
 
 }  // namespace mxfa

@@ -47,10 +47,10 @@ struct BatchParams {
     // attention (fa_batch_items.h): the most rows (new tokens x query heads of a
     // KV head) of a sequence that the few-row form takes (0: it takes none) and
     // its work-groups per KV head; per form (few, many) the least stages of a run
-    // or share; the many-row form's work-groups resident at once, 1 / that, and
-    // the slots of its shares and the split units there can be; the forms' parts of
-    // the workspace
-    int few_rows, few_groups, least[2], resident, slots, splits;
+    // or share; of the many-row form: the stages up to which nothing is split, the
+    // work-groups resident at once, 1 / that, the slots of its shares and the split
+    // units there can be; the forms' parts of the workspace and their notes
+    int few_rows, few_groups, least[2], whole, resident, slots, splits;
     float per_resident;
     float *part[2];
     int *notes[2];
