@@ -106,13 +106,12 @@ __device__ __forceinline__ void pages_fork_plan(const PagesParams &p, const int 
                 copy = (len & part) != 0;
             }
         }
-        int total;
-        const int k = need + plan_prefix(copy, sums, &total);
-        need += total;
+        int total;  // (both counts in one, up to kPlan each)
+        const int k = need + (plan_prefix(copy + (no << 16), sums, &total) & 0xffff);
+        need += total & 0xffff;
+        refused += total >> 16;
         // the copy's number, in the child's own row for now
         if (copy) p.table[(long long)children[i] * p.table_stride + (status[i] >> p.bs_shift)] = k;
-        plan_prefix(no, sums, &total);
-        refused += total;
     }
     // the lowest `need` blocks that nobody uses
     int found = 0;
@@ -188,20 +187,32 @@ constexpr int kPlanEach = 8;  // consecutive blocks per thread and turn
 __device__ __forceinline__ void pages_compact_plan(const PagesParams &p, int *new_refs, int *pairs, int *counts) {
     __shared__ int sums[kPlan / 64];
     const int tid = threadIdx.x;
-    int used = 0, live;
-    for (int b = tid; b < p.n_blocks; b += kPlan) used += p.refs[b] > 0;
-    plan_prefix(used, sums, &live);
-    int moved = 0, holes = 0;
-    for (int b0 = 0; b0 < p.n_blocks; b0 += kPlanEach * kPlan) {
-        int r[kPlanEach], nm = 0, nh = 0;
+    int r[kPlanEach], used = 0, live;
+    auto read = [&](int b0) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < kPlanEach; ++e) {
             const int b = b0 + kPlanEach * tid + e;
             r[e] = b < p.n_blocks ? max(p.refs[b], 0) : 0;
-            nm += b < p.n_blocks && b >= live && r[e] > 0;
-            nh += b < live && r[e] == 0;
         }
-        int tm, th, km = moved + plan_prefix(nm, sums, &tm), kh = holes + plan_prefix(nh, sums, &th);
+    };
+    for (int b0 = 0; b0 < p.n_blocks; b0 += kPlanEach * kPlan) {
+        read(b0);
+#pragma unroll
+        for (int e = 0; e < kPlanEach; ++e) used += r[e] > 0;
+    }
+    plan_prefix(used, sums, &live);
+    int moved = 0, holes = 0;
+    for (int b0 = 0; b0 < p.n_blocks; b0 += kPlanEach * kPlan) {
+        if (p.n_blocks > kPlanEach * kPlan) read(b0);  // (else still there)
+        int n = 0;  // moves, and holes from bit 16 on: up to kPlanEach kPlan each
+#pragma unroll
+        for (int e = 0; e < kPlanEach; ++e) {
+            const int b = b0 + kPlanEach * tid + e;
+            n += (b >= live && r[e] > 0) + ((b < live && r[e] == 0) << 16);
+        }
+        int total;
+        const int k = plan_prefix(n, sums, &total);
+        int km = moved + (k & 0xffff), kh = holes + (k >> 16);
 #pragma unroll
         for (int e = 0; e < kPlanEach; ++e) {
             const int b = b0 + kPlanEach * tid + e;
@@ -211,8 +222,8 @@ __device__ __forceinline__ void pages_compact_plan(const PagesParams &p, int *ne
                 new_refs[b] = b < live ? r[e] : 0;
             }
         }
-        moved += tm;
-        holes += th;
+        moved += total & 0xffff;
+        holes += total >> 16;
     }
     __syncthreads();
     for (int j = tid; j < moved; j += kPlan) new_refs[pairs[2 * j + 1]] = p.refs[pairs[2 * j]];
