@@ -545,13 +545,6 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
 
 // ----------------------------------------------------------------- the many rows
 
-// The item of the many-row form's work-group `block`, in the order by which a CU's
-// resident ones have long and short units (cu_order_wg); neighbours in eights
-// (the XCDs) stay together.
-__device__ __forceinline__ int batch_order(const BatchParams &p, int block) {
-    return cu_order_wg(block >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + (block & 7);
-}
-
 template <class Pol>
 struct BatchManySmem {
     typename Pol::T k[2][Pol::ROWS * Pol::D], v[2][Pol::ROWS * Pol::D];

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "fa_cache.h"
+#include "fa_device.h"
 
 namespace mxfa {
 
@@ -208,6 +209,14 @@ __host__ __device__ inline bool batch_item(const BatchParams &p, const SeqItems 
     return it.slot < p.slots;
 }
 
+// The item of the many-row form's work-group `block`, in the order by which a CU's
+// resident ones have long and short units (cu_order_wg); neighbours in eights
+// (the XCDs) stay together. It permutes the resident ones: a launch of more than
+// one a CU has them all (batch_many_form).
+__host__ __device__ inline int batch_order(const BatchParams &p, int block) {
+    return cu_order_wg(block >> 3, kCusPerXcd, p.resident / (8 * kCusPerXcd)) * 8 + (block & 7);
+}
+
 // Whether a note of the join is one that find_item's items write (whatever the
 // workspace holds where none was written).
 __host__ __device__ inline bool note_holds(const BatchParams &p, const ManyNote &n, int ROWS) {
@@ -294,7 +303,7 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;
     if (batch_most_stages(*p) <= p->whole) {  // nothing to split
-        f.groups = units;
+        f.groups = units <= kBatchCus ? units : more_of(units, (long long)p->resident);  // (batch_order)
         f.joins = f.slots = 0;
     } else {
         f.groups = units <= p->resident ? p->resident : units + more;

@@ -77,6 +77,14 @@ def test_split_over_keys(pairs, bf16, hd):
     assert torch.equal(out, again) and torch.equal(lse, lse2)  # equal calls, equal bits
 
 
+@pytest.mark.parametrize("pairs", [[(1000, 1000)] * 4, [(600, 900), (777, 1000)] * 2, [(900, 1010)] * 5])
+def test_more_units_than_cus_that_stay_whole(pairs):
+    """Tables too short for any split: a launch of more work-groups than CUs, in the
+    order that balances those a CU holds, has them all."""
+    b = Batch(pairs, 14, 2, 64, 16, True, seed=len(pairs))
+    check(b, *run(b))
+
+
 @pytest.mark.parametrize("n_seq", [63, 64, 65, 130])
 def test_many_sequences(n_seq):
     """More sequences than a wave's lanes, some without new tokens."""
