@@ -456,7 +456,7 @@ int mxfa_check_batch(const mxfa_batch_shape *shape);
  * (mxfa_prefill_batch_workspace_bytes, 16-byte aligned, no contents needed) is
  * used until the call completes: calls that may overlap need their own. The
  * key ranges of long sequences are joined in a fixed order: equal calls give
- * equal bits. */
+ * equal bits. out may be q (the same pointer and stride). */
 size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *shape);
 int mxfa_run_prefill_batch(const mxfa_batch_shape *shape, const void *q, const void *kcache, const void *vcache,
                            void *out, float *lse, const int *block_table, const int *cu_q, const int *lens,
@@ -466,9 +466,9 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *shape, const void *q, const v
  * n_kv_head key heads, then its value heads; Q turns into q_out row r, K turns
  * into kcache and V is copied into vcache, at the rows of the tokens'
  * positions. rotary_dim = 0 (frequencies NULL): copies only. head_dim as for
- * mxfa_rotary_shape. q_out may be qkv (the same pointer and stride); any other
- * overlap of q_out, kcache or vcache with qkv or each other is the caller's to
- * avoid. */
+ * mxfa_rotary_shape. q_out may be qkv (the same pointer and stride), or other
+ * columns of the same rows; where it lies over qkv otherwise the call is refused
+ * (MXFA_ERR_UNSUPPORTED). Any other overlap is the caller's to avoid. */
 typedef struct {
     int rotary_dim, interleaved;
     float factor;
@@ -504,8 +504,8 @@ int mxfa_run_pages_fork(const mxfa_pages_shape *shape, int *block_table, int *le
                         const int *children, int n, int *pairs, int *status, int *counts, void *stream);
 /* The used blocks to the pool's low end: with L blocks in use, the j-th used
  * one at or above L moves to the j-th unused one below it. Writes the tables
- * and counts as they are after the moves (new_table may be block_table;
- * new_refs may not be refs), the moves to pairs (n_blocks / 2 pairs of space,
+ * and counts as they are after the moves (new_table may be block_table, with the
+ * same stride, and else lies apart from it; new_refs lies apart from refs), the moves to pairs (n_blocks / 2 pairs of space,
  * at least one), and to counts how many and L. Until the blocks that were left
  * are used again, the old tables stay valid too. */
 int mxfa_run_pages_compact(const mxfa_pages_shape *shape, const int *block_table, const int *lens, const int *refs,

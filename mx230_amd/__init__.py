@@ -877,6 +877,15 @@ def _dev(t, name, dtype=None, like=None):
     return t
 
 
+def _c_int(**values):
+    """The values, which must be whole numbers that a C int holds (ctypes would cut
+    them)."""
+    import operator
+    for name, v in values.items():
+        if not -2 ** 31 <= operator.index(v) < 2 ** 31:
+            raise ValueError(f"{name} {v}: past 32 bits")
+
+
 def _ints(t, name, n, like):
     """A contiguous int32 vector of at least n elements."""
     torch = _torch()
@@ -955,6 +964,7 @@ def run_rotary(q, k, q_out, k_out, frequencies, positions=None, pos0: int = 0, i
             raise ValueError(f"positions: expected [{N}] or [{B}, {N}] with contiguous rows, got "
                              f"{tuple(positions.shape)} strides {positions.stride()}")
         pp, pbs = ctypes.c_void_p(positions.data_ptr()), positions.stride(0) if positions.dim() == 2 else 0
+    _c_int(pos0=pos0, B=B, Hq=Hq, Hkv=Hkv, N=N)
     sh = MxfaRotaryShape(B, Hq, Hkv, N, d, dim, int(bool(interleaved)), int(bool(inverse)),
                          MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, pos0, factor, *qs, *ks, *qos, *kos, pbs)
     with _on(q.device):
@@ -984,6 +994,7 @@ def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, l
     _dev(q, "q")
     if q.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"q: dtype {q.dtype}; bf16 or float32 expected")
+    _c_int(max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, block_size=block_size)
     if n_head < 1 or n_kv_head < 1 or head_dim < 1 or block_size < 1:
         raise ValueError("n_head, n_kv_head, head_dim and block_size must be positive")
     n_tok = q.shape[0] if q.dim() == 2 else -1
@@ -998,6 +1009,8 @@ def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, l
     lp = _ints(lens, "lens", 1, q)
     cp = _ints(cu_q, "cu_q", n_seq + 1, q)
     tp, wide, ts = _block_table(block_table, n_seq, q)
+    _c_int(n_tok=n_tok, n_blocks=kcache.shape[0] // block_size, table_stride=ts, q_stride=qs, kv_stride=ks,
+           out_stride=os_)
     sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, kcache.shape[0] // block_size,
                         wide, ts, qs, ks, os_, MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
     return sh, qp, kp, vp, op, tp, cp, lp
@@ -1037,8 +1050,9 @@ def prefill_batch_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head: in
                                   bf16: bool = True) -> int:
     """mxfa_prefill_batch_workspace_bytes: what run_prefill_batch needs for such a
     batch, whatever its lengths (0 for one it does not take)."""
-    # (a table of any width: at 2^20 positions every form has all its work-groups)
-    w, entries = n_head * head_dim, 1 << 20
+    # (a table of any width: at 2^17 positions every form has all its work-groups)
+    w, entries = n_head * head_dim, 1 << 17
+    _c_int(n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, q_stride=w)
     sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w,
                         n_kv_head * head_dim, w, MXFA_BF16 if bf16 else MXFA_F32, 0.0)
     return int(load_library().mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh)))
@@ -1052,7 +1066,7 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
     (run_cache_append). Lengths and tables are read on the device.
 
     q: [n_tok, >= n_head head_dim] (may be the columns of a fused QKV buffer),
-    out likewise; the caches, block_table, cu_q and lens as for
+    out likewise (may be q); the caches, block_table, cu_q and lens as for
     run_cache_append; max_q: at least the most new tokens any sequence has
     (rows past it are not computed). lse: None, or float32 [n_tok, n_head] for
     the rows' log-sum-exp. workspace: a contiguous device tensor of
@@ -1098,6 +1112,7 @@ def _pages_args(block_table, block_size, lens, refs):
     torch = _torch()
     _dev(lens, "lens", torch.int32)
     tp, wide, ts = _block_table(block_table, lens.numel(), lens)
+    _c_int(block_size=block_size, table_stride=ts)
     sh = MxfaPagesShape(lens.numel(), wide, ts, block_size, refs.numel() if isinstance(refs, torch.Tensor) else 0)
     return sh, tp, _ints(lens, "lens", 1, lens), _ints(refs, "refs", 1, lens)
 

@@ -208,7 +208,7 @@ __device__ __forceinline__ void rotary_body(const RotaryParams &p) {
 template <class T, int VEC>
 __device__ __forceinline__ void append_body(const BatchParams &p) {
     const int U = rotary_units<VEC>(p.d, p.dim), tid = threadIdx.x;
-    const int per = U <= 256 ? 256 / U : 1;
+    const int per = 256 / U;  // a row has at most 255 units
     __shared__ int seq_of[256], pos_of[256];
     __shared__ long long row_of[256];
     const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, p.n_tok);
@@ -238,34 +238,32 @@ __device__ __forceinline__ void append_body(const BatchParams &p) {
     __syncthreads();
     const int H = p.Hq + 2 * p.Hkv;
     const int h0 = (int)blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, H);
-    for (int i = tid; i < per * U; i += 256) {  // one turn unless a row has more than 256 units
-        const int k = i / U, u = i - k * U, t = t0 + k;
-        if (t >= t1 || pos_of[k] < 0) continue;
-        const long long crow = row_of[k];
-        const Unit<T, VEC> un(u, p.dim, p.interleaved, p.freq, pos_of[k], p.factor, 1.0f);
-        const T *in = static_cast<const T *>(p.q) + (long long)t * p.q_rs;
-        for (int h = h0; h < h1; h += kHeadsAhead) {
-            Chunk<T, VEC> x[kHeadsAhead], y[kHeadsAhead];
+    const int k = tid / U, u = tid - k * U, t = t0 + k;
+    if (k >= per || t >= t1 || pos_of[k] < 0) return;
+    const long long crow = row_of[k];
+    const Unit<T, VEC> un(u, p.dim, p.interleaved, p.freq, pos_of[k], p.factor, 1.0f);
+    const T *in = static_cast<const T *>(p.q) + (long long)t * p.q_rs;
+    for (int h = h0; h < h1; h += kHeadsAhead) {
+        Chunk<T, VEC> x[kHeadsAhead], y[kHeadsAhead];
 #pragma unroll
-            for (int j = 0; j < kHeadsAhead; ++j) {
-                if (h + j >= h1) break;
-                x[j].load(in + (h + j) * p.d + un.e0);
-                if (un.e1 >= 0) y[j].load(in + (h + j) * p.d + un.e1);
-            }
+        for (int j = 0; j < kHeadsAhead; ++j) {
+            if (h + j >= h1) break;
+            x[j].load(in + (h + j) * p.d + un.e0);
+            if (un.e1 >= 0) y[j].load(in + (h + j) * p.d + un.e1);
+        }
 #pragma unroll
-            for (int j = 0; j < kHeadsAhead; ++j) {
-                if (h + j >= h1) break;
-                const int hh = h + j, kv = hh - p.Hq;
-                if (kv >= 0 && crow < 0) continue;
-                T *row = kv < 0 ? static_cast<T *>(p.o) + (long long)t * p.o_rs + hh * p.d
-                         : kv < p.Hkv ? static_cast<T *>(p.k) + crow * p.kv_rs + kv * p.d
-                                      : static_cast<T *>(p.v) + crow * p.kv_rs + (kv - p.Hkv) * p.d;
-                if (un.e1 >= 0) {
-                    if (kv < p.Hkv) turn<T, VEC>(x[j], y[j], un.c, un.s, p.interleaved);
-                    y[j].store(row + un.e1);
-                }
-                x[j].store(row + un.e0);
+        for (int j = 0; j < kHeadsAhead; ++j) {
+            if (h + j >= h1) break;
+            const int hh = h + j, kv = hh - p.Hq;
+            if (kv >= 0 && crow < 0) continue;
+            T *row = kv < 0 ? static_cast<T *>(p.o) + (long long)t * p.o_rs + hh * p.d
+                     : kv < p.Hkv ? static_cast<T *>(p.k) + crow * p.kv_rs + kv * p.d
+                                  : static_cast<T *>(p.v) + crow * p.kv_rs + (kv - p.Hkv) * p.d;
+            if (un.e1 >= 0) {
+                if (kv < p.Hkv) turn<T, VEC>(x[j], y[j], un.c, un.s, p.interleaved);
+                y[j].store(row + un.e1);
             }
+            x[j].store(row + un.e0);
         }
     }
 }
@@ -314,7 +312,7 @@ hipError_t launch_rotary(RotaryParams p, int dtype_bf16, hipStream_t stream) {
 
 hipError_t launch_append(BatchParams p, int dtype_bf16, hipStream_t stream) {
     const int v = rotary_vec(p.dim, dtype_bf16), U = rotary_row_units(p.d, p.dim, dtype_bf16);
-    const int H = p.Hq + 2 * p.Hkv, per = U <= 256 ? 256 / U : 1;
+    const int H = p.Hq + 2 * p.Hkv, per = 256 / U;
     p.hpt = heads_per_thread((long long)p.n_tok * U, H);
     const KernelId id = dtype_bf16 ? (v == 8 ? k_mxfa_append_b : v == 4 ? k_mxfa_append_b4 : k_mxfa_append_b1)
                                    : (v == 4 ? k_mxfa_append_f : k_mxfa_append_f1);

@@ -717,6 +717,19 @@ int check_batch(const mxfa_batch_shape *s, long long qw) {
     return MXFA_OK;
 }
 
+// Whether `rows` output rows of `ow` bytes and as many input rows of `iw` share
+// memory in any way but as the same rows: where the strides are equal they may
+// also be columns of the same wider rows.
+bool rows_collide(const void *out, long long os, long long ow, const void *in, long long is, long long iw, int rows) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+    if (rows == 1) os = is = ow > iw ? ow : iw;
+    if (o == i && os == is) return false;
+    if (o >= i + (uintptr_t)(is * (rows - 1) + iw) || i >= o + (uintptr_t)(os * (rows - 1) + ow)) return false;
+    if (os != is) return true;
+    const uintptr_t at = o > i ? (o - i) % (uintptr_t)os : ((uintptr_t)os - (i - o) % (uintptr_t)os) % (uintptr_t)os;
+    return at < (uintptr_t)iw || at + (uintptr_t)ow > (uintptr_t)os;
+}
+
 mxfa::BatchParams batch_params(const mxfa_batch_shape *s, const void *q, void *k, void *v, void *o, const int *table,
                                const int *cu_q, const int *lens) {
     mxfa::BatchParams p;
@@ -813,6 +826,10 @@ int mxfa_run_cache_append(const mxfa_batch_shape *s, const mxfa_append_rotary *r
     if (rc != MXFA_OK) return rc;
     rc = check_ints({block_table, cu_q, lens});
     if (rc != MXFA_OK) return rc;
+    const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, row = esz * s->head_dim;
+    if (rows_collide(q_out, s->out_stride * esz, s->n_head * row, qkv, s->q_stride * esz,
+                     (s->n_head + 2LL * s->n_kv_head) * row, s->n_tok))
+        return MXFA_ERR_UNSUPPORTED;
     mxfa::BatchParams p = batch_params(s, qkv, kcache, vcache, q_out, block_table, cu_q, lens);
     p.freq = r->frequencies;
     p.dim = r->rotary_dim;
@@ -870,6 +887,10 @@ int mxfa_run_pages_compact(const mxfa_pages_shape *s, const int *block_table, co
     if (rc != MXFA_OK) return rc;
     // the counts are read again after the new ones are written
     if (refs < new_refs + s->n_blocks && new_refs < refs + s->n_blocks) return MXFA_ERR_UNSUPPORTED;
+    // and a table's entries by one thread each
+    if (rows_collide(new_table, 4LL * new_stride, 4LL * s->max_blocks, block_table, 4LL * s->table_stride,
+                     4LL * s->max_blocks, s->n_seq))
+        return MXFA_ERR_UNSUPPORTED;
     return from_hip(mxfa::launch_pages_compact(pages_params(s, block_table, lens, refs), new_table, new_stride,
                                                new_refs, pairs, counts, static_cast<hipStream_t>(stream)));
 }

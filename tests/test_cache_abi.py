@@ -133,6 +133,18 @@ def test_append_arguments(lib):
     assert go((64, 0, 1.0), n_tok=2 ** 29) == SHAPE
 
 
+def test_append_over_its_input(lib):
+    """q_out may be qkv or other columns of its rows; otherwise it lies apart."""
+    def go(off, stride, n_tok=4):  # (bf16, 4/2 heads of 64: Q 512 bytes, a row of qkv 1024)
+        s = batch_shape(n_tok=n_tok, n_head=4, n_kv_head=2, head_dim=64, q_stride=1024, out_stride=stride, kv_stride=128)
+        base = 1 << 20
+        return lib.mxfa_run_cache_append(ctypes.byref(s), ctypes.byref(mx.MxfaAppendRotary(64, 0, 1.0, P)),
+                                         ctypes.c_void_p(base), ctypes.c_void_p(base + off), P, P, P, P, P, None)
+    for off, stride, n in ((512, 1024, 4), (-256, 1024, 4), (0, 512, 4), (1024, 512, 4), (16, 1024, 4), (1536 + 16, 1024, 4),
+                           (2048 + 512, 1024, 4), (512, 512, 1), (16, 256, 1), (-16, 256, 1)):
+        assert go(off, stride, n) == UNSUPPORTED, (off, stride, n)
+
+
 def pages_shape(**kw):
     base = dict(n_seq=3, max_blocks=5, table_stride=5, block_size=16, n_blocks=10)
     base.update(kw)
@@ -158,6 +170,9 @@ def test_pages_arguments(lib):
     assert lib.mxfa_run_pages_compact(s, P, P, P, P, 4, far, P, P, None) == SHAPE
     assert lib.mxfa_run_pages_compact(s, P, P, P, P, 5, P, P, P, None) == UNSUPPORTED  # counts over counts
     assert lib.mxfa_run_pages_compact(s, P, P, P, P, 5, ctypes.c_void_p(4097), P, P, None) == ALIGN
+    # a new table over the old one in any way but as the same rows
+    assert lib.mxfa_run_pages_compact(s, P, P, P, P, 6, far, P, P, None) == UNSUPPORTED
+    assert lib.mxfa_run_pages_compact(s, P, P, P, ctypes.c_void_p(4096 + 40), 5, far, P, P, None) == UNSUPPORTED
     copy = lib.mxfa_run_pages_copy
     assert copy(P, 1, 0, 10, 0, P, 1, None, None) == SHAPE
     assert copy(P, 1, 0, 10, 24, P, 1, None, None) == ALIGN
@@ -185,6 +200,14 @@ def test_python_layer_refuses_host_tensors():
             call()
     with pytest.raises(TypeError):
         mx.run_rotary(None, None, None, None, f)
+
+
+def test_numbers_past_32_bits():
+    with pytest.raises(ValueError, match="past 32 bits"):
+        mx.prefill_batch_workspace_bytes(2 ** 32 + 1, 1, 1, 4, 2)
+    with pytest.raises(TypeError):
+        mx.prefill_batch_workspace_bytes(5, 1, 1.5, 4, 2)
+    assert mx.prefill_batch_workspace_bytes(150000, 150000, 1, 1, 1) > 0
 
 
 def test_rotary_frequencies():

@@ -177,6 +177,31 @@ def test_strides_and_shared_rows():
                              3, nh, nkv, hd)
 
 
+@pytest.mark.parametrize("pairs", [[(1, 900), (3, 5000), (1, 1)], [(150, 4000), (1, 3000), (200, 200)], [(90, 90)]])
+def test_output_over_the_queries(pairs):
+    b = Batch(pairs, 14, 2, 64, 16, True, seed=len(pairs))
+    k, v, table, cu, lens, qkv = b.cuda("k", "v", "table", "cu_q", "lens", "qkv")
+    q = qkv[:, :b.nh * b.hd].clone()
+    out, _ = run(b, lse=False)
+    mx.run_prefill_batch(q, k, v, q, table, b.bs, cu, lens, b.max_q, b.nh, b.nkv, b.hd)
+    torch.cuda.synchronize()
+    assert torch.equal(q[:b.n_new].cpu(), out[:b.n_new])
+
+
+def test_numbers_past_32_bits():
+    b = Batch([(1, 9)], 4, 2, 64, 16, True, seed=1)
+    k, v, table, cu, lens, qkv = b.cuda("k", "v", "table", "cu_q", "lens", "qkv")
+    out = torch.empty(b.n_tok, b.nh * b.hd, dtype=b.dt, device="cuda")
+    for kw in (dict(max_q=2 ** 32 + 1), dict(block_size=2 ** 32 + 16), dict(n_head=2 ** 32 + 4)):
+        a = dict(block_table=table, block_size=b.bs, cu_q=cu, lens=lens, max_q=1, n_head=b.nh, n_kv_head=b.nkv, head_dim=b.hd)
+        with pytest.raises(ValueError, match="past 32 bits"):
+            mx.run_prefill_batch(qkv[:, :b.nh * b.hd], k, v, out, **(a | kw))
+    f, _ = mx.rotary_frequencies(64)
+    x = torch.zeros(1, 2, 3, 64, device="cuda")
+    with pytest.raises(ValueError, match="past 32 bits"):
+        mx.run_rotary(x, None, x, None, f, pos0=2 ** 32)
+
+
 def test_max_q_bounds_the_rows():
     """Rows of a sequence past max_q are left as they were."""
     b = Batch([(6, 100), (2, 30)], 4, 2, 64, 16, True, seed=15)
