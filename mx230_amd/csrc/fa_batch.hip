@@ -212,19 +212,22 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
     const int lane = threadIdx.x & 63;
     BatchSeq b = batch_seq<false, ROWS>(p, lane);
     float all = seq_stages<ROWS>(p, b), units = (float)b.units;
-    bool any_long = b.stages > p.whole;
     for (int s0 = 64; s0 < p.n_seq; s0 += 64) {
         const BatchSeq c = batch_seq<false, ROWS>(p, s0 + lane);
         all += seq_stages<ROWS>(p, c);
         units += (float)c.units;
-        any_long |= c.stages > p.whole;
     }
-    any_long = __builtin_amdgcn_ballot_w64(any_long) != 0;
-    const unsigned quota = batch_quota(p, wave_sum(all), wave_sum(units), any_long, [&](unsigned q) __attribute__((always_inline)) {
+    auto count = [&](unsigned q) __attribute__((always_inline)) {
         int n = seq_items<ROWS>(p, b, q).items;
         for (int s0 = 64; s0 < p.n_seq; s0 += 64) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s0 + lane), q).items;
         return (float)wave_sum(n);
-    });
+    };
+    auto longer = [&](unsigned x) __attribute__((always_inline)) {
+        bool is = (unsigned)b.stages > x;
+        for (int s0 = 64; s0 < p.n_seq; s0 += 64) is |= (unsigned)batch_seq<false, ROWS>(p, s0 + lane).stages > x;
+        return __builtin_amdgcn_ballot_w64(is) != 0;
+    };
+    const unsigned quota = batch_quota(p, wave_sum(all), wave_sum(units), count, longer);
     if (w == 0 && p.splits > 0) {
         int n = seq_items<ROWS>(p, b, quota).split;
         for (int s0 = 64; s0 < p.n_seq; s0 += 64) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s0 + lane), quota).split;

@@ -148,26 +148,30 @@ __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchS
 }
 
 // The quota, from the sums of seq_stages and of the units over the sequences (of
-// one KV head), whether any has more than p.whole stages, and the count of all items
-// at a quota. Without one nothing is split: that takes about the join's time, or
-// less (bf16, 1000 tokens of 14/2 heads: 12 us whole, 20 in shares of 8 stages).
-// Where the units fit the
-// work-groups that are resident at once (p.resident), it is about the least one
-// by which their shares still do, found by raising an even share's (INT_MAX,
-// no split, where that takes too long); else one and a half even shares. It
-// depends on lengths alone.
+// one KV head), the count of all items at a quota, and whether a sequence has
+// more stages than a number. Where the units fit the work-groups that are resident
+// at once (p.resident), it is about the least one by which their shares still
+// do, found by raising an even share's (INT_MAX, no split, where that takes too
+// long); else one and a half even shares. It depends on lengths alone.
+//
+// A split costs a join of about p.whole stages' time and p.per_item stages' for
+// each share's part written and read again; where the longest unit is over a
+// share's by no more, all units stay whole. us, whole and split: bf16, 14/2 heads,
+// 4 chunks of 700 tokens after 700 32 and 39, one of 500 after 1500 31 and 23,
+// 1000 tokens 19 and 21; 32/8 heads, d = 128, 1000 tokens 27 and 35; fp32, 14/2
+// heads, 500 tokens 28 and 29, 1000 51 and 35.
 constexpr float kManySplit = 1.5f;
-template <class Count>
-__host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, bool any_long, Count count) {
-    if (!any_long) return INT_MAX;
+template <class Count, class Longer>
+__host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, Count count, Longer longer) {
     all = less_of(all * (float)p.Hkv * 1.001f, 1e18f);  // (more than its rounding)
     const float resident = (float)p.resident, even = less_of(all * p.per_resident + 1.0f, 1e9f);
     const float least = (float)p.least[1];
-    if (units * (float)p.Hkv > resident) return (unsigned)more_of(kManySplit * even, least);
-    unsigned q = (unsigned)more_of(even, least);
+    const bool fit = units * (float)p.Hkv <= resident;
+    unsigned q = (unsigned)more_of(fit ? even : kManySplit * even, least);
+    if (p.slots == 0) return INT_MAX;
     for (int i = 0; i < 8; ++i) {
         const float items = count(q);
-        if (items <= resident) return q;
+        if (!fit || items <= resident) return longer(q + p.whole + (unsigned)(p.per_item * items)) ? q : INT_MAX;
         q = more_of(q + 1, (unsigned)((float)q * items * p.per_resident));
     }
     return INT_MAX;
@@ -302,7 +306,10 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     p->per_resident = 1.0f / (float)p->resident;
     const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
     const long long more = (long long)p->resident * 4 / 3 + 1;
-    if (batch_most_stages(*p) <= p->whole) {  // nothing to split
+    // nothing is split, and no join launched, where batch_quota would hardly ever
+    // find it worth it: some 3 shares of a unit
+    const float shares = 3.0f * (float)less_of(units, (long long)p->resident / 2);
+    if ((float)batch_most_stages(*p) <= (float)(p->least[1] + p->whole) + p->per_item * shares) {
         f.groups = units <= kBatchCus ? units : more_of(units, (long long)p->resident);  // (batch_order)
         f.joins = f.slots = 0;
     } else {
@@ -318,13 +325,13 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
 }
 
 // The least stages of a share or run: one for each of the few-row form's waves; 4
-// of the many-row form's, whose units all stay whole if none has more than
-// p.whole (a stage takes 0.6 us in bf16, 2.5 in fp32, and the join 5).
+// of the many-row form's.
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
     p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
     p->least[1] = 4;
-    p->whole = dtype_bf16 ? 16 : 4;
+    p->whole = dtype_bf16 ? 6 : 4;
+    p->per_item = dtype_bf16 ? 0.024f : 0.007f;
 }
 
 }  // namespace mxfa

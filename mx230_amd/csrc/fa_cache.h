@@ -47,11 +47,12 @@ struct BatchParams {
     // attention (fa_batch_items.h): the most rows (new tokens x query heads of a
     // KV head) of a sequence that the few-row form takes (0: it takes none) and
     // its work-groups per KV head; per form (few, many) the least stages of a run
-    // or share; of the many-row form: the stages up to which nothing is split, the
-    // work-groups resident at once, 1 / that, the slots of its shares and the split
-    // units there can be; the forms' parts of the workspace and their notes
+    // or share; of the many-row form: what a split costs, in stages and in stages
+    // per item (batch_quota), the work-groups resident at once, 1 / that, the slots
+    // of its shares and the split units there can be; the forms' parts of the
+    // workspace and their notes
     int few_rows, few_groups, least[2], whole, resident, slots, splits;
-    float per_resident;
+    float per_item, per_resident;
     float *part[2];
     int *notes[2];
 };

@@ -42,18 +42,23 @@ static int g_fail = 0;
 template <int ROWS>
 static bool find(const BatchParams &p, int w, BatchItem &it, int *total = nullptr) {
     float all = 0, units = 0;
-    bool any_long = false;
     for (int s = 0; s < p.n_seq; ++s) {
         const BatchSeq b = batch_seq<false, ROWS>(p, s);
-        any_long |= b.stages > p.whole;
         all += seq_stages<ROWS>(p, b);
         units += (float)b.units;
     }
-    const unsigned quota = batch_quota(p, all, units, any_long, [&](unsigned q) {
+    auto count = [&](unsigned q) {
         int n = 0;
         for (int s = 0; s < p.n_seq; ++s) n += seq_items<ROWS>(p, batch_seq<false, ROWS>(p, s), q).items;
         return (float)n;
-    });
+    };
+    auto longer = [&](unsigned x) {
+        for (int s = 0; s < p.n_seq; ++s) {
+            if ((unsigned)batch_seq<false, ROWS>(p, s).stages > x) return true;
+        }
+        return false;
+    };
+    const unsigned quota = batch_quota(p, all, units, count, longer);
     int before = 0, slots = 0, splits = 0;
     bool found = false;
     for (int s = 0; s < p.n_seq; ++s) {
