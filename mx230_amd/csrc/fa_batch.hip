@@ -372,14 +372,12 @@ __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchIte
     if (part != nullptr && c == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m, l);
 }
 
-// A slot of a form's workspace: ROWS rows of D floats, and their (max, sum).
-template <int ROWS>
-__device__ __forceinline__ float *batch_part(float *part, int slot, int d) {
-    return part + (size_t)slot * ROWS * d;
+// A slot of a form's workspace: its units' rows of d floats, and their (max, sum).
+__device__ __forceinline__ float *batch_part(float *part, int slot, int rows, int d) {
+    return part + (size_t)slot * rows * d;
 }
-template <int ROWS>
-__device__ __forceinline__ float *batch_ml(float *part, int slots, int slot, int d) {
-    return part + (size_t)slots * ROWS * d + (size_t)slot * ROWS * 2;
+__device__ __forceinline__ float *batch_ml(float *part, int slots, int slot, int rows, int d) {
+    return part + (size_t)slots * rows * d + (size_t)slot * rows * 2;
 }
 __device__ __forceinline__ int few_slots(const BatchParams &p) { return 2 * p.few_groups * p.Hkv; }
 
@@ -491,8 +489,8 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
     __syncthreads();
     float *part = nullptr, *ml = nullptr;
     if (slot >= 0) {
-        part = batch_part<ROWS>(p.part[0], slot, D);
-        ml = batch_ml<ROWS>(p.part[0], few_slots(p), slot, D);
+        part = batch_part(p.part[0], slot, ROWS, D);
+        ml = batch_ml(p.part[0], few_slots(p), slot, ROWS, D);
     }
     if (sm.merge.bad) {
         if (tid < 4 * ROWS) batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
@@ -664,8 +662,8 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
     }
     float *part = nullptr, *ml = nullptr;
     if (it.shares > 1) {
-        part = batch_part<ROWS>(p.part[1], it.slot, D);
-        ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
+        part = batch_part(p.part[1], it.slot, ROWS, D);
+        ml = batch_ml(p.part[1], p.slots, it.slot, ROWS, D);
     }
     const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
     if (lane == 0) sm.bad[wave] = bad;
@@ -704,7 +702,7 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
 // are then run in plain arithmetic. 2000 tokens of 14/2 heads after 2096, us: on
 // v_mfma_f32_16x16x4_f32 235, parts with 4 waves and 64 rows 203.
 __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block, FwdSplitSmem &sm) {
-    constexpr int D = 64, XT = 4, BK = 64, NW = kBatchF32Waves, NT = 64 * NW, ROWS = batch_many_rows(false);
+    constexpr int D = 64, XT = 4, BK = 64, NW = kBatchF32Waves, NT = 64 * NW, ROWS = 16 * NW;
     using PL = PolBF16<64>;  // the parts' layout
     using Stage = SplitStage<NT>;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -868,8 +866,8 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
     if (low) z = NAN;
     float *part = nullptr, *ml = nullptr;
     if (it.shares > 1) {
-        part = batch_part<ROWS>(p.part[1], it.slot, D);
-        ml = batch_ml<ROWS>(p.part[1], p.slots, it.slot, D);
+        part = batch_part(p.part[1], it.slot, ROWS, D);
+        ml = batch_ml(p.part[1], p.slots, it.slot, ROWS, D);
     }
     if (any_nonfinite<NW>(z, sm.flags, wave, lane)) {
         batch_plain<float, D, ROWS>(p, it, 0, s_lo * BK, s_hi * BK, part, ml);
@@ -899,9 +897,9 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
 // rows several groups take turns over its parts and meet in LDS. Bound by
 // latency: the (max, sum) pairs of all parts are one round of loads, and eight
 // parts of a thread's turn another.
-template <class T, int D, int ROWS, class At>
-__device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int first, int end, int S,
-                                                float *parts, int slots, At at) {
+template <class T, int D, class At>
+__device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int rows, int first, int end,
+                                                int S, float *parts, int slots, At at) {
     constexpr int C = D / 4, NG = 256 / C, PARTS = 128, EACH = PARTS / C;
     __shared__ __attribute__((aligned(16))) f32x4 so[NG][C];
     __shared__ float weights[NG][PARTS];
@@ -921,7 +919,7 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
             for (int i = 0; i < EACH; ++i) {
                 v[i] = make_float2(-INFINITY, 0.f);
                 if (i * C + c < n)
-                    v[i] = *reinterpret_cast<const float2 *>(batch_ml<ROWS>(parts, slots, at(s0 + i * C + c), D) + 2 * r);
+                    v[i] = *reinterpret_cast<const float2 *>(batch_ml(parts, slots, at(s0 + i * C + c), rows, D) + 2 * r);
             }
             float mx = M;
 #pragma unroll
@@ -950,7 +948,7 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
                 for (int i = 0; i < 8; ++i) {
                     const int j = min(s + i * together, n - 1);
                     w[i] = s + i * together < n ? weights[grp][j] : 0.f;
-                    x[i] = *reinterpret_cast<const f32x4 *>(batch_part<ROWS>(parts, at(s0 + j), D) + r * D + 4 * c);
+                    x[i] = *reinterpret_cast<const f32x4 *>(batch_part(parts, at(s0 + j), rows, D) + r * D + 4 * c);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o += x[i] * w[i];
@@ -965,7 +963,7 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
                 for (int k = 1; k < together; ++k) o += so[grp + k][c];
             }
         }
-        if (have && turn == 0) batch_store<T>(p, it, it.unit * ROWS + r, D, 4 * c, o, M, L);
+        if (have && turn == 0) batch_store<T>(p, it, it.unit * rows + r, D, 4 * c, o, M, L);
     }
 }
 
@@ -973,7 +971,8 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
 // then the pieces of the split units that the many-row form may have.
 template <class T, int D>
 __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
-    constexpr int ROWS = batch_many_rows(sizeof(T) == 2), JOIN = join_rows(D), PIECES = ROWS / JOIN;
+    constexpr int JOIN = join_rows(D);
+    const int rows = p.many_rows, pieces = rows / JOIN;
     BatchItem it;
     if ((int)blockIdx.x < few_cuts) {
         // the cut at the end of work-group g's run
@@ -985,21 +984,21 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
         it.head = head;
         it.unit = 0;
         it.s.q0 = n.q0;
-        batch_join_rows<T, D, kBatchFew>(p, it, first, end, n.parts, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
+        batch_join_rows<T, D>(p, it, kBatchFew, first, end, n.parts, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
             return i == 0 ? few_first_slot(run, heads, head) : few_next_slot(run, heads, head) + 2 * heads * (i - 1);
         });
         return;
     }
-    const int w = (int)blockIdx.x - few_cuts, unit = w / PIECES;
+    const int w = (int)blockIdx.x - few_cuts, unit = w / pieces;
     const int count = p.notes[1][0];
     const ManyNote n = reinterpret_cast<const ManyNote *>(p.notes[1])[1 + unit];
-    if (unit >= count || !note_holds(p, n, ROWS)) return;
-    const int first = w % PIECES * JOIN, end = min(first + JOIN, n.rows - n.unit * ROWS);
+    if (unit >= count || !note_holds(p, n)) return;
+    const int first = w % pieces * JOIN, end = min(first + JOIN, n.rows - n.unit * rows);
     if (first >= end) return;
     it.head = n.head;
     it.unit = n.unit;
     it.s.q0 = n.q0;
-    batch_join_rows<T, D, ROWS>(p, it, first, end, n.shares, p.part[1], p.slots,
+    batch_join_rows<T, D>(p, it, rows, first, end, n.shares, p.part[1], p.slots,
                                 [&](int i) __attribute__((always_inline)) { return n.slot + i * p.Hkv; });
 }
 
@@ -1007,16 +1006,15 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
 // tiles a quarter of its work-group's (bf16, d = 64) or half of it, so that LDS
 // holds as many of them as of the many-row form's: their reads and its matrix
 // products then share the CUs.
-__device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<PolRows<64>> &sm) {
-    batch_many_body<PolRows<64>, 2>(p, block, sm);
+template <int QT, class Pol>
+__device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
+    batch_many_body<Pol, QT>(p, block, sm);
 }
-__device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<PolRows<128>> &sm) {
-    batch_many_body<PolRows<128>, 2>(p, block, sm);
-}
+template <int QT>
 __device__ __forceinline__ void batch_many(const BatchParams &p, int block, FwdSplitSmem &sm) {
     batch_many_parts(p, block, sm);
 }
-template <class Pol, class Many, int NW, int THREADS>
+template <class Pol, class Many, int QT, int NW, int THREADS>
 __device__ __forceinline__ void batch_both_body(const BatchParams &p, int few_groups) {
     __shared__ __attribute__((aligned(16))) union {
         BatchFewSmem<Pol, NW> few;
@@ -1025,28 +1023,36 @@ __device__ __forceinline__ void batch_both_body(const BatchParams &p, int few_gr
     if ((int)blockIdx.x < few_groups) {
         batch_few_body<Pol, NW, THREADS>(p, blockIdx.x, sm.few);
     } else {
-        batch_many(p, (int)blockIdx.x - few_groups, sm.many);
+        batch_many<QT>(p, (int)blockIdx.x - few_groups, sm.many);
     }
 }
 
-#define MXFA_BATCH(SUFFIX, POL, MANY, THREADS, WPS, NW, BOTH_NW)                                             \
+// (MANY: of units of 64 QT rows, WPS waves per SIMD)
+#define MXFA_BATCH_MANY(NAME, BOTH, POL, MANY, QT, THREADS, WPS, BOTH_NW, BOTH_WPS)                          \
+    extern "C" __global__ __launch_bounds__(THREADS, WPS) void mxfa_batch_##NAME(BatchParams p) {            \
+        __shared__ __attribute__((aligned(16))) MANY sm;                                                     \
+        batch_many<QT>(p, blockIdx.x, sm);                                                                   \
+    }                                                                                                        \
+    extern "C" __global__ __launch_bounds__(THREADS, BOTH_WPS) void mxfa_batch_##BOTH(BatchParams p, int few_groups) { \
+        batch_both_body<POL, MANY, QT, BOTH_NW, THREADS>(p, few_groups);                                     \
+    }
+#define MXFA_BATCH(SUFFIX, POL, NW)                                                                          \
     extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##SUFFIX##_few(BatchParams p) {         \
         __shared__ __attribute__((aligned(16))) BatchFewSmem<POL, NW> sm;                                    \
         batch_few_body<POL, NW, 64 * NW>(p, blockIdx.x, sm);                                                 \
     }                                                                                                        \
-    extern "C" __global__ __launch_bounds__(THREADS, WPS) void mxfa_batch_##SUFFIX##_many(BatchParams p) {   \
-        __shared__ __attribute__((aligned(16))) MANY sm;                                                     \
-        batch_many(p, blockIdx.x, sm);                                                                       \
-    }                                                                                                        \
-    extern "C" __global__ __launch_bounds__(THREADS, WPS) void mxfa_batch_##SUFFIX##_both(BatchParams p, int few_groups) { \
-        batch_both_body<POL, MANY, BOTH_NW, THREADS>(p, few_groups);                                         \
-    }                                                                                                        \
     extern "C" __global__ __launch_bounds__(256) void mxfa_batch_##SUFFIX##_join(BatchParams p, int few_groups) { \
         batch_join<POL::T, POL::D>(p, few_groups);                                                           \
     }
-MXFA_BATCH(b64, PolRows<64>, BatchManySmem<PolRows<64>>, 256, 3, 8, 3)
-MXFA_BATCH(b128, PolRows<128>, BatchManySmem<PolRows<128>>, 256, 2, 4, 2)
-MXFA_BATCH(f64, PolF32, FwdSplitSmem, 64 * kBatchF32Waves, 4, 4, 2)
+MXFA_BATCH(b64, PolRows<64>, 8)
+MXFA_BATCH_MANY(b64_many, b64_both, PolRows<64>, BatchManySmem<PolRows<64>>, 2, 256, 3, 3, 3)
+MXFA_BATCH_MANY(b64_many64, b64_both64, PolRows<64>, BatchManySmem<PolRows<64>>, 1, 256, 4, 3, 3)
+MXFA_BATCH(b128, PolRows<128>, 4)
+MXFA_BATCH_MANY(b128_many, b128_both, PolRows<128>, BatchManySmem<PolRows<128>>, 2, 256, 2, 2, 2)
+MXFA_BATCH_MANY(b128_many64, b128_both64, PolRows<128>, BatchManySmem<PolRows<128>>, 1, 256, 2, 2, 2)
+MXFA_BATCH(f64, PolF32, 4)
+MXFA_BATCH_MANY(f64_many, f64_both, PolF32, FwdSplitSmem, 2, 64 * kBatchF32Waves, 4, 2, 4)
+#undef MXFA_BATCH_MANY
 #undef MXFA_BATCH
 #endif
 
@@ -1074,13 +1080,16 @@ long long batch_groups(const BatchParams &q, int dtype_bf16) {
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
-    static constexpr KernelId ids[3][4] = {
-        {k_mxfa_batch_b64_few, k_mxfa_batch_b64_many, k_mxfa_batch_b64_join, k_mxfa_batch_b64_both},
-        {k_mxfa_batch_b128_few, k_mxfa_batch_b128_many, k_mxfa_batch_b128_join, k_mxfa_batch_b128_both},
-        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_many, k_mxfa_batch_f64_join, k_mxfa_batch_f64_both}};
+    static constexpr KernelId ids[3][6] = {
+        {k_mxfa_batch_b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_b64_many, k_mxfa_batch_b64_both,
+         k_mxfa_batch_b64_many64, k_mxfa_batch_b64_both64},
+        {k_mxfa_batch_b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_b128_many, k_mxfa_batch_b128_both,
+         k_mxfa_batch_b128_many64, k_mxfa_batch_b128_both64},
+        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_f64_many, k_mxfa_batch_f64_both}};
     const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
     BatchForm f[2];
     batch_forms(&p, dtype_bf16, f);
+    const KernelId *many = id + (p.many_rows == 64 ? 4 : 2);
     float *next = static_cast<float *>(workspace);
     for (int i = 0; i < 2; ++i) {  // (notes of 16 and 32 bytes, slots of a multiple of that)
         p.part[i] = next;
@@ -1095,15 +1104,15 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     if (f[1].groups == 0) {
         e = launch_kernel(id[0], dim3(few_groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
     } else if (few_groups == 0) {
-        e = launch_kernel(id[1], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
+        e = launch_kernel(many[0], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
     } else {
-        e = launch_kernel(id[3], dim3((unsigned)(few_groups + f[1].groups)), dim3(threads), args, stream);
+        e = launch_kernel(many[1], dim3((unsigned)(few_groups + f[1].groups)), dim3(threads), args, stream);
     }
     int cuts = (int)f[0].joins * kFewJoins;
     const unsigned joins = (unsigned)(cuts + f[1].joins * (f[1].rows / join_rows(p.d)));
     if (e != hipSuccess || joins == 0) return e;
     void *jargs[] = {&p, &cuts};
-    return launch_kernel(id[2], dim3(joins), dim3(256), jargs, stream);
+    return launch_kernel(id[1], dim3(joins), dim3(256), jargs, stream);
 }
 
 }  // namespace mxfa

@@ -19,9 +19,9 @@ constexpr int kCusPerXcd = 32;  // of 8 XCDs
 // in a hundred pieces.
 __host__ __device__ constexpr int join_rows(int d) { return 1024 / d; }
 constexpr int kFewJoins = 4;
-// Rows of the many-row form's units: 4 waves of 2 query tiles (bf16), 8 of one.
+// Waves of the many-row form's work-groups in fp32, of 16 rows each (bf16: 4, of 16
+// or 32: batch_many_rows).
 constexpr int kBatchF32Waves = 8;
-__host__ __device__ constexpr int batch_many_rows(bool bf16) { return bf16 ? 128 : 16 * kBatchF32Waves; }
 
 // The workspace holds the shares of split units: `slots` of them, each ROWS rows
 // of D floats and their (max, sum) pairs; then what the join reads about them,
@@ -149,10 +149,11 @@ __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchS
 
 // The quota, from the sums of seq_stages and of the units over the sequences (of
 // one KV head), the count of all items at a quota, and whether a sequence has
-// more stages than a number. Where the units fit the work-groups that are resident
-// at once (p.resident), it is about the least one by which their shares still
-// do, found by raising an even share's (INT_MAX, no split, where that takes too
-// long); else one and a half even shares. It depends on lengths alone.
+// more stages than a number. It is about the least one, up to two even shares, by
+// which all shares fit the work-groups that are resident at once (p.resident), found
+// by raising an even share's; without one, one and a half even shares, if the launch
+// has room for those (p.roomy; else the search goes on). INT_MAX: no split. It depends
+// on lengths alone.
 //
 // A split costs a join of about p.whole stages' time and p.per_item stages' for
 // each share's part written and read again; where the longest unit is over a
@@ -163,18 +164,23 @@ __host__ __device__ inline SeqItems seq_items(const BatchParams &p, const BatchS
 constexpr float kManySplit = 1.5f;
 template <class Count, class Longer>
 __host__ __device__ inline unsigned batch_quota(const BatchParams &p, float all, float units, Count count, Longer longer) {
-    all = less_of(all * (float)p.Hkv * 1.001f, 1e18f);  // (more than its rounding)
-    const float resident = (float)p.resident, even = less_of(all * p.per_resident + 1.0f, 1e9f);
-    const float least = (float)p.least[1];
-    const bool fit = units * (float)p.Hkv <= resident;
-    unsigned q = (unsigned)more_of(fit ? even : kManySplit * even, least);
     if (p.slots == 0) return INT_MAX;
-    for (int i = 0; i < 8; ++i) {
+    all = less_of(all * (float)p.Hkv * 1.001f, 1e18f);  // (more than its rounding)
+    const float resident = (float)p.resident, even = less_of(all * p.per_resident + 1.0f, 1e8f);
+    const float least = (float)p.least[1];
+    auto worth = [&](unsigned q, float items) {
+        return longer(q + p.whole + (unsigned)(p.per_item * items)) ? q : (unsigned)INT_MAX;
+    };
+    unsigned q = (unsigned)more_of(even, least);
+    for (int i = 0; i < 12 && units * (float)p.Hkv <= resident; ++i) {
         const float items = count(q);
-        if (!fit || items <= resident) return longer(q + p.whole + (unsigned)(p.per_item * items)) ? q : INT_MAX;
-        q = more_of(q + 1, (unsigned)((float)q * items * p.per_resident));
+        if (items <= resident) return worth(q, items);
+        q = (unsigned)more_of((float)q * 1.125f + 1.0f, (float)q * items * p.per_resident);
+        if (p.roomy && (float)q > 2.0f * even) break;
     }
-    return INT_MAX;
+    if (!p.roomy) return INT_MAX;
+    q = (unsigned)more_of(kManySplit * even, least);
+    return worth(q, count(q));
 }
 
 struct BatchItem {
@@ -223,10 +229,10 @@ __host__ __device__ inline int batch_order(const BatchParams &p, int block) {
 
 // Whether a note of the join is one that find_item's items write (whatever the
 // workspace holds where none was written).
-__host__ __device__ inline bool note_holds(const BatchParams &p, const ManyNote &n, int ROWS) {
+__host__ __device__ inline bool note_holds(const BatchParams &p, const ManyNote &n) {
     return n.shares > 1 && n.slot >= 0 && (long long)n.slot + (long long)(n.shares - 1) * p.Hkv < p.slots && n.q0 >= 0 &&
            n.rows > 0 && n.q0 + (long long)(n.rows - 1) / p.group < p.n_tok && n.unit >= 0 &&
-           (long long)n.unit * ROWS < n.rows && n.head >= 0 && n.head < p.Hkv;
+           (long long)n.unit * p.many_rows < n.rows && n.head >= 0 && n.head < p.Hkv;
 }
 
 // The share's stages of the unit's n.
@@ -244,9 +250,11 @@ __host__ __device__ inline void share_stages(const BatchItem &it, int n, int &lo
 // ---- the launcher's side
 
 // Work-groups resident at once: the few-row form's have a CU each, the many-row
-// form's share one in twos or threes.
+// form's share one in twos, threes or fours (the kernels' registers and LDS).
 constexpr int kBatchCus = 256;
-inline int batch_resident(int dtype_bf16, int d) { return dtype_bf16 && d == 64 ? 3 * kBatchCus : 2 * kBatchCus; }
+inline int batch_resident(int dtype_bf16, int d, int rows, bool both) {
+    return kBatchCus * (!dtype_bf16 || d == 128 ? 2 : rows == 64 && !both ? 4 : 3);
+}
 
 // Which forms a call launches, by what the host knows: the few-row form alone
 // where no sequence can have more rows; the many-row form alone where one
@@ -257,6 +265,31 @@ inline int batch_few_rows(const BatchParams &p) {
 }
 inline bool batch_may_be_many(const BatchParams &p) {
     return (long long)less_of(p.max_q, p.n_tok) * p.group > kBatchFew || p.few_rows == 0;
+}
+
+// Units of the many-row form at most.
+inline long long batch_units(const BatchParams &p, int rows) {
+    return ((long long)p.n_tok * p.group / rows + less_of(p.n_seq, p.n_tok)) * p.Hkv;
+}
+
+// Whether most sequences are of few rows, by what the host knows: the others have
+// max_q tokens at most.
+inline bool batch_mostly_few(const BatchParams &p) {
+    if (p.few_rows == 0) return false;
+    const long long few_tok = p.few_rows / p.group;
+    return 2 * (more_of((long long)p.n_tok - p.n_seq * few_tok, 0LL) / p.max_q) < p.n_seq;
+}
+
+// Rows of its units (bf16: 4 waves of 16 or of 32). 32 a wave halve the LDS reads of
+// K and V for each product, 16 give twice the work-groups: taken where units of 128
+// rows are at most one and a half (d = 128: one) per CU. us, by 64 and by 128 rows:
+// 14/2 heads, 1000 tokens 14 and 19, 2000 25 and 34, 4 chunks of 700 after 700 28 and
+// 33, 8 of 512 after 3584 111 and 92; 32/8 heads, d = 128, 1000 tokens 23 and 28,
+// 2 chunks of 1000 after 2000 134 and 106. Beside the few-row form's work-groups, which
+// leave a CU room for two more of either, 128: 4 chunks and 28 tokens 58 and 52.
+inline int batch_many_rows(const BatchParams &p, int dtype_bf16) {
+    if (!dtype_bf16) return 16 * kBatchF32Waves;
+    return !batch_mostly_few(p) && batch_units(p, 128) <= (p.d == 64 ? 3 * kBatchCus / 2 : kBatchCus) ? 64 : 128;
 }
 
 // Stages that a sequence has at most, by its table.
@@ -284,27 +317,23 @@ inline BatchForm batch_few_form(BatchParams *p) {
     return f;
 }
 
-// Many rows. The units are full but for a sequence's last. Where they fit the
-// resident work-groups, so do all items, the shares of split units among them.
-// Else the quota is at least one and a half even shares, and find_item's sum of
+// Many rows. The units are full but for a sequence's last. Where they are up to
+// half of the resident work-groups, all items fit those, the shares of split units
+// among them. Else the quota may be at least one and a half even shares, and find_item's sum of
 // stages at least half of units x the last one's in each sequence: then the
 // shares of split units, ceil(last one's / quota) each, are at most 4/3 of the
 // resident + the split units, those at most 4/3 of the resident and the units.
 inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
     BatchForm f;
-    f.rows = batch_many_rows(dtype_bf16);
-    p->resident = batch_resident(dtype_bf16, p->d);
-    // Beside the few-row form's work-groups a CU holds two of these. The host
-    // knows how many sequences can be of few rows: the others have max_q tokens at
-    // most. us, 14/2 heads, d = 64: 4 chunks and 28 tokens 57.6 (61 by three a CU);
-    // 8 chunks 84 by three (104 by two)
-    if (p->few_rows > 0) {
-        const long long few_tok = p->few_rows / p->group;
-        const long long chunks = more_of((long long)p->n_tok - p->n_seq * few_tok, 0LL) / p->max_q;
-        if (2 * chunks < p->n_seq) p->resident = 2 * kBatchCus;
-    }
+    f.rows = p->many_rows;
+    p->roomy = 0;
+    p->resident = batch_resident(dtype_bf16, p->d, p->many_rows, p->few_rows > 0);
+    // Beside the few-row form's work-groups a CU holds two of these. us, 14/2 heads,
+    // d = 64: 4 chunks and 28 tokens 57.6 (61 by three a CU); 8 chunks 84 by three
+    // (104 by two)
+    if (batch_mostly_few(*p)) p->resident = 2 * kBatchCus;
     p->per_resident = 1.0f / (float)p->resident;
-    const long long units = ((long long)p->n_tok * p->group / f.rows + less_of(p->n_seq, p->n_tok)) * p->Hkv;
+    const long long units = batch_units(*p, f.rows);
     const long long more = (long long)p->resident * 4 / 3 + 1;
     // nothing is split, and no join launched, where batch_quota would hardly ever
     // find it worth it: some 3 shares of a unit
@@ -313,9 +342,10 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
         f.groups = units <= kBatchCus ? units : more_of(units, (long long)p->resident);  // (batch_order)
         f.joins = f.slots = 0;
     } else {
-        f.groups = units <= p->resident ? p->resident : units + more;
-        const long long split = units <= p->resident ? less_of(units, (long long)p->resident / 2) : less_of(units, more);
-        f.slots = units <= p->resident ? p->resident : more + split;
+        p->roomy = units > p->resident / 2;
+        f.groups = p->roomy ? units + more : p->resident;
+        const long long split = less_of(units, more);
+        f.slots = p->roomy ? more + split : p->resident;
         f.joins = split;
     }
     p->slots = (int)f.slots;
@@ -328,6 +358,7 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
 // of the many-row form's.
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
+    p->many_rows = batch_many_rows(*p, dtype_bf16);
     p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
     p->least[1] = 4;
     p->whole = dtype_bf16 ? 6 : 4;

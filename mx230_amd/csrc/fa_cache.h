@@ -46,12 +46,12 @@ struct BatchParams {
     int hpt;  // heads per thread
     // attention (fa_batch_items.h): the most rows (new tokens x query heads of a
     // KV head) of a sequence that the few-row form takes (0: it takes none) and
-    // its work-groups per KV head; per form (few, many) the least stages of a run
-    // or share; of the many-row form: what a split costs, in stages and in stages
-    // per item (batch_quota), the work-groups resident at once, 1 / that, the slots
-    // of its shares and the split units there can be; the forms' parts of the
+    // its work-groups per KV head; the rows of the many-row form's
+    // units; per form the least stages of a run or share; of the many-row form: what a split costs, in stages and in stages
+    // per item (batch_quota), the work-groups resident at once, 1 / that, whether a
+    // launch has more than those, the slots of its shares and the split units there can be; the forms' parts of the
     // workspace and their notes
-    int few_rows, few_groups, least[2], whole, resident, slots, splits;
+    int few_rows, few_groups, many_rows, least[2], whole, resident, roomy, slots, splits;
     float per_item, per_resident;
     float *part[2];
     int *notes[2];

@@ -46,6 +46,7 @@
     /* attention of a batch over a paged cache (fa_batch.hip) */                              \
     X(mxfa_batch_b64_few) X(mxfa_batch_b64_many) X(mxfa_batch_b64_join) X(mxfa_batch_b64_both)                       \
     X(mxfa_batch_b128_few) X(mxfa_batch_b128_many) X(mxfa_batch_b128_join) X(mxfa_batch_b128_both)                    \
+    X(mxfa_batch_b64_many64) X(mxfa_batch_b64_both64) X(mxfa_batch_b128_many64) X(mxfa_batch_b128_both64)             \
     X(mxfa_batch_f64_few) X(mxfa_batch_f64_many) X(mxfa_batch_f64_join) X(mxfa_batch_f64_both)                       \
     /* rotary positions and the cache append (fa_rotary.hip): 16-byte, 8-byte, single-element chunks */ \
     X(mxfa_rotary_b) X(mxfa_rotary_b4) X(mxfa_rotary_b1) X(mxfa_rotary_f) X(mxfa_rotary_f1)   \

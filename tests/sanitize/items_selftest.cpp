@@ -119,7 +119,7 @@ static void check_many(BatchParams p, int bf16, bool sound) {
                 const int k = (int)(r() % 4);
                 *x = k == 0 ? (int)r() : k == 1 ? (int)(r() % 300) : k == 2 ? 0 : INT_MAX;
             }
-            if (!note_holds(p, n, f.rows)) continue;
+            if (!note_holds(p, n)) continue;
             CHECK(n.slot >= 0 && n.slot + (n.shares - 1LL) * p.Hkv < f.slots, "slots %d + %d", n.slot, n.shares);
             CHECK(n.q0 >= 0 && n.q0 + (long long)(n.rows - 1) / p.group < p.n_tok, "rows %d from %d", n.rows, n.q0);
         }
@@ -139,7 +139,7 @@ static void check_many(BatchParams p, int bf16, bool sound) {
             CHECK(x.split >= 0 && x.split < total, "split unit %d of %d", x.split, total);
             CHECK(joined.emplace(x.split, x).second, "split unit %d twice", x.split);
             const ManyNote n{x.shares, x.slot, x.s.q0, x.s.rows, x.unit, x.head, {0, 0}};
-            CHECK(note_holds(p, n, f.rows), "the note of split unit %d", x.split);
+            CHECK(note_holds(p, n), "the note of split unit %d", x.split);
         }
     }
     CHECK((int)joined.size() == total, "%zu joins for %d split units", joined.size(), total);
@@ -291,8 +291,8 @@ int main() {
         batch_plan(&p, bf16);
         if (p.few_rows > 0) check_few(p, sound);
         if (batch_may_be_many(p)) {
-            if (bf16) check_many<batch_many_rows(true)>(p, bf16, sound);
-            else check_many<batch_many_rows(false)>(p, bf16, sound);
+            if (p.many_rows == 64) check_many<64>(p, bf16, sound);
+            else check_many<128>(p, bf16, sound);
         } else if (sound) {
             for (int s = 0; s < p.n_seq; ++s) CHECK((batch_seq<false, 64>(p, s).rows == 0), "rows that no form takes");
         }

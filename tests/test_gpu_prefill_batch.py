@@ -85,6 +85,16 @@ def test_more_units_than_cus_that_stay_whole(pairs):
     check(b, *run(b))
 
 
+@pytest.mark.parametrize("pairs,nh,nkv,hd", [
+    ([(400, 1500)], 14, 2, 64), ([(350, 900), (64, 2000)], 14, 2, 64),    # units of 64 rows
+    ([(900, 1100)] * 4 + [(1, 40)], 14, 2, 64),                          # of 128
+    ([(1100, 1200)], 4, 1, 128), ([(600, 700)] * 2, 32, 4, 128),
+    ([(129, 1400), (1, 3000), (1, 200), (1, 64)], 14, 2, 64)])           # beside few rows
+def test_unit_sizes(pairs, nh, nkv, hd):
+    b = Batch(pairs, nh, nkv, hd, 16, True, seed=hd)
+    check(b, *run(b))
+
+
 @pytest.mark.parametrize("n_seq", [63, 64, 65, 130])
 def test_many_sequences(n_seq):
     """More sequences than a wave's lanes, some without new tokens."""
