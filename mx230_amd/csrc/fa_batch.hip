@@ -8,16 +8,33 @@
 // one pass over the keys with the running maximum m and sum. A sequence's rows
 // of one KV head are its new tokens times the head's query heads (row r: token
 // r / group, query head r % group), so that a key that is read serves the whole
-// group. Two forms take them in units of rows:
-//   * few (at most 16 rows): every wave holds the same rows and takes 64-key
-//     stages of its own; bound by the reads of K and V;
-//   * many: 128 rows (fp32: 64), 32 (16) per wave, the waves sharing each stage; bound by the
-//     matrix products.
-// The host knows neither lengths nor units: a work-group finds its item (a
-// unit's share of its keys) from cu_q and lens itself (find_item). A unit is
-// split over its keys where the whole work, spread over the target count of
-// items, gives each less than the unit has; its shares' unnormalised outputs
-// are then joined by a second launch, in a fixed order.
+// group. Sums, maxima and O are fp32; in bf16 p is rounded to bf16 for the product
+// with V (relative 2^-8 at most, each p by itself), as the matrix instruction takes
+// it, and its sum is of the values before that. fp32 operands keep 24 bits.
+//
+// Two forms take a sequence's rows in units:
+//   * few (at most 16 rows, one unit): every wave holds the same rows and takes
+//     64-key stages of its own; bound by the reads of K and V;
+//   * many: units of 128 or (bf16) 64 rows, the waves sharing each stage; bound by
+//     the matrix products.
+// The host knows neither lengths nor units, only the buffers' sizes: a work-group
+// finds its part of the work from cu_q and lens itself (fa_batch_items.h has the
+// arithmetic). Where a sequence's or unit's keys are several work-groups', their
+// unnormalised outputs are joined by a second launch, in a fixed order, so equal
+// calls give equal bits. A counter per unit would save that launch (4 to 7 us), but
+// has to be cleared before each call, and an only reader per unit of up to 128
+// parts takes longer than the many of the launch.
+//
+// Measured (us; the rates count the keys each sequence has once, or the products of
+// the positions that rows see):
+//   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: 385 and
+//         the join 6 (5.7 TB/s; a plain read of all memory reaches 6.4);
+//         one token after 4095, 32/4 heads, d = 64: 7.1 and 4.5;
+//   many: 2048 tokens after 30720, 32/8 heads, d = 128: 960 (1110 TFLOP/s; a large
+//         library product 1173); 4096 tokens, 32/4 heads, d = 64: 88 (780);
+//         fp32, 2000 tokens after 2096, 14/2 heads: 179 (124; in fp32 150);
+//   both: 28 single tokens and 4 chunks of up to 512, to 8192 long, 14/2 heads,
+//         d = 64: 48.5 and the join 7 (one after the other: 41 and 18).
 #include <algorithm>
 #include <type_traits>
 
@@ -34,8 +51,8 @@ namespace mxfa {
 // ------------------------------------------------- fp32 on its own instructions
 
 // fp32 inputs (d = 64) on v_mfma_f32_16x16x4_f32, in the policy form of
-// fwd_stage, for the few-row form, which the reads bound. LDS rows of 256 bytes hold their 16-byte chunk c at c ^ (row & 15),
-// so the 16 rows of a score operand and the 16 chunks of a V row both cover
+// fwd_stage, for the few-row form, which the reads bound. LDS rows of 256 bytes
+// hold their 16-byte chunk c at c ^ (row & 15), so the 16 rows of a score operand and the 16 chunks of a V row both cover
 // all banks. Score k-steps: MFMA (c, e) takes element 16c + 4g + e of lane
 // group g. In the chained product a lane reads 4 columns of a V row at once, so
 // tile xt's row 4g + r of O^T is column 4 (4g + r) + xt.
@@ -321,8 +338,8 @@ __device__ __forceinline__ f32x4 batch_quad(const f32x4 (&acc)[XT][QT], int i, i
 // A unit's share in plain fp32 arithmetic, keys a row does not see left out
 // altogether: taken where a value was not finite, since in the matrix products
 // an infinity or NaN in the V of a key that a row does not see reaches it as 0
-// x inf. 4 threads per row, rows from row0 of the unit. A row's running (max, sum) and output go where
-// the form's would: to the workspace slot, or (part null) finished.
+// x inf. 4 threads per row, rows from row0 of the unit. Some 6 times the time of the
+// products. A row's running (max, sum) and output go where the form's would: to the workspace slot, or (part null) finished.
 template <class T, int D, int ROWS>
 __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchItem &it, int row0, int key0, int key1,
                                             float *part, float *ml) {
@@ -401,6 +418,11 @@ union BatchFewSmem {
 // sums and O meet in LDS. The stage's blocks come through LDS too, two stages
 // ahead: as loads into registers the compiler would wait for them with
 // vmcnt(0), and with them for every staging load in flight.
+//
+// Bound by the reads: 128 KB of tiles in flight per CU (8 waves of 16 KB, d = 128: 4
+// of 32), and nothing but the next tile's loads between two waits. us, 64 sequences
+// of 2000-16384 positions, 32/8 heads, d = 128: 411 where a load reads whole rows,
+// 510 by 32 bytes of each of 32 rows.
 template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
                                                 BatchFewSmem<Pol, NW> &sm) {
@@ -518,7 +540,10 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
     }
 }
 
-// Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line.
+// Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line. Equal
+// runs, one work-group to a CU (its tiles take the LDS): 64 sequences of 2000-16384
+// positions in 393 us with the join, 415 with a work-group per share of a sequence
+// (d = 64: 471 and 504), whose count the host can only bound: thousands are empty.
 template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
     const unsigned all = few_line(p), run = few_run(p, all);
@@ -552,6 +577,9 @@ struct BatchManySmem {
     int bad[4];
 };
 
+// One unit's share, 16 QT rows per wave: K and V double-buffered in LDS, staged by
+// all four waves and read by each. 2048 tokens after 30720, 32/8 heads, d = 128: 960
+// us, 1110 TFLOP/s.
 template <class Pol, int QT>
 __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
     using T = typename Pol::T;
@@ -699,8 +727,9 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
 // (Split3): K and V pass through registers, loaded one stage ahead, and are
 // split once per work-group into one LDS buffer; two work-groups per CU. Operands
 // that the parts cannot hold (kPartMin, infinities) flag the unit, whose rows
-// are then run in plain arithmetic. 2000 tokens of 14/2 heads after 2096, us: on
-// v_mfma_f32_16x16x4_f32 235, parts with 4 waves and 64 rows 203.
+// are then run in plain arithmetic. Bound by the splitting beside the products. us,
+// 2000 tokens of 14/2 heads after 2096: 176; 203 with 4 waves and 64 rows; on
+// v_mfma_f32_16x16x4_f32 235.
 __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block, FwdSplitSmem &sm) {
     constexpr int D = 64, XT = 4, BK = 64, NW = kBatchF32Waves, NT = 64 * NW, ROWS = 16 * NW;
     using PL = PolBF16<64>;  // the parts' layout
@@ -896,7 +925,9 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
 // group of D / 4 threads, four elements each, has a row; where there are few
 // rows several groups take turns over its parts and meet in LDS. Bound by
 // latency: the (max, sum) pairs of all parts are one round of loads, and eight
-// parts of a thread's turn another.
+// parts of a thread's turn another. us, one token after 65535, 14/2 heads (128 parts
+// of 7 rows): 7.4, and 11.2 with one group to a row; 28 tokens and 4 chunks: 7.2
+// with the notes, 12.8 where each work-group found its unit in the lengths.
 template <class T, int D, class At>
 __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int rows, int first, int end,
                                                 int S, float *parts, int slots, At at) {
@@ -1005,7 +1036,9 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
 // Both forms in one launch: the few-row form's work-groups first, each wave's
 // tiles a quarter of its work-group's (bf16, d = 64) or half of it, so that LDS
 // holds as many of them as of the many-row form's: their reads and its matrix
-// products then share the CUs.
+// products then share the CUs (us, 28 tokens and 4 chunks: 48.5; 41 + 17 in two
+// launches). In fp32 the few-row form has to spill at the other's 128 registers; two
+// launches took the same (6 tokens and 2 chunks: 13 + 55 and 55).
 template <int QT, class Pol>
 __device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
     batch_many_body<Pol, QT>(p, block, sm);
