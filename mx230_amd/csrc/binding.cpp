@@ -327,40 +327,56 @@ at::Tensor rows16(const at::Tensor &x) {
     return good ? x : x.contiguous();
 }
 
+// Q and K turned, in new tensors.
+struct RotaryOptions {
+    int64_t pos0;
+    bool interleaved;
+    double factor;
+    bool inverse;
+};
+torch::autograd::variable_list turned(const at::Tensor &q0, const at::Tensor &k0, const at::Tensor &f,
+                                      const at::Tensor *pos, const RotaryOptions &o) {
+    const at::Tensor q = rows16(q0), k = rows16(k0);
+    at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    const RotaryArgs r{&q, &k, &qo, &ko, &f, pos};
+    mxfa_rotary_shape s{};
+    TORCH_CHECK_VALUE(r.shape(&s), "rotary_embedding: tensors that do not fit together or are on another device");
+    s.pos0 = (int)o.pos0;
+    s.interleaved = o.interleaved;
+    s.factor = (float)o.factor;
+    s.inverse = o.inverse;
+    const int rc = r.run(s);
+    TORCH_CHECK(rc == 0, "rotary_embedding: mxfa_run_rotary returned ", rc);
+    return {qo, ko};
+}
+
 // The differentiable rotation (autograd.rotary_embedding): its gradient is the
 // transposed rotation of the outputs' gradients, itself such a node where a
 // graph of it is asked for.
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q0,
-                                                  const at::Tensor &k0, const at::Tensor &f,
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q,
+                                                  const at::Tensor &k, const at::Tensor &f,
                                                   const std::optional<at::Tensor> &pos,
                                                   int64_t pos0, bool interleaved, double factor, bool inverse) {
         ctx->save_for_backward({f, pos ? *pos : at::Tensor()});
-        ctx->saved_data["pos0"] = pos0;
-        ctx->saved_data["interleaved"] = interleaved;
-        ctx->saved_data["factor"] = factor;
-        ctx->saved_data["inverse"] = inverse;
-        const at::Tensor q = rows16(q0), k = rows16(k0);
-        at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
-        const RotaryArgs r{&q, &k, &qo, &ko, &f, pos ? &*pos : nullptr};
-        mxfa_rotary_shape s{};
-        TORCH_CHECK_VALUE(r.shape(&s), "rotary_embedding: tensors that do not fit together or are on another device");
-        s.pos0 = (int)pos0;
-        s.interleaved = interleaved;
-        s.factor = (float)factor;
-        s.inverse = inverse;
-        const int rc = r.run(s);
-        TORCH_CHECK(rc == 0, "rotary_embedding: mxfa_run_rotary returned ", rc);
-        return {qo, ko};
+        ctx->saved_data["options"] = std::make_tuple(pos0, interleaved, factor, inverse);
+        return turned(q, k, f, pos ? &*pos : nullptr, RotaryOptions{pos0, interleaved, factor, inverse});
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list g) {
         const auto saved = ctx->get_saved_variables();
-        std::optional<at::Tensor> pos;
-        if (saved[1].defined()) pos = saved[1];
-        auto out = apply(g[0], g[1], saved[0], pos, ctx->saved_data["pos0"].toInt(),
-                         ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(),
-                         !ctx->saved_data["inverse"].toBool());
+        const auto o = ctx->saved_data["options"].toTuple();
+        const auto &e = o->elements();
+        const RotaryOptions back{e[0].toInt(), e[1].toBool(), e[2].toDouble(), !e[3].toBool()};
+        const bool given = saved[1].defined();
+        torch::autograd::variable_list out;
+        if (c10::GradMode::is_enabled()) {
+            std::optional<at::Tensor> pos;
+            if (given) pos = saved[1];
+            out = apply(g[0], g[1], saved[0], pos, back.pos0, back.interleaved, back.factor, back.inverse);
+        } else {
+            out = turned(g[0], g[1], saved[0], given ? &saved[1] : nullptr, back);
+        }
         const at::Tensor none;
         return {out[0], out[1], none, none, none, none, none, none};
     }
