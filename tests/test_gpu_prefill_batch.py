@@ -7,6 +7,7 @@ sequence's."""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -210,6 +211,31 @@ def test_numbers_past_32_bits():
     x = torch.zeros(1, 2, 3, 64, device="cuda")
     with pytest.raises(ValueError, match="past 32 bits"):
         mx.run_rotary(x, None, x, None, f, pos0=2 ** 32)
+
+
+@pytest.mark.parametrize("fill", [0, 1, 0x7f, 0xff])
+@pytest.mark.parametrize("pairs", [[(1, 5000), (1, 70), (2, 2500)], [(200, 4000), (1, 3000), (1, 9), (1, 6000)], [(300, 5000)],
+                                   [(1, 3000)] * 3 + [(0, 0)]])
+def test_what_the_workspace_holds_before(pairs, fill):
+    """Whatever it is, notes of another call among it: outputs are those of a fresh one."""
+    b = Batch(pairs, 14, 2, 64, 16, True, seed=len(pairs))
+    other = Batch([(120, 6000), (1, 5000), (1, 40)], 14, 2, 64, 16, True, seed=5)
+    n = max(mx.prefill_batch_workspace_bytes(x.n_tok, len(x.pairs), 300, 14, 2, 64) for x in (b, other))
+    ws = torch.full((n,), fill, dtype=torch.uint8, device="cuda")
+    got, glse = run(b, max_q=300, workspace=ws)
+    want, wlse = run(b, max_q=300)
+    check(b, got, glse)
+    assert torch.equal(got, want) and torch.equal(glse, wlse)
+    run(other, max_q=300, workspace=ws)
+    again, _ = run(b, max_q=300, workspace=ws)
+    assert torch.equal(again, want)
+
+
+def test_hundreds_of_sequences():
+    r = random.Random(4)
+    pairs = [(n, r.randint(max(n, 1), 700)) for n in (r.choice([0, 1, 1, 1, 1, 2, 40]) for _ in range(700))]
+    b = Batch(pairs, 4, 2, 64, 16, True, seed=3)
+    check(b, *run(b))
 
 
 def test_max_q_bounds_the_rows():
