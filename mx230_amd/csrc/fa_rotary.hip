@@ -10,8 +10,7 @@
 // thread has one unit of a row, two 16-byte chunks of pairs or one of the
 // copied rest, computes its angles once and walks hpt heads with them: no table
 // of cosines is read or kept, and the angles' 64-bit arithmetic hides behind the
-// loads (20 us at B4, 12 + 12 heads, N4096, d = 64 bf16: 100 MB at 5.1 TB/s, the rate
-// of a copy).
+// first loads (B4, 12 + 12 heads, N4096, d = 64 bf16, 100 MB: 18 us, a copy 20).
 #include <algorithm>
 
 #include "fa_cache.h"
@@ -137,21 +136,19 @@ __host__ __device__ constexpr int rotary_units(int d, int dim) {
     return dim / (2 * VEC) + (d - dim) / VEC;
 }
 
-// Unit u of a row: where its chunks lie, and its angles at `pos`.
+// Unit u of a row: where its chunks lie, and, once `at` was called, its angles at a
+// position.
 template <class T, int VEC>
 struct Unit {
     int e0, e1;  // first elements of the chunks (e1 < 0: a single chunk, copied)
     float c[VEC], s[VEC];
-    __device__ __forceinline__ Unit(int u, int dim, int interleaved, const double *freq, int pos, float factor,
-                                    float sin_sign) {
+    __device__ __forceinline__ Unit(int u, int dim, int interleaved) {
         const int nr = dim / (2 * VEC);
-        if (u >= nr) {
-            e0 = dim + (u - nr) * VEC;
-            e1 = -1;
-            return;
-        }
-        e0 = interleaved ? 2 * VEC * u : VEC * u;
-        e1 = interleaved ? e0 + VEC : e0 + dim / 2;
+        e0 = u >= nr ? dim + (u - nr) * VEC : interleaved ? 2 * VEC * u : VEC * u;
+        e1 = u >= nr ? -1 : interleaved ? e0 + VEC : e0 + dim / 2;
+    }
+    __device__ __forceinline__ void at(int u, const double *freq, int pos, float factor, float sin_sign) {
+        if (e1 < 0) return;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             turn_angle((double)pos * (freq[VEC * u + e] * kTurn), c[e], s[e]);
@@ -161,8 +158,34 @@ struct Unit {
     }
 };
 
-// Heads in flight per thread: their loads go out together.
+// A thread's heads h0 .. h1 - 1 of a row, the chunks at e0 and (e1 >= 0) e1 of each:
+// from(h) is where head h is read, put(h, x, y) turns and stores it. The loads of
+// kHeadsAhead heads go out together, and the first of them before first(), which
+// finds what put needs.
 constexpr int kHeadsAhead = 4;
+template <class T, int VEC, class From, class First, class Put>
+__device__ __forceinline__ void walk_heads(int h0, int h1, int e0, int e1, From from, First first, Put put) {
+    Chunk<T, VEC> x[kHeadsAhead], y[kHeadsAhead];
+    auto load = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kHeadsAhead; ++j) {
+            if (h + j >= h1) break;
+            const T *row = from(h + j);
+            x[j].load(row + e0);
+            if (e1 >= 0) y[j].load(row + e1);
+        }
+    };
+    load(h0);
+    first();
+    for (int h = h0; h < h1; h += kHeadsAhead) {
+        if (h > h0) load(h);
+#pragma unroll
+        for (int j = 0; j < kHeadsAhead; ++j) {
+            if (h + j >= h1) break;
+            put(h + j, x[j], y[j]);
+        }
+    }
+}
 
 // Grid: (units of all tokens in work-groups of 256, heads of Q then K in
 // groups of hpt, batches).
@@ -173,33 +196,28 @@ __device__ __forceinline__ void rotary_body(const RotaryParams &p) {
     const int n = (int)(i / (unsigned)U), u = (int)(i - (unsigned)n * (unsigned)U);
     if (n >= p.N) return;
     const int b = blockIdx.z;
-    const int pos = p.positions != nullptr ? p.positions[b * p.pos_bs + n] : p.pos0 + n;
-    const Unit<T, VEC> un(u, p.dim, p.interleaved, p.freq, pos, p.factor, p.sin_sign);
+    Unit<T, VEC> un(u, p.dim, p.interleaved);
     const int h0 = (int)blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H[0] + p.H[1]);
-    for (int h = h0; h < h1; h += kHeadsAhead) {
-        Chunk<T, VEC> x[kHeadsAhead], y[kHeadsAhead];
-#pragma unroll
-        for (int k = 0; k < kHeadsAhead; ++k) {
-            if (h + k >= h1) break;
-            const int t = h + k >= p.H[0], hh = h + k - (t ? p.H[0] : 0);
+    walk_heads<T, VEC>(
+        h0, h1, un.e0, un.e1,
+        [&](int h) __attribute__((always_inline)) {
+            const int t = h >= p.H[0], hh = h - (t ? p.H[0] : 0);
             const HeadView &v = p.x[t];
-            const T *row = static_cast<const T *>(v.in) + b * v.in_bs + hh * v.in_hs + n * v.in_ts;
-            x[k].load(row + un.e0);
-            if (un.e1 >= 0) y[k].load(row + un.e1);
-        }
-#pragma unroll
-        for (int k = 0; k < kHeadsAhead; ++k) {
-            if (h + k >= h1) break;
-            const int t = h + k >= p.H[0], hh = h + k - (t ? p.H[0] : 0);
+            return static_cast<const T *>(v.in) + b * v.in_bs + hh * v.in_hs + n * v.in_ts;
+        },
+        [&]() __attribute__((always_inline)) {
+            un.at(u, p.freq, p.positions != nullptr ? p.positions[b * p.pos_bs + n] : p.pos0 + n, p.factor, p.sin_sign);
+        },
+        [&](int h, Chunk<T, VEC> &x, Chunk<T, VEC> &y) __attribute__((always_inline)) {
+            const int t = h >= p.H[0], hh = h - (t ? p.H[0] : 0);
             const HeadView &v = p.x[t];
             T *row = static_cast<T *>(v.out) + b * v.out_bs + hh * v.out_hs + n * v.out_ts;
             if (un.e1 >= 0) {
-                turn<T, VEC>(x[k], y[k], un.c, un.s, p.interleaved);
-                y[k].store(row + un.e1);
+                turn<T, VEC>(x, y, un.c, un.s, p.interleaved);
+                y.store(row + un.e1);
             }
-            x[k].store(row + un.e0);
-        }
-    }
+            x.store(row + un.e0);
+        });
 }
 
 // The cache append: rows of [Q heads | K heads | V heads] of new tokens; Q is
@@ -208,69 +226,56 @@ __device__ __forceinline__ void rotary_body(const RotaryParams &p) {
 // it first finds each token's sequence: every sequence that has tokens among
 // them writes its index beside those, so the search costs one load of cu_q
 // instead of a bisection's chain of them. Bound by memory where there are many
-// tokens (5400 of 32/8 heads, d = 128: 25 us, 5.3 TB/s), by the chain of loads cu_q, length,
+// tokens (5400 of 32/8 heads, d = 128, 132 MB: 23.5 us, 32 from memory that no cache
+// holds, where a copy takes 26), by the chain of loads cu_q, length,
 // block, row where there are few (16 of 14/2 heads: 4.1 us).
 template <class T, int VEC>
 __device__ __forceinline__ void append_body(const BatchParams &p) {
-    const int U = rotary_units<VEC>(p.d, p.dim), tid = threadIdx.x;
-    const int per = 256 / U;  // a row has at most 255 units
-    __shared__ int seq_of[256], pos_of[256];
-    __shared__ long long row_of[256];
+    const int U = rotary_units<VEC>(p.d, p.dim), tid = threadIdx.x;  // (U is at most 255)
+    const int per = 256 / U;
+    __shared__ int seq_of[256];
     const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, p.n_tok);
-    if (tid < per) seq_of[tid] = -1;
-    __syncthreads();
-    for (int s = tid; s < p.n_seq; s += 256) {
-        const int lo = max(p.cu_q[s], t0), hi = min(p.cu_q[s + 1], t1);
-        for (int t = lo; t < hi; ++t) seq_of[t - t0] = s;
-    }
-    __syncthreads();
-    if (tid < t1 - t0) {
-        const int s = seq_of[tid];
-        long long row = -1;
-        int pos = -1;
-        if (s >= 0) {
-            pos = p.lens[s] - p.cu_q[s + 1] + t0 + tid;
-            const int blk = pos >> p.bs_shift;
-            if (pos >= 0 && blk < p.max_blocks) {
-                const int e = p.table[(long long)s * p.table_stride + blk];
-                if ((unsigned)e < (unsigned)p.n_blocks)
-                    row = ((long long)e << p.bs_shift) + (pos & ((1 << p.bs_shift) - 1));
-            }
-        }
-        pos_of[tid] = pos;
-        row_of[tid] = row;
-    }
-    __syncthreads();
-    const int H = p.Hq + 2 * p.Hkv;
-    const int h0 = (int)blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, H);
     const int k = tid / U, u = tid - k * U, t = t0 + k;
-    if (k >= per || t >= t1 || pos_of[k] < 0) return;
-    const long long crow = row_of[k];
-    const Unit<T, VEC> un(u, p.dim, p.interleaved, p.freq, pos_of[k], p.factor, 1.0f);
+    const bool mine = k < per && t < t1;  // (every thread takes part in the search)
+    const int h0 = (int)blockIdx.y * p.hpt, h1 = mine ? min(h0 + p.hpt, p.Hq + 2 * p.Hkv) : h0;
     const T *in = static_cast<const T *>(p.q) + (long long)t * p.q_rs;
-    for (int h = h0; h < h1; h += kHeadsAhead) {
-        Chunk<T, VEC> x[kHeadsAhead], y[kHeadsAhead];
-#pragma unroll
-        for (int j = 0; j < kHeadsAhead; ++j) {
-            if (h + j >= h1) break;
-            x[j].load(in + (h + j) * p.d + un.e0);
-            if (un.e1 >= 0) y[j].load(in + (h + j) * p.d + un.e1);
+    Unit<T, VEC> un(u, p.dim, p.interleaved);
+    int pos = -1;
+    long long crow = -1;
+    auto search = [&]() __attribute__((always_inline)) {
+        if (tid < per) seq_of[tid] = -1;
+        __syncthreads();
+        for (int s = tid; s < p.n_seq; s += 256) {
+            const int lo = max(p.cu_q[s], t0), hi = min(p.cu_q[s + 1], t1);
+            for (int i = lo; i < hi; ++i) seq_of[i - t0] = s;
         }
-#pragma unroll
-        for (int j = 0; j < kHeadsAhead; ++j) {
-            if (h + j >= h1) break;
-            const int hh = h + j, kv = hh - p.Hq;
-            if (kv >= 0 && crow < 0) continue;
-            T *row = kv < 0 ? static_cast<T *>(p.o) + (long long)t * p.o_rs + hh * p.d
+        __syncthreads();
+        if (!mine || seq_of[k] < 0) return;
+        const int s = seq_of[k];
+        pos = p.lens[s] - p.cu_q[s + 1] + t;
+        if (pos < 0) return;
+        const int blk = pos >> p.bs_shift;
+        if (blk < p.max_blocks) {
+            const int e = p.table[(long long)s * p.table_stride + blk];
+            if ((unsigned)e < (unsigned)p.n_blocks)
+                crow = ((long long)e << p.bs_shift) + (pos & ((1 << p.bs_shift) - 1));
+        }
+        un.at(u, p.freq, pos, p.factor, 1.0f);
+    };
+    walk_heads<T, VEC>(
+        h0, h1, un.e0, un.e1, [&](int h) __attribute__((always_inline)) { return in + h * p.d; }, search,
+        [&](int h, Chunk<T, VEC> &x, Chunk<T, VEC> &y) __attribute__((always_inline)) {
+            const int kv = h - p.Hq;
+            if (pos < 0 || (kv >= 0 && crow < 0)) return;
+            T *row = kv < 0 ? static_cast<T *>(p.o) + (long long)t * p.o_rs + h * p.d
                      : kv < p.Hkv ? static_cast<T *>(p.k) + crow * p.kv_rs + kv * p.d
                                   : static_cast<T *>(p.v) + crow * p.kv_rs + (kv - p.Hkv) * p.d;
             if (un.e1 >= 0) {
-                if (kv < p.Hkv) turn<T, VEC>(x[j], y[j], un.c, un.s, p.interleaved);
-                y[j].store(row + un.e1);
+                if (kv < p.Hkv) turn<T, VEC>(x, y, un.c, un.s, p.interleaved);
+                y.store(row + un.e1);
             }
-            x[j].store(row + un.e0);
-        }
-    }
+            x.store(row + un.e0);
+        });
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -285,11 +290,12 @@ MXFA_ROTARY(f1, float, 1)
 #undef MXFA_ROTARY
 #endif
 
-// Heads per thread: as many as leave 2^17 threads (8 waves on each SIMD's
-// CU), so that a thread's angles serve many heads of a large call and a small
-// one still spreads over the GPU.
+// Heads per thread: as many as leave 2^18 threads (4 waves on each SIMD), so that a
+// thread's angles serve many heads of a large call and a small one still spreads
+// over the GPU. us, 5400 tokens of 32/8 heads, d = 128, from memory that no cache
+// holds: 32.5 (2^17: 36, 2^19: 36).
 static int heads_per_thread(long long units, int heads) {
-    const long long want = units * heads / (1 << 17);
+    const long long want = units * heads / (1 << 18);
     return (int)std::clamp<long long>(want, 1, heads);
 }
 
