@@ -18,7 +18,7 @@
 
 namespace mxfa {
 
-// cos and sin of a whole angle given in turns, |result error| below 1e-7: the
+// cos and sin of a whole angle given in turns, off by about 1.2e-7 at most: the
 // position times the frequency is formed and reduced to [-1/8, 1/8] turns in
 // 64 bits (in 32 a position of 2^20 would be off by 0.06 radians), then
 // Taylor's series, whose first terms left out are z^11 / 11! <= 1.8e-9 and
@@ -27,7 +27,7 @@ __device__ __forceinline__ void turn_angle(double turns, float &c, float &s) {
     turns -= __builtin_rint(turns);
     const double quarter = __builtin_rint(4.0 * turns);
     const float z = 6.283185307179586f * (float)__builtin_fma(-0.25, quarter, turns);
-    const int q = (int)quarter & 3;  // -2 .. 2
+    const int q = (int)quarter & 3;  // (quarter: -2 .. 2)
     const float w = z * z;
     float sn = __builtin_fmaf(w, 2.75573192e-6f, -1.98412698e-4f);
     sn = __builtin_fmaf(w, sn, 8.33333333e-3f);
