@@ -76,8 +76,9 @@ __device__ __forceinline__ void pages_free_body(const PagesParams &p, const int 
 // named for the first time, a parent that exists, a free block where the last
 // one must be copied), the copies in the order of the pairs, from the lowest
 // free blocks up, and the children's lengths and last blocks.
+template <class Share>
 __device__ __forceinline__ void pages_fork_plan(const PagesParams &p, const int *parents, const int *children, int m,
-                                                int *pairs, int *status, int *counts) {
+                                                int *pairs, int *status, int *counts, Share share) {
     __shared__ int sums[kPlan / 64];
     const int tid = threadIdx.x, part = (1 << p.bs_shift) - 1;
     // the parent's length where the pair may be taken, else -1
@@ -167,21 +168,28 @@ __device__ __forceinline__ void pages_fork_plan(const PagesParams &p, const int 
         counts[0] = found;
         counts[1] = refused + need - found;
     }
+    __syncthreads();
+    share();
 }
 
-// The fork's rows, a work-group per pair: the parent's whole blocks are shared.
+// Entry j of pair i's rows: a whole block of the parent is shared.
+__device__ __forceinline__ void pages_fork_entry(const PagesParams &p, const int *parents, const int *children,
+                                                 const int *status, int i, int j) {
+    if (status[i] != 0) return;
+    const int c = children[i];
+    if (j >= load_now(p.lens + c) >> p.bs_shift) return;
+    const int b = p.table[(long long)parents[i] * p.table_stride + j];
+    p.table[(long long)c * p.table_stride + j] = b;
+    if ((unsigned)b < (unsigned)p.n_blocks) atomicAdd(p.refs + b, 1);
+}
+
+// The fork's rows where they are many, a work-group per pair.
 __device__ __forceinline__ void pages_fork_rows(const PagesParams &p, const int *parents, const int *children,
                                                 const int *status) {
     const int i = blockIdx.x;
     if (status[i] != 0) return;
-    const int a = parents[i], c = children[i], n = p.lens[c] >> p.bs_shift;
-    const int *from = p.table + (long long)a * p.table_stride;
-    int *to = p.table + (long long)c * p.table_stride;
-    for (int j = threadIdx.x; j < n; j += 256) {
-        const int b = from[j];
-        to[j] = b;
-        if ((unsigned)b < (unsigned)p.n_blocks) atomicAdd(p.refs + b, 1);
-    }
+    const int n = p.lens[children[i]] >> p.bs_shift;
+    for (int j = threadIdx.x; j < n; j += 256) pages_fork_entry(p, parents, children, status, i, j);
 }
 
 // The compaction's plan, one work-group: with L used blocks in all, the j-th
@@ -297,8 +305,13 @@ extern "C" __global__ __launch_bounds__(256) void mxfa_pages_free(PagesParams p,
 }
 extern "C" __global__ __launch_bounds__(kPlan) void mxfa_pages_fork_plan(PagesParams p, const int *parents,
                                                                          const int *children, int m, int *pairs,
-                                                                         int *status, int *counts) {
-    pages_fork_plan(p, parents, children, m, pairs, status, counts);
+                                                                         int *status, int *counts, int rows) {
+    pages_fork_plan(p, parents, children, m, pairs, status, counts, [&]() __attribute__((always_inline)) {
+        for (int x = threadIdx.x; x < rows; x += kPlan) {
+            const int i = x / p.max_blocks;
+            pages_fork_entry(p, parents, children, status, i, x - i * p.max_blocks);
+        }
+    });
 }
 extern "C" __global__ __launch_bounds__(256) void mxfa_pages_fork_rows(PagesParams p, const int *parents,
                                                                        const int *children, const int *status) {
@@ -326,12 +339,18 @@ hipError_t launch_pages_free(const PagesParams &p, const int *rows, int n, hipSt
     return launch_kernel(k_mxfa_pages_free, dim3(n), dim3(256), args, stream);
 }
 
+// Entries of all pairs' rows up to which the plan's work-group shares the blocks
+// itself instead of a second launch. us, rows ended and forked again: 4 pairs of 64
+// blocks 9.0 (two launches 11.0), 8 of 256 11.7 (11.8), 16 of 256 14.5 (11.8).
+constexpr int kForkOwn = 2048;
 hipError_t launch_pages_fork(const PagesParams &p, const int *parents, const int *children, int n, int *pairs,
                              int *status, int *counts, hipStream_t stream) {
     PagesParams q = p;
-    void *plan[] = {&q, &parents, &children, &n, &pairs, &status, &counts};
+    const long long entries = (long long)n * p.max_blocks;
+    int own = entries <= kForkOwn ? (int)entries : 0;
+    void *plan[] = {&q, &parents, &children, &n, &pairs, &status, &counts, &own};
     const hipError_t e = launch_kernel(k_mxfa_pages_fork_plan, dim3(1), dim3(kPlan), plan, stream);
-    if (e != hipSuccess || n == 0) return e;
+    if (e != hipSuccess || entries == own) return e;
     void *rows[] = {&q, &parents, &children, &status};
     return launch_kernel(k_mxfa_pages_fork_rows, dim3(n), dim3(256), rows, stream);
 }

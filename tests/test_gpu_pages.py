@@ -85,6 +85,19 @@ def test_fork(seed):
     assert (t.tolist(), ln.tolist(), rf.tolist()) == want[2:]
 
 
+@pytest.mark.parametrize("entries", [1, 255, 256, 257, 700])
+def test_fork_long_rows(entries):
+    """Rows shared by the plan's own launch (8 pairs of up to 256 entries) and by a second."""
+    r = random.Random(entries)
+    lens = [16 * entries, max(1, 16 * entries - 5)] + [0] * 8
+    table, lens, refs, _ = make(r, lens, 16, 2 * entries + 9, entries)
+    parents, children = [0, 1] * 4, list(range(2, 10))
+    want = plain_fork(table, lens, refs, 16, parents, children)
+    t, ln, rf, pairs, status, counts = fork(table, lens, refs, 16, parents, children)
+    assert status.tolist() == want[0] and pairs[:len(want[1])].tolist() == want[1]
+    assert (t.tolist(), ln.tolist(), rf.tolist()) == want[2:]
+
+
 def test_fork_more_pairs_than_threads():
     r = random.Random(9)
     n = 3000
