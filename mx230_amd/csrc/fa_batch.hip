@@ -30,7 +30,7 @@
 //   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: 385 and
 //         the join 6 (5.7 TB/s; a plain read of all memory reaches 6.4);
 //         one token after 4095, 32/4 heads, d = 64: 7.1 and 4.5;
-//   many: 2048 tokens after 30720, 32/8 heads, d = 128: 960 (1110 TFLOP/s; a large
+//   many: the last 2048 tokens of 32768, 32/8 heads, d = 128: 960 (1110 TFLOP/s; a large
 //         library product 1173); 4096 tokens, 32/4 heads, d = 64: 88 (780);
 //         fp32, 2000 tokens after 2096, 14/2 heads: 179 (124; in fp32 150);
 //   both: 28 single tokens and 4 chunks of up to 512, to 8192 long, 14/2 heads,
@@ -578,7 +578,7 @@ struct BatchManySmem {
 };
 
 // One unit's share, 16 QT rows per wave: K and V double-buffered in LDS, staged by
-// all four waves and read by each. 2048 tokens after 30720, 32/8 heads, d = 128: 960
+// all four waves and read by each. the last 2048 tokens of 32768, 32/8 heads, d = 128: 960
 // us, 1110 TFLOP/s.
 template <class Pol, int QT>
 __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
