@@ -578,7 +578,7 @@ struct BatchManySmem {
 };
 
 // One unit's share, 16 QT rows per wave: K and V double-buffered in LDS, staged by
-// all four waves and read by each. the last 2048 tokens of 32768, 32/8 heads, d = 128: 960
+// all four waves and read by each. The last 2048 of 32768 tokens, 32/8 heads, d = 128: 960
 // us, 1110 TFLOP/s.
 template <class Pol, int QT>
 __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
