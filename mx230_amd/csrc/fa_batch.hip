@@ -169,18 +169,23 @@ struct BatchRows {
 
 // The loads of one 64-key tile by NT threads: load k fills 16-byte positions k NT
 // + tid, whole rows of the cache; off holds the loads' byte offsets in the cache
-// (row_of(r): the cache row of the tile's row r).
+// (row_of(r): the cache row of the tile's row r). Rows may be more than 4 GiB
+// apart: a stride of INT_MAX elements in bytes fits 32 bits in bf16 (one 32 x 32 bit
+// product per load; with the shift of a product of elements instead 0.7% of
+// 960 us, 2048 tokens of 32768, d = 128), in fp32 it takes 64.
 template <class Pol, int NT>
 struct BatchStage {
     static constexpr int CPR = Pol::D / Pol::EPC, LOADS = 64 * CPR / NT;
+    using Stride = std::conditional_t<sizeof(typename Pol::T) == 2, unsigned, unsigned long long>;
     unsigned long long off[LOADS];
+    __device__ static __forceinline__ Stride stride_bytes(int stride) { return (Stride)stride * (Stride)sizeof(typename Pol::T); }
     template <class RowOf>
-    __device__ __forceinline__ void rows(int tid, unsigned stride_bytes, RowOf row_of) {
+    __device__ __forceinline__ void rows(int tid, Stride stride, RowOf row_of) {
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) {
             int row, c;
             Pol::chunk_at(k * NT + tid, row, c);
-            off[k] = (unsigned long long)row_of(row) * stride_bytes + 16 * c;
+            off[k] = (unsigned long long)row_of(row) * stride + 16 * c;
         }
     }
     __device__ __forceinline__ void load(typename Pol::T *tile, const typename Pol::T *X, int wave) const {
@@ -434,7 +439,7 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
     const int g = lane >> 4, l16 = lane & 15;
     const T *K = static_cast<const T *>(p.k) + it.head * D, *V = static_cast<const T *>(p.v) + it.head * D;
     const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, it.s.keys, (unsigned)(p.n_blocks - 1)};
-    const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
+    const typename Stage::Stride stride = Stage::stride_bytes(p.kv_rs);
     // waves past the NW that have tiles only take part in the join
     const int own = NW * 64 < THREADS ? min(wave, NW - 1) : wave;
     T *sk = sm.t.k[own], *sv = sm.t.v[own];
@@ -621,7 +626,7 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
 
     const int Nk = min(it.s.keys, max(pos_hi + 1, 0)), n = (Nk + BK - 1) / BK;
     const BatchRows rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, Nk, (unsigned)(p.n_blocks - 1)};
-    const unsigned stride = (unsigned)p.kv_rs * (unsigned)sizeof(T);
+    const typename Stage::Stride stride = Stage::stride_bytes(p.kv_rs);
     int s_lo, s_hi;
     share_stages(it, n, s_lo, s_hi);
     // each wave's lanes hold the blocks of the 64 rows of the stage to be staged
