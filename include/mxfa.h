@@ -450,7 +450,8 @@ int mxfa_check_batch(const mxfa_batch_shape *shape);
  * included, as mxfa_run_cache_append writes them). Query row r holds head h at
  * elements [h * head_dim, (h + 1) * head_dim), a cache row KV head h, the
  * output row likewise; head_dim 64 (fp32, bf16) or 128 (bf16). A row that sees
- * no position (a token at a negative one) is zeros, its lse -infinity. lse:
+ * no position (a token at a negative one) is zeros, its lse -infinity; one whose
+ * every seen score is -infinity has no softmax: NaN, its lse -infinity. lse:
  * NULL, or n_tok x n_head floats. A position that a row does not see never
  * reaches it, whatever its K and V hold. The workspace
  * (mxfa_prefill_batch_workspace_bytes, 16-byte aligned, no contents needed) is

@@ -273,7 +273,7 @@ __device__ __forceinline__ bool find_item(const BatchParams &p, int w, BatchItem
                 return false;
             if (it.shares > 1 && it.share == 0 && it.split < p.splits && threadIdx.x == 0)
                 reinterpret_cast<ManyNote *>(p.notes[1])[1 + it.split] =
-                    ManyNote{it.shares, it.slot, it.s.q0, it.s.rows, it.unit, it.head, {0, 0}};
+                    ManyNote{it.shares, it.slot, it.s.q0, it.s.rows, it.unit, it.head, {it.s.pos, 0}};
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -317,12 +317,17 @@ __device__ __forceinline__ size_t batch_lse(const BatchParams &p, const BatchIte
     return (size_t)(it.s.q0 + r / p.group) * p.Hq + it.head * p.group + r % p.group;
 }
 
+// What the sum of V of a row at position `pos` is multiplied by, l being the sum
+// of its weights: 0 where it sees no position; where every score that it sees is
+// -infinity (K infinite, or products past the range) there is no softmax: NaN.
+__device__ __forceinline__ float batch_inverse(float l, int pos) { return l != 0.f ? 1.0f / l : pos < 0 ? 0.f : NAN; }
+
 // Four elements of a finished row, and its lse by the row's first thread.
 template <class T>
 __device__ __forceinline__ void batch_store(const BatchParams &p, const BatchItem &it, int r, int d, int c, f32x4 o,
                                             float m, float l) {
     T *O = static_cast<T *>(p.o) + batch_elem(p, it, r, p.o_rs, d) + c;
-    store4<T>(O, o, l > 0.f || l != l ? 1.0f / l : 0.f);  // a row that sees no key is zeros
+    store4<T>(O, o, batch_inverse(l, it.s.pos + r / p.group));
     if (p.lse != nullptr && c == 0) p.lse[batch_lse(p, it, r)] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
 }
 
@@ -566,7 +571,7 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
         it.seq = seq;
         it.s = s;
         const FewPiece f = few_piece(x, x1, u0, u1, g);
-        if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, s.q0, s.rows, 0});
+        if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, s.q0, s.rows, s.pos});
         batch_few_piece<Pol, NW, THREADS>(p, it, f.lo, f.hi, f.slot, sm);
         x = f.end;
         if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
@@ -718,7 +723,7 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
             }
             continue;
         }
-        const float inv = ltot[qt] > 0.f ? 1.0f / ltot[qt] : 0.f;
+        const float inv = batch_inverse(ltot[qt], qpos.at[qt]);
         T *O = static_cast<T *>(p.o) + batch_elem(p, it, min(r, last_row), p.o_rs, D);
 #pragma unroll
         for (int xt = 0; xt < XT; xt += 2)
@@ -1020,6 +1025,7 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
         it.head = head;
         it.unit = 0;
         it.s.q0 = n.q0;
+        it.s.pos = n.pos;
         batch_join_rows<T, D>(p, it, kBatchFew, first, end, n.parts, p.part[0], few_slots(p), [&](int i) __attribute__((always_inline)) {
             return i == 0 ? few_first_slot(run, heads, head) : few_next_slot(run, heads, head) + 2 * heads * (i - 1);
         });
@@ -1034,6 +1040,7 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
     it.head = n.head;
     it.unit = n.unit;
     it.s.q0 = n.q0;
+    it.s.pos = n.pos[0];
     batch_join_rows<T, D>(p, it, rows, first, end, n.shares, p.part[1], p.slots,
                                 [&](int i) __attribute__((always_inline)) { return n.slot + i * p.Hkv; });
 }

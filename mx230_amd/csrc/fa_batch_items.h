@@ -30,12 +30,13 @@ __host__ __device__ constexpr size_t batch_slot_floats(long long slots, int rows
     return (size_t)slots * rows * (d + 2);
 }
 // The join's notes. Few rows: per work-group the pieces of the sequence that its
-// run ends in (0: none) and its rows. Many rows: the count of split units, then each.
+// run ends in (0: none), its rows and first position. Many rows: the count of split
+// units, then each.
 struct FewNote {
-    int parts, q0, rows, unused;
+    int parts, q0, rows, pos;
 };
 struct ManyNote {
-    int shares, slot, q0, rows, unit, head, unused[2];
+    int shares, slot, q0, rows, unit, head, pos[2];  // (pos[1]: to 32 bytes)
 };
 
 template <class X>

@@ -57,3 +57,50 @@ def test_rows_past_32_bits_apart(bf16, stride, nh, n):
     order = table[0].long()
     assert torch.equal(k[order], two[:, nh * hd:(nh + 1) * hd]) and torch.equal(v[order], two[:, (nh + 1) * hd:])
     assert torch.equal(out, two[:, :nh * hd])
+
+
+@pytest.mark.parametrize("bf16,hd", TYPES)
+@pytest.mark.parametrize("how", ["infinite", "overflow"])
+@pytest.mark.parametrize("pairs", [
+    [(1, 40), (1, 1), (2, 130)], [(80, 100), (70, 200)], [(1, 3000), (3, 2900)], [(70, 6000)], [(40, 5000), (1, 4500), (5, 3)]])
+def test_scores_all_minus_infinity(pairs, how, bf16, hd):
+    """Every score that a row of the first KV head sees is -infinity, by K or by
+    products past the type's range: no softmax exists, so NaN, its lse -infinity (not
+    the zeros of a row that sees no position). The other head is as ever."""
+    b = Batch(pairs, 4, 2, hd, 16, bf16, seed=21)
+    rows = torch.cat(b.rows)
+    for h in range(2):
+        b.qkv[:, h * hd] = 3e38 if how == "overflow" else b.qkv[:, h * hd].abs() + 0.5
+    b.k[rows, 0] = -3e38 if how == "overflow" else -math.inf
+    out, lse = run(b)
+    t0 = 0
+    for n, ln in pairs:
+        for i in range(t0, t0 + n):
+            got = out[i, :2 * hd]
+            assert not got.any() if ln - n + i - t0 < 0 else bool(torch.isnan(got).all()), (n, ln, i - t0)
+        t0 += n
+    assert bool((lse[:, :2] == -math.inf).all())
+    want, mag, wlse, _ = b.attention()
+    reach, other = reach_of(b, (2, 3)), slice(2 * hd, None)
+    assert bool(((out.double() - want).abs() <= b.tolerance(want, mag, reach))[:, other].all())
+    fine = torch.isfinite(wlse[:, 2:])
+    assert torch.equal(lse[:, 2:][~fine].double(), wlse[:, 2:][~fine])
+    assert float((lse.double() - wlse)[:, 2:][fine].abs().max()) <= b.lse_tolerance(reach)
+
+
+@pytest.mark.parametrize("bf16,hd", TYPES)
+@pytest.mark.parametrize("pairs", [[(1, 200), (3, 190)], [(80, 200)], [(1, 5000), (3, 4900)], [(70, 6000)]])
+def test_scores_minus_infinity_at_first(pairs, bf16, hd):
+    """Keys whose score is -infinity weigh nothing beside others: the first 100
+    positions, whole stages and shares among them."""
+    b = Batch(pairs, 2, 1, hd, 16, bf16, seed=22)
+    b.qkv[:, 0], b.qkv[:, hd] = (b.qkv[:, c].abs() + 0.5 for c in (0, hd))
+    for s in range(len(pairs)):
+        b.k[b.rows[s][:100], 0] = -math.inf
+    out, lse = run(b)
+    want, mag, wlse, _ = b.attention()
+    assert bool(torch.isfinite(want).all())
+    reach = reach_of(b, (0, 1), skip=100)
+    off = (out.double() - want).abs()
+    assert bool((off <= b.tolerance(want, mag, reach)).all()), float(off.max())
+    assert float((lse.double() - wlse).abs().max()) <= b.lse_tolerance(reach)
