@@ -992,7 +992,10 @@ __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const Batc
                     x[i] = *reinterpret_cast<const f32x4 *>(batch_part(parts, at(s0 + j), rows, D) + r * D + 4 * c);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o += x[i] * w[i];
+                for (int i = 0; i < 8; ++i) {
+                    // (past the last part: its load again, which adds nothing, also where it is infinite)
+                    o += (s + i * together < n ? x[i] : zero4()) * w[i];
+                }
             }
             wait_lds();
         }

@@ -104,3 +104,26 @@ def test_scores_minus_infinity_at_first(pairs, bf16, hd):
     off = (out.double() - want).abs()
     assert bool((off <= b.tolerance(want, mag, reach)).all()), float(off.max())
     assert float((lse.double() - wlse).abs().max()) <= b.lse_tolerance(reach)
+
+
+@pytest.mark.parametrize("bf16,hd", TYPES)
+@pytest.mark.parametrize("pairs", [[(1, 200), (3, 190)], [(80, 200)], [(1, 5000), (3, 4900)], [(70, 6000)],
+                                   [(1, 9000)], [(1, 30), (40, 3000)]])
+@pytest.mark.parametrize("signs", ["+", "-", "+-"])
+def test_infinite_values(pairs, signs, bf16, hd):
+    """An infinite V that a row sees, in the last position: the sum is that infinity,
+    and NaN where both are seen, whether the keys are split or not."""
+    b = Batch(pairs, 4, 2, hd, 16, bf16, seed=23)
+    for s, (n, ln) in enumerate(pairs):
+        last = b.rows[s][ln - n:]
+        b.v[last, :hd] = -math.inf if signs == "-" else math.inf
+        if signs == "+-":
+            b.v[b.rows[s][0], :hd] = -math.inf
+    out, lse = run(b)
+    want, _, wlse, reach = b.attention()
+    c = slice(0, 2 * hd)
+    assert torch.equal(torch.isnan(out[:, c]), torch.isnan(want[:, c]))
+    fine = ~torch.isnan(want[:, c])
+    assert torch.equal(out[:, c][fine].double(), want[:, c][fine])
+    assert bool(torch.isfinite(out[:, 2 * hd:]).all())
+    assert float((lse.double() - wlse).abs().max()) <= b.lse_tolerance(reach)
