@@ -457,7 +457,9 @@ int mxfa_check_batch(const mxfa_batch_shape *shape);
  * (mxfa_prefill_batch_workspace_bytes, 16-byte aligned, no contents needed) is
  * used until the call completes: calls that may overlap need their own. The
  * key ranges of long sequences are joined in a fixed order: equal calls give
- * equal bits. out may be q (the same pointer and stride). */
+ * equal bits. out may be q (the same pointer and stride) or other columns of the
+ * same rows; where it lies over q otherwise, or out, lse or the workspace over a
+ * cache, q or each other, the call is refused (MXFA_ERR_UNSUPPORTED). */
 size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *shape);
 int mxfa_run_prefill_batch(const mxfa_batch_shape *shape, const void *q, const void *kcache, const void *vcache,
                            void *out, float *lse, const int *block_table, const int *cu_q, const int *lens,

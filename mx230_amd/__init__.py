@@ -1066,7 +1066,8 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
     (run_cache_append). Lengths and tables are read on the device.
 
     q: [n_tok, >= n_head head_dim] (may be the columns of a fused QKV buffer),
-    out likewise (may be q); the caches, block_table, cu_q and lens as for
+    out likewise (may be q, or other columns of its rows; refused where it lies
+    over q or a cache otherwise); the caches, block_table, cu_q and lens as for
     run_cache_append; max_q: at least the most new tokens any sequence has
     (rows past it are not computed). lse: None, or float32 [n_tok, n_head] for
     the rows' log-sum-exp. workspace: a contiguous device tensor of

@@ -717,17 +717,25 @@ int check_batch(const mxfa_batch_shape *s, long long qw) {
     return MXFA_OK;
 }
 
-// Whether `rows` output rows of `ow` bytes and as many input rows of `iw` share
-// memory in any way but as the same rows: where the strides are equal they may
-// also be columns of the same wider rows.
+// Whether `an` rows of `aw` bytes, `as` apart, share memory with `bn` rows of `bw`.
+// Where the strides are equal, or one of them is a single row, that is the rows
+// themselves (they may be columns of the same wider rows); else what they span.
+bool rows_meet(const void *a, long long as, long long aw, long long an, const void *b, long long bs, long long bw,
+               long long bn) {
+    using Wide = unsigned __int128;  // (no span passes it)
+    if (an == 1) as = bn == 1 ? aw + bw : bs;
+    if (bn == 1) bs = as;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if ((Wide)x >= y + (Wide)bs * (Wide)(bn - 1) + (Wide)bw || (Wide)y >= x + (Wide)as * (Wide)(an - 1) + (Wide)aw)
+        return false;
+    if (as != bs) return true;
+    const uintptr_t s = (uintptr_t)as, at = x > y ? (x - y) % s : (s - (y - x) % s) % s;
+    return at < (uintptr_t)bw || at + (uintptr_t)aw > s;
+}
+
+// Whether output rows and as many input rows meet in any way but as the same rows.
 bool rows_collide(const void *out, long long os, long long ow, const void *in, long long is, long long iw, int rows) {
-    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
-    if (rows == 1) os = is = ow > iw ? ow : iw;
-    if (o == i && os == is) return false;
-    if (o >= i + (uintptr_t)(is * (rows - 1) + iw) || i >= o + (uintptr_t)(os * (rows - 1) + ow)) return false;
-    if (os != is) return true;
-    const uintptr_t at = o > i ? (o - i) % (uintptr_t)os : ((uintptr_t)os - (i - o) % (uintptr_t)os) % (uintptr_t)os;
-    return at < (uintptr_t)iw || at + (uintptr_t)ow > (uintptr_t)os;
+    return !(out == in && (os == is || rows == 1)) && rows_meet(out, os, ow, rows, in, is, iw, rows);
 }
 
 mxfa::BatchParams batch_params(const mxfa_batch_shape *s, const void *q, void *k, void *v, void *o, const int *table,
@@ -801,7 +809,28 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void 
                                        cu_q, lens);
     p.lse = lse;
     p.scale_log2 = (s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * mxfa::kLog2e;
-    if (workspace_bytes < mxfa::batch_workspace_bytes(p, s->dtype == MXFA_BF16)) return MXFA_ERR_WORKSPACE;
+    const size_t need = mxfa::batch_workspace_bytes(p, s->dtype == MXFA_BF16);
+    if (workspace_bytes < need) return MXFA_ERR_WORKSPACE;
+    // what is written lies apart from what is read: other work-groups may still read it
+    struct Rows {
+        const void *at;
+        long long stride, width, rows;
+    };
+    const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, qw = esz * s->n_head * s->head_dim;
+    const long long kw = esz * s->n_kv_head * s->head_dim, pool = (long long)s->n_blocks * s->block_size;
+    const long long lw = lse == nullptr ? 0 : 4LL * s->n_tok * s->n_head;
+    const Rows all[] = {{q, s->q_stride * esz, qw, s->n_tok}, {kcache, s->kv_stride * esz, kw, pool},
+                        {vcache, s->kv_stride * esz, kw, pool}, {out, s->out_stride * esz, qw, s->n_tok},
+                        {lse, lw, lw, 1}, {workspace, (long long)need, (long long)need, 1}};
+    if (rows_collide(out, s->out_stride * esz, qw, q, s->q_stride * esz, qw, s->n_tok)) return MXFA_ERR_UNSUPPORTED;
+    for (int w = 3; w < 6; ++w) {
+        for (int r = w == 3 ? 1 : 0; r < w; ++r) {  // (out over q: above)
+            const Rows &x = all[w], &y = all[r];
+            if (x.width > 0 && y.width > 0 &&
+                rows_meet(x.at, x.stride, x.width, x.rows, y.at, y.stride, y.width, y.rows))
+                return MXFA_ERR_UNSUPPORTED;
+        }
+    }
     return from_hip(mxfa::launch_batch(p, s->dtype == MXFA_BF16, workspace, static_cast<hipStream_t>(stream)));
 }
 

@@ -1,0 +1,62 @@
+"""More argument checks of the operators around the paged cache (no GPU needed, nothing
+is launched): outputs that lie over inputs, tables of the largest width, rows that do
+not begin on 16 bytes, and frequencies worked out by hand."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import mx230_amd as mx
+from test_cache_abi import OK, SHAPE, UNSUPPORTED, P, batch_shape, lib, pages_shape  # noqa: F401
+
+BASE = 1 << 30
+FAR = [BASE + (i << 28) for i in range(1, 6)]  # nothing is there
+
+
+def attend(lib, s, q=FAR[0], k=FAR[1], v=FAR[2], out=FAR[3], lse=None, ws=FAR[4]):
+    """The status of a call that has to be refused."""
+    n = lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(s))
+    p = [None if x is None else ctypes.c_void_p(x) for x in (q, k, v, out, lse)]
+    return lib.mxfa_run_prefill_batch(ctypes.byref(s), *p, P, P, P, ctypes.c_void_p(ws), n, None)
+
+
+# bf16, 4/2 heads of 64, 8 tokens, a pool of 160 rows: a row of Q or out 512 bytes, of K or V 256
+@pytest.mark.parametrize("q_stride,out_stride,off", [
+    (512, 512, 16), (512, 512, -16), (512, 512, 1024), (512, 512, 256), (256, 512, 0), (512, 256, 0), (512, 256, 1024 * 7 + 496),
+    (256, 512, -1024 * 7), (512, 512, 1024 + 256), (512, 512, 1024 - 496), (256, 264, 512 * 7)])
+def test_output_over_the_queries(lib, q_stride, out_stride, off):  # noqa: F811
+    s = batch_shape(q_stride=q_stride, out_stride=out_stride)
+    assert attend(lib, s, out=FAR[0] + off) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("off,n_tok", [(16, 1), (-16, 1), (496, 1), (-496, 1)])
+def test_output_over_one_query_row(lib, off, n_tok):  # noqa: F811
+    s = batch_shape(n_tok=n_tok, n_seq=1, max_q=1)
+    assert attend(lib, s, out=FAR[0] + off) == UNSUPPORTED
+
+
+def test_output_over_the_caches(lib):  # noqa: F811
+    for which in ("k", "v"):
+        at = dict(k=FAR[1], v=FAR[2])[which]
+        for off in (0, 256 * 159 + 240, 16, 256 * 80, -512 * 7 - 16):
+            assert attend(lib, batch_shape(), out=at + off) == UNSUPPORTED, off
+        # columns of the same wide rows that the cache has itself
+        s = batch_shape(kv_stride=1024, out_stride=1024)
+        for off in (0, 240, -496, 2048 * 5 + 240, 2048 * 159 + 16):
+            assert attend(lib, s, out=at + off) == UNSUPPORTED, off
+        # one token's row inside a wide cache row's columns
+        s = batch_shape(n_tok=1, n_seq=1, max_q=1, kv_stride=1024)
+        assert attend(lib, s, out=at + 2048 * 7 + 240) == UNSUPPORTED
+
+
+def test_lse_and_workspace_over_the_rest(lib):  # noqa: F811
+    s = batch_shape()
+    n = lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(s))
+    for x in (FAR[0], FAR[1], FAR[2], FAR[3]):
+        assert attend(lib, s, ws=x) == UNSUPPORTED
+        assert attend(lib, s, ws=x - n // 16 * 16 + 16) == UNSUPPORTED
+        assert attend(lib, s, lse=x + 4) == UNSUPPORTED
+    assert attend(lib, s, lse=FAR[4]) == UNSUPPORTED
+    assert attend(lib, s, lse=FAR[4] + n - 4) == UNSUPPORTED

@@ -127,3 +127,27 @@ def test_infinite_values(pairs, signs, bf16, hd):
     assert torch.equal(out[:, c][fine].double(), want[:, c][fine])
     assert bool(torch.isfinite(out[:, 2 * hd:]).all())
     assert float((lse.double() - wlse).abs().max()) <= b.lse_tolerance(reach)
+
+
+@pytest.mark.parametrize("pairs", [[(1, 900), (3, 700), (1, 1)], [(150, 400), (1, 300)], [(1, 1)]])
+def test_neighbours_in_memory(pairs):
+    """The output in the free columns of q's rows, and every tensor right behind the
+    one before it in one allocation, are not over each other."""
+    nh, nkv, hd = 2, 1, 64
+    b = Batch(pairs, nh, nkv, hd, 16, True, seed=25)
+    k, v, table, cu, lens, qkv = b.cuda("k", "v", "table", "cu_q", "lens", "qkv")
+    mx.run_prefill_batch(qkv[:, :nh * hd], k, v, qkv[:, nh * hd:], table, 16, cu, lens, b.max_q, nh, nkv, hd)
+    check(b, qkv[:, nh * hd:].cpu(), None)
+    assert torch.equal(qkv[:, :nh * hd].cpu(), b.qkv[:, :nh * hd])
+    need = mx.prefill_batch_workspace_bytes(b.n_tok, len(pairs), b.max_q, nh, nkv, hd)
+    rows = -(-need // (2 * hd))
+    arena = torch.full((2 * k.shape[0] + 2 * nh * b.n_tok + rows + -(-2 * nh * b.n_tok // hd), hd), 7.0, dtype=b.dt,
+                       device="cuda")
+    parts = arena.split([k.shape[0], nh * b.n_tok, k.shape[0], nh * b.n_tok, rows, -(-2 * nh * b.n_tok // hd)])
+    ak, aq, av, ao, ws, lse = parts
+    aq, ao = aq.view(b.n_tok, nh * hd), ao.view(b.n_tok, nh * hd)
+    lse = lse.view(torch.float32).flatten()[:b.n_tok * nh].view(b.n_tok, nh)
+    for x, y in ((ak, k), (av, v), (aq, b.qkv[:, :nh * hd])):
+        x.copy_(y)
+    mx.run_prefill_batch(aq, ak, av, ao, table, 16, cu, lens, b.max_q, nh, nkv, hd, lse=lse, workspace=ws)
+    check(b, ao.cpu(), lse.cpu())
