@@ -314,6 +314,14 @@ def _stream(stream):
     return ctypes.c_void_p(s.cuda_stream)
 
 
+def _scratch(nbytes: int, device, stream):
+    """Device bytes for a launch on `stream` (None: the current one), of that stream's
+    own memory: what another stream's pool gives may still be in use there."""
+    torch = _torch()
+    with torch.cuda.stream(stream):  # (None: does nothing)
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
 def shape_of(q, k, causal: bool, scale: float = 0.0) -> Shape:
     """Shape of an attention call from Q [B,Hq,N,d] and K [B,Hkv,N,d]."""
     torch = _torch()
@@ -1071,9 +1079,9 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
     run_cache_append; max_q: at least the most new tokens any sequence has
     (rows past it are not computed). lse: None, or float32 [n_tok, n_head] for
     the rows' log-sum-exp. workspace: a contiguous device tensor of
-    prefill_batch_workspace_bytes bytes (allocated when None); returned. Calls
-    that may overlap need their own. bf16 with head_dim 64 or 128, or fp32 with
-    64."""
+    prefill_batch_workspace_bytes bytes (allocated when None, as memory of
+    `stream`); returned. Calls that may overlap need their own. bf16 with
+    head_dim 64 or 128, or fp32 with 64."""
     torch = _torch()
     if stream is None:
         rc = _calls().prefill_batch(q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head,
@@ -1094,10 +1102,7 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
     _check("mxfa_check_batch", lib.mxfa_check_batch(ctypes.byref(sh)))
     with _on(q.device):
         if workspace is None:
-            workspace = torch.empty(int(lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh))), dtype=torch.uint8,
-                                    device=q.device)
-            if stream is not None:
-                workspace.record_stream(stream)
+            workspace = _scratch(int(lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh))), q.device, stream)
         elif not _dev(workspace, "workspace", None, q).is_contiguous():
             raise ValueError("workspace: expected a contiguous device tensor")
         _check("mxfa_run_prefill_batch",

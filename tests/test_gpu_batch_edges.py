@@ -129,6 +129,33 @@ def test_infinite_values(pairs, signs, bf16, hd):
     assert float((lse.double() - wlse).abs().max()) <= b.lse_tolerance(reach)
 
 
+def test_workspace_belongs_to_the_stream():
+    """The workspace that a call on a given stream allocates comes from that stream's
+    memory: not what a call on the current stream still uses, whose tensor is gone."""
+    b = Batch([(1, 4000), (1, 300), (40, 2500)], 4, 2, 64, 16, True, seed=24)
+    want, _ = run(b)
+    k, v, table, cu, lens, qkv = b.cuda("k", "v", "table", "cu_q", "lens", "qkv")
+    out = [torch.zeros(b.n_tok, b.nh * b.hd, dtype=b.dt, device="cuda") for _ in range(3)]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def call(o, stream):
+        return mx.run_prefill_batch(qkv[:, :b.nh * b.hd], k, v, o, table, b.bs, cu, lens, 40, b.nh, b.nkv, b.hd, stream=stream)
+    ws = call(out[0], None)
+    mine, size = ws.data_ptr(), ws.numel()
+    del ws
+    ws = call(out[1], s)
+    assert ws.data_ptr() + ws.numel() <= mine or mine + size <= ws.data_ptr()
+    theirs = ws.data_ptr()
+    del ws
+    # and the other way about: the next call here does not get the stream's
+    ws = call(out[2], None)
+    assert ws.data_ptr() + ws.numel() <= theirs or theirs + size <= ws.data_ptr()
+    torch.cuda.synchronize()
+    for o in out:
+        assert torch.equal(o.cpu(), want)
+
+
 @pytest.mark.parametrize("pairs", [[(1, 900), (3, 700), (1, 1)], [(150, 400), (1, 300)], [(1, 1)]])
 def test_neighbours_in_memory(pairs):
     """The output in the free columns of q's rows, and every tensor right behind the
