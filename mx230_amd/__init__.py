@@ -318,7 +318,9 @@ def _scratch(nbytes: int, device, stream):
     """Device bytes for a launch on `stream` (None: the current one), of that stream's
     own memory: what another stream's pool gives may still be in use there."""
     torch = _torch()
-    with torch.cuda.stream(stream):  # (None: does nothing)
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
@@ -754,7 +756,7 @@ def run_prefill_paged(q, kcache, vcache, out, block_table, block_size: int, pos0
                lib.mxfa_run_prefill_paged(ctypes.byref(sh), qp, kp, vp, op, ctypes.c_void_p(block_table.data_ptr()),
                                           int(block_size), _stream(stream)))
         return None
-    workspace = _split_workspace(lib, sh, workspace, q.device)
+    workspace = _split_workspace(lib, sh, workspace, q.device, stream)
     _check("mxfa_run_prefill_paged_ws",
            lib.mxfa_run_prefill_paged_ws(ctypes.byref(sh), qp, kp, vp, op, ctypes.c_void_p(block_table.data_ptr()),
                                          int(block_size), ctypes.c_void_p(workspace.data_ptr()),
@@ -762,12 +764,12 @@ def run_prefill_paged(q, kcache, vcache, out, block_table, block_size: int, pos0
     return workspace
 
 
-def _split_workspace(lib, sh, workspace, device):
+def _split_workspace(lib, sh, workspace, device, stream):
     """The split prefill's workspace: `workspace` checked, or a new one of the size the shape needs."""
     torch = _torch()
     if workspace is None:
         need = int(lib.mxfa_prefill_workspace_bytes(ctypes.byref(sh)))
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        workspace = _scratch(max(need, 16), device, stream)
     if not isinstance(workspace, torch.Tensor) or workspace.device.type != "cuda" or not workspace.is_contiguous():
         raise ValueError("workspace: expected a contiguous device tensor")
     return workspace
@@ -810,7 +812,7 @@ def run_prefill_split(q, kcache, vcache, out, pos0: int, n_head: int, n_kv_head:
     sh = MxfaPrefillShape(n_tok, n_head, n_kv_head, head_dim, pos0, qs, ks, os_,
                           MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
     lib = load_library()
-    workspace = _split_workspace(lib, sh, workspace, q.device)
+    workspace = _split_workspace(lib, sh, workspace, q.device, stream)
     have = workspace.numel() * workspace.element_size()
     _check("mxfa_run_prefill_ws",
            lib.mxfa_run_prefill_ws(ctypes.byref(sh), qp, kp, vp, op, ctypes.c_void_p(workspace.data_ptr()),
@@ -1258,10 +1260,10 @@ def attention_bwd(q, k, v, o, lse, do, causal: bool, scale: float = 0.0, stream=
         if r is not NotImplemented:
             _check("mxfa_run_bwd_ws", r)
     sh = shape_of(q, k, causal, scale)
-    delta = torch.empty((sh.B, sh.Hq, sh.N), dtype=torch.float32, device=q.device)
+    delta = _scratch(4 * sh.B * sh.Hq * sh.N, q.device, stream).view(torch.float32).view(sh.B, sh.Hq, sh.N)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     nws = bwd_workspace_bytes(q, k, causal)
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    ws = _scratch(nws, q.device, stream) if nws else None
     run_bwd_ws(q, k, v, o, do, lse, delta, dq, dk, dv, ws, causal, scale, stream)
     return dq, dk, dv
 
