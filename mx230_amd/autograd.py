@@ -49,7 +49,7 @@ def _rows16(x):
     es = x.element_size()
     if x.shape[-1] > 1 and x.stride(-1) != 1 or x.data_ptr() % 16 or \
             any(n > 1 and s * es % 16 for n, s in zip(x.shape[:-1], x.stride()[:-1])):
-        return x.contiguous()
+        return x.clone(memory_format=torch.contiguous_format)  # (contiguous() leaves where it begins)
     return x
 
 

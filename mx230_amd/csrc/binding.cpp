@@ -324,7 +324,7 @@ at::Tensor rows16(const at::Tensor &x) {
     const int64_t es = (int64_t)x.element_size();
     bool good = (x.size(-1) < 2 || x.stride(-1) == 1) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) good = good && (x.size(i) < 2 || x.stride(i) * es % 16 == 0);
-    return good ? x : x.contiguous();
+    return good ? x : x.clone(at::MemoryFormat::Contiguous);  // (contiguous() leaves where it begins)
 }
 
 // Q and K turned, in new tensors.

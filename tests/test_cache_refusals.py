@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import mx230_amd as mx
+from mx230_amd.autograd import _rows16
 from test_cache_abi import OK, SHAPE, UNSUPPORTED, P, batch_shape, lib, pages_shape  # noqa: F401
 
 BASE = 1 << 30
@@ -60,3 +61,12 @@ def test_lse_and_workspace_over_the_rest(lib):  # noqa: F811
         assert attend(lib, s, lse=x + 4) == UNSUPPORTED
     assert attend(lib, s, lse=FAR[4]) == UNSUPPORTED
     assert attend(lib, s, lse=FAR[4] + n - 4) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_rows_begin_on_16_bytes(dt):
+    base = torch.zeros(2 * 3 * 5 * 64 + 8, dtype=dt)
+    for off in range(8):
+        x = base[off:off + 2 * 3 * 5 * 64].view(2, 3, 5, 64)
+        y = _rows16(x)
+        assert y.data_ptr() % 16 == 0 and torch.equal(x, y) and (y is x) == (x.data_ptr() % 16 == 0)
