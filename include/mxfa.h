@@ -471,7 +471,9 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *shape, const void *q, const v
  * positions. rotary_dim = 0 (frequencies NULL): copies only. head_dim as for
  * mxfa_rotary_shape. q_out may be qkv (the same pointer and stride), or other
  * columns of the same rows; where it lies over qkv otherwise the call is refused
- * (MXFA_ERR_UNSUPPORTED). Any other overlap is the caller's to avoid. */
+ * (MXFA_ERR_UNSUPPORTED). Any other overlap is the caller's to avoid. A token at
+ * a negative position is left out, its q_out row too; one past the table has its
+ * q_out row only. */
 typedef struct {
     int rotary_dim, interleaved;
     float factor;

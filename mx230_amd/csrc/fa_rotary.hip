@@ -11,6 +11,8 @@
 // copied rest, computes its angles once and walks hpt heads with them: no table
 // of cosines is read or kept, and the angles' 64-bit arithmetic hides behind the
 // first loads (B4, 12 + 12 heads, N4096, d = 64 bf16, 100 MB: 18 us, a copy 20).
+#include <limits.h>
+
 #include <algorithm>
 
 #include "fa_cache.h"
@@ -252,8 +254,9 @@ __device__ __forceinline__ void append_body(const BatchParams &p) {
         __syncthreads();
         if (!mine || seq_of[k] < 0) return;
         const int s = seq_of[k];
-        pos = p.lens[s] - p.cu_q[s + 1] + t;
-        if (pos < 0) return;
+        const long long at = (long long)p.lens[s] - p.cu_q[s + 1] + t;  // (may pass 32 bits either way)
+        if (at < 0 || at > INT_MAX) return;
+        pos = (int)at;
         const int blk = pos >> p.bs_shift;
         if (blk < p.max_blocks) {
             const int e = p.table[(long long)s * p.table_stride + blk];

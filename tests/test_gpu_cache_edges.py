@@ -35,3 +35,16 @@ def test_embedding_of_rows_off_16_bytes(dt, python, monkeypatch):
     torch.autograd.backward(got, (off(wq), off(wk)))
     for x, y in zip((*want, q.grad, k.grad), (*got, a.grad, b.grad)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("length", [-2 ** 31, -2 ** 31 + 1, -1, 0])
+def test_append_at_negative_positions(length):
+    """A token at a position below 0, however far, is left out."""
+    bs = 1 << 24
+    table = torch.full((1, 128), 0, dtype=torch.int32, device="cuda")
+    k, v = (torch.full((bs, 8), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    qkv = torch.ones(2, 24, dtype=torch.bfloat16, device="cuda")
+    out = torch.full((2, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 2], [length]))
+    mx.run_cache_append(qkv, out, k, v, table, bs, cu, lens, 1, 1, 8, mx.rotary_frequencies(8)[0])
+    assert bool((out == 7.0).all()) and bool((k == 7.0).all()) and bool((v == 7.0).all())
