@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -873,6 +874,8 @@ int mxfa_check_pages(const mxfa_pages_shape *s) {
     if (s->n_seq > kMaxGridY) return MXFA_ERR_SHAPE;
     // the plans count blocks in ints, a few thousand past the last
     if (s->n_blocks > (1 << 30)) return MXFA_ERR_SHAPE;
+    // and a table's entries by work-groups of 256
+    if (s->max_blocks > INT_MAX - 255) return MXFA_ERR_SHAPE;
     if (!power_of_two(s->block_size) || s->block_size > (1 << 24)) return MXFA_ERR_UNSUPPORTED;
     return MXFA_OK;
 }

@@ -63,6 +63,13 @@ def test_lse_and_workspace_over_the_rest(lib):  # noqa: F811
     assert attend(lib, s, lse=FAR[4] + n - 4) == UNSUPPORTED
 
 
+def test_widest_table(lib):  # noqa: F811
+    """A table's entries are counted in ints, a work-group past the last."""
+    for wide, want in ((2 ** 31 - 1, SHAPE), (2 ** 31 - 255, SHAPE), (2 ** 31 - 256, OK)):
+        s = pages_shape(n_seq=1, max_blocks=wide, table_stride=wide)
+        assert lib.mxfa_check_pages(ctypes.byref(s)) == want
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_rows_begin_on_16_bytes(dt):
     base = torch.zeros(2 * 3 * 5 * 64 + 8, dtype=dt)
