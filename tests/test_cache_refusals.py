@@ -77,3 +77,16 @@ def test_rows_begin_on_16_bytes(dt):
         x = base[off:off + 2 * 3 * 5 * 64].view(2, 3, 5, 64)
         y = _rows16(x)
         assert y.data_ptr() % 16 == 0 and torch.equal(x, y) and (y is x) == (x.data_ptr() % 16 == 0)
+
+
+def test_yarn_between_its_ends():
+    """dim 64, base 10^4, 4096 positions: a pair that turns 32 times is number 10.5 and
+    one that turns once 22.5, so the ramp goes from 10 to 23: pair i is divided by 8 to
+    (i - 10) / 13."""
+    f, _ = mx.rotary_frequencies(64, 10000.0, "yarn", 8.0, 4096, device="cpu")
+    for i in (10, 11, 12, 16, 20, 22, 23):
+        part = (i - 10) / 13
+        assert f[i].item() == pytest.approx(10.0 ** (-i / 8) * (1 - part * 7 / 8), rel=1e-14)
+    assert f[16].item() == pytest.approx(0.01 * 62 / 104, rel=1e-14)
+    assert f[9].item() == pytest.approx(10.0 ** (-9 / 8), rel=1e-14)
+    assert f[24].item() == pytest.approx(10.0 ** -3 / 8, rel=1e-14)
