@@ -25,16 +25,20 @@
 // has to be cleared before each call, and an only reader per unit of up to 128
 // parts takes longer than the many of the launch.
 //
-// Measured (us; the rates count the keys each sequence has once, or the products of
-// the positions that rows see):
-//   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: 385 and
-//         the join 6 (5.7 TB/s; a plain read of all memory reaches 6.4);
-//         one token after 4095, 32/4 heads, d = 64: 7.1 and 4.5;
-//   many: the last 2048 tokens of 32768, 32/8 heads, d = 128: 960 (1110 TFLOP/s; a large
-//         library product 1173); 4096 tokens, 32/4 heads, d = 64: 88 (780);
-//         fp32, 2000 tokens after 2096, 14/2 heads: 179 (124; in fp32 150);
+// Measured (us, medians of a kernel trace; the rates count the keys each sequence
+// has once, or the products of the positions that rows see):
+//   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: 391 and
+//         the join 6 (2.2 GB, 5.6 TB/s; a plain read of all memory reaches 6.4), d =
+//         64 221 and 6 (5.0), fp32 (d = 64) 414 and 7 (5.3);
+//         one token after 4095, 32/4 heads, d = 64: 7.1 and 4.0, fp32 8.8 and 4.1;
+//   many: the last 2048 tokens of 32768, 32/8 heads, d = 128: 920 to 970 in runs of
+//         calls on different cards (1100 to 1150 TFLOP/s; a large library product
+//         1180); 4096 tokens, 32/4 heads, d = 64: 87 to 90 (770); fp32, 2000 tokens
+//         after 2096, 14/2 heads: 169 to 180 with the join (123 to 131; in fp32 150);
 //   both: 28 single tokens and 4 chunks of up to 512, to 8192 long, 14/2 heads,
-//         d = 64: 48.5 and the join 7 (one after the other: 41 and 18).
+//         d = 64: 48.6 and the join 7 (one after the other: 41 and 18); 32/8 heads, d
+//         = 128: 213 with the join (98.7 GFLOP, 0.65 GB); fp32, 6 tokens and 2 chunks
+//         of up to 500, to 4096 long, 14/2 heads: 55 and 7.
 #include <algorithm>
 #include <type_traits>
 
@@ -103,9 +107,11 @@ struct PolF32 {
 // take 32 bytes of each of 32 rows). Chunk c of row r (bits r0, r1, ...) is at
 // slot c ^ swz(r). The 16 rows of a score operand differ in r0, r1, r3, r4, a
 // transposing read of V takes two neighbouring chunks of rows differing in r0
-// and r1 (two lane groups: r3), and with the bit patterns below each of these
-// covers all banks, in 128- and in 256-byte halves. r2 and r5 (tile t or half h,
-// block) stay out of it: plain additions.
+// and r1 (two lane groups: r3), and the bit patterns below are to spread each of
+// these over the banks, in 128- and in 256-byte halves. r2 and r5 (tile t or half h,
+// block) stay out of it: plain additions. The counters still show conflicts in 31%
+// of the LDS-active cycles of the many-row form, 25% of the few-row form's (PolBF16's
+// tiles have none).
 template <int D_>
 struct PolRows {
     using Base = PolBF16<D_>;
@@ -431,8 +437,8 @@ union BatchFewSmem {
 //
 // Bound by the reads: 128 KB of tiles in flight per CU (8 waves of 16 KB, d = 128: 4
 // of 32), and nothing but the next tile's loads between two waits. us, 64 sequences
-// of 2000-16384 positions, 32/8 heads, d = 128: 411 where a load reads whole rows,
-// 510 by 32 bytes of each of 32 rows.
+// of 2000-16384 positions, 32/8 heads, d = 128, at the step that brought it: 411
+// where a load reads whole rows, 510 by 32 bytes of each of 32 rows.
 template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
                                                 BatchFewSmem<Pol, NW> &sm) {
@@ -552,8 +558,9 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
 
 // Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line. Equal
 // runs, one work-group to a CU (its tiles take the LDS): 64 sequences of 2000-16384
-// positions in 393 us with the join, 415 with a work-group per share of a sequence
-// (d = 64: 471 and 504), whose count the host can only bound: thousands are empty.
+// positions, 32/8 heads, d = 128, in 393 us with the join, at the step that brought
+// them, 415 with a work-group per share of a sequence, whose count the host can only
+// bound: thousands are empty.
 template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
     const unsigned all = few_line(p), run = few_run(p, all);
@@ -589,7 +596,7 @@ struct BatchManySmem {
 
 // One unit's share, 16 QT rows per wave: K and V double-buffered in LDS, staged by
 // all four waves and read by each. The last 2048 of 32768 tokens, 32/8 heads, d = 128: 960
-// us, 1110 TFLOP/s.
+// us, 1110 TFLOP/s, the matrix units busy in half of the cycles, at 1.9 GHz.
 template <class Pol, int QT>
 __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
     using T = typename Pol::T;
@@ -738,8 +745,8 @@ __device__ __forceinline__ void batch_many_body(const BatchParams &p, int block,
 // split once per work-group into one LDS buffer; two work-groups per CU. Operands
 // that the parts cannot hold (kPartMin, infinities) flag the unit, whose rows
 // are then run in plain arithmetic. Bound by the splitting beside the products. us,
-// 2000 tokens of 14/2 heads after 2096: 176; 203 with 4 waves and 64 rows; on
-// v_mfma_f32_16x16x4_f32 235.
+// 2000 tokens of 14/2 heads after 2096: 177 (matrix units busy 33%); at the step that
+// brought it 176, 203 with 4 waves and 64 rows, 235 on v_mfma_f32_16x16x4_f32.
 __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block, FwdSplitSmem &sm) {
     constexpr int D = 64, XT = 4, BK = 64, NW = kBatchF32Waves, NT = 64 * NW, ROWS = 16 * NW;
     using PL = PolBF16<64>;  // the parts' layout
@@ -936,7 +943,7 @@ __device__ __forceinline__ void batch_many_parts(const BatchParams &p, int block
 // rows several groups take turns over its parts and meet in LDS. Bound by
 // latency: the (max, sum) pairs of all parts are one round of loads, and eight
 // parts of a thread's turn another. us, one token after 65535, 14/2 heads (128 parts
-// of 7 rows): 7.4, and 11.2 with one group to a row; 28 tokens and 4 chunks: 7.2
+// of 7 rows): 6.6; 7.4 when it came, and 11.2 with one group to a row; 28 tokens and 4 chunks: 7.2
 // with the notes, 12.8 where each work-group found its unit in the lengths.
 template <class T, int D, class At>
 __device__ __forceinline__ void batch_join_rows(const BatchParams &p, const BatchItem &it, int rows, int first, int end,
@@ -1051,9 +1058,9 @@ __device__ __forceinline__ void batch_join(const BatchParams &p, int few_cuts) {
 // Both forms in one launch: the few-row form's work-groups first, each wave's
 // tiles a quarter of its work-group's (bf16, d = 64) or half of it, so that LDS
 // holds as many of them as of the many-row form's: their reads and its matrix
-// products then share the CUs (us, 28 tokens and 4 chunks: 48.5; 41 + 17 in two
-// launches). In fp32 the few-row form has to spill at the other's 128 registers; two
-// launches took the same (6 tokens and 2 chunks: 13 + 55 and 55).
+// products then share the CUs (us, 28 tokens and 4 chunks: 48.6; 41 + 17 in two
+// launches). In fp32 the few-row form has to spill 96 at the other's 128 registers;
+// two launches took the same (6 tokens and 2 chunks: 13 + 55 and 55).
 template <int QT, class Pol>
 __device__ __forceinline__ void batch_many(const BatchParams &p, int block, BatchManySmem<Pol> &sm) {
     batch_many_body<Pol, QT>(p, block, sm);

@@ -5,8 +5,8 @@
 // TB/s, a large copy's rate); the rest by latency (tables of some thousand
 // entries): one work-group plans what needs an order, so that equal inputs
 // give equal blocks, and the rest is spread. us, 8 parents with 8 children of up to
-// 4096 tokens: free 3.3, plan 6.2, rows 3.5, copies in 48 pools 5.2; the plan of a
-// compaction of 8192 blocks 14, its tables 5.6.
+// 4096 tokens: free 3.2, plan 5.7, rows 3.9, copies in 48 pools 5.4; the plan of a
+// compaction of 8192 blocks 13.4, its tables 5.7.
 #include <algorithm>
 
 #include "fa_cache.h"

@@ -10,7 +10,10 @@
 // thread has one unit of a row, two 16-byte chunks of pairs or one of the
 // copied rest, computes its angles once and walks hpt heads with them: no table
 // of cosines is read or kept, and the angles' 64-bit arithmetic hides behind the
-// first loads (B4, 12 + 12 heads, N4096, d = 64 bf16, 100 MB: 18 us, a copy 20).
+// first loads (B4, 12 + 12 heads, N4096, d = 64 bf16, 100 MB: 18 us, a copy 20; fp32, 200
+// MB: 44, 4.6 TB/s). A short call stays below the copy's rate: fp32, B3, 10 + 10
+// heads, N777, 24 MB: 6.6 us (3.6 TB/s), and 7.2 where half of each row is only
+// copied: of a row's 12 threads then 4 have pairs and angles and 8 a single chunk.
 #include <limits.h>
 
 #include <algorithm>
@@ -20,9 +23,11 @@
 
 namespace mxfa {
 
-// cos and sin of a whole angle given in turns, off by about 1.2e-7 at most: the
-// position times the frequency is formed and reduced to [-1/8, 1/8] turns in
-// 64 bits (in 32 a position of 2^20 would be off by 0.06 radians), then
+// cos and sin of a whole angle given in turns, off by about 1.2e-7 at most, and by
+// what the angle itself is: the position times the frequency is formed, rounded
+// three times (with 1 / 2 pi), in 64 bits, so by up to 3 x 2^-53 of the angle (a
+// position of 2^20 at a frequency of 1 3.5e-10 radians, of 2^31 7e-7; in 32 bits
+// 2^20 would be off by 0.06). It is reduced to [-1/8, 1/8] turns there, then
 // Taylor's series, whose first terms left out are z^11 / 11! <= 1.8e-9 and
 // z^12 / 12! <= 1.2e-10 at z = pi / 4.
 __device__ __forceinline__ void turn_angle(double turns, float &c, float &s) {
@@ -230,7 +235,8 @@ __device__ __forceinline__ void rotary_body(const RotaryParams &p) {
 // instead of a bisection's chain of them. Bound by memory where there are many
 // tokens (5400 of 32/8 heads, d = 128, 132 MB: 23.5 us, 32 from memory that no cache
 // holds, where a copy takes 26), by the chain of loads cu_q, length,
-// block, row where there are few (16 of 14/2 heads: 4.1 us).
+// block, row where there are few (16 of 14/2 heads: 4.0 us). fp32, d = 64: 22.4
+// (132 MB) and 3.7.
 template <class T, int VEC>
 __device__ __forceinline__ void append_body(const BatchParams &p) {
     const int U = rotary_units<VEC>(p.d, p.dim), tid = threadIdx.x;  // (U is at most 255)
