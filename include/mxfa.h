@@ -407,8 +407,8 @@ typedef struct {
 int mxfa_check_rotary(const mxfa_rotary_shape *shape);
 /* One launch for Q and K. positions: int32 on the device, N per batch, any
  * sign; NULL: pos0 + n. frequencies: rotary_dim / 2 doubles on the device.
- * An output may be its own input (the same pointer and strides); an output
- * that overlaps its input otherwise gives MXFA_ERR_UNSUPPORTED, and Q and K
+ * An output may be its own input (the same pointer and strides); one whose
+ * span overlaps its input's otherwise gives MXFA_ERR_UNSUPPORTED, and Q and K
  * outputs must not overlap each other or the other's input (not checked: they
  * may be columns of the same rows). */
 int mxfa_run_rotary(const mxfa_rotary_shape *shape, const void *q, const void *k, void *q_out, void *k_out,

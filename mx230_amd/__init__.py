@@ -320,6 +320,8 @@ def _scratch(nbytes: int, device, stream):
     torch = _torch()
     if stream is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if not isinstance(stream, torch.cuda.Stream):  # anything with a cuda_stream, as _stream takes it
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 

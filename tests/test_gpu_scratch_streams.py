@@ -67,3 +67,25 @@ def test_backward(monkeypatch):
     torch.cuda.synchronize()
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+def test_streams_of_other_kinds():
+    """Whatever has a cuda_stream is a stream."""
+    class Other:
+        def __init__(self, s):
+            self.cuda_stream = s.cuda_stream
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, do = (torch.randn(1, 4, 300, 64, device="cuda", generator=g).bfloat16() for _ in range(2))
+    k, v = (torch.randn(1, 2, 300, 64, device="cuda", generator=g).bfloat16() for _ in range(2))
+    o, lse = mx.attention_fwd(q, k, v, True)
+    want = mx.attention_bwd(q, k, v, o, lse, do, True)
+    rows = torch.randn(8, 4 * 64, device="cuda", generator=g).bfloat16()
+    cache = torch.randn(4096, 2 * 64, device="cuda", generator=g).bfloat16()
+    out, two = torch.empty_like(rows), torch.empty_like(rows)
+    mx.run_prefill_split(rows, cache, cache, out, 4000, 4, 2, 64)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = mx.attention_bwd(q, k, v, o, lse, do, True, stream=Other(s))
+    mx.run_prefill_split(rows, cache, cache, two, 4000, 4, 2, 64, stream=Other(s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(out, two)
