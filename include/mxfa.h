@@ -483,6 +483,56 @@ int mxfa_run_cache_append(const mxfa_batch_shape *shape, const mxfa_append_rotar
                           void *q_out, void *kcache, void *vcache, const int *block_table, const int *cu_q,
                           const int *lens, void *stream);
 
+/* ---- A microscaled cache: the paged cache in 8 or 4 bits a value. Of each head's
+ * row, 32 neighbouring elements share a power of two 2^(E - 127), one byte E;
+ * an element is a code of `bits` bits, e4m3 (8) or e2m1 (4; two to a byte, the
+ * even element in the low half), and stands for 2^(E - 127) code, exactly a bf16.
+ * kcache and vcache are blocks of bytes, shape.kv_stride BYTES apart (a multiple
+ * of 16, at least mxfa_mx_block_bytes); in a block lie the codes [KV head][token]
+ * [head_dim bits / 8], then the bytes E [KV head][token][head_dim / 32]. The other
+ * fields of mxfa_batch_shape, and the tables, are as for the ordinary cache; dtype
+ * is that of qkv, q and the outputs. The upkeep of pages is the ordinary one
+ * (mxfa_run_pages_copy with a block of kv_stride bytes). */
+/* The least bytes of a block, a multiple of 16; 0 where bits, head_dim (a multiple
+ * of 32, at most 256) or block_size (a power of two) is not taken or they pass
+ * an int. */
+size_t mxfa_mx_block_bytes(int block_size, int n_kv_head, int head_dim, int bits);
+
+/* As mxfa_run_cache_append, K and V quantised as they are written. E is the least,
+ * 10 or more, by which the largest of the 32 is at most 448 2^(E - 127) (8 bits)
+ * or 7 2^(E - 127) (4 bits: from 6 on it rounds to 6); the codes are the nearest,
+ * on a tie the even one (elements above 1.75 2^127 count as that, whose code is in
+ * the types' range). 32 elements of which one is not finite get E = 255 and
+ * read back as NaN. K turns in 64 bits, rounded to 32, so equal tokens get equal
+ * codes whatever computes them; factor is one of 64 bits for that. head_dim: a
+ * multiple of 32, at most 256. */
+typedef struct {
+    int rotary_dim, interleaved;
+    double factor;
+    const double *frequencies; /* device, rotary_dim / 2 */
+} mxfa_append_rotary_mx;
+int mxfa_run_cache_append_mx(const mxfa_batch_shape *shape, int bits, const mxfa_append_rotary_mx *rotary,
+                             const void *qkv, void *q_out, void *kcache, void *vcache, const int *block_table,
+                             const int *cu_q, const int *lens, void *stream);
+
+/* Rows back out of it: row r of k_out and v_out (n_tok rows, out_stride elements
+ * apart, KV head h at elements [h head_dim, (h + 1) head_dim)) is what the cache
+ * holds at the position of the append's row r for the same cu_q and lens: of each
+ * sequence its last cu_q[s + 1] - cu_q[s] positions, all of them where that is
+ * lens[s]. Rows at negative positions, past the table or in a block outside the
+ * pool stay as they were. Reads neither n_head, q_stride nor scale. k_out and v_out
+ * must not lie over each other or the caches (MXFA_ERR_UNSUPPORTED). */
+int mxfa_run_cache_read_mx(const mxfa_batch_shape *shape, int bits, const void *kcache, const void *vcache, void *k_out,
+                           void *v_out, const int *block_table, const int *cu_q, const int *lens, void *stream);
+
+/* As mxfa_run_prefill_batch over what a microscaled cache holds. The workspace is
+ * sized by mxfa_prefill_batch_mx_workspace_bytes. */
+int mxfa_check_batch_mx(const mxfa_batch_shape *shape, int bits);
+size_t mxfa_prefill_batch_mx_workspace_bytes(const mxfa_batch_shape *shape, int bits);
+int mxfa_run_prefill_batch_mx(const mxfa_batch_shape *shape, int bits, const void *q, const void *kcache,
+                              const void *vcache, void *out, float *lse, const int *block_table, const int *cu_q,
+                              const int *lens, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- The pages of a cache: block tables (int32, table_stride elements between
  * rows), lengths and use counts of the blocks (int32 per block, how many table
  * rows hold it), all on the device. A sequence of lens[s] tokens holds its

@@ -62,6 +62,8 @@ EXPORTS = (
     "mxfa_check_rotary", "mxfa_run_rotary", "mxfa_check_batch", "mxfa_prefill_batch_workspace_bytes",
     "mxfa_run_prefill_batch", "mxfa_run_cache_append", "mxfa_check_pages", "mxfa_run_pages_free",
     "mxfa_run_pages_fork", "mxfa_run_pages_compact", "mxfa_run_pages_copy",
+    "mxfa_mx_block_bytes", "mxfa_run_cache_append_mx", "mxfa_run_cache_read_mx", "mxfa_check_batch_mx",
+    "mxfa_prefill_batch_mx_workspace_bytes", "mxfa_run_prefill_batch_mx",
 )
 # Every symbol include/mxfa_probes.h declares.
 PROBE_EXPORTS = (
@@ -110,6 +112,11 @@ class MxfaBatchShape(ctypes.Structure):
 
 class MxfaAppendRotary(ctypes.Structure):
     _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("factor", ctypes.c_float),
+                ("frequencies", ctypes.c_void_p)]
+
+
+class MxfaAppendRotaryMx(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("factor", ctypes.c_double),
                 ("frequencies", ctypes.c_void_p)]
 
 
@@ -199,6 +206,14 @@ def load_library(path: str | None = None):
     lib.mxfa_run_pages_fork.argtypes = [gp, vp, vp, vp, vp, vp, ci, vp, vp, vp, vp]
     lib.mxfa_run_pages_compact.argtypes = [gp, vp, vp, vp, vp, ci, vp, vp, vp, vp]
     lib.mxfa_run_pages_copy.argtypes = [vp, ci, cl, ci, cl, vp, ci, vp, vp]
+    lib.mxfa_mx_block_bytes.argtypes = [ci, ci, ci, ci]
+    lib.mxfa_mx_block_bytes.restype = ctypes.c_size_t
+    lib.mxfa_run_cache_append_mx.argtypes = [bp, ci, ctypes.POINTER(MxfaAppendRotaryMx), vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mxfa_run_cache_read_mx.argtypes = [bp, ci, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.mxfa_check_batch_mx.argtypes = [bp, ci]
+    lib.mxfa_prefill_batch_mx_workspace_bytes.argtypes = [bp, ci]
+    lib.mxfa_prefill_batch_mx_workspace_bytes.restype = ctypes.c_size_t
+    lib.mxfa_run_prefill_batch_mx.argtypes = [bp, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     op = ctypes.POINTER(MxfaBwdOptions)
     lib.mxfa_set_bwd_options.argtypes = [op]
     lib.mxfa_get_bwd_options.argtypes = [op]
@@ -207,7 +222,8 @@ def load_library(path: str | None = None):
     for name in EXPORTS + PROBE_EXPORTS:
         if name not in ("mxfa_version", "mxfa_strerror", "mxfa_bwd_workspace_bytes",
                         "mxfa_naive_scratch_bytes", "mxfa_bwd_noalloc_scratch_bytes",
-                        "mxfa_prefill_workspace_bytes", "mxfa_prefill_batch_workspace_bytes"):
+                        "mxfa_prefill_workspace_bytes", "mxfa_prefill_batch_workspace_bytes",
+                        "mxfa_mx_block_bytes", "mxfa_prefill_batch_mx_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_int
     if path is None:
         _lib = lib
@@ -226,6 +242,7 @@ class _NoBinding:
         return NotImplemented
     attention_fwd = attention_bwd = prefill = _other
     rotary = rotary_embedding = cache_append = prefill_batch = pages_free = pages_fork = pages_compact = pages_copy = _other
+    cache_append_mx = cache_read_mx = prefill_batch_mx = _other
 
 
 def _calls():
@@ -250,7 +267,9 @@ def _calls():
             "mxfa_run_flash_lse", "mxfa_run_bwd_ws", "mxfa_bwd_workspace_bytes", "mxfa_run_prefill",
             "mxfa_run_prefill_ws", "mxfa_run_prefill_paged", "mxfa_run_prefill_paged_ws", "mxfa_run_rotary",
             "mxfa_run_cache_append", "mxfa_run_prefill_batch", "mxfa_prefill_batch_workspace_bytes",
-            "mxfa_run_pages_free", "mxfa_run_pages_fork", "mxfa_run_pages_compact", "mxfa_run_pages_copy")))
+            "mxfa_run_pages_free", "mxfa_run_pages_fork", "mxfa_run_pages_compact", "mxfa_run_pages_copy",
+            "mxfa_mx_block_bytes", "mxfa_run_cache_append_mx", "mxfa_run_cache_read_mx", "mxfa_run_prefill_batch_mx",
+            "mxfa_prefill_batch_mx_workspace_bytes")))
         _native = ext
     return _native
 
@@ -1001,7 +1020,8 @@ def _block_table(block_table, n_seq, like):
 
 
 def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head, n_kv_head,
-                head_dim, scale):
+                head_dim, scale, bits=None):
+    """bits: None for a cache of rows in q's type, else blocks of bytes of so many bits a value."""
     torch = _torch()
     _dev(q, "q")
     if q.dtype not in (torch.bfloat16, torch.float32):
@@ -1011,8 +1031,11 @@ def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, l
         raise ValueError("n_head, n_kv_head, head_dim and block_size must be positive")
     n_tok = q.shape[0] if q.dim() == 2 else -1
     qp, qs = _rows(q, "q", q.dtype, 1, q_cols * head_dim)
-    kp, ks = _rows(_dev(kcache, "kcache", q.dtype, q), "kcache", q.dtype, block_size, n_kv_head * head_dim)
-    vp, vs = _rows(_dev(vcache, "vcache", q.dtype, q), "vcache", q.dtype, block_size, n_kv_head * head_dim)
+    kt, least, wide = q.dtype, block_size, n_kv_head * head_dim
+    if bits is not None:
+        kt, least, wide = torch.uint8, 1, mx_block_bytes(block_size, n_kv_head, head_dim, bits)
+    kp, ks = _rows(_dev(kcache, "kcache", kt, q), "kcache", kt, least, wide)
+    vp, vs = _rows(_dev(vcache, "vcache", kt, q), "vcache", kt, least, wide)
     if ks != vs or kcache.shape[0] != vcache.shape[0]:
         raise ValueError(f"kcache and vcache must share their rows and row stride ({kcache.shape[0]}, {ks} and "
                          f"{vcache.shape[0]}, {vs})")
@@ -1021,10 +1044,10 @@ def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, l
     lp = _ints(lens, "lens", 1, q)
     cp = _ints(cu_q, "cu_q", n_seq + 1, q)
     tp, wide, ts = _block_table(block_table, n_seq, q)
-    _c_int(n_tok=n_tok, n_blocks=kcache.shape[0] // block_size, table_stride=ts, q_stride=qs, kv_stride=ks,
+    n_blocks = kcache.shape[0] // least
+    _c_int(n_tok=n_tok, n_blocks=n_blocks, table_stride=ts, q_stride=qs, kv_stride=ks,
            out_stride=os_)
-    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, kcache.shape[0] // block_size,
-                        wide, ts, qs, ks, os_, MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, n_blocks, wide, ts, qs, ks, os_, MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
     return sh, qp, kp, vp, op, tp, cp, lp
 
 
@@ -1086,7 +1109,6 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
     prefill_batch_workspace_bytes bytes (allocated when None, as memory of
     `stream`); returned. Calls that may overlap need their own. bf16 with
     head_dim 64 or 128, or fp32 with 64."""
-    torch = _torch()
     if stream is None:
         rc = _calls().prefill_batch(q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head,
                                     n_kv_head, head_dim, scale, lse, workspace)
@@ -1094,8 +1116,16 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
             if isinstance(rc, int):
                 _check("mxfa_run_prefill_batch", rc)
             return rc
+    return _run_attention("mxfa_run_prefill_batch", (), q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q,
+                          n_head, n_kv_head, head_dim, scale, lse, workspace, stream)
+
+
+def _run_attention(func, bits, q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head, n_kv_head,
+                   head_dim, scale, lse, workspace, stream):
+    """The attention over either cache; bits: () or (the bits,)."""
+    torch = _torch()
     sh, qp, kp, vp, op, tp, cp, lp = _batch_args(q, n_head, kcache, vcache, out, block_table, block_size, cu_q, lens,
-                                                 max_q, n_head, n_kv_head, head_dim, scale)
+                                                 max_q, n_head, n_kv_head, head_dim, scale, *bits)
     ep = None
     if lse is not None:
         _dev(lse, "lse", torch.float32, q)
@@ -1103,17 +1133,114 @@ def run_prefill_batch(q, kcache, vcache, out, block_table, block_size: int, cu_q
             raise ValueError(f"lse: expected a contiguous [{sh.n_tok}, {n_head}], got {tuple(lse.shape)}")
         ep = ctypes.c_void_p(lse.data_ptr())
     lib = load_library()
-    _check("mxfa_check_batch", lib.mxfa_check_batch(ctypes.byref(sh)))
+    check, need, run = (getattr(lib, n) for n in (func.replace("run_prefill", "check"),
+                                                  func.replace("run_", "") + "_workspace_bytes", func))
+    _check("mxfa_check_batch" + func[len("mxfa_run_prefill_batch"):], check(ctypes.byref(sh), *bits))
     with _on(q.device):
         if workspace is None:
-            workspace = _scratch(int(lib.mxfa_prefill_batch_workspace_bytes(ctypes.byref(sh))), q.device, stream)
+            workspace = _scratch(int(need(ctypes.byref(sh), *bits)), q.device, stream)
         elif not _dev(workspace, "workspace", None, q).is_contiguous():
             raise ValueError("workspace: expected a contiguous device tensor")
-        _check("mxfa_run_prefill_batch",
-               lib.mxfa_run_prefill_batch(ctypes.byref(sh), qp, kp, vp, op, ep, tp, cp, lp,
-                                          ctypes.c_void_p(workspace.data_ptr()),
-                                          workspace.numel() * workspace.element_size(), _stream(stream)))
+        _check(func, run(ctypes.byref(sh), *bits, qp, kp, vp, op, ep, tp, cp, lp, ctypes.c_void_p(workspace.data_ptr()),
+                         workspace.numel() * workspace.element_size(), _stream(stream)))
     return workspace
+
+
+# ------------------------------------------------------- a microscaled cache --
+
+def mx_block_bytes(block_size: int, n_kv_head: int, head_dim: int = 64, bits: int = 8) -> int:
+    """mxfa_mx_block_bytes: the bytes of a block of a microscaled cache (a multiple of
+    16): of each head's row, 32 neighbouring elements share a power of two 2^(E -
+    127), one byte E, and are codes of 8 bits (e4m3) or 4 (e2m1) that stand for 2^(E
+    - 127) code. A pool is uint8 [blocks, at least this], its row stride a multiple
+    of 16; kcache and vcache are two of them. run_pages_copy(pool, 1, pairs) copies
+    its blocks."""
+    _c_int(block_size=block_size, n_kv_head=n_kv_head, head_dim=head_dim, bits=bits)
+    n = int(load_library().mxfa_mx_block_bytes(block_size, n_kv_head, head_dim, bits))
+    if n == 0:
+        raise ValueError(f"no microscaled blocks of block_size {block_size} (a power of two), {n_kv_head} KV heads, head_dim "
+                         f"{head_dim} (a multiple of 32, at most 256), {bits} bits (8 or 4)")
+    return n
+
+
+def run_cache_append_mx(qkv, q_out, kcache, vcache, bits: int, block_table, block_size: int, cu_q, lens, n_head: int,
+                        n_kv_head: int, head_dim: int = 64, frequencies=None, interleaved: bool = False,
+                        factor: float = 1.0, stream=None):
+    """mxfa_run_cache_append_mx: as run_cache_append, into a microscaled cache of `bits`
+    (8 or 4) bits a value: K, turned, and V are quantised as they are written, each
+    group of 32 elements by its own power of two, to the nearest code. kcache,
+    vcache: uint8 [blocks, at least mx_block_bytes]. A group of which an element is
+    not finite reads back as NaN. The other arguments are as for run_cache_append;
+    head_dim is a multiple of 32, at most 256."""
+    if stream is None:
+        rc = _calls().cache_append_mx(qkv, q_out, kcache, vcache, block_table, block_size, cu_q, lens, n_head, n_kv_head,
+                                      head_dim, frequencies, interleaved, factor, bits)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_cache_append_mx", rc)
+    sh, qp, kp, vp, op, tp, cp, lp = _batch_args(qkv, n_head + 2 * n_kv_head, kcache, vcache, q_out, block_table,
+                                                 block_size, cu_q, lens, 1, n_head, n_kv_head, head_dim, 0.0, bits)
+    fp, dim = (None, 0) if frequencies is None else _freqs(frequencies, head_dim, qkv)
+    rot = MxfaAppendRotaryMx(dim, int(bool(interleaved)), factor, fp)
+    with _on(qkv.device):
+        _check("mxfa_run_cache_append_mx",
+               load_library().mxfa_run_cache_append_mx(ctypes.byref(sh), bits, ctypes.byref(rot), qp, op, kp, vp, tp, cp,
+                                                       lp, _stream(stream)))
+
+
+def run_cache_read_mx(kcache, vcache, bits: int, k_out, v_out, block_table, block_size: int, cu_q, lens, n_kv_head: int,
+                      head_dim: int = 64, stream=None):
+    """mxfa_run_cache_read_mx: rows of a microscaled cache as bf16 or fp32 again (its
+    values are exact in either): row r of k_out and v_out ([rows, >= n_kv_head
+    head_dim], one row stride) is what the cache holds at the position of row r of
+    run_cache_append_mx for the same cu_q and lens, that is each sequence's last
+    cu_q[s + 1] - cu_q[s] positions: what an append wrote, or with the lengths' own
+    sums for cu_q the whole sequences. Rows of no position, and those past
+    cu_q[-1], stay as they were."""
+    torch = _torch()
+    if stream is None:
+        rc = _calls().cache_read_mx(kcache, vcache, k_out, v_out, block_table, block_size, cu_q, lens, n_kv_head, head_dim,
+                                    bits)
+        if rc is not NotImplemented:
+            return _check("mxfa_run_cache_read_mx", rc)
+    sh, op, kp, vp, _, tp, cp, lp = _batch_args(k_out, n_kv_head, kcache, vcache, k_out, block_table, block_size, cu_q,
+                                                lens, 1, n_kv_head, n_kv_head, head_dim, 0.0, bits)
+    wp, ws = _rows(_dev(v_out, "v_out", k_out.dtype, k_out), "v_out", k_out.dtype, sh.n_tok, n_kv_head * head_dim)
+    if v_out.shape[0] != sh.n_tok or (sh.n_tok > 1 and ws != sh.out_stride):
+        raise ValueError(f"k_out and v_out must share their rows and row stride ({sh.n_tok}, {sh.out_stride} and "
+                         f"{v_out.shape[0]}, {ws})")
+    with _on(k_out.device):
+        _check("mxfa_run_cache_read_mx",
+               load_library().mxfa_run_cache_read_mx(ctypes.byref(sh), bits, kp, vp, op, wp, tp, cp, lp, _stream(stream)))
+
+
+def prefill_batch_mx_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head: int, n_kv_head: int, head_dim: int = 64,
+                                     bf16: bool = True, bits: int = 8) -> int:
+    """mxfa_prefill_batch_mx_workspace_bytes: what run_prefill_batch_mx needs for such a
+    batch, whatever its lengths (0 for one it does not take)."""
+    w, entries = n_head * head_dim, 1 << 17
+    _c_int(n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, q_stride=w)
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w,
+                        mx_block_bytes(1, n_kv_head, head_dim, bits), w, MXFA_BF16 if bf16 else MXFA_F32, 0.0)
+    return int(load_library().mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(sh), bits))
+
+
+def run_prefill_batch_mx(q, kcache, vcache, bits: int, out, block_table, block_size: int, cu_q, lens, max_q: int,
+                         n_head: int, n_kv_head: int, head_dim: int = 64, scale: float = 0.0, lse=None, workspace=None,
+                         stream=None):
+    """mxfa_run_prefill_batch_mx: as run_prefill_batch, over what a microscaled cache of
+    `bits` (8 or 4) bits a value holds (run_cache_append_mx): K and V enter the
+    products as the values that their codes stand for, without another rounding. The
+    workspace is of prefill_batch_mx_workspace_bytes; the other arguments are as
+    for run_prefill_batch."""
+    if stream is None:
+        rc = _calls().prefill_batch_mx(q, kcache, vcache, out, block_table, block_size, cu_q, lens, max_q, n_head,
+                                       n_kv_head, head_dim, scale, lse, workspace, bits)
+        if rc is not NotImplemented:
+            if isinstance(rc, int):
+                _check("mxfa_run_prefill_batch_mx", rc)
+            return rc
+    return _run_attention("mxfa_run_prefill_batch_mx", (bits,), q, kcache, vcache, out, block_table, block_size, cu_q, lens,
+                          max_q, n_head, n_kv_head, head_dim, scale, lse, workspace, stream)
 
 
 # ------------------------------------------------------- the pages of a cache --

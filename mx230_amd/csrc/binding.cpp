@@ -38,6 +38,11 @@ struct {
     decltype(&mxfa_run_pages_fork) pages_fork;
     decltype(&mxfa_run_pages_compact) pages_compact;
     decltype(&mxfa_run_pages_copy) pages_copy;
+    decltype(&mxfa_mx_block_bytes) mx_block_bytes;
+    decltype(&mxfa_run_cache_append_mx) cache_append_mx;
+    decltype(&mxfa_run_cache_read_mx) cache_read_mx;
+    decltype(&mxfa_run_prefill_batch_mx) prefill_batch_mx;
+    decltype(&mxfa_prefill_batch_mx_workspace_bytes) prefill_batch_mx_workspace_bytes;
 } abi;
 
 PyObject *other() { Py_RETURN_NOTIMPLEMENTED; }
@@ -425,7 +430,7 @@ struct Batch {
     const at::Tensor *q, *k, *v, *o, *table, *cu_q, *lens;
     mxfa_batch_shape s;
     bool read(PyObject *q_, PyObject *k_, PyObject *v_, PyObject *o_, PyObject *table_, PyObject *block, PyObject *cu_,
-              PyObject *lens_, PyObject *heads_, PyObject *kv_heads, PyObject *head_dim, int kv_in_q) {
+              PyObject *lens_, PyObject *heads_, PyObject *kv_heads, PyObject *head_dim, int kv_in_q, int bits = 0) {
         q = plain(q_), k = plain(k_), v = plain(v_), o = plain(o_), table = plain(table_), cu_q = plain(cu_);
         lens = plain(lens_);
         s = mxfa_batch_shape{};
@@ -437,38 +442,46 @@ struct Batch {
             return false;
         const at::ScalarType t = q->scalar_type();
         const int64_t d = s.head_dim, kw = s.n_kv_head * d;
-        if (!rows_of(q, t, 1, (s.n_head + kv_in_q * (int64_t)s.n_kv_head) * d, &s.q_stride) ||
-            !rows_of(k, t, s.block_size, kw, &ks) || !rows_of(v, t, s.block_size, kw, &vs) || ks != vs ||
+        // a cache row in q's type; a block of bytes
+        const at::ScalarType kt = bits ? at::kByte : t;
+        const int64_t least = bits ? 1 : s.block_size;
+        const int64_t wide = bits ? (int64_t)abi.mx_block_bytes(s.block_size, s.n_kv_head, s.head_dim, bits) : kw;
+        if (wide < 1 || !rows_of(q, t, 1, (s.n_head + kv_in_q * (int64_t)s.n_kv_head) * d, &s.q_stride) ||
+            !rows_of(k, kt, least, wide, &ks) || !rows_of(v, kt, least, wide, &vs) || ks != vs ||
             k->size(0) != v->size(0) || !rows_of(o, t, q->size(0), s.n_head * d, &s.out_stride) ||
             !vec(lens, at::kInt, 1) || !vec(cu_q, at::kInt, lens->numel() + 1) ||
             !table_of(table, lens->numel(), &s.max_blocks, &s.table_stride) ||
-            k->size(0) / s.block_size > INT32_MAX)
+            k->size(0) / least > INT32_MAX)
             return false;
         s.n_tok = (int)q->size(0);
         s.n_seq = (int)lens->numel();
         s.max_q = 1;
-        s.n_blocks = (int)(k->size(0) / s.block_size);
+        s.n_blocks = (int)(k->size(0) / least);
         s.kv_stride = ks;
         s.dtype = t == at::kBFloat16 ? MXFA_BF16 : MXFA_F32;
         return true;
     }
 };
 
-// cache_append(qkv, q_out, kcache, vcache, table, block_size, cu_q, lens, n_head, n_kv_head,
-// head_dim, frequencies or None, interleaved, factor): the status
-PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (n != 14 || abi.cache_append == nullptr) return other();
+// `bits` of a microscaled cache, where a call is of one.
+bool mx_bits(PyObject *o, int *bits) { return integer(o, bits) && (*bits == 8 || *bits == 4); }
+
+// The append into either cache (R: its rotation), bits from *more.
+template <class R, class Run>
+PyObject *append_to(PyObject *const *a, PyObject *more, Run run) {
     return guarded([&]() -> PyObject * {
         Batch b;
-        mxfa_append_rotary r{};
+        R r{};
         double factor;
+        int bits = 0;
+        if (more != nullptr && !mx_bits(more, &bits)) return other();
         const bool turned = a[11] != Py_None;
         const at::Tensor *f = turned ? plain(a[11]) : nullptr;
-        if (!b.read(a[0], a[2], a[3], a[1], a[4], a[5], a[6], a[7], a[8], a[9], a[10], 2) ||
+        if (!b.read(a[0], a[2], a[3], a[1], a[4], a[5], a[6], a[7], a[8], a[9], a[10], 2, bits) ||
             !flag(a[12], &r.interleaved) || !number(a[13], &factor) ||
             (turned && (!vec(f, at::kDouble, 1) || 2 * f->numel() > b.s.head_dim)))
             return other();
-        r.factor = (float)factor;
+        r.factor = (decltype(r.factor))factor;
         if (turned) {
             r.rotary_dim = 2 * (int)f->numel();
             r.frequencies = static_cast<const double *>(f->data_ptr());
@@ -478,28 +491,66 @@ PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int *table = ints(b.table), *cu = ints(b.cu_q), *lens = ints(b.lens);
         int rc;
         Py_BEGIN_ALLOW_THREADS;
-        rc = abi.cache_append(&b.s, &r, q, o, k, v, table, cu, lens, stream);
+        rc = run(&b.s, bits, &r, q, o, k, v, table, cu, lens, stream);
         Py_END_ALLOW_THREADS;
         return status(rc);
     });
 }
 
-// prefill_batch(q, kcache, vcache, out, table, block_size, cu_q, lens, max_q, n_head, n_kv_head,
-// head_dim, scale, lse or None, workspace or None): the workspace, or the status
-PyObject *prefill_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (n != 15 || abi.prefill_batch == nullptr) return other();
+// cache_append(qkv, q_out, kcache, vcache, table, block_size, cu_q, lens, n_head, n_kv_head,
+// head_dim, frequencies or None, interleaved, factor): the status
+PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 14 || abi.cache_append == nullptr) return other();
+    return append_to<mxfa_append_rotary>(a, nullptr, [](const mxfa_batch_shape *s, int, auto... x) {
+        return abi.cache_append(s, x...);
+    });
+}
+// cache_append_mx(the same, bits)
+PyObject *cache_append_mx(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 15 || abi.cache_append_mx == nullptr) return other();
+    return append_to<mxfa_append_rotary_mx>(a, a[14], [](auto... x) { return abi.cache_append_mx(x...); });
+}
+
+// cache_read_mx(kcache, vcache, k_out, v_out, table, block_size, cu_q, lens, n_kv_head, head_dim,
+// bits): the status
+PyObject *cache_read_mx(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 11 || abi.cache_read_mx == nullptr) return other();
+    return guarded([&]() -> PyObject * {
+        Batch b;
+        int bits, vs;
+        const at::Tensor *v_out = plain(a[3]);
+        // (k_out in the place of q too: its rows are the batch's)
+        if (!mx_bits(a[10], &bits) || !b.read(a[2], a[0], a[1], a[2], a[4], a[5], a[6], a[7], a[8], a[8], a[9], 0, bits) ||
+            !here(v_out) || !rows_of(v_out, b.o->scalar_type(), b.s.n_tok, (int64_t)b.s.n_kv_head * b.s.head_dim, &vs) ||
+            v_out->size(0) != b.s.n_tok || (b.s.n_tok > 1 && vs != b.s.out_stride))
+            return other();
+        const void *k = b.k->data_ptr(), *v = b.v->data_ptr();
+        void *ko = b.o->data_ptr(), *vo = v_out->data_ptr(), *stream = current_stream();
+        const int *table = ints(b.table), *cu = ints(b.cu_q), *lens = ints(b.lens);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = abi.cache_read_mx(&b.s, bits, k, v, ko, vo, table, cu, lens, stream);
+        Py_END_ALLOW_THREADS;
+        return status(rc);
+    });
+}
+
+// The attention over either cache, bits from *more.
+PyObject *attend(PyObject *const *a, PyObject *more) {
     return guarded([&]() -> PyObject * {
         Batch b;
         double sc;
+        int bits = 0;
+        if (more != nullptr && !mx_bits(more, &bits)) return other();
         const bool want_lse = a[13] != Py_None, given = a[14] != Py_None;
         const at::Tensor *lse = want_lse ? plain(a[13]) : nullptr, *ws = given ? plain(a[14]) : nullptr;
-        if (!b.read(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[9], a[10], a[11], 0) ||
+        if (!b.read(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[9], a[10], a[11], 0, bits) ||
             !integer(a[8], &b.s.max_q) || !number(a[12], &sc) || (given && (!here(ws) || !ws->is_contiguous())) ||
             (want_lse && (!here(lse) || lse->scalar_type() != at::kFloat || lse->dim() != 2 ||
                           !lse->is_contiguous() || lse->size(0) != b.s.n_tok || lse->size(1) != b.s.n_head)))
             return other();
         b.s.scale = (float)sc;
-        const size_t need = abi.prefill_batch_workspace_bytes(&b.s);
+        const size_t need = bits ? abi.prefill_batch_mx_workspace_bytes(&b.s, bits) : abi.prefill_batch_workspace_bytes(&b.s);
         at::Tensor own;
         if (!given) {
             if (need == 0) return other();  // a shape it does not take
@@ -513,13 +564,23 @@ PyObject *prefill_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const size_t bytes = (size_t)ws->numel() * ws->element_size();
         int rc;
         Py_BEGIN_ALLOW_THREADS;
-        rc = abi.prefill_batch(&b.s, q, k, v, o, lp, table, cu, lens, wp, bytes, stream);
+        rc = bits ? abi.prefill_batch_mx(&b.s, bits, q, k, v, o, lp, table, cu, lens, wp, bytes, stream)
+                  : abi.prefill_batch(&b.s, q, k, v, o, lp, table, cu, lens, wp, bytes, stream);
         Py_END_ALLOW_THREADS;
         if (rc != 0) return status(rc);
         if (!given) return THPVariable_Wrap(std::move(own));
         Py_INCREF(a[14]);
         return a[14];
     });
+}
+// prefill_batch(q, kcache, vcache, out, table, block_size, cu_q, lens, max_q, n_head, n_kv_head,
+// head_dim, scale, lse or None, workspace or None): the workspace, or the status
+PyObject *prefill_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return n != 15 || abi.prefill_batch == nullptr ? other() : attend(a, nullptr);
+}
+// prefill_batch_mx(the same, bits)
+PyObject *prefill_batch_mx(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return n != 16 || abi.prefill_batch_mx == nullptr ? other() : attend(a, a[15]);
 }
 
 // The tables of the pages' calls: block_table, block_size, lens, refs.
@@ -606,7 +667,7 @@ PyObject *pages_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 // bind(addresses of the ABI functions, in the order of `abi`)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    constexpr int kCount = 15;
+    constexpr int kCount = 20;
     if (n != kCount) {
         PyErr_Format(PyExc_TypeError, "bind: %d addresses expected", kCount);
         return nullptr;
@@ -631,6 +692,11 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     abi.pages_fork = reinterpret_cast<decltype(abi.pages_fork)>(f[12]);
     abi.pages_compact = reinterpret_cast<decltype(abi.pages_compact)>(f[13]);
     abi.pages_copy = reinterpret_cast<decltype(abi.pages_copy)>(f[14]);
+    abi.mx_block_bytes = reinterpret_cast<decltype(abi.mx_block_bytes)>(f[15]);
+    abi.cache_append_mx = reinterpret_cast<decltype(abi.cache_append_mx)>(f[16]);
+    abi.cache_read_mx = reinterpret_cast<decltype(abi.cache_read_mx)>(f[17]);
+    abi.prefill_batch_mx = reinterpret_cast<decltype(abi.prefill_batch_mx)>(f[18]);
+    abi.prefill_batch_mx_workspace_bytes = reinterpret_cast<decltype(abi.prefill_batch_mx_workspace_bytes)>(f[19]);
     Py_RETURN_NONE;
 }
 
@@ -639,7 +705,8 @@ PyMethodDef methods[] = {MXFA_METHOD(bind), MXFA_METHOD(attention_fwd), MXFA_MET
                          MXFA_METHOD(prefill), MXFA_METHOD(rotary), MXFA_METHOD(rotary_embedding),
                          MXFA_METHOD(cache_append),
                          MXFA_METHOD(prefill_batch), MXFA_METHOD(pages_free), MXFA_METHOD(pages_fork),
-                         MXFA_METHOD(pages_compact), MXFA_METHOD(pages_copy), {nullptr, nullptr, 0, nullptr}};
+                         MXFA_METHOD(pages_compact), MXFA_METHOD(pages_copy), MXFA_METHOD(cache_append_mx),
+                         MXFA_METHOD(cache_read_mx), MXFA_METHOD(prefill_batch_mx), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

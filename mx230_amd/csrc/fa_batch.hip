@@ -64,6 +64,7 @@ struct PolF32 {
     static constexpr int D = 64;
     using T = float;
     using Frag = f32x4;
+    using QFrag = Frag;
     static constexpr int EPC = 4, NC = 4, ROWS = 64;
     __device__ static __forceinline__ void chunk_at(int P, int &row, int &chunk) {
         row = P >> 4;
@@ -118,6 +119,7 @@ struct PolRows {
     static constexpr int D = D_, EPC = 8, NC = Base::NC, ROWS = 64, CPR = D / 8;
     using T = u16;
     using Frag = typename Base::Frag;
+    using QFrag = Frag;
     using ChainB = typename Base::ChainB;
     __device__ static __forceinline__ int arow(int t, int m) { return Base::arow(t, m); }
     __device__ static __forceinline__ int bidx(int t, int g, int r) { return Base::bidx(t, g, r); }
@@ -133,15 +135,18 @@ struct PolRows {
 #pragma unroll
         for (int c = 0; c < NC; ++c) f[c] = *reinterpret_cast<const Frag *>(base + (x ^ (64 * c)));
     }
-    __device__ static __forceinline__ f32x4 chain(f32x4 acc, const ChainB &b, const T *tile, int y0, int blk, int g,
-                                                  int l16) {
+    __device__ static __forceinline__ Frag chain_a(const T *tile, int y0, int blk, int g, int l16) {
         const int r0 = blk + 8 * g + (l16 >> 2);
         const char *base = reinterpret_cast<const char *>(tile) + r0 * (2 * D) + ((l16 & 1) << 3);
         const int x = (((l16 >> 1) & 1) ^ swz(r0)) << 4;
         const int off = x ^ (2 * y0);
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(base + off));
         const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(base + off + 4 * (2 * D)));
-        return mma(__builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), b, acc);
+        return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ static __forceinline__ f32x4 chain(f32x4 acc, const ChainB &b, const T *tile, int y0, int blk, int g,
+                                                  int l16) {
+        return mma(chain_a(tile, y0, blk, g, l16), b, acc);
     }
     // the chunk at 16-byte position P of the tile, and its row
     __device__ static __forceinline__ void chunk_at(int P, int &row, int &chunk) {
@@ -351,12 +356,41 @@ __device__ __forceinline__ f32x4 batch_quad(const f32x4 (&acc)[XT][QT], int i, i
     }
 }
 
+// A sequence's K and V of one KV head, E elements from column c of each position, as
+// floats, for batch_plain.
+template <class T, int D>
+struct PlainRows {
+    static constexpr int E = D / 4;
+    const T *K, *V;
+    const int *table;
+    int shift, stride;
+    unsigned last;
+    __device__ __forceinline__ PlainRows(const BatchParams &p, const BatchItem &it, int c)
+        : K(static_cast<const T *>(p.k) + it.head * D + c), V(static_cast<const T *>(p.v) + it.head * D + c),
+          table(p.table + (long long)it.seq * p.table_stride), shift(p.bs_shift), stride(p.kv_rs),
+          last((unsigned)(p.n_blocks - 1)) {}
+    __device__ __forceinline__ void read(int k, float (&kf)[E], float (&vf)[E]) const {
+        const size_t b = min((unsigned)table[k >> shift], last);
+        const size_t at = ((b << shift) + (k & ((1 << shift) - 1))) * (size_t)stride;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if constexpr (sizeof(T) == 2) {
+                kf[e] = __uint_as_float((uint32_t)K[at + e] << 16);
+                vf[e] = __uint_as_float((uint32_t)V[at + e] << 16);
+            } else {
+                kf[e] = K[at + e];
+                vf[e] = V[at + e];
+            }
+        }
+    }
+};
+
 // A unit's share in plain fp32 arithmetic, keys a row does not see left out
 // altogether: taken where a value was not finite, since in the matrix products
 // an infinity or NaN in the V of a key that a row does not see reaches it as 0
 // x inf. 4 threads per row, rows from row0 of the unit. Some 6 times the time of the
 // products. A row's running (max, sum) and output go where the form's would: to the workspace slot, or (part null) finished.
-template <class T, int D, int ROWS>
+template <class T, int D, int ROWS, class Rows = PlainRows<T, D>>
 __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchItem &it, int row0, int key0, int key1,
                                             float *part, float *ml) {
     constexpr int E = D / 4;
@@ -376,21 +410,20 @@ __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchIte
         acc[e] = 0.f;
     }
     const int kend = min(min(key1, it.s.keys), it.s.pos + row / p.group + 1);
-    const int *table = p.table + (long long)it.seq * p.table_stride;
+    const Rows rows(p, it, c);
     for (int k = key0; k < kend; ++k) {
-        const size_t b = min((unsigned)table[k >> p.bs_shift], (unsigned)(p.n_blocks - 1));
-        const size_t at = ((b << p.bs_shift) + (k & ((1 << p.bs_shift) - 1))) * (size_t)p.kv_rs + it.head * D + c;
-        const T *K = static_cast<const T *>(p.k) + at, *V = static_cast<const T *>(p.v) + at;
+        float kf[E], vf[E];
+        rows.read(k, kf, vf);
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = __builtin_fmaf(q[e], val(K[e]), s);
+        for (int e = 0; e < E; ++e) s = __builtin_fmaf(q[e], kf[e], s);
         s = quad_sum(s);
         const float mn = fmaxf(m, s), mref = mn == -INFINITY ? 0.f : mn;
         const float corr = fast_exp2(m - mref), pv = fast_exp2(s - mref);
         m = mn;
         l = l * corr + pv;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(pv, val(V[e]), acc[e] * corr);
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(pv, vf[e], acc[e] * corr);
     }
     if (!have) return;
 #pragma unroll
@@ -416,18 +449,75 @@ __device__ __forceinline__ int few_slots(const BatchParams &p) { return 2 * p.fe
 
 // ------------------------------------------------------------------ the few rows
 
+// Where a piece's waves meet.
+template <int D, int NW>
+struct BatchFewMerge {
+    float acc[NW][kBatchFew][D + 4];
+    float ml[NW][kBatchFew][2];
+    int bad;
+};
+
 template <class Pol, int NW>
 union BatchFewSmem {
     struct {
         typename Pol::T k[NW][Pol::ROWS * Pol::D], v[NW][Pol::ROWS * Pol::D];
         int blk[NW][2][64];
     } t;
-    struct {
-        float acc[NW][kBatchFew][Pol::D + 4];
-        float ml[NW][kBatchFew][2];
-        int bad;
-    } merge;
+    BatchFewMerge<Pol::D, NW> merge;
 };
+
+// The end of a piece: the NW waves' maxima, sums and O are added and go to the
+// workspace slot or (slot < 0) out. quad(i): 4 columns from col(i) of the lane's
+// row, i < D / 16; lw: its sum over the wave's keys; bad: not finite, or flagged;
+// plain(part, ml): the piece in plain arithmetic.
+template <class T, int D, int NW, int THREADS, class Quad, class Col, class Plain>
+__device__ __forceinline__ void batch_few_finish(const BatchParams &p, const BatchItem &it, int slot,
+                                                 BatchFewMerge<D, NW> &sm, float m, float lw, bool bad, Quad quad, Col col,
+                                                 Plain plain) {
+    constexpr int ROWS = kBatchFew;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    __syncthreads();  // every wave is done with the tiles
+    if (tid == 0) sm.bad = 0;
+    __syncthreads();
+    if (bad && lane == 0) sm.bad = 1;
+    if (wave < NW) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4 *>(&sm.acc[wave][l16][col(i)]) = quad(i);
+        if (g == 0) *reinterpret_cast<float2 *>(sm.ml[wave][l16]) = make_float2(m, lw);
+    }
+    __syncthreads();
+    float *part = nullptr, *ml = nullptr;
+    if (slot >= 0) {
+        part = batch_part(p.part[0], slot, ROWS, D);
+        ml = batch_ml(p.part[0], few_slots(p), slot, ROWS, D);
+    }
+    if (sm.bad) {
+        if (tid < 4 * ROWS) plain(part, ml);
+        return;
+    }
+    for (int i = tid; i < it.s.rows * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), c = 4 * (i % (D / 4));
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm.ml[w][r][0]);
+        const float mref = M == -INFINITY ? 0.f : M;  // no key of the row here: weight 0
+        f32x4 o = zero4();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float x = fast_exp2(sm.ml[w][r][0] - mref);
+            L += x * sm.ml[w][r][1];
+            o += *reinterpret_cast<const f32x4 *>(&sm.acc[w][r][c]) * x;
+        }
+        if (part != nullptr) {
+            store4<float>(part + r * D + c, o, 1.0f);
+            if (c == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(M, L);
+        } else {
+            batch_store<T>(p, it, r, D, c, o, M, L);
+        }
+    }
+}
 
 // One piece of a sequence: each of the NW waves takes every NW-th of its stages
 // [s_lo, s_hi), staged into its own tiles with no barrier; the waves' maxima,
@@ -514,46 +604,13 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
 #pragma unroll
     for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt][0]);
     const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
-    __syncthreads();  // every wave is done with the tiles
-    if (tid == 0) sm.merge.bad = 0;
-    __syncthreads();
-    if (bad && lane == 0) sm.merge.bad = 1;
-    if (wave < NW) {
-#pragma unroll
-        for (int i = 0; i < XT; ++i)
-            *reinterpret_cast<f32x4 *>(&sm.merge.acc[own][l16][batch_col<Pol>(i, g)]) = batch_quad<Pol>(acc, i, 0);
-        if (g == 0) *reinterpret_cast<float2 *>(sm.merge.ml[own][l16]) = make_float2(m[0], lw);
-    }
-    __syncthreads();
-    float *part = nullptr, *ml = nullptr;
-    if (slot >= 0) {
-        part = batch_part(p.part[0], slot, ROWS, D);
-        ml = batch_ml(p.part[0], few_slots(p), slot, ROWS, D);
-    }
-    if (sm.merge.bad) {
-        if (tid < 4 * ROWS) batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
-        return;
-    }
-    for (int i = tid; i < it.s.rows * (D / 4); i += THREADS) {
-        const int r = i / (D / 4), c = 4 * (i % (D / 4));
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm.merge.ml[w][r][0]);
-        const float mref = M == -INFINITY ? 0.f : M;  // no key of the row here: weight 0
-        f32x4 o = zero4();
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float x = fast_exp2(sm.merge.ml[w][r][0] - mref);
-            L += x * sm.merge.ml[w][r][1];
-            o += *reinterpret_cast<const f32x4 *>(&sm.merge.acc[w][r][c]) * x;
-        }
-        if (part != nullptr) {
-            store4<float>(part + r * D + c, o, 1.0f);
-            if (c == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(M, L);
-        } else {
-            batch_store<T>(p, it, r, D, c, o, M, L);
-        }
-    }
+    batch_few_finish<T, D, NW, THREADS>(
+        p, it, slot, sm.merge, m[0], lw, bad,
+        [&](int i) __attribute__((always_inline)) { return batch_quad<Pol>(acc, i, 0); },
+        [&](int i) __attribute__((always_inline)) { return batch_col<Pol>(i, g); },
+        [&](float *part, float *ml) __attribute__((always_inline)) {
+            batch_plain<T, D, ROWS>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
+        });
 }
 
 // Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line. Equal
@@ -561,8 +618,9 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
 // positions, 32/8 heads, d = 128, in 393 us with the join, at the step that brought
 // them, 415 with a work-group per share of a sequence, whose count the host can only
 // bound: thousands are empty.
-template <class Pol, int NW, int THREADS>
-__device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
+// (piece(item, first and last stage, slot): as batch_few_piece)
+template <class Piece>
+__device__ __forceinline__ void batch_few_run(const BatchParams &p, int g, Piece piece) {
     const unsigned all = few_line(p), run = few_run(p, all);
     unsigned x = (unsigned)(g / p.Hkv) * run;
     const unsigned x1 = min(x + run, all);
@@ -579,10 +637,16 @@ __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, Batc
         it.s = s;
         const FewPiece f = few_piece(x, x1, u0, u1, g);
         if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, s.q0, s.rows, s.pos});
-        batch_few_piece<Pol, NW, THREADS>(p, it, f.lo, f.hi, f.slot, sm);
+        piece(it, f.lo, f.hi, f.slot);
         x = f.end;
         if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
         return x >= x1;
+    });
+}
+template <class Pol, int NW, int THREADS>
+__device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
+    batch_few_run(p, g, [&](const BatchItem &it, int lo, int hi, int slot) __attribute__((always_inline)) {
+        batch_few_piece<Pol, NW, THREADS>(p, it, lo, hi, slot, sm);
     });
 }
 
@@ -1111,14 +1175,6 @@ MXFA_BATCH_MANY(f64_many, f64_both, PolF32, FwdSplitSmem, 2, 64 * kBatchF32Waves
 #undef MXFA_BATCH
 #endif
 
-// The forms of a call; groups = 0: not launched.
-static void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2]) {
-    batch_plan(p, dtype_bf16);
-    f[0] = f[1] = BatchForm{0, 0, 0, 0, 0};
-    if (p->few_rows > 0) f[0] = batch_few_form(p);
-    if (batch_may_be_many(*p)) f[1] = batch_many_form(p, dtype_bf16);
-}
-
 size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
     BatchParams p = q;
     BatchForm f[2];
@@ -1135,13 +1191,21 @@ long long batch_groups(const BatchParams &q, int dtype_bf16) {
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
-    static constexpr KernelId ids[3][6] = {
+    static constexpr KernelId ids[9][6] = {
         {k_mxfa_batch_b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_b64_many, k_mxfa_batch_b64_both,
          k_mxfa_batch_b64_many64, k_mxfa_batch_b64_both64},
         {k_mxfa_batch_b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_b128_many, k_mxfa_batch_b128_both,
          k_mxfa_batch_b128_many64, k_mxfa_batch_b128_both64},
-        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_f64_many, k_mxfa_batch_f64_both}};
-    const KernelId *id = ids[!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0];
+        {k_mxfa_batch_f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_f64_many, k_mxfa_batch_f64_both},
+#define MXFA_IDS(BITS)                                                                                                  \
+    {k_mxfa_batch_x##BITS##b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_x##BITS##b64_many, k_mxfa_batch_x##BITS##b64_both, \
+     k_mxfa_batch_x##BITS##b64_many64, k_mxfa_batch_x##BITS##b64_both64},                                               \
+        {k_mxfa_batch_x##BITS##b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_x##BITS##b128_many,                       \
+         k_mxfa_batch_x##BITS##b128_both, k_mxfa_batch_x##BITS##b128_many64, k_mxfa_batch_x##BITS##b128_both64},        \
+    {k_mxfa_batch_x##BITS##f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_x##BITS##f64_many, k_mxfa_batch_x##BITS##f64_both}
+        MXFA_IDS(8), MXFA_IDS(4)};
+#undef MXFA_IDS
+    const KernelId *id = ids[(p.bits == 0 ? 0 : p.bits == 8 ? 3 : 6) + (!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0)];
     BatchForm f[2];
     batch_forms(&p, dtype_bf16, f);
     const KernelId *many = id + (p.many_rows == 64 ? 4 : 2);
@@ -1157,7 +1221,7 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     int few_groups = (int)f[0].groups;
     void *args[] = {&p, &few_groups};
     if (f[1].groups == 0) {
-        e = launch_kernel(id[0], dim3(few_groups), dim3(dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+        e = launch_kernel(id[0], dim3(few_groups), dim3(p.bits != 0 || (dtype_bf16 && p.d == 64) ? 512 : 256), args, stream);
     } else if (few_groups == 0) {
         e = launch_kernel(many[0], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
     } else {

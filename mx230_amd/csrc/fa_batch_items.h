@@ -360,10 +360,18 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
     p->many_rows = batch_many_rows(*p, dtype_bf16);
-    p->least[0] = dtype_bf16 && p->d == 64 ? 8 : 4;
+    p->least[0] = p->bits != 0 || (dtype_bf16 && p->d == 64) ? 8 : 4;
     p->least[1] = 4;
     p->whole = dtype_bf16 ? 6 : 4;
     p->per_item = dtype_bf16 ? 0.024f : 0.007f;
+}
+
+// The forms of a call; groups = 0: not launched.
+inline void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2]) {
+    batch_plan(p, dtype_bf16);
+    f[0] = f[1] = BatchForm{0, 0, 0, 0, 0};
+    if (p->few_rows > 0) f[0] = batch_few_form(p);
+    if (batch_may_be_many(*p)) f[1] = batch_many_form(p, dtype_bf16);
 }
 
 }  // namespace mxfa

@@ -1,0 +1,605 @@
+// Attention of a batch over a paged cache in 8 or 4 bits (fa_mx.h): the work of
+// fa_batch.hip, whose parts, units, shares and joins these kernels share, with K and
+// V made bf16 on their way to the matrix products, exactly. bf16 operands of Q and
+// p are as there; in fp32 Q and p are three bf16 parts (Split3), and a product
+// is three of the matrix instruction's, not six, since K and V are whole in one.
+//
+//   * few rows: codes and E go to LDS as they lie in the cache (a wave's own tiles, by
+//     direct loads); a lane takes a quarter of a key's row, 16 bytes at d = 128 and 4
+//     bits, as its share of the contraction over d, so K is converted in registers,
+//     E's power in the same instruction. V is read from LDS transposed, still as
+//     codes (ds_read_b64_tr_b4 / _b8): a lane has 16 keys of one column, whose powers
+//     differ, so these multiply p before it is rounded for the product.
+//   * many rows: a thread loads a part of a key's row a stage ahead and converts it
+//     once for the work-group, into the bf16 tiles of fa_batch.hip's products.
+#include "fa_batch_items.h"
+#include "fa_launch.h"
+#include "fa_mx.h"
+
+namespace mxfa {
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+template <int BITS_, int D_>
+struct Mx {
+    static constexpr int BITS = BITS_, D = D_;
+    static constexpr int CB = mx_code_bytes(D, BITS), SB = mx_scale_bytes(D);  // bytes of a head's row
+    static constexpr int QB = CB / 4, CH = CB / 16;  // of a quarter of it; 16-byte chunks
+    static constexpr int TILE = 64 * CB;
+};
+
+// The byte offsets of positions' codes in a pool; blocks as in BatchRows.
+template <class F>
+struct MxRows {
+    BatchRows rows;
+    unsigned stride;
+    MxHead head;
+    __device__ __forceinline__ MxRows(const BatchParams &p, const BatchItem &it, int keys)
+        : rows{p.table + (long long)it.seq * p.table_stride, p.bs_shift, keys, (unsigned)(p.n_blocks - 1)},
+          stride((unsigned)p.kv_rs), head(mx_head(p, it.head)) {}
+    __device__ __forceinline__ unsigned inside(int t) const {
+        return (unsigned)min(t, rows.keys - 1) & ((1u << rows.shift) - 1u);
+    }
+    __device__ __forceinline__ size_t block(int blk) const { return (size_t)min((unsigned)blk, rows.last) * stride; }
+    __device__ __forceinline__ size_t codes(int blk, int t) const { return block(blk) + head.codes + inside(t) * F::CB; }
+    __device__ __forceinline__ size_t scales(int blk, int t) const { return block(blk) + head.scales + inside(t) * F::SB; }
+};
+
+// For batch_plain: elements c .. c + D / 4 - 1, a quarter of a row, of one group.
+template <class F>
+struct MxPlainRows {
+    static constexpr int E = F::D / 4;
+    MxRows<F> rows;
+    const char *k, *v;
+    int quarter;
+    __device__ __forceinline__ MxPlainRows(const BatchParams &p, const BatchItem &it, int c)
+        : rows(p, it, INT_MAX), k(static_cast<const char *>(p.k)), v(static_cast<const char *>(p.v)), quarter(c / E) {}
+    __device__ __forceinline__ void read_one(const char *x, size_t codes, size_t scales, float (&f)[E]) const {
+        uint32_t w[F::QB / 4];
+        load_words(w, x + codes + quarter * F::QB);
+        const float power = mx_power((unsigned char)x[scales + quarter * E / kMxGroup]);
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i) {
+            const bf16x8 y = mx_values<F::BITS>(w + i * (F::BITS / 4), power);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[8 * i + e] = (float)y[e];
+        }
+    }
+    __device__ __forceinline__ void read(int t, float (&kf)[E], float (&vf)[E]) const {
+        const int blk = rows.rows.table[t >> rows.rows.shift];
+        const size_t codes = rows.codes(blk, t), scales = rows.scales(blk, t);
+        read_one(k, codes, scales, kf);
+        read_one(v, codes, scales, vf);
+    }
+};
+
+// A product's operand in registers, and c + a b, for bf16 and (three parts) fp32.
+template <class T>
+struct MxOperand;
+template <>
+struct MxOperand<u16> {
+    using B = bf16x8;
+    static constexpr float kUp = 1.f, kDown = 1.f;
+    __device__ static __forceinline__ B pack(const f32x4 &a, const f32x4 &b) { return PolBF16<64>::pack(a, b); }
+    __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) { return PolBF16<64>::mma(a, b, c); }
+};
+template <>
+struct MxOperand<float> {
+    using B = Split3;
+    // p times a power of down to 2^-117 keeps its parts (kPartMin)
+    static constexpr float kUp = kPartUp, kDown = kPartDown;
+    __device__ static __forceinline__ B pack(const f32x4 &a, const f32x4 &b) { return split3(a, b); }
+    __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) {
+        c = PolBF16<64>::mma(a, b.l, c);
+        c = PolBF16<64>::mma(a, b.m, c);
+        return PolBF16<64>::mma(a, b.h, c);
+    }
+};
+
+// A lane's D / 4 elements of a row of Q, quarter g, in the order of K's codes. True
+// for the wave where a row's parts are not 24 bits (fp32: as split_row).
+template <class F, class T>
+__device__ __forceinline__ bool mx_row(typename MxOperand<T>::B (&f)[F::D / 32], const T *row, int g) {
+    row += g * (F::D / 4);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int c = 0; c < F::D / 32; ++c) f[c] = *reinterpret_cast<const bf16x8 *>(row + 8 * c);
+        return false;
+    } else {
+        float mx = 0.f;
+#pragma unroll
+        for (int c = 0; c < F::D / 32; ++c) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(row + 8 * c), b = *reinterpret_cast<const f32x4 *>(row + 8 * c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(a[e]), fabsf(b[e])));
+            f[c] = split3(a, b);
+        }
+        uint64_t some = __builtin_amdgcn_ballot_w64(mx > 0.f), enough = __builtin_amdgcn_ballot_w64(mx >= kPartMin);
+        some |= some >> 32;
+        enough |= enough >> 32;
+        return (((some | some >> 16) & ~(enough | enough >> 16)) & 0xffff) != 0;
+    }
+}
+
+// ------------------------------------------------------------------ the few rows
+
+template <class F, int NW>
+union MxFewSmem {
+    struct {
+        char k[NW][F::TILE], v[NW][F::TILE];
+        uint32_t ke[NW][64], ve[NW][64];  // E of a key in its low SB bytes
+        int blk[NW][2][64];
+    } t;
+    BatchFewMerge<F::D, NW> merge;
+};
+
+// Codes in LDS: chunk c of row r at slot c ^ kswz(r) (K) or c ^ vswz(r) (V).
+template <class F>
+__device__ __forceinline__ int mx_kswz(int r) {
+    // a score operand reads rows that differ in bits 0, 1, 4, 5, one quarter at a time
+    return F::CH == 8 ? (((r >> 1) & 1) | ((r >> 4) & 3) << 1) : F::CH == 4 ? (r >> 4) & 3 : (r >> 4) & 1;
+}
+template <class F>
+__device__ __forceinline__ int mx_vswz(int r) {
+    // a transposing read: rows that differ in their low bits
+    return F::CH == 8 ? (((r >> 1) & 3) | ((r >> 4) & 1) << 2) : F::CH == 4 ? (r >> 2) & 3 : (r >> 3) & 1;
+}
+
+// A wave's loads of a stage's codes, CH of 64 chunks, and E.
+template <class F>
+struct MxStage {
+    static constexpr int LOADS = F::CH + 1;
+    template <class Swz>
+    __device__ static __forceinline__ void load(char *tile, uint32_t *es, const char *X, const MxRows<F> &rows, const int *blk,
+                                                int k0, int lane, Swz swz) {
+        const uint32_t base = lds_addr(tile);
+#pragma unroll
+        for (int k = 0; k < F::CH; ++k) {
+            const int P = k * 64 + lane, row = P / F::CH, c = (P % F::CH) ^ swz(row);
+            lds_dma16(base + k * 1024, X + rows.codes(blk[row], k0 + row) + 16 * c);
+        }
+        const char *e = X + rows.scales(blk[lane], k0 + lane);
+        if constexpr (F::SB == 4) {
+            lds_dma4(lds_addr(es), e);
+        } else {
+            lds_dma2(lds_addr(es), e);
+        }
+    }
+};
+
+// One 64-key stage: key 16 a + 4 t + b of it is row 4 a + b of score tile t, so a lane
+// (g, l16) holds the scores of keys 16 g .. 16 g + 15 of row l16, in order: the 16
+// keys whose codes a transposing read of V brings it.
+template <class F, class T, bool MASK, class AfterK, class BeforeV>
+__device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, float &lsum,
+                                             const typename MxOperand<T>::B (&qf)[F::D / 32], const char *sk,
+                                             const uint32_t *ke, const char *sv, const uint32_t *ve, int lim, int g, int l16,
+                                             float xmul, AfterK after_k, BeforeV before_v) {
+    using Op = MxOperand<T>;
+    constexpr int NC = F::D / 32, XT = F::D / 16;
+    f32x4 s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int row = 16 * (l16 >> 2) + 4 * t + (l16 & 3);
+        uint32_t w[F::QB / 4];
+        if constexpr (F::QB >= 16) {
+#pragma unroll
+            for (int i = 0; i < F::QB / 16; ++i) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(sk + row * F::CB + (((F::QB / 16 * g + i) ^ mx_kswz<F>(row)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * i + e] = x[e];
+            }
+        } else {  // (half a chunk)
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(sk + row * F::CB + (((g >> 1) ^ mx_kswz<F>(row)) << 4) + 8 * (g & 1));
+            w[0] = x[0];
+            w[1] = x[1];
+        }
+        const float power = mx_power((ke[row] >> (8 * (g * F::SB / 4))) & 255u);
+        f32x4 c = zero4();
+#pragma unroll
+        for (int i = 0; i < NC; ++i) c = Op::mma(mx_values<F::BITS>(w + i * (F::BITS / 4), power), qf[i], c);
+        s[t] = c;
+    }
+    after_k();
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float v = s[t][r] * xmul;
+            if constexpr (MASK) v = 4 * t + r > lim ? -INFINITY : v;
+            s[t][r] = v;
+            mx = fmaxf(mx, v);
+        }
+    }
+    mx = xg_max(mx);
+    const float mnew = fmaxf(m, mx), mref = mnew == -INFINITY ? 0.f : mnew;
+    const float corr = fast_exp2(m - mref);
+    m = mnew;
+    lsum *= corr;
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) acc[xt] *= corr;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float pv = fast_exp2(s[t][r] - mref);
+            lsum += pv;
+            s[t][r] = pv * Op::kUp;
+        }
+    }
+    before_v();
+    u32x4 es[4];  // E of the lane's keys
+#pragma unroll
+    for (int t = 0; t < 4; ++t) es[t] = *reinterpret_cast<const u32x4 *>(ve + 16 * g + 4 * t);
+#pragma unroll
+    for (int grp = 0; grp < F::SB; ++grp) {
+        typename Op::B pf[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4 a[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[t][r] = s[2 * h + t][r] * mx_power((es[2 * h + t][r] >> (8 * grp)) & 255u);
+            }
+            pf[h] = Op::pack(a[0], a[1]);
+        }
+#pragma unroll
+        for (int xt = 2 * grp; xt < 2 * grp + 2; ++xt) {
+            uint32_t w[F::BITS / 2];  // 16 keys of column 16 xt + l16
+            if constexpr (F::BITS == 4) {
+                const int row = 16 * g + l16;
+                const i32x2 x = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                    (lds_i32x2 *)(sv + row * F::CB + (((xt >> 1) ^ mx_vswz<F>(row)) << 4) + 8 * (xt & 1)));
+                w[0] = x[0];
+                w[1] = x[1];
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = 16 * g + 8 * h + (l16 >> 1);
+                    const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (lds_i32x2 *)(sv + row * F::CB + ((xt ^ mx_vswz<F>(row)) << 4) + 8 * (l16 & 1)));
+                    w[2 * h] = x[0];
+                    w[2 * h + 1] = x[1];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[xt] = Op::mma(mx_values<F::BITS>(w + h * (F::BITS / 4), 1.0f), pf[h], acc[xt]);
+        }
+    }
+}
+
+// One piece of a sequence, as batch_few_piece: its loads and waits.
+template <class F, class T, int NW>
+__device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
+                                             MxFewSmem<F, NW> &sm) {
+    using Stage = MxStage<F>;
+    constexpr int D = F::D, XT = D / 16, ROWS = kBatchFew, NL = Stage::LOADS;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    const char *K = static_cast<const char *>(p.k), *V = static_cast<const char *>(p.v);
+    const int Nk = it.s.keys;
+    const MxRows<F> rows(p, it, Nk);
+    char *sk = sm.t.k[wave], *sv = sm.t.v[wave];
+    uint32_t *ke = sm.t.ke[wave], *ve = sm.t.ve[wave];
+
+    auto fetch = [&](int st, int n) __attribute__((always_inline)) {
+        lds_dma4(lds_addr(sm.t.blk[wave][n & 1]), rows.rows.table + rows.rows.block_at(st * 64 + lane));
+    };
+    auto load_k = [&](int st, int n) __attribute__((always_inline)) {
+        Stage::load(sk, ke, K, rows, sm.t.blk[wave][n & 1], st * 64, lane, mx_kswz<F>);
+    };
+    auto load_v = [&](int st, int n) __attribute__((always_inline)) {
+        Stage::load(sv, ve, V, rows, sm.t.blk[wave][n & 1], st * 64, lane, mx_vswz<F>);
+    };
+    int st = s_lo + wave, n = 0;
+    if (st < s_hi) fetch(st, 0);
+    const int row = min(l16, it.s.rows - 1);
+    const int qpos = it.s.pos + row / p.group;
+    typename MxOperand<T>::B qf[D / 32];
+    const bool low = mx_row<F, T>(qf, static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
+    if (st < s_hi) {
+        wait_loads<0>();
+        if (st + NW < s_hi) fetch(st + NW, 1);
+        load_k(st, 0);
+        load_v(st, 0);
+    }
+    f32x4 acc[XT];
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) acc[xt] = zero4();
+    float m = -INFINITY, lsum = 0.f;
+    // stages before `whole` hold no key that a row does not see
+    const int whole = min(Nk, it.s.pos + 1) / 64;
+    for (; st < s_hi; st += NW, ++n) {
+        const bool more = st + NW < s_hi, after = st + 2 * NW < s_hi;
+        wait_loads<NL>();
+        auto after_k = [&]() __attribute__((always_inline)) {
+            wait_lds();
+            if (more) {
+                fetch(after ? st + 2 * NW : st, n);  // (this stage's blocks: its V is out already)
+                load_k(st + NW, n + 1);
+            }
+        };
+        auto before_v = [&]() __attribute__((always_inline)) {
+            if (more) {
+                wait_loads<NL + 1>();
+            } else {
+                wait_loads<0>();
+            }
+        };
+        const int lim = min(qpos, Nk - 1) - st * 64 - 16 * g;
+        if (st < whole) {
+            mx_few_stage<F, T, false>(acc, m, lsum, qf, sk, ke, sv, ve, lim, g, l16, p.scale_log2, after_k, before_v);
+        } else {
+            mx_few_stage<F, T, true>(acc, m, lsum, qf, sk, ke, sv, ve, lim, g, l16, p.scale_log2, after_k, before_v);
+        }
+        wait_lds();
+        if (more) load_v(st + NW, n + 1);
+    }
+    const float lw = xg_sum(lsum);
+    float z = 0.f * lw;
+#pragma unroll
+    for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt]);
+    const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0 || low;
+    batch_few_finish<T, D, NW, 64 * NW>(
+        p, it, slot, sm.merge, m, lw, bad,
+        [&](int i) __attribute__((always_inline)) { return acc[i] * MxOperand<T>::kDown; },
+        [&](int i) __attribute__((always_inline)) { return 16 * i + 4 * g; },
+        [&](float *part, float *ml) __attribute__((always_inline)) {
+            batch_plain<T, D, ROWS, MxPlainRows<F>>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
+        });
+}
+template <class F, class T, int NW>
+__device__ __forceinline__ void mx_few_body(const BatchParams &p, int g, MxFewSmem<F, NW> &sm) {
+    batch_few_run(p, g, [&](const BatchItem &it, int lo, int hi, int slot) __attribute__((always_inline)) {
+        mx_few_piece<F, T, NW>(p, it, lo, hi, slot, sm);
+    });
+}
+
+// ----------------------------------------------------------------- the many rows
+
+// The products' policy: K and V as bf16 tiles, Q and p in bf16 or in three parts.
+template <int D_>
+struct PolMxF32 : PolRows<D_> {
+    using Base = PolRows<D_>;
+    using Op = MxOperand<float>;
+    using Frag = typename Base::Frag;
+    using T = u16;
+    using QFrag = Split3;
+    using ChainB = Split3;
+    __device__ static __forceinline__ f32x4 mma(Frag a, const QFrag &b, f32x4 c) { return Op::mma(a, b, c); }
+    __device__ static __forceinline__ ChainB pack(const f32x4 &a, const f32x4 &b) { return split3(a, b); }
+    __device__ static __forceinline__ f32x4 chain(f32x4 acc, const ChainB &b, const T *tile, int y0, int blk, int g, int l16) {
+        return Op::mma(Base::chain_a(tile, y0, blk, g, l16), b, acc);
+    }
+};
+template <class T, int D>
+using PolMx = std::conditional_t<sizeof(T) == 2, PolRows<D>, PolMxF32<D>>;
+
+template <int D, int NW>
+struct MxManySmem {
+    __attribute__((aligned(16))) u16 k[2][64 * D], v[2][64 * D];
+    int bad[NW];
+};
+
+// A thread's part of a stage of K or V, of NT threads': loaded as codes, written to
+// the tile as bf16.
+template <class F, int NT>
+struct MxPart {
+    static constexpr int TPR = NT / 64, E = F::D / TPR, B = E * F::BITS / 8;  // threads of a row, elements, bytes
+    uint32_t w[B / 4];
+    float power;
+    __device__ __forceinline__ void load(const char *X, size_t codes, size_t scales, int part) {
+        load_words(w, X + codes + part * B);
+        power = mx_power((unsigned char)X[scales + part * E / kMxGroup]);
+    }
+    __device__ __forceinline__ void write(u16 *tile, int row, int part) const {
+        char *base = reinterpret_cast<char *>(tile) + row * (2 * F::D);
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i)
+            *reinterpret_cast<bf16x8 *>(base + ((((part * E) / 8 + i) ^ PolRows<F::D>::swz(row)) << 4)) =
+                mx_values<F::BITS>(w + i * (F::BITS / 4), power);
+    }
+};
+
+// One unit's share, as batch_many_body, NW waves of 16 QT rows.
+template <class F, class T, int QT, int NW>
+__device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, MxManySmem<F::D, NW> &sm) {
+    using Pol = PolMx<T, F::D>;
+    using Part = MxPart<F, 64 * NW>;
+    constexpr int D = F::D, XT = D / 16, BK = 64, ROWS = 16 * QT * NW;
+    constexpr bool kPrio = true;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    BatchItem it;
+    if (!find_item<ROWS>(p, batch_order(p, block), it)) return;
+    const char *K = static_cast<const char *>(p.k), *V = static_cast<const char *>(p.v);
+
+    const int r0 = it.unit * ROWS, rw = r0 + wave * 16 * QT;  // the unit's and the wave's first row
+    const int last_row = it.s.rows - 1;
+    RowPos<QT> qpos;
+    typename Pol::QFrag qf[QT][Pol::NC];
+    bool low = false;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int row = min(rw + 16 * qt + l16, last_row);
+        qpos.at[qt] = it.s.pos + row / p.group;
+        const T *q = static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D);
+        if constexpr (sizeof(T) == 2) {
+            row_frags<Pol>(qf[qt], q, g);
+        } else {
+            low |= split_row(qf[qt], q, g, 1.0f, true);
+        }
+    }
+    const int pos_lo = it.s.pos + r0 / p.group;
+    const int pos_hi = it.s.pos + min(r0 + ROWS - 1, last_row) / p.group;
+    const int pos_w = it.s.pos + min(rw + 16 * QT - 1, last_row) / p.group;
+    f32x4 acc[XT][QT];
+    float m[QT], lsum[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) acc[xt][qt] = zero4();
+        m[qt] = -INFINITY;
+        lsum[qt] = 0.f;
+    }
+    const int Nk = min(it.s.keys, max(pos_hi + 1, 0)), n = (Nk + BK - 1) / BK;
+    const MxRows<F> rows(p, it, Nk);
+    int s_lo, s_hi;
+    share_stages(it, n, s_lo, s_hi);
+
+    // the stage after the next: its block; the next: its codes, in registers
+    const int key = tid / Part::TPR, part = tid % Part::TPR;
+    Part xk, xv;
+    int blk = 0;
+    auto fetch = [&](int st) __attribute__((always_inline)) { blk = rows.rows.table[rows.rows.block_at(st * BK + key)]; };
+    auto load = [&](int st) __attribute__((always_inline)) {
+        const size_t codes = rows.codes(blk, st * BK + key), scales = rows.scales(blk, st * BK + key);
+        xk.load(K, codes, scales, part);
+        xv.load(V, codes, scales, part);
+        if (st + 1 < s_hi) fetch(st + 1);
+    };
+    auto write = [&](int buf) __attribute__((always_inline)) {
+        xk.write(sm.k[buf], key, part);
+        xv.write(sm.v[buf], key, part);
+    };
+    if (s_lo < s_hi) {
+        fetch(s_lo);
+        load(s_lo);
+        write(0);
+    }
+    __syncthreads();
+    const int whole = min(s_hi, min(Nk, pos_lo + 1) / BK);
+    const bool some = rw <= last_row;  // the wave has rows
+    auto main_stage = [&](auto buf, auto first, int st) __attribute__((always_inline)) {
+        constexpr int B = decltype(buf)::value;
+        if (st + 1 < s_hi) load(st + 1);
+        if (some) {
+            if constexpr (decltype(first)::value) {
+                fwd_stage<Pol, QT, true, false, kPrio>(acc, m, lsum, qf, sm.k[B], sm.v[B], st * BK, qpos, Nk, g, l16,
+                                                       p.scale_log2);
+            } else {
+                fwd_stage_lazy<Pol, QT, true, false, kPrio>(acc, m, lsum, qf, sm.k[B], sm.v[B], st * BK, qpos, Nk, g, l16,
+                                                            p.scale_log2);
+            }
+        }
+        if (st + 1 < s_hi) write(B ^ 1);
+        __syncthreads();
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    int st = s_lo;
+    if (st < whole) main_stage(B0{}, std::true_type{}, st++);
+    for (; st + 1 < whole; st += 2) {
+        main_stage(B1{}, std::false_type{}, st);
+        main_stage(B0{}, std::false_type{}, st + 1);
+    }
+    if (st < whole) main_stage(B1{}, std::false_type{}, st++);
+    for (; st < s_hi; ++st) {
+        const int cur = (st - s_lo) & 1;
+        if (st + 1 < s_hi) load(st + 1);
+        if (some && st * BK <= pos_w)  // else no row of the wave sees the stage
+            fwd_stage<Pol, QT, true, true, kPrio, true>(acc, m, lsum, qf, sm.k[cur], sm.v[cur], st * BK, qpos, Nk, g, l16,
+                                                        p.scale_log2);
+        if (st + 1 < s_hi) write(cur ^ 1);
+        __syncthreads();
+    }
+    float ltot[QT], z = 0.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        ltot[qt] = xg_sum(lsum[qt]);
+        z += 0.f * ltot[qt];
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt][qt]);
+    }
+    float *ws = nullptr, *ml = nullptr;
+    if (it.shares > 1) {
+        ws = batch_part(p.part[1], it.slot, ROWS, D);
+        ml = batch_ml(p.part[1], p.slots, it.slot, ROWS, D);
+    }
+    const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0 || low;
+    if (lane == 0) sm.bad[wave] = bad;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any |= sm.bad[w];
+    if (any) {
+        for (int i = 0; i < ROWS; i += 16 * NW)
+            batch_plain<T, D, ROWS, MxPlainRows<F>>(p, it, i, s_lo * BK, s_hi * BK, ws, ml);
+        return;
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int r = rw + 16 * qt + l16, rl = r - r0;
+        const bool have = r < it.s.rows;
+        if (it.shares > 1) {
+            if (have) {
+#pragma unroll
+                for (int i = 0; i < XT; ++i) store4<float>(ws + rl * D + 16 * i + 4 * g, acc[i][qt], 1.0f);
+                if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * rl) = make_float2(m[qt], ltot[qt]);
+            }
+            continue;
+        }
+        const float inv = batch_inverse(ltot[qt], qpos.at[qt]);
+        T *O = static_cast<T *>(p.o) + batch_elem(p, it, min(r, last_row), p.o_rs, D);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int xt = 0; xt < XT; xt += 2)
+                store8_pair_bf16(O, 16 * xt, g, acc[xt][qt], acc[xt + 1][qt], inv, have);
+        } else if (have) {
+#pragma unroll
+            for (int xt = 0; xt < XT; ++xt) store4<float>(O + 16 * xt + 4 * g, acc[xt][qt], inv);
+        }
+        if (p.lse != nullptr && have && g == 0)
+            p.lse[batch_lse(p, it, r)] = ltot[qt] > 0.f ? (m[qt] + fast_log2(ltot[qt])) * kLn2 : -INFINITY;
+    }
+}
+
+// Both forms in one launch, as batch_both_body.
+template <class F, class T, int QT, int NW>
+__device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_groups) {
+    __shared__ __attribute__((aligned(16))) union {
+        MxFewSmem<F, NW> few;
+        MxManySmem<F::D, NW> many;
+    } sm;
+    if ((int)blockIdx.x < few_groups) {
+        mx_few_body<F, T, NW>(p, blockIdx.x, sm.few);
+    } else {
+        mx_many_body<F, T, QT, NW>(p, (int)blockIdx.x - few_groups, sm.many);
+    }
+}
+
+#define MXFA_BATCH_MX_FEW(NAME, BITS, D, T, NW)                                                              \
+    extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##NAME##_few(BatchParams p) {           \
+        __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, NW> sm;                               \
+        mx_few_body<Mx<BITS, D>, T, NW>(p, blockIdx.x, sm);                                                  \
+    }
+#define MXFA_BATCH_MX_MANY(MANY, BOTH, BITS, D, T, QT, NW, WPS, BOTH_WPS)                                    \
+    extern "C" __global__ __launch_bounds__(64 * NW, WPS) void mxfa_batch_##MANY(BatchParams p) {            \
+        __shared__ __attribute__((aligned(16))) MxManySmem<D, NW> sm;                                        \
+        mx_many_body<Mx<BITS, D>, T, QT, NW>(p, blockIdx.x, sm);                                             \
+    }                                                                                                        \
+    extern "C" __global__ __launch_bounds__(64 * NW, BOTH_WPS) void mxfa_batch_##BOTH(BatchParams p, int few_groups) { \
+        mx_both_body<Mx<BITS, D>, T, QT, NW>(p, few_groups);                                                 \
+    }
+#define MXFA_BATCH_MX(BITS)                                                                                  \
+    MXFA_BATCH_MX_FEW(x##BITS##b64, BITS, 64, u16, 8)                                                        \
+    MXFA_BATCH_MX_MANY(x##BITS##b64_many, x##BITS##b64_both, BITS, 64, u16, 2, 4, 3, 3)                      \
+    MXFA_BATCH_MX_MANY(x##BITS##b64_many64, x##BITS##b64_both64, BITS, 64, u16, 1, 4, 4, 3)                  \
+    MXFA_BATCH_MX_FEW(x##BITS##b128, BITS, 128, u16, 8)                                                      \
+    MXFA_BATCH_MX_MANY(x##BITS##b128_many, x##BITS##b128_both, BITS, 128, u16, 2, 4, 2, 2)                   \
+    MXFA_BATCH_MX_MANY(x##BITS##b128_many64, x##BITS##b128_both64, BITS, 128, u16, 1, 4, 2, 2)               \
+    MXFA_BATCH_MX_FEW(x##BITS##f64, BITS, 64, float, 8)                                                      \
+    MXFA_BATCH_MX_MANY(x##BITS##f64_many, x##BITS##f64_both, BITS, 64, float, 1, kBatchF32Waves, 4, 4)
+MXFA_BATCH_MX(8)
+MXFA_BATCH_MX(4)
+#undef MXFA_BATCH_MX
+#undef MXFA_BATCH_MX_MANY
+#undef MXFA_BATCH_MX_FEW
+
+#endif
+
+}  // namespace mxfa

@@ -38,6 +38,7 @@ struct BatchParams {
     const int *table, *cu_q, *lens;
     int n_tok, n_seq, max_q, Hq, Hkv, group, d;
     int q_rs, kv_rs, o_rs, bs_shift, n_blocks, max_blocks, table_stride;
+    int bits;  // 0: cache rows in the type of q; 8 or 4: microscaled blocks (fa_mx.h), kv_rs bytes apart
     float scale_log2;
     // append: the rotation of Q and K (dim = 0: none)
     const double *freq;
@@ -66,12 +67,16 @@ struct PagesParams {
 int rotary_row_units(int d, int dim, int dtype_bf16);
 hipError_t launch_rotary(RotaryParams p, int dtype_bf16, hipStream_t stream);
 hipError_t launch_append(BatchParams p, int dtype_bf16, hipStream_t stream);
+// The same into a microscaled cache, its rotation's factor in 64 bits, and the read
+// of rows back (p.k, p.v: the caches; p.q unused; p.o and v_out: rows of o_rs).
+hipError_t launch_append_mx(BatchParams p, double factor, int dtype_bf16, hipStream_t stream);
+hipError_t launch_read_mx(BatchParams p, void *v_out, int dtype_bf16, hipStream_t stream);
 
 // Attention of the batch's new tokens over the cache; p.part from a workspace of
 // batch_workspace_bytes (set by the launcher).
 size_t batch_workspace_bytes(const BatchParams &p, int dtype_bf16);
 long long batch_groups(const BatchParams &p, int dtype_bf16);  // of the largest launch
-hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream);
+hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream);  // (p.bits: either cache)
 
 hipError_t launch_pages_free(const PagesParams &p, const int *rows, int n, hipStream_t stream);
 hipError_t launch_pages_fork(const PagesParams &p, const int *parents, const int *children, int n, int *pairs,

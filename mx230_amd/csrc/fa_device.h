@@ -262,6 +262,7 @@ struct PolBF16 {
     static constexpr int D = D_;
     using T = u16;
     using Frag = bf16x8;
+    using QFrag = Frag;                // the scores' other operand
     static constexpr int EPC = 8;      // elements per 16-byte chunk
     static constexpr int NC = D / 32;  // MFMAs over D per first-GEMM tile
     static constexpr int ROWS = 64;    // rows of every LDS tile
@@ -583,6 +584,17 @@ __device__ __forceinline__ void lds_dma16(uint32_t base, const void *src) {
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
         "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+        : "=&s"(save)
+        : "v"(src), "s"(__builtin_amdgcn_readfirstlane(base)));
+#endif
+}
+// (two bytes, zero-extended to the lane's 4)
+__device__ __forceinline__ void lds_dma2(uint32_t base, const void *src) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    uint32_t save;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+        "global_load_lds_ushort %1, off\n\ts_mov_b32 m0, %0"
         : "=&s"(save)
         : "v"(src), "s"(__builtin_amdgcn_readfirstlane(base)));
 #endif

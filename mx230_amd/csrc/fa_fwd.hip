@@ -54,7 +54,7 @@ struct FwdNothing {
 template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, bool EMPTY_ROWS = false,
           class AfterK = FwdNothing, class BeforeV = FwdNothing, class Pos = int>
 __device__ __forceinline__ void fwd_stage(f32x4 (&acc)[Pol::D / 16][QT], float (&m)[QT], float (&lsum)[QT],
-                                          const typename Pol::Frag (&qf)[QT][Pol::NC],
+                                          const typename Pol::QFrag (&qf)[QT][Pol::NC],
                                           const typename Pol::T *sk, const typename Pol::T *sv, int k0,
                                           const Pos &qpos0, int Nk, int g, int l16, float xmul, AfterK after_k = {},
                                           BeforeV before_v = {}) {
@@ -161,7 +161,7 @@ constexpr float kLazySum = 65536.0f;
 // fp32 result is multiplied by xmul = scale log2(e).
 template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, class Pos = int>
 __device__ __forceinline__ void fwd_scores(f32x4 (&s)[2][2][QT], const float (&m)[QT],
-                                           const typename Pol::Frag (&qf)[QT][Pol::NC], const typename Pol::T *sk,
+                                           const typename Pol::QFrag (&qf)[QT][Pol::NC], const typename Pol::T *sk,
                                            int k0, const Pos &qpos0, int Nk, int g, int l16, float xmul) {
     using Frag = typename Pol::Frag;
     constexpr int NC = Pol::NC;
@@ -231,7 +231,7 @@ __device__ __forceinline__ void fwd_exp_sum(f32x4 (&s)[2][2][QT], float (&l)[QT]
 
 template <class Pol, int QT, bool CAUSAL, bool MASK, bool PRIO = false, class Pos = int>
 __device__ __forceinline__ void fwd_stage_lazy(f32x4 (&acc)[Pol::D / 16][QT], float (&m)[QT], float (&lsum)[QT],
-                                               const typename Pol::Frag (&qf)[QT][Pol::NC],
+                                               const typename Pol::QFrag (&qf)[QT][Pol::NC],
                                                const typename Pol::T *sk, const typename Pol::T *sv, int k0,
                                                const Pos &qpos0, int Nk, int g, int l16, float xmul) {
     constexpr int XT = Pol::D / 16;

@@ -341,3 +341,6 @@ hipError_t launch_append(BatchParams p, int dtype_bf16, hipStream_t stream) {
 }
 
 }  // namespace mxfa
+
+// the append into a cache of fewer bits, and its read
+#include "fa_mx.hip"

@@ -5,6 +5,7 @@
 #include "fa_bwd.hip"
 #include "fa_naive.hip"
 #include "fa_batch.hip"
+#include "fa_batch_mx.hip"
 #include "fa_rotary.hip"
 #include "fa_pages.hip"
 #include "probe.hip"

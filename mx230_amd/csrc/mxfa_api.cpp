@@ -14,6 +14,7 @@
 
 #include "fa_cache.h"
 #include "fa_launch.h"
+#include "fa_mx.h"
 
 namespace {
 
@@ -700,22 +701,34 @@ int mxfa_run_rotary(const mxfa_rotary_shape *s, const void *q, const void *k, vo
 
 namespace {
 
-// What the append and the attention of a batch have in common; qw: the columns
-// of a q / qkv row.
-int check_batch(const mxfa_batch_shape *s, long long qw) {
+// What the calls on a batch have in common; qw, ow and kw: the least q_stride,
+// out_stride and kv_stride.
+int check_rows(const mxfa_batch_shape *s, long long qw, long long ow, long long kw) {
     if (s->dtype != MXFA_F32 && s->dtype != MXFA_BF16) return MXFA_ERR_DTYPE;
     if (s->n_tok < 1 || s->n_seq < 1 || s->n_head < 1 || s->n_kv_head < 1 || s->head_dim < 1 || s->n_blocks < 1 ||
         s->max_blocks < 1 || s->table_stride < s->max_blocks)
         return MXFA_ERR_SHAPE;
     if (s->n_head % s->n_kv_head != 0) return MXFA_ERR_SHAPE;
     if (!power_of_two(s->block_size) || s->block_size > (1 << 24)) return MXFA_ERR_UNSUPPORTED;
-    const long long ow = (long long)s->n_head * s->head_dim, kw = (long long)s->n_kv_head * s->head_dim;
     if (s->q_stride < qw || s->out_stride < ow || s->kv_stride < kw) return MXFA_ERR_SHAPE;
     const int esz = s->dtype == MXFA_BF16 ? 2 : 4;
-    if (((long long)s->q_stride * esz) % 16 || ((long long)s->kv_stride * esz) % 16 ||
-        ((long long)s->out_stride * esz) % 16)
-        return MXFA_ERR_ALIGN;
+    if ((qw > 0 && ((long long)s->q_stride * esz) % 16) || ((long long)s->out_stride * esz) % 16) return MXFA_ERR_ALIGN;
     return MXFA_OK;
+}
+// The append and the attention over rows of the type.
+int check_batch(const mxfa_batch_shape *s, long long qw) {
+    const int rc = check_rows(s, qw, (long long)s->n_head * s->head_dim, (long long)s->n_kv_head * s->head_dim);
+    if (rc != MXFA_OK) return rc;
+    return (long long)s->kv_stride * (s->dtype == MXFA_BF16 ? 2 : 4) % 16 ? MXFA_ERR_ALIGN : MXFA_OK;
+}
+// Over a microscaled cache.
+int check_mx(const mxfa_batch_shape *s, int bits, long long qw, long long ow) {
+    const int rc = check_rows(s, qw, ow, 0);
+    if (rc != MXFA_OK) return rc;
+    if ((bits != 8 && bits != 4) || s->head_dim % mxfa::kMxGroup != 0 || s->head_dim > 256) return MXFA_ERR_UNSUPPORTED;
+    const size_t block = mxfa_mx_block_bytes(s->block_size, s->n_kv_head, s->head_dim, bits);
+    if (block == 0 || (size_t)s->kv_stride < block) return MXFA_ERR_SHAPE;
+    return s->kv_stride % 16 ? MXFA_ERR_ALIGN : MXFA_OK;
 }
 
 // Whether `an` rows of `aw` bytes, `as` apart, share memory with `bn` rows of `bw`.
@@ -769,10 +782,10 @@ mxfa::BatchParams batch_params(const mxfa_batch_shape *s, const void *q, void *k
 
 }  // namespace
 
-int mxfa_check_batch(const mxfa_batch_shape *s) {
-    if (s == nullptr) return MXFA_ERR_NULL;
-    const int rc = check_batch(s, (long long)s->n_head * s->head_dim);
-    if (rc != MXFA_OK) return rc;
+namespace {
+
+// The attention's own checks; p.bits: of which cache.
+int check_attention(const mxfa_batch_shape *s, int bits) {
     if (s->max_q < 1) return MXFA_ERR_SHAPE;
     if (!(s->scale >= 0.0f) || std::isinf(s->scale)) return MXFA_ERR_SHAPE;
     if (s->head_dim != 64 && s->head_dim != 128) return MXFA_ERR_UNSUPPORTED;
@@ -785,23 +798,24 @@ int mxfa_check_batch(const mxfa_batch_shape *s) {
     // the stages of all sequences, and the caches' rows, in 32 bits
     if (((double)s->max_blocks * s->block_size / 64 + 2) * s->n_seq > 2147483648.0) return MXFA_ERR_SHAPE;
     if ((long long)s->n_blocks * s->block_size > 0x80000000LL) return MXFA_ERR_SHAPE;
-    const mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    p.bits = bits;
     if (mxfa::batch_groups(p, s->dtype == MXFA_BF16) > 0x7fffffffLL / 512) return MXFA_ERR_SHAPE;
     return MXFA_OK;
 }
 
-size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *s) {
-    if (mxfa_check_batch(s) != MXFA_OK) return 0;
-    return mxfa::batch_workspace_bytes(batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr),
-                                       s->dtype == MXFA_BF16);
+size_t attention_workspace(const mxfa_batch_shape *s, int bits) {
+    mxfa::BatchParams p = batch_params(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    p.bits = bits;
+    return mxfa::batch_workspace_bytes(p, s->dtype == MXFA_BF16);
 }
 
-int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void *kcache, const void *vcache, void *out,
-                           float *lse, const int *block_table, const int *cu_q, const int *lens, void *workspace,
-                           size_t workspace_bytes, void *stream) {
-    int rc = mxfa_check_batch(s);
-    if (rc != MXFA_OK) return rc;
-    rc = check_ptrs({q, kcache, vcache, out, workspace});
+// The attention of a checked shape over a cache of `pool` rows (blocks, where bits is
+// not 0) of kw bytes, ks apart.
+int run_attention(const mxfa_batch_shape *s, int bits, long long pool, long long kw, long long ks, const void *q,
+                  const void *kcache, const void *vcache, void *out, float *lse, const int *block_table, const int *cu_q,
+                  const int *lens, void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = check_ptrs({q, kcache, vcache, out, workspace});
     if (rc != MXFA_OK) return rc;
     rc = check_ints({block_table, cu_q, lens});
     if (rc != MXFA_OK) return rc;
@@ -809,6 +823,7 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void 
     mxfa::BatchParams p = batch_params(s, q, const_cast<void *>(kcache), const_cast<void *>(vcache), out, block_table,
                                        cu_q, lens);
     p.lse = lse;
+    p.bits = bits;
     p.scale_log2 = (s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * mxfa::kLog2e;
     const size_t need = mxfa::batch_workspace_bytes(p, s->dtype == MXFA_BF16);
     if (workspace_bytes < need) return MXFA_ERR_WORKSPACE;
@@ -818,10 +833,8 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void 
         long long stride, width, rows;
     };
     const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, qw = esz * s->n_head * s->head_dim;
-    const long long kw = esz * s->n_kv_head * s->head_dim, pool = (long long)s->n_blocks * s->block_size;
     const long long lw = lse == nullptr ? 0 : 4LL * s->n_tok * s->n_head;
-    const Rows all[] = {{q, s->q_stride * esz, qw, s->n_tok}, {kcache, s->kv_stride * esz, kw, pool},
-                        {vcache, s->kv_stride * esz, kw, pool}, {out, s->out_stride * esz, qw, s->n_tok},
+    const Rows all[] = {{q, s->q_stride * esz, qw, s->n_tok}, {kcache, ks, kw, pool}, {vcache, ks, kw, pool}, {out, s->out_stride * esz, qw, s->n_tok},
                         {lse, lw, lw, 1}, {workspace, (long long)need, (long long)need, 1}};
     if (rows_collide(out, s->out_stride * esz, qw, q, s->q_stride * esz, qw, s->n_tok)) return MXFA_ERR_UNSUPPORTED;
     for (int w = 3; w < 6; ++w) {
@@ -833,6 +846,59 @@ int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void 
         }
     }
     return from_hip(mxfa::launch_batch(p, s->dtype == MXFA_BF16, workspace, static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace
+
+int mxfa_check_batch(const mxfa_batch_shape *s) {
+    if (s == nullptr) return MXFA_ERR_NULL;
+    const int rc = check_batch(s, (long long)s->n_head * s->head_dim);
+    return rc != MXFA_OK ? rc : check_attention(s, 0);
+}
+
+size_t mxfa_prefill_batch_workspace_bytes(const mxfa_batch_shape *s) {
+    return mxfa_check_batch(s) == MXFA_OK ? attention_workspace(s, 0) : 0;
+}
+
+int mxfa_run_prefill_batch(const mxfa_batch_shape *s, const void *q, const void *kcache, const void *vcache, void *out,
+                           float *lse, const int *block_table, const int *cu_q, const int *lens, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+    const int rc = mxfa_check_batch(s);
+    if (rc != MXFA_OK) return rc;
+    const long long esz = s->dtype == MXFA_BF16 ? 2 : 4;
+    return run_attention(s, 0, (long long)s->n_blocks * s->block_size, esz * s->n_kv_head * s->head_dim, s->kv_stride * esz,
+                         q, kcache, vcache, out, lse, block_table, cu_q, lens, workspace, workspace_bytes, stream);
+}
+
+size_t mxfa_mx_block_bytes(int block_size, int n_kv_head, int head_dim, int bits) {
+    if ((bits != 8 && bits != 4) || head_dim < 1 || head_dim > 256 || head_dim % mxfa::kMxGroup != 0 || n_kv_head < 1 ||
+        !power_of_two(block_size) || block_size > (1 << 24))
+        return 0;
+    const double rows = (double)block_size * n_kv_head;
+    const int row = mxfa::mx_code_bytes(head_dim, bits) + mxfa::mx_scale_bytes(head_dim);
+    if (rows * row > (double)(INT_MAX - 15)) return 0;
+    return ((size_t)block_size * n_kv_head * row + 15) / 16 * 16;
+}
+
+int mxfa_check_batch_mx(const mxfa_batch_shape *s, int bits) {
+    if (s == nullptr) return MXFA_ERR_NULL;
+    const long long w = (long long)s->n_head * s->head_dim;
+    const int rc = check_mx(s, bits, w, w);
+    return rc != MXFA_OK ? rc : check_attention(s, bits);
+}
+
+size_t mxfa_prefill_batch_mx_workspace_bytes(const mxfa_batch_shape *s, int bits) {
+    return mxfa_check_batch_mx(s, bits) == MXFA_OK ? attention_workspace(s, bits) : 0;
+}
+
+int mxfa_run_prefill_batch_mx(const mxfa_batch_shape *s, int bits, const void *q, const void *kcache, const void *vcache,
+                              void *out, float *lse, const int *block_table, const int *cu_q, const int *lens,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = mxfa_check_batch_mx(s, bits);
+    if (rc != MXFA_OK) return rc;
+    return run_attention(s, bits, s->n_blocks, (long long)mxfa_mx_block_bytes(s->block_size, s->n_kv_head, s->head_dim, bits),
+                         s->kv_stride, q, kcache, vcache, out, lse, block_table, cu_q, lens, workspace, workspace_bytes,
+                         stream);
 }
 
 int mxfa_run_cache_append(const mxfa_batch_shape *s, const mxfa_append_rotary *r, const void *qkv, void *q_out,
@@ -866,6 +932,64 @@ int mxfa_run_cache_append(const mxfa_batch_shape *s, const mxfa_append_rotary *r
     p.interleaved = r->interleaved;
     p.factor = r->factor;
     return from_hip(mxfa::launch_append(p, s->dtype == MXFA_BF16, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_cache_append_mx(const mxfa_batch_shape *s, int bits, const mxfa_append_rotary_mx *r, const void *qkv,
+                             void *q_out, void *kcache, void *vcache, const int *block_table, const int *cu_q,
+                             const int *lens, void *stream) {
+    if (s == nullptr || r == nullptr) return MXFA_ERR_NULL;
+    const long long heads = (long long)s->n_head + 2LL * s->n_kv_head;
+    int rc = check_mx(s, bits, heads * s->head_dim, (long long)s->n_head * s->head_dim);
+    if (rc != MXFA_OK) return rc;
+    if (r->rotary_dim != 0) {
+        rc = check_rotated(s->head_dim, r->rotary_dim, r->interleaved, (float)r->factor);
+        if (rc != MXFA_OK) return rc;
+        if (r->frequencies == nullptr) return MXFA_ERR_NULL;
+        if (reinterpret_cast<uintptr_t>(r->frequencies) % 8 != 0) return MXFA_ERR_ALIGN;
+    }
+    if (heads > kMaxGridY) return MXFA_ERR_SHAPE;
+    if ((double)s->n_tok * (s->head_dim / 8) > 0x7fffffff / 2 - 512.0) return MXFA_ERR_SHAPE;  // a launch's threads
+    rc = check_ptrs({qkv, q_out, kcache, vcache});
+    if (rc != MXFA_OK) return rc;
+    rc = check_ints({block_table, cu_q, lens});
+    if (rc != MXFA_OK) return rc;
+    const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, row = esz * s->head_dim;
+    if (rows_collide(q_out, s->out_stride * esz, s->n_head * row, qkv, s->q_stride * esz, heads * row, s->n_tok))
+        return MXFA_ERR_UNSUPPORTED;
+    mxfa::BatchParams p = batch_params(s, qkv, kcache, vcache, q_out, block_table, cu_q, lens);
+    p.bits = bits;
+    p.freq = r->frequencies;
+    p.dim = r->rotary_dim;
+    p.interleaved = r->interleaved;
+    return from_hip(mxfa::launch_append_mx(p, r->factor, s->dtype == MXFA_BF16, static_cast<hipStream_t>(stream)));
+}
+
+int mxfa_run_cache_read_mx(const mxfa_batch_shape *shape, int bits, const void *kcache, const void *vcache, void *k_out,
+                           void *v_out, const int *block_table, const int *cu_q, const int *lens, void *stream) {
+    if (shape == nullptr) return MXFA_ERR_NULL;
+    mxfa_batch_shape s = *shape;
+    s.n_head = s.n_kv_head;
+    s.q_stride = 0;
+    const long long w = (long long)s.n_kv_head * s.head_dim;
+    int rc = check_mx(&s, bits, 0, w);
+    if (rc != MXFA_OK) return rc;
+    if (2LL * s.n_kv_head > kMaxGridY || (double)s.n_tok * (s.head_dim / 8) > 0x7fffffff / 2 - 512.0) return MXFA_ERR_SHAPE;
+    rc = check_ptrs({kcache, vcache, k_out, v_out});
+    if (rc != MXFA_OK) return rc;
+    rc = check_ints({block_table, cu_q, lens});
+    if (rc != MXFA_OK) return rc;
+    const long long esz = s.dtype == MXFA_BF16 ? 2 : 4, os = s.out_stride * esz, ow = w * esz;
+    const long long bytes = (long long)mxfa_mx_block_bytes(s.block_size, s.n_kv_head, s.head_dim, bits);
+    if (rows_meet(k_out, os, ow, s.n_tok, v_out, os, ow, s.n_tok)) return MXFA_ERR_UNSUPPORTED;
+    for (const void *o : {k_out, v_out}) {
+        for (const void *c : {kcache, vcache}) {
+            if (rows_meet(o, os, ow, s.n_tok, c, s.kv_stride, bytes, s.n_blocks)) return MXFA_ERR_UNSUPPORTED;
+        }
+    }
+    mxfa::BatchParams p = batch_params(&s, nullptr, const_cast<void *>(kcache), const_cast<void *>(vcache), k_out,
+                                       block_table, cu_q, lens);
+    p.bits = bits;
+    return from_hip(mxfa::launch_read_mx(p, v_out, s.dtype == MXFA_BF16, static_cast<hipStream_t>(stream)));
 }
 
 int mxfa_check_pages(const mxfa_pages_shape *s) {
