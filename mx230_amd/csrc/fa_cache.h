@@ -44,7 +44,7 @@ struct BatchParams {
     const double *freq;
     int dim, interleaved;
     float factor;
-    int hpt;  // heads per thread
+    int hpt, hpt_kv;  // heads per thread; of K or V, where they have threads of their own
     // attention (fa_batch_items.h): the most rows (new tokens x query heads of a
     // KV head) of a sequence that the few-row form takes (0: it takes none) and
     // its work-groups per KV head; the rows of the many-row form's
