@@ -369,20 +369,20 @@ struct PlainRows {
         : K(static_cast<const T *>(p.k) + it.head * D + c), V(static_cast<const T *>(p.v) + it.head * D + c),
           table(p.table + (long long)it.seq * p.table_stride), shift(p.bs_shift), stride(p.kv_rs),
           last((unsigned)(p.n_blocks - 1)) {}
-    __device__ __forceinline__ void read(int k, float (&kf)[E], float (&vf)[E]) const {
+    size_t row;
+    __device__ __forceinline__ void at(int k) {
         const size_t b = min((unsigned)table[k >> shift], last);
-        const size_t at = ((b << shift) + (k & ((1 << shift) - 1))) * (size_t)stride;
+        row = ((b << shift) + (k & ((1 << shift) - 1))) * (size_t)stride;
+    }
+    __device__ __forceinline__ void read(const T *X, float (&f)[E]) const {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if constexpr (sizeof(T) == 2) {
-                kf[e] = __uint_as_float((uint32_t)K[at + e] << 16);
-                vf[e] = __uint_as_float((uint32_t)V[at + e] << 16);
-            } else {
-                kf[e] = K[at + e];
-                vf[e] = V[at + e];
-            }
+            if constexpr (sizeof(T) == 2) f[e] = __uint_as_float((uint32_t)X[row + e] << 16);
+            else f[e] = X[row + e];
         }
     }
+    __device__ __forceinline__ void read_k(float (&f)[E]) const { read(K, f); }
+    __device__ __forceinline__ void read_v(float (&f)[E]) const { read(V, f); }
 };
 
 // A unit's share in plain fp32 arithmetic, keys a row does not see left out
@@ -410,20 +410,22 @@ __device__ __forceinline__ void batch_plain(const BatchParams &p, const BatchIte
         acc[e] = 0.f;
     }
     const int kend = min(min(key1, it.s.keys), it.s.pos + row / p.group + 1);
-    const Rows rows(p, it, c);
+    Rows rows(p, it, c);
     for (int k = key0; k < kend; ++k) {
-        float kf[E], vf[E];
-        rows.read(k, kf, vf);
+        float x[E];
+        rows.at(k);
+        rows.read_k(x);
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = __builtin_fmaf(q[e], kf[e], s);
+        for (int e = 0; e < E; ++e) s = __builtin_fmaf(q[e], x[e], s);
         s = quad_sum(s);
         const float mn = fmaxf(m, s), mref = mn == -INFINITY ? 0.f : mn;
         const float corr = fast_exp2(m - mref), pv = fast_exp2(s - mref);
         m = mn;
         l = l * corr + pv;
+        rows.read_v(x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(pv, vf[e], acc[e] * corr);
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(pv, x[e], acc[e] * corr);
     }
     if (!have) return;
 #pragma unroll
@@ -1221,7 +1223,7 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     int few_groups = (int)f[0].groups;
     void *args[] = {&p, &few_groups};
     if (f[1].groups == 0) {
-        e = launch_kernel(id[0], dim3(few_groups), dim3(p.bits != 0 || (dtype_bf16 && p.d == 64) ? 512 : 256), args, stream);
+        e = launch_kernel(id[0], dim3(few_groups), dim3(p.bits != 0 ? 64 * kMxFewWaves : dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
     } else if (few_groups == 0) {
         e = launch_kernel(many[0], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
     } else {

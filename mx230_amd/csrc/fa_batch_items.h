@@ -19,6 +19,8 @@ constexpr int kCusPerXcd = 32;  // of 8 XCDs
 // in a hundred pieces.
 __host__ __device__ constexpr int join_rows(int d) { return 1024 / d; }
 constexpr int kFewJoins = 4;
+// Waves of the few-row form's work-groups over a microscaled cache.
+constexpr int kMxFewWaves = 8;
 // Waves of the many-row form's work-groups in fp32, of 16 rows each (bf16: 4, of 16
 // or 32: batch_many_rows).
 constexpr int kBatchF32Waves = 8;
@@ -360,7 +362,7 @@ inline BatchForm batch_many_form(BatchParams *p, int dtype_bf16) {
 inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->few_rows = batch_few_rows(*p);
     p->many_rows = batch_many_rows(*p, dtype_bf16);
-    p->least[0] = p->bits != 0 || (dtype_bf16 && p->d == 64) ? 8 : 4;
+    p->least[0] = p->bits != 0 ? kMxFewWaves : dtype_bf16 && p->d == 64 ? 8 : 4;
     p->least[1] = 4;
     p->whole = dtype_bf16 ? 6 : 4;
     p->per_item = dtype_bf16 ? 0.024f : 0.007f;

@@ -54,7 +54,13 @@ struct MxPlainRows {
     int quarter;
     __device__ __forceinline__ MxPlainRows(const BatchParams &p, const BatchItem &it, int c)
         : rows(p, it, INT_MAX), k(static_cast<const char *>(p.k)), v(static_cast<const char *>(p.v)), quarter(c / E) {}
-    __device__ __forceinline__ void read_one(const char *x, size_t codes, size_t scales, float (&f)[E]) const {
+    size_t codes, scales;
+    __device__ __forceinline__ void at(int t) {
+        const int blk = rows.rows.table[t >> rows.rows.shift];
+        codes = rows.codes(blk, t);
+        scales = rows.scales(blk, t);
+    }
+    __device__ __forceinline__ void read(const char *x, float (&f)[E]) const {
         uint32_t w[F::QB / 4];
         load_words(w, x + codes + quarter * F::QB);
         const float power = mx_power((unsigned char)x[scales + quarter * E / kMxGroup]);
@@ -65,34 +71,80 @@ struct MxPlainRows {
             for (int e = 0; e < 8; ++e) f[8 * i + e] = (float)y[e];
         }
     }
-    __device__ __forceinline__ void read(int t, float (&kf)[E], float (&vf)[E]) const {
-        const int blk = rows.rows.table[t >> rows.rows.shift];
-        const size_t codes = rows.codes(blk, t), scales = rows.scales(blk, t);
-        read_one(k, codes, scales, kf);
-        read_one(v, codes, scales, vf);
-    }
+    __device__ __forceinline__ void read_k(float (&f)[E]) const { read(k, f); }
+    __device__ __forceinline__ void read_v(float (&f)[E]) const { read(v, f); }
 };
 
-// A product's operand in registers, and c + a b, for bf16 and (three parts) fp32.
+// A product's operand in registers, c + a b, and p times the powers of V's keys, for
+// bf16 and (three parts) fp32.
+//
+// bf16: the powers multiply p after it is rounded, by adding to its exponent, two
+// keys at a time: (p + (E << 7)) - (127 << 7) in 16 bits, 0 where that is negative (the
+// result would be below 2^-126). p = 0 becomes 2^(E - 254), as good as 0 beside V's
+// 2^(E - 127), but not for a key that the row does not see: stages that hold such
+// multiply in fp32. With E up to kMxMost no sum passes 16 bits; a piece that met a larger
+// one (V above 2^63, or NaN) runs in plain arithmetic.
+constexpr unsigned kMxMost = 190;
 template <class T>
 struct MxOperand;
 template <>
 struct MxOperand<u16> {
     using B = bf16x8;
-    static constexpr float kUp = 1.f, kDown = 1.f;
-    __device__ static __forceinline__ B pack(const f32x4 &a, const f32x4 &b) { return PolBF16<64>::pack(a, b); }
+    using Power = u16;
+    static constexpr float kDown = 1.f;
+    struct Packed {
+        u32x4 w[2];  // keys 2 i, 2 i + 1 in word i
+    };
+    __device__ static __forceinline__ Power power(unsigned E) { return (u16)(E << 7); }
     __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) { return PolBF16<64>::mma(a, b, c); }
+    __device__ static __forceinline__ Packed prepare(const f32x4 (&p)[4]) {
+        return Packed{{__builtin_bit_cast(u32x4, PolBF16<64>::pack(p[0], p[1])), __builtin_bit_cast(u32x4, PolBF16<64>::pack(p[2], p[3]))}};
+    }
+    template <bool EXACT>
+    __device__ static __forceinline__ void scaled(B (&f)[2], const Packed &pk, const f32x4 (&p)[4], const Power *power) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 e = *reinterpret_cast<const u32x4 *>(power + 8 * h);
+            if constexpr (EXACT) {
+                f32x4 x[2];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i / 4][i % 4] = p[2 * h + i / 4][i % 4] * __uint_as_float(i & 1 ? e[i / 2] & 0xffff0000u : e[i / 2] << 16);
+                f[h] = PolBF16<64>::pack(x[0], x[1]);
+            } else {
+                u32x4 r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a = pk.w[h][i], b = e[i];
+                    const u16x2 up = __builtin_bit_cast(u16x2, a) + __builtin_bit_cast(u16x2, b);
+                    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(up, u16x2{127 << 7, 127 << 7}));
+                }
+                f[h] = __builtin_bit_cast(B, r);
+            }
+        }
+    }
 };
 template <>
 struct MxOperand<float> {
     using B = Split3;
+    using Power = float;
     // p times a power of down to 2^-117 keeps its parts (kPartMin)
-    static constexpr float kUp = kPartUp, kDown = kPartDown;
-    __device__ static __forceinline__ B pack(const f32x4 &a, const f32x4 &b) { return split3(a, b); }
+    static constexpr float kDown = kPartDown;
+    struct Packed {};
+    __device__ static __forceinline__ Power power(unsigned E) { return mx_power(E); }
     __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) {
         c = PolBF16<64>::mma(a, b.l, c);
         c = PolBF16<64>::mma(a, b.m, c);
         return PolBF16<64>::mma(a, b.h, c);
+    }
+    __device__ static __forceinline__ Packed prepare(const f32x4 (&)[4]) { return Packed{}; }
+    template <bool EXACT>
+    __device__ static __forceinline__ void scaled(B (&f)[2], const Packed &, const f32x4 (&p)[4], const Power *power) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 *e = reinterpret_cast<const f32x4 *>(power + 8 * h);
+            f[h] = split3(p[2 * h] * kPartUp * e[0], p[2 * h + 1] * kPartUp * e[1]);
+        }
     }
 };
 
@@ -123,13 +175,14 @@ __device__ __forceinline__ bool mx_row(typename MxOperand<T>::B (&f)[F::D / 32],
 
 // ------------------------------------------------------------------ the few rows
 
-template <class F, int NW>
+template <class F, class T, int NW>
 union MxFewSmem {
-    struct {
-        char k[NW][F::TILE], v[NW][F::TILE];
-        uint32_t ke[NW][64], ve[NW][64];  // E of a key in its low SB bytes
-        int blk[NW][2][64];
-    } t;
+    struct Wave {
+        char k[F::TILE], v[F::TILE];
+        uint32_t ke[64], ve[64];  // E of a key in its low SB bytes
+        typename MxOperand<T>::Power vp[F::SB][64];
+        int blk[2][64];
+    } t[NW];
     BatchFewMerge<F::D, NW> merge;
 };
 
@@ -145,20 +198,33 @@ __device__ __forceinline__ int mx_vswz(int r) {
     return F::CH == 8 ? (((r >> 1) & 3) | ((r >> 4) & 1) << 2) : F::CH == 4 ? (r >> 2) & 3 : (r >> 3) & 1;
 }
 
-// A wave's loads of a stage's codes, CH of 64 chunks, and E.
+// A wave's loads of a stage's codes, CH of 64 chunks, and E. A load's 64 / CH rows
+// lie in a run where blocks are as large (`runs`): its address is then a uniform one
+// and the lane's constant. The stage that ends the sequence goes by each row's
+// own, the last one's past it: what lies behind a sequence is not read.
 template <class F>
 struct MxStage {
-    static constexpr int LOADS = F::CH + 1;
+    static constexpr int LOADS = F::CH + 1, ROWS = 64 / F::CH;
     template <class Swz>
     __device__ static __forceinline__ void load(char *tile, uint32_t *es, const char *X, const MxRows<F> &rows, const int *blk,
-                                                int k0, int lane, Swz swz) {
+                                                int k0, int lane, bool runs, Swz swz) {
         const uint32_t base = lds_addr(tile);
+        const int mine = blk[lane];
+        if (runs && k0 + 64 <= rows.rows.keys) {
 #pragma unroll
-        for (int k = 0; k < F::CH; ++k) {
-            const int P = k * 64 + lane, row = P / F::CH, c = (P % F::CH) ^ swz(row);
-            lds_dma16(base + k * 1024, X + rows.codes(blk[row], k0 + row) + 16 * c);
+            for (int k = 0; k < F::CH; ++k) {
+                const int row = k * ROWS + lane / F::CH;
+                const char *at = X + rows.codes(__builtin_amdgcn_readlane(mine, k * ROWS), k0 + k * ROWS);
+                lds_dma16_u(base + k * 1024, at, (uint32_t)((lane / F::CH) * F::CB + (((lane % F::CH) ^ swz(row)) << 4)));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < F::CH; ++k) {
+                const int row = k * ROWS + lane / F::CH, c = (lane % F::CH) ^ swz(row);
+                lds_dma16(base + k * 1024, X + rows.codes(blk[row], k0 + row) + 16 * c);
+            }
         }
-        const char *e = X + rows.scales(blk[lane], k0 + lane);
+        const char *e = X + rows.scales(mine, k0 + lane);
         if constexpr (F::SB == 4) {
             lds_dma4(lds_addr(es), e);
         } else {
@@ -169,15 +235,19 @@ struct MxStage {
 
 // One 64-key stage: key 16 a + 4 t + b of it is row 4 a + b of score tile t, so a lane
 // (g, l16) holds the scores of keys 16 g .. 16 g + 15 of row l16, in order: the 16
-// keys whose codes a transposing read of V brings it.
-template <class F, class T, bool MASK, class AfterK, class BeforeV>
-__device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, float &lsum,
+// keys whose codes a transposing read of V brings it. p is relative to the running
+// m, which rises only where a lane's sum of p passes kLazySum (fwd_stage_lazy's
+// reasons), or at the wave's FIRST stage. most: the largest E of V so far.
+template <class F, class T, bool FIRST, bool MASK, class AfterK, class BeforeV>
+__device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, float &lsum, unsigned &most,
                                              const typename MxOperand<T>::B (&qf)[F::D / 32], const char *sk,
-                                             const uint32_t *ke, const char *sv, const uint32_t *ve, int lim, int g, int l16,
-                                             float xmul, AfterK after_k, BeforeV before_v) {
+                                             const uint32_t *ke, const char *sv, const uint32_t *ve,
+                                             typename MxOperand<T>::Power (*vp)[64], int lim, int lane, float xmul,
+                                             AfterK after_k, BeforeV before_v) {
     using Op = MxOperand<T>;
     constexpr int NC = F::D / 32, XT = F::D / 16;
-    f32x4 s[4];
+    const int g = lane >> 4, l16 = lane & 15;
+    f32x4 s[4], pv[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const int row = 16 * (l16 >> 2) + 4 * t + (l16 & 3);
@@ -194,57 +264,75 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
             w[0] = x[0];
             w[1] = x[1];
         }
-        const float power = mx_power((ke[row] >> (8 * (g * F::SB / 4))) & 255u);
+        const float power = mx_power(reinterpret_cast<const unsigned char *>(ke + row)[g * F::SB / 4]);
         f32x4 c = zero4();
 #pragma unroll
         for (int i = 0; i < NC; ++i) c = Op::mma(mx_values<F::BITS>(w + i * (F::BITS / 4), power), qf[i], c);
         s[t] = c;
     }
     after_k();
-    float mx = -INFINITY;
+    if constexpr (MASK) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float v = s[t][r] * xmul;
-            if constexpr (MASK) v = 4 * t + r > lim ? -INFINITY : v;
-            s[t][r] = v;
-            mx = fmaxf(mx, v);
+            for (int r = 0; r < 4; ++r) s[t][r] = 4 * t + r > lim ? -INFINITY : s[t][r];
         }
     }
-    mx = xg_max(mx);
-    const float mnew = fmaxf(m, mx), mref = mnew == -INFINITY ? 0.f : mnew;
-    const float corr = fast_exp2(m - mref);
-    m = mnew;
-    lsum *= corr;
+    auto exps = [&](float sub) __attribute__((always_inline)) {
+        float ls = 0.f;
 #pragma unroll
-    for (int xt = 0; xt < XT; ++xt) acc[xt] *= corr;
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+            for (int r = 0; r < 4; ++r) {
+                pv[t][r] = fast_exp2(__builtin_fmaf(s[t][r], xmul, -sub));
+                ls += pv[t][r];
+            }
+        }
+        return ls;
+    };
+    auto raise = [&]() __attribute__((always_inline)) {
+        float mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float pv = fast_exp2(s[t][r] - mref);
-            lsum += pv;
-            s[t][r] = pv * Op::kUp;
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+        }
+        mx = fmaxf(xg_max(mx) * xmul, m);
+        const float to = mx == -INFINITY ? 0.f : mx;  // (a row that sees no key)
+        if constexpr (!FIRST) {
+            const float corr = fast_exp2(m - to);
+            lsum *= corr;
+#pragma unroll
+            for (int xt = 0; xt < XT; ++xt) acc[xt] *= corr;
+        }
+        m = mx;
+        lsum += exps(to);
+    };
+    if constexpr (FIRST) {
+        raise();
+    } else {
+        const float ls = exps(m == -INFINITY ? 0.f : m);
+        if (__builtin_amdgcn_ballot_w64(ls > kLazySum) != 0) {
+            raise();
+        } else {
+            lsum += ls;
         }
     }
     before_v();
-    u32x4 es[4];  // E of the lane's keys
+    // the powers of V's keys, a lane a key
+    const uint32_t e = ve[lane];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) es[t] = *reinterpret_cast<const u32x4 *>(ve + 16 * g + 4 * t);
+    for (int grp = 0; grp < F::SB; ++grp) {
+        const unsigned E = (e >> (8 * grp)) & 255u;
+        most = max(most, E);
+        vp[grp][lane] = Op::power(E);
+    }
+    wait_lds();
+    const typename Op::Packed pk = Op::prepare(pv);
 #pragma unroll
     for (int grp = 0; grp < F::SB; ++grp) {
         typename Op::B pf[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            f32x4 a[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) a[t][r] = s[2 * h + t][r] * mx_power((es[2 * h + t][r] >> (8 * grp)) & 255u);
-            }
-            pf[h] = Op::pack(a[0], a[1]);
-        }
+        Op::template scaled<MASK>(pf, pk, pv, vp[grp] + 16 * g);
 #pragma unroll
         for (int xt = 2 * grp; xt < 2 * grp + 2; ++xt) {
             uint32_t w[F::BITS / 2];  // 16 keys of column 16 xt + l16
@@ -273,7 +361,7 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
 // One piece of a sequence, as batch_few_piece: its loads and waits.
 template <class F, class T, int NW>
 __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
-                                             MxFewSmem<F, NW> &sm) {
+                                             MxFewSmem<F, T, NW> &sm) {
     using Stage = MxStage<F>;
     constexpr int D = F::D, XT = D / 16, ROWS = kBatchFew, NL = Stage::LOADS;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -282,17 +370,18 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
     const char *K = static_cast<const char *>(p.k), *V = static_cast<const char *>(p.v);
     const int Nk = it.s.keys;
     const MxRows<F> rows(p, it, Nk);
-    char *sk = sm.t.k[wave], *sv = sm.t.v[wave];
-    uint32_t *ke = sm.t.ke[wave], *ve = sm.t.ve[wave];
+    const bool runs = (1 << p.bs_shift) >= Stage::ROWS;
+    auto &t = sm.t[wave];
 
+    // stage `st` is the wave's n-th: its blocks in buffer n & 1
     auto fetch = [&](int st, int n) __attribute__((always_inline)) {
-        lds_dma4(lds_addr(sm.t.blk[wave][n & 1]), rows.rows.table + rows.rows.block_at(st * 64 + lane));
+        lds_dma4(lds_addr(t.blk[n & 1]), rows.rows.table + rows.rows.block_at(st * 64 + lane));
     };
     auto load_k = [&](int st, int n) __attribute__((always_inline)) {
-        Stage::load(sk, ke, K, rows, sm.t.blk[wave][n & 1], st * 64, lane, mx_kswz<F>);
+        Stage::load(t.k, t.ke, K, rows, t.blk[n & 1], st * 64, lane, runs, mx_kswz<F>);
     };
     auto load_v = [&](int st, int n) __attribute__((always_inline)) {
-        Stage::load(sv, ve, V, rows, sm.t.blk[wave][n & 1], st * 64, lane, mx_vswz<F>);
+        Stage::load(t.v, t.ve, V, rows, t.blk[n & 1], st * 64, lane, runs, mx_vswz<F>);
     };
     int st = s_lo + wave, n = 0;
     if (st < s_hi) fetch(st, 0);
@@ -302,7 +391,7 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
     const bool low = mx_row<F, T>(qf, static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
     if (st < s_hi) {
         wait_loads<0>();
-        if (st + NW < s_hi) fetch(st + NW, 1);
+        fetch(st + NW, 1);
         load_k(st, 0);
         load_v(st, 0);
     }
@@ -310,15 +399,21 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
 #pragma unroll
     for (int xt = 0; xt < XT; ++xt) acc[xt] = zero4();
     float m = -INFINITY, lsum = 0.f;
+    unsigned most = 0;
     // stages before `whole` hold no key that a row does not see
     const int whole = min(Nk, it.s.pos + 1) / 64;
-    for (; st < s_hi; st += NW, ++n) {
-        const bool more = st + NW < s_hi, after = st + 2 * NW < s_hi;
+    // The wave's next stage: its K goes out once this one's K has been read, with the
+    // blocks of the stage after it, and its V once this one's V has. vmcnt counts in
+    // order: NL loads (this stage's V) follow K, NL + 1 (the blocks and the next K)
+    // follow V. A second buffer for each, with both in flight all the time, was slower (64
+    // sequences, 4 bits: 124 us and 115): the reads are not what waits.
+    auto stage = [&](auto first, auto mask) __attribute__((always_inline)) {
+        const bool more = st + NW < s_hi;
         wait_loads<NL>();
         auto after_k = [&]() __attribute__((always_inline)) {
             wait_lds();
             if (more) {
-                fetch(after ? st + 2 * NW : st, n);  // (this stage's blocks: its V is out already)
+                fetch(st + 2 * NW, n);  // (this stage's blocks: its V is out already)
                 load_k(st + NW, n + 1);
             }
         };
@@ -330,19 +425,23 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
             }
         };
         const int lim = min(qpos, Nk - 1) - st * 64 - 16 * g;
-        if (st < whole) {
-            mx_few_stage<F, T, false>(acc, m, lsum, qf, sk, ke, sv, ve, lim, g, l16, p.scale_log2, after_k, before_v);
-        } else {
-            mx_few_stage<F, T, true>(acc, m, lsum, qf, sk, ke, sv, ve, lim, g, l16, p.scale_log2, after_k, before_v);
-        }
+        mx_few_stage<F, T, decltype(first)::value, decltype(mask)::value>(acc, m, lsum, most, qf, t.k, t.ke, t.v, t.ve, t.vp,
+                                                                          lim, lane, p.scale_log2, after_k, before_v);
         wait_lds();
         if (more) load_v(st + NW, n + 1);
-    }
+        st += NW;
+        ++n;
+    };
+    using std::false_type;
+    using std::true_type;
+    if (st < s_hi) stage(true_type{}, true_type{});
+    while (st < min(s_hi, whole)) stage(false_type{}, false_type{});
+    while (st < s_hi) stage(false_type{}, true_type{});
     const float lw = xg_sum(lsum);
     float z = 0.f * lw;
 #pragma unroll
     for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt]);
-    const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f) != 0 || low;
+    const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f || most > kMxMost) != 0 || low;
     batch_few_finish<T, D, NW, 64 * NW>(
         p, it, slot, sm.merge, m, lw, bad,
         [&](int i) __attribute__((always_inline)) { return acc[i] * MxOperand<T>::kDown; },
@@ -352,7 +451,7 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
         });
 }
 template <class F, class T, int NW>
-__device__ __forceinline__ void mx_few_body(const BatchParams &p, int g, MxFewSmem<F, NW> &sm) {
+__device__ __forceinline__ void mx_few_body(const BatchParams &p, int g, MxFewSmem<F, T, NW> &sm) {
     batch_few_run(p, g, [&](const BatchItem &it, int lo, int hi, int slot) __attribute__((always_inline)) {
         mx_few_piece<F, T, NW>(p, it, lo, hi, slot, sm);
     });
@@ -391,9 +490,9 @@ struct MxPart {
     static constexpr int TPR = NT / 64, E = F::D / TPR, B = E * F::BITS / 8;  // threads of a row, elements, bytes
     uint32_t w[B / 4];
     float power;
-    __device__ __forceinline__ void load(const char *X, size_t codes, size_t scales, int part) {
-        load_words(w, X + codes + part * B);
-        power = mx_power((unsigned char)X[scales + part * E / kMxGroup]);
+    __device__ __forceinline__ void load(const char *codes, const char *scales) {
+        load_words(w, codes);
+        power = mx_power((unsigned char)*scales);
     }
     __device__ __forceinline__ void write(u16 *tile, int row, int part) const {
         char *base = reinterpret_cast<char *>(tile) + row * (2 * F::D);
@@ -457,9 +556,10 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
     int blk = 0;
     auto fetch = [&](int st) __attribute__((always_inline)) { blk = rows.rows.table[rows.rows.block_at(st * BK + key)]; };
     auto load = [&](int st) __attribute__((always_inline)) {
-        const size_t codes = rows.codes(blk, st * BK + key), scales = rows.scales(blk, st * BK + key);
-        xk.load(K, codes, scales, part);
-        xv.load(V, codes, scales, part);
+        const size_t codes = rows.codes(blk, st * BK + key) + part * Part::B;
+        const size_t scales = rows.scales(blk, st * BK + key) + part * Part::E / kMxGroup;
+        xk.load(K + codes, K + scales);
+        xv.load(V + codes, V + scales);
         if (st + 1 < s_hi) fetch(st + 1);
     };
     auto write = [&](int buf) __attribute__((always_inline)) {
@@ -471,7 +571,7 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
         load(s_lo);
         write(0);
     }
-    __syncthreads();
+    barrier_lds();
     const int whole = min(s_hi, min(Nk, pos_lo + 1) / BK);
     const bool some = rw <= last_row;  // the wave has rows
     auto main_stage = [&](auto buf, auto first, int st) __attribute__((always_inline)) {
@@ -487,7 +587,7 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
             }
         }
         if (st + 1 < s_hi) write(B ^ 1);
-        __syncthreads();
+        barrier_lds();
     };
     using B0 = std::integral_constant<int, 0>;
     using B1 = std::integral_constant<int, 1>;
@@ -505,7 +605,7 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
             fwd_stage<Pol, QT, true, true, kPrio, true>(acc, m, lsum, qf, sm.k[cur], sm.v[cur], st * BK, qpos, Nk, g, l16,
                                                         p.scale_log2);
         if (st + 1 < s_hi) write(cur ^ 1);
-        __syncthreads();
+        barrier_lds();
     }
     float ltot[QT], z = 0.f;
 #pragma unroll
@@ -562,7 +662,7 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
 template <class F, class T, int QT, int NW>
 __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_groups) {
     __shared__ __attribute__((aligned(16))) union {
-        MxFewSmem<F, NW> few;
+        MxFewSmem<F, T, NW> few;
         MxManySmem<F::D, NW> many;
     } sm;
     if ((int)blockIdx.x < few_groups) {
@@ -572,10 +672,10 @@ __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_group
     }
 }
 
-#define MXFA_BATCH_MX_FEW(NAME, BITS, D, T, NW)                                                              \
-    extern "C" __global__ __launch_bounds__(64 * NW) void mxfa_batch_##NAME##_few(BatchParams p) {           \
-        __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, NW> sm;                               \
-        mx_few_body<Mx<BITS, D>, T, NW>(p, blockIdx.x, sm);                                                  \
+#define MXFA_BATCH_MX_FEW(NAME, BITS, D, T)                                                                  \
+    extern "C" __global__ __launch_bounds__(64 * kMxFewWaves) void mxfa_batch_##NAME##_few(BatchParams p) {  \
+        __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, T, kMxFewWaves> sm;                   \
+        mx_few_body<Mx<BITS, D>, T, kMxFewWaves>(p, blockIdx.x, sm);                                         \
     }
 #define MXFA_BATCH_MX_MANY(MANY, BOTH, BITS, D, T, QT, NW, WPS, BOTH_WPS)                                    \
     extern "C" __global__ __launch_bounds__(64 * NW, WPS) void mxfa_batch_##MANY(BatchParams p) {            \
@@ -586,13 +686,13 @@ __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_group
         mx_both_body<Mx<BITS, D>, T, QT, NW>(p, few_groups);                                                 \
     }
 #define MXFA_BATCH_MX(BITS)                                                                                  \
-    MXFA_BATCH_MX_FEW(x##BITS##b64, BITS, 64, u16, 8)                                                        \
+    MXFA_BATCH_MX_FEW(x##BITS##b64, BITS, 64, u16)                                                           \
     MXFA_BATCH_MX_MANY(x##BITS##b64_many, x##BITS##b64_both, BITS, 64, u16, 2, 4, 3, 3)                      \
     MXFA_BATCH_MX_MANY(x##BITS##b64_many64, x##BITS##b64_both64, BITS, 64, u16, 1, 4, 4, 3)                  \
-    MXFA_BATCH_MX_FEW(x##BITS##b128, BITS, 128, u16, 8)                                                      \
+    MXFA_BATCH_MX_FEW(x##BITS##b128, BITS, 128, u16)                                                         \
     MXFA_BATCH_MX_MANY(x##BITS##b128_many, x##BITS##b128_both, BITS, 128, u16, 2, 4, 2, 2)                   \
     MXFA_BATCH_MX_MANY(x##BITS##b128_many64, x##BITS##b128_both64, BITS, 128, u16, 1, 4, 2, 2)               \
-    MXFA_BATCH_MX_FEW(x##BITS##f64, BITS, 64, float, 8)                                                      \
+    MXFA_BATCH_MX_FEW(x##BITS##f64, BITS, 64, float)                                                         \
     MXFA_BATCH_MX_MANY(x##BITS##f64_many, x##BITS##f64_both, BITS, 64, float, 1, kBatchF32Waves, 4, 4)
 MXFA_BATCH_MX(8)
 MXFA_BATCH_MX(4)

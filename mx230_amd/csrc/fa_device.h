@@ -760,6 +760,19 @@ __device__ __forceinline__ void lds_dma16_s(uint32_t base, const void *sbase, ui
 #endif
 }
 
+// The same where a vector instruction may have written the base's registers, which
+// a vector-memory instruction may read 5 wait states later.
+__device__ __forceinline__ void lds_dma16_u(uint32_t base, const void *sbase, uint32_t voff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    uint32_t save;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+        : "=&s"(save)
+        : "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane(base)));
+#endif
+}
+
 // Where each of a thread's staging loads of a tile reads from: load k fills
 // 16-byte position P = k NT + tid of the tile, which holds chunk c of row r
 // (Pol::chunk_at). Computed once per kernel and kept packed in one register
