@@ -1217,11 +1217,16 @@ def prefill_batch_mx_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head:
                                      bf16: bool = True, bits: int = 8) -> int:
     """mxfa_prefill_batch_mx_workspace_bytes: what run_prefill_batch_mx needs for such a
     batch, whatever its lengths (0 for one it does not take)."""
-    w, entries = n_head * head_dim, 1 << 17
+    w, lib, block = n_head * head_dim, load_library(), mx_block_bytes(1, n_kv_head, head_dim, bits)
     _c_int(n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, q_stride=w)
-    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w,
-                        mx_block_bytes(1, n_kv_head, head_dim, bits), w, MXFA_BF16 if bf16 else MXFA_F32, 0.0)
-    return int(load_library().mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(sh), bits))
+
+    def of(entries):
+        sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w, block, w,
+                            MXFA_BF16 if bf16 else MXFA_F32, 0.0)
+        return int(lib.mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(sh), bits))
+    # (tables of any width: the widest of short contexts, whose units may be smaller and
+    # their shares more, and 2^17 positions, at which every form has all its work-groups)
+    return max(of(64 * ((40 + max(min(max_q, n_tok), 0) // 64) // 2)), of(1 << 17))
 
 
 def run_prefill_batch_mx(q, kcache, vcache, bits: int, out, block_table, block_size: int, cu_q, lens, max_q: int,

@@ -283,6 +283,9 @@ inline bool batch_mostly_few(const BatchParams &p) {
     return 2 * (more_of((long long)p.n_tok - p.n_seq * few_tok, 0LL) / p.max_q) < p.n_seq;
 }
 
+// Stages that a sequence has at most, by its table.
+inline long long batch_most_stages(const BatchParams &p) { return (((long long)p.max_blocks << p.bs_shift) + 63) / 64; }
+
 // Rows of its units (bf16: 4 waves of 16 or of 32). 32 a wave halve the LDS reads of
 // K and V for each product, 16 give twice the work-groups: taken where units of 128
 // rows are at most one and a half (d = 128: one) per CU. us, by 64 and by 128 rows:
@@ -290,13 +293,19 @@ inline bool batch_mostly_few(const BatchParams &p) {
 // 33, 8 of 512 after 3584 111 and 92; 32/8 heads, d = 128, 1000 tokens 23 and 28,
 // 2 chunks of 1000 after 2000 134 and 106. Beside the few-row form's work-groups, which
 // leave a CU room for two more of either, 128: 4 chunks and 28 tokens 58 and 52.
+//
+// Over a microscaled cache, whose keys each work-group converts, 64 rows also cost
+// twice the conversions, and where there are stages enough to share out a unit's keys
+// fill the CUs as well: 128 where a row of the longest chunk sees more than 20 stages
+// on average. us, 4 bits, by 64 and by 128 rows: 14/2 heads, d = 64, 2000 tokens from
+// the start (16) 29 and 33, 4 chunks of 700 to 1400 (16) 29 and 34, 1000 to 2048 (24) 31
+// and 28, 4 of 512 to 8192 (124) 137 and 95; 32/8 heads, d = 128, 500 to 1000 (12) 24 and 30,
+// 500 to 2048 (28) 45 and 38, to 8192 112 and 82.
 inline int batch_many_rows(const BatchParams &p, int dtype_bf16) {
     if (!dtype_bf16) return 16 * kBatchF32Waves;
+    if (p.bits != 0 && 2 * batch_most_stages(p) - less_of(p.max_q, p.n_tok) / 64 > 40) return 128;
     return !batch_mostly_few(p) && batch_units(p, 128) <= (p.d == 64 ? 3 * kBatchCus / 2 : kBatchCus) ? 64 : 128;
 }
-
-// Stages that a sequence has at most, by its table.
-inline long long batch_most_stages(const BatchParams &p) { return (((long long)p.max_blocks << p.bs_shift) + 63) / 64; }
 
 // A form's launch: its work-groups and the join's, and the workspace's slots.
 struct BatchForm {

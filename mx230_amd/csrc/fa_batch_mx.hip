@@ -9,9 +9,22 @@
 //     bits, as its share of the contraction over d, so K is converted in registers,
 //     E's power in the same instruction. V is read from LDS transposed, still as
 //     codes (ds_read_b64_tr_b4 / _b8): a lane has 16 keys of one column, whose powers
-//     differ, so these multiply p before it is rounded for the product.
+//     differ, so these multiply p.
 //   * many rows: a thread loads a part of a key's row a stage ahead and converts it
 //     once for the work-group, into the bf16 tiles of fa_batch.hip's products.
+//
+// Measured (us, as in fa_batch.hip; in brackets the ordinary cache, bf16 or fp32):
+//   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: in 8 bits
+//         202 and the join 5 (1.11 GB, 5.5 TB/s), in 4 bits 115 and 5 (0.57 GB, 5.0
+//         TB/s: a head's 64 bytes of E come as whole lines, 6% more) [391 and 6]; d =
+//         64 122 and 89 in all [248]; fp32 45 and 41 [125];
+//         24 sequences of 1 to 4 tokens, to 8192 long, d = 128, 8 bits: 49 and 5;
+//   many: the last 2048 tokens of 32768, 32/8 heads, d = 128, 4 bits: 955 [950]; 1000
+//         to 4000 tokens of short contexts 10 to 18% more than the ordinary cache: the
+//         conversions and addresses, some 60 instructions a stage beside the softmax's
+//         260, share the vector unit with it; fp32, 2000 tokens of 14/2 heads 39 [56];
+//   both: 28 single tokens and 4 chunks of up to 512, to 8192 long, 14/2 heads, d = 64,
+//         8 bits: 60 with the join [61]; fp32, 4 bits, 6 tokens and 2 chunks: 54 [57].
 #include "fa_batch_items.h"
 #include "fa_launch.h"
 #include "fa_mx.h"
@@ -237,7 +250,8 @@ struct MxStage {
 // (g, l16) holds the scores of keys 16 g .. 16 g + 15 of row l16, in order: the 16
 // keys whose codes a transposing read of V brings it. p is relative to the running
 // m, which rises only where a lane's sum of p passes kLazySum (fwd_stage_lazy's
-// reasons), or at the wave's FIRST stage. most: the largest E of V so far.
+// reasons), is above 0 while m is still -infinity, or at the wave's FIRST stage. most:
+// the largest E of V so far.
 template <class F, class T, bool FIRST, bool MASK, class AfterK, class BeforeV>
 __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, float &lsum, unsigned &most,
                                              const typename MxOperand<T>::B (&qf)[F::D / 32], const char *sk,
@@ -311,8 +325,9 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
     if constexpr (FIRST) {
         raise();
     } else {
-        const float ls = exps(m == -INFINITY ? 0.f : m);
-        if (__builtin_amdgcn_ballot_w64(ls > kLazySum) != 0) {
+        const bool none = m == -INFINITY;  // no key seen, or every score so far -infinity
+        const float ls = exps(none ? 0.f : m);
+        if (__builtin_amdgcn_ballot_w64(ls > (none ? 0.f : kLazySum)) != 0) {
             raise();
         } else {
             lsum += ls;
@@ -375,7 +390,7 @@ __device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchIt
 
     // stage `st` is the wave's n-th: its blocks in buffer n & 1
     auto fetch = [&](int st, int n) __attribute__((always_inline)) {
-        lds_dma4(lds_addr(t.blk[n & 1]), rows.rows.table + rows.rows.block_at(st * 64 + lane));
+        lds_dma4(lds_addr(t.blk[n & 1]), rows.rows.table + rows.rows.block_at(min(st, s_hi - 1) * 64 + lane));
     };
     auto load_k = [&](int st, int n) __attribute__((always_inline)) {
         Stage::load(t.k, t.ke, K, rows, t.blk[n & 1], st * 64, lane, runs, mx_kswz<F>);

@@ -354,6 +354,8 @@ __device__ __forceinline__ void append_any(const BatchParams &p, double factor) 
                 }
             }
             if (w.of == 0) {
+                // (q_out may be qkv: the wave has all of the row's partners before it stores)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 store8<T>(out + h * p.d, x);
             } else {
                 const MxRow r = mx_row_of<BITS>(p, at, w.of == 1 ? p.k : p.v, h);
