@@ -143,3 +143,20 @@ def test_format_by_hand():
     assert torch.equal(c.to(torch.uint8), (x * p).to(torch.float8_e4m3fn).view(torch.uint8))
     assert torch.equal(stands_for(c, e, 8).float(), (x * p).to(torch.float8_e4m3fn).float() / p)
     assert bool((x * p).abs().unflatten(-1, (-1, 32)).amax(-1).gt(224).all())
+
+
+@pytest.mark.parametrize("bf16,hd", [(True, 64), (True, 128), (False, 64)])
+def test_workspace_for_tables_of_any_width(lib, bf16, hd):  # noqa: F811
+    """prefill_batch_mx_workspace_bytes holds what a call needs, whatever its table."""
+    for n_tok, n_seq, max_q in ((1, 1, 1), (64, 64, 1), (96, 24, 4), (500, 1, 500), (700, 4, 512), (2000, 1, 2000), (4000, 8, 700),
+                                (1000, 3, 4096), (30, 30, 7)):
+        for nh, nkv in ((14, 2), (32, 8), (4, 1), (40, 1)):
+            got = mx.prefill_batch_mx_workspace_bytes(n_tok, n_seq, max_q, nh, nkv, hd, bf16, 4)
+            for wide in (1, 64, 256, 500, 700, 1000, 1280, 1281, 1500, 2000, 2304, 2305, 3000, 4000, 6000, 10 ** 4, 10 ** 5, 10 ** 6):
+                for bs in (1, 16):
+                    n = -(-wide // bs)
+                    s = shape(4, n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=nh, n_kv_head=nkv, head_dim=hd, block_size=bs,
+                              max_blocks=n, table_stride=n, q_stride=nh * hd, out_stride=nh * hd, kv_stride=1 << 20,
+                              dtype=mx.MXFA_BF16 if bf16 else mx.MXFA_F32)
+                    need = lib.mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(s), 4)
+                    assert 0 < need <= got, (n_tok, n_seq, max_q, nh, nkv, wide, bs, need, got)
