@@ -52,7 +52,7 @@ typedef enum {
     MXFA_ERR_ALIGN = -5,       /* a device pointer is not 16-byte aligned */
     MXFA_ERR_LAUNCH = -6,      /* the HIP runtime rejected a launch */
     MXFA_ERR_DEVICE = -7,      /* no usable gfx950 device */
-    MXFA_ERR_WORKSPACE = -8,   /* a workspace smaller than mxfa_{bwd,prefill,prefill_batch}_workspace_bytes(shape) */
+    MXFA_ERR_WORKSPACE = -8,   /* a workspace smaller than mxfa_{bwd,prefill,prefill_batch,prefill_batch_mx}_workspace_bytes */
     MXFA_ERR_CODE_OBJECT = -9, /* the gfx950 code object is missing, malformed, for another
                                   processor, or lacks a kernel */
     MXFA_ERR_SCRATCH = -10     /* mxfa_run_bwd_noalloc: the shape needs more than
