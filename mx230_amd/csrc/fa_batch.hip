@@ -301,24 +301,60 @@ __device__ __forceinline__ unsigned few_line(const BatchParams &p) {
     return wave_sum(all);
 }
 
-// f(sequence's number, BatchSeq, its begin and end on the line) for the sequences
-// from position x of the line on, until f returns true.
-template <class F>
-__device__ __forceinline__ void few_walk(const BatchParams &p, unsigned x, F f) {
-    const int lane = threadIdx.x & 63;
-    unsigned before = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-        const BatchSeq b = batch_seq<true, kBatchFew>(p, s0 + lane);
-        const unsigned w = few_weight(b), upto = before + wave_prefix(w);
-        unsigned long long left = __builtin_amdgcn_ballot_w64(w > 0 && upto > x);
-        for (; left != 0; left &= left - 1) {
-            const int l = __builtin_ctzll(left);
-            const unsigned u1 = __builtin_amdgcn_readlane(upto, l);
-            if (f(s0 + l, seq_of_lane(b, l), u1 - __builtin_amdgcn_readlane(w, l), u1)) return;
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
+// The pieces of work-group g of the few-row form in their order: KV head g % Hkv, run
+// g / Hkv of its line. Equal runs, one work-group to a CU (its tiles take the LDS): 64
+// sequences of 2000-16384 positions, 32/8 heads, d = 128, in 393 us with the join, at the step
+// that brought them, 415 with a work-group per share of a sequence, whose count the host can
+// only bound: thousands are empty.
+struct FewRun {
+    const BatchParams &p;
+    const int g;
+    unsigned run, x, x1;
+    BatchSeq b;          // of 64 sequences, a lane each
+    unsigned w, upto, before = 0;
+    int s0 = 0;          // the next 64
+    unsigned long long left = 0;  // of these, the ones that the run meets
+    // what the join of a sequence that the run ends in reads
+    __device__ __forceinline__ void note(const FewNote &n) const {
+        if (threadIdx.x == 0 && p.few_groups > 1) reinterpret_cast<FewNote *>(p.notes[0])[g] = n;
     }
-}
+    __device__ __forceinline__ FewRun(const BatchParams &p_, int g_) : p(p_), g(g_) {
+        const unsigned all = few_line(p);
+        // (scalars from the start: a division is the vector unit's)
+        run = __builtin_amdgcn_readfirstlane(few_run(p, all));
+        x = (unsigned)__builtin_amdgcn_readfirstlane(g / p.Hkv) * run;
+        x1 = min(x + run, all);
+        if (x >= x1) note(FewNote{0, 0, 0, 0});
+    }
+    __device__ __forceinline__ BatchItem item() const {
+        BatchItem it;
+        it.head = __builtin_amdgcn_readfirstlane(g % p.Hkv);
+        it.unit = 0;
+        return it;
+    }
+    // the next piece: its sequence into `it`, from item()
+    __device__ __forceinline__ bool next(BatchItem &it, FewPiece &f) {
+        if (x >= x1) return false;
+        while (left == 0) {
+            if (s0 >= p.n_seq) return false;
+            b = batch_seq<true, kBatchFew>(p, s0 + (threadIdx.x & 63));
+            w = few_weight(b);
+            upto = before + wave_prefix(w);
+            left = __builtin_amdgcn_ballot_w64(w > 0 && upto > x);
+            before = __builtin_amdgcn_readlane(upto, 63);
+            s0 += 64;
+        }
+        const int l = __builtin_ctzll(left);
+        left &= left - 1;
+        const unsigned u1 = __builtin_amdgcn_readlane(upto, l), u0 = u1 - __builtin_amdgcn_readlane(w, l);
+        it.seq = s0 - 64 + l;
+        it.s = seq_of_lane(b, l);
+        f = few_piece(x, x1, u0, u1, g);
+        if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, it.s.q0, it.s.rows, it.s.pos});
+        x = f.end;
+        return true;
+    }
+};
 
 // Row r of a unit's sequence: its elements in q or o, and its index in lse.
 __device__ __forceinline__ size_t batch_elem(const BatchParams &p, const BatchItem &it, int r, int stride, int d) {
@@ -480,16 +516,16 @@ __device__ __forceinline__ void batch_few_finish(const BatchParams &p, const Bat
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
-    __syncthreads();  // every wave is done with the tiles
+    barrier_lds();  // every wave is done with the tiles
     if (tid == 0) sm.bad = 0;
-    __syncthreads();
+    barrier_lds();
     if (bad && lane == 0) sm.bad = 1;
     if (wave < NW) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4 *>(&sm.acc[wave][l16][col(i)]) = quad(i);
         if (g == 0) *reinterpret_cast<float2 *>(sm.ml[wave][l16]) = make_float2(m, lw);
     }
-    __syncthreads();
+    barrier_lds();
     float *part = nullptr, *ml = nullptr;
     if (slot >= 0) {
         part = batch_part(p.part[0], slot, ROWS, D);
@@ -615,41 +651,16 @@ __device__ __forceinline__ void batch_few_piece(const BatchParams &p, const Batc
         });
 }
 
-// Work-group g of the few-row form: KV head g % Hkv, run g / Hkv of its line. Equal
-// runs, one work-group to a CU (its tiles take the LDS): 64 sequences of 2000-16384
-// positions, 32/8 heads, d = 128, in 393 us with the join, at the step that brought
-// them, 415 with a work-group per share of a sequence, whose count the host can only
-// bound: thousands are empty.
-// (piece(item, first and last stage, slot): as batch_few_piece)
-template <class Piece>
-__device__ __forceinline__ void batch_few_run(const BatchParams &p, int g, Piece piece) {
-    const unsigned all = few_line(p), run = few_run(p, all);
-    unsigned x = (unsigned)(g / p.Hkv) * run;
-    const unsigned x1 = min(x + run, all);
-    // what the join of a sequence that the run ends in reads
-    auto note = [&](const FewNote &n) __attribute__((always_inline)) {
-        if (threadIdx.x == 0 && p.few_groups > 1) reinterpret_cast<FewNote *>(p.notes[0])[g] = n;
-    };
-    if (x >= x1) return note(FewNote{0, 0, 0, 0});
-    BatchItem it;
-    it.head = g % p.Hkv;
-    it.unit = 0;
-    few_walk(p, x, [&](int seq, const BatchSeq &s, unsigned u0, unsigned u1) __attribute__((always_inline)) {
-        it.seq = seq;
-        it.s = s;
-        const FewPiece f = few_piece(x, x1, u0, u1, g);
-        if (f.end >= x1) note(FewNote{f.slot == 2 * g + 1 ? few_parts(run, u0, u1) : 0, s.q0, s.rows, s.pos});
-        piece(it, f.lo, f.hi, f.slot);
-        x = f.end;
-        if (x < x1) __syncthreads();  // the next piece's tiles are this one's join
-        return x >= x1;
-    });
-}
 template <class Pol, int NW, int THREADS>
 __device__ __forceinline__ void batch_few_body(const BatchParams &p, int g, BatchFewSmem<Pol, NW> &sm) {
-    batch_few_run(p, g, [&](const BatchItem &it, int lo, int hi, int slot) __attribute__((always_inline)) {
-        batch_few_piece<Pol, NW, THREADS>(p, it, lo, hi, slot, sm);
-    });
+    FewRun run(p, g);
+    BatchItem it = run.item();
+    FewPiece f;
+    for (bool more = run.next(it, f); more;) {
+        batch_few_piece<Pol, NW, THREADS>(p, it, f.lo, f.hi, f.slot, sm);
+        more = run.next(it, f);
+        if (more) __syncthreads();  // the next piece's tiles are this one's join
+    }
 }
 
 // ----------------------------------------------------------------- the many rows
@@ -1193,18 +1204,19 @@ long long batch_groups(const BatchParams &q, int dtype_bf16) {
 }
 
 hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStream_t stream) {
-    static constexpr KernelId ids[9][6] = {
+    static constexpr KernelId ids[9][7] = {
         {k_mxfa_batch_b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_b64_many, k_mxfa_batch_b64_both,
          k_mxfa_batch_b64_many64, k_mxfa_batch_b64_both64},
         {k_mxfa_batch_b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_b128_many, k_mxfa_batch_b128_both,
          k_mxfa_batch_b128_many64, k_mxfa_batch_b128_both64},
         {k_mxfa_batch_f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_f64_many, k_mxfa_batch_f64_both},
-#define MXFA_IDS(BITS)                                                                                                  \
-    {k_mxfa_batch_x##BITS##b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_x##BITS##b64_many, k_mxfa_batch_x##BITS##b64_both, \
-     k_mxfa_batch_x##BITS##b64_many64, k_mxfa_batch_x##BITS##b64_both64},                                               \
-        {k_mxfa_batch_x##BITS##b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_x##BITS##b128_many,                       \
-         k_mxfa_batch_x##BITS##b128_both, k_mxfa_batch_x##BITS##b128_many64, k_mxfa_batch_x##BITS##b128_both64},        \
-    {k_mxfa_batch_x##BITS##f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_x##BITS##f64_many, k_mxfa_batch_x##BITS##f64_both}
+#define MXFA_IDS(BITS)                                                                                                 \
+    {k_mxfa_batch_x##BITS##b64_few, k_mxfa_batch_b64_join, k_mxfa_batch_x##BITS##b64_many, k_mxfa_batch_x##BITS##b64_both,\
+     k_mxfa_batch_x##BITS##b64_many64, k_mxfa_batch_x##BITS##b64_both64, k_mxfa_batch_x##BITS##b64_one},               \
+    {k_mxfa_batch_x##BITS##b128_few, k_mxfa_batch_b128_join, k_mxfa_batch_x##BITS##b128_many, k_mxfa_batch_x##BITS##b128_both,\
+     k_mxfa_batch_x##BITS##b128_many64, k_mxfa_batch_x##BITS##b128_both64, k_mxfa_batch_x##BITS##b128_one},            \
+    {k_mxfa_batch_x##BITS##f64_few, k_mxfa_batch_f64_join, k_mxfa_batch_x##BITS##f64_many, k_mxfa_batch_x##BITS##f64_both,\
+     {}, {}, k_mxfa_batch_x##BITS##f64_one}
         MXFA_IDS(8), MXFA_IDS(4)};
 #undef MXFA_IDS
     const KernelId *id = ids[(p.bits == 0 ? 0 : p.bits == 8 ? 3 : 6) + (!dtype_bf16 ? 2 : p.d == 128 ? 1 : 0)];
@@ -1223,7 +1235,8 @@ hipError_t launch_batch(BatchParams p, int dtype_bf16, void *workspace, hipStrea
     int few_groups = (int)f[0].groups;
     void *args[] = {&p, &few_groups};
     if (f[1].groups == 0) {
-        e = launch_kernel(id[0], dim3(few_groups), dim3(p.bits != 0 ? 64 * kMxFewWaves : dtype_bf16 && p.d == 64 ? 512 : 256), args, stream);
+        const int few_threads = p.bits != 0 ? 64 * kMxFewWaves : dtype_bf16 && p.d == 64 ? 512 : 256;
+        e = launch_kernel(id[p.bits != 0 && p.n_seq == 1 ? 6 : 0], dim3(few_groups), dim3(few_threads), args, stream);
     } else if (few_groups == 0) {
         e = launch_kernel(many[0], dim3((unsigned)f[1].groups), dim3(threads), args, stream);
     } else {

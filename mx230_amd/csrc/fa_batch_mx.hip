@@ -15,10 +15,11 @@
 //
 // Measured (us, as in fa_batch.hip; in brackets the ordinary cache, bf16 or fp32):
 //   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: in 8 bits
-//         202 and the join 5 (1.11 GB, 5.5 TB/s), in 4 bits 115 and 5 (0.57 GB, 5.0
+//         198 and the join 5 (1.11 GB, 5.6 TB/s), in 4 bits 108 and 5 (0.57 GB, 5.3
 //         TB/s: a head's 64 bytes of E come as whole lines, 6% more) [391 and 6]; d =
-//         64 122 and 89 in all [248]; fp32 45 and 41 [125];
-//         24 sequences of 1 to 4 tokens, to 8192 long, d = 128, 8 bits: 49 and 5;
+//         64 122 and 80 in all [248]; fp32 43 and 40 [125]; 512 sequences of 900, d = 128
+//         186 and 128 in all;
+//         24 sequences of 1 to 4 tokens, to 8192 long, d = 128, 8 bits: 46 and 5;
 //   many: the last 2048 tokens of 32768, 32/8 heads, d = 128, 4 bits: 955 [950]; 1000
 //         to 4000 tokens of short contexts 10 to 18% more than the ordinary cache: the
 //         conversions and addresses, some 60 instructions a stage beside the softmax's
@@ -186,17 +187,51 @@ __device__ __forceinline__ bool mx_row(typename MxOperand<T>::B (&f)[F::D / 32],
     }
 }
 
+// Waits for Q's loads. The compiler knows of no others, and where a use may be the first
+// after them it waits until none of any kind is left: without this in every stage (64
+// sequences of 2000-16384, 32/8 heads, d = 128, 4 bits: 121 us and 110).
+template <class T, int N>
+__device__ __forceinline__ void mx_arrived(typename MxOperand<T>::B (&f)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if constexpr (sizeof(T) == 2) {
+            asm volatile("" : "+v"(f[c]));
+        } else {
+            asm volatile("" : "+v"(f[c].h), "+v"(f[c].m), "+v"(f[c].l));
+        }
+    }
+}
+
 // ------------------------------------------------------------------ the few rows
 
-template <class F, class T, int NW>
-union MxFewSmem {
-    struct Wave {
-        char k[F::TILE], v[F::TILE];
-        uint32_t ke[64], ve[64];  // E of a key in its low SB bytes
-        typename MxOperand<T>::Power vp[F::SB][64];
-        int blk[2][64];
-    } t[NW];
-    BatchFewMerge<F::D, NW> merge;
+// V's tiles, and where the waves meet at a piece's end: in the same LDS, or apart where a
+// work-group sends for the next piece before and has a CU's LDS to itself.
+template <class Values, class Merge>
+union MxFewShared {
+    Values values;
+    Merge merge;
+};
+template <class Values, class Merge>
+struct MxFewApart {
+    Values values;
+    alignas(16) Merge merge;
+};
+template <class F, class T, int NW, bool AHEAD>
+struct MxFewSmem {
+    struct Keys {
+        char k[F::TILE];
+        uint32_t e[64];             // E of a key in its low SB bytes
+        int blk[2][64], first[64];  // blocks of its stages; of the next piece's first
+    };
+    struct Values {
+        char v[NW][F::TILE];
+        uint32_t e[NW][64];
+        typename MxOperand<T>::Power power[NW][F::SB][64];
+    };
+    using Merge = BatchFewMerge<F::D, NW>;
+    static constexpr bool APART = AHEAD && NW * sizeof(Keys) + sizeof(Values) + sizeof(Merge) + 16 <= 160 * 1024;
+    Keys keys[NW];
+    std::conditional_t<APART, MxFewApart<Values, Merge>, MxFewShared<Values, Merge>> end;
 };
 
 // Codes in LDS: chunk c of row r at slot c ^ kswz(r) (K) or c ^ vswz(r) (V).
@@ -373,103 +408,157 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
     }
 }
 
-// One piece of a sequence, as batch_few_piece: its loads and waits.
-template <class F, class T, int NW>
-__device__ __forceinline__ void mx_few_piece(const BatchParams &p, const BatchItem &it, int s_lo, int s_hi, int slot,
-                                             MxFewSmem<F, T, NW> &sm) {
+// A work-group's run of pieces, as batch_few_piece: their loads and waits. AHEAD: a wave
+// that is done with a piece sends for its first stage of the next one before the waves
+// meet, V only where its tiles are not what they meet in (APART); Q has come a piece
+// ahead. us, without and with it: 512 sequences of 900 tokens, 32/8 heads, d = 128, 8 bits
+// 204 and 186, 4 bits 150 and 128 (V after they met: 135); 64 of 2000-16384, 4 bits
+// 110 and 107; one of 4096, which has no next piece, 7.0 and 7.7: a batch of one does
+// without (`one`), and beside the many-row form's registers it brought nothing.
+template <class F, class T, int NW, bool AHEAD>
+__device__ __forceinline__ void mx_few_body(const BatchParams &p, int group, MxFewSmem<F, T, NW, AHEAD> &sm) {
     using Stage = MxStage<F>;
     constexpr int D = F::D, XT = D / 16, ROWS = kBatchFew, NL = Stage::LOADS;
+    constexpr bool APART = MxFewSmem<F, T, NW, AHEAD>::APART;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     const char *K = static_cast<const char *>(p.k), *V = static_cast<const char *>(p.v);
-    const int Nk = it.s.keys;
-    const MxRows<F> rows(p, it, Nk);
     const bool runs = (1 << p.bs_shift) >= Stage::ROWS;
-    auto &t = sm.t[wave];
+    auto &t = sm.keys[wave];
+    auto &values = sm.end.values;
 
-    // stage `st` is the wave's n-th: its blocks in buffer n & 1
-    auto fetch = [&](int st, int n) __attribute__((always_inline)) {
-        lds_dma4(lds_addr(t.blk[n & 1]), rows.rows.table + rows.rows.block_at(min(st, s_hi - 1) * 64 + lane));
+    // the blocks of stage `st` of a piece that ends before stage `hi`
+    auto fetch = [&](int *to, const BatchItem &of, int st, int hi) __attribute__((always_inline)) {
+        const MxRows<F> rows(p, of, of.s.keys);
+        lds_dma4(lds_addr(to), rows.rows.table + rows.rows.block_at(min(st, hi - 1) * 64 + lane));
     };
-    auto load_k = [&](int st, int n) __attribute__((always_inline)) {
-        Stage::load(t.k, t.ke, K, rows, t.blk[n & 1], st * 64, lane, runs, mx_kswz<F>);
+    auto load_k = [&](const BatchItem &of, int st, const int *blk) __attribute__((always_inline)) {
+        Stage::load(t.k, t.e, K, MxRows<F>(p, of, of.s.keys), blk, st * 64, lane, runs, mx_kswz<F>);
     };
-    auto load_v = [&](int st, int n) __attribute__((always_inline)) {
-        Stage::load(t.v, t.ve, V, rows, t.blk[n & 1], st * 64, lane, runs, mx_vswz<F>);
+    auto load_v = [&](const BatchItem &of, int st, const int *blk) __attribute__((always_inline)) {
+        Stage::load(values.v[wave], values.e[wave], V, MxRows<F>(p, of, of.s.keys), blk, st * 64, lane, runs, mx_vswz<F>);
     };
-    int st = s_lo + wave, n = 0;
-    if (st < s_hi) fetch(st, 0);
-    const int row = min(l16, it.s.rows - 1);
-    const int qpos = it.s.pos + row / p.group;
+    auto load_q = [&](typename MxOperand<T>::B (&to)[D / 32], const BatchItem &of) __attribute__((always_inline)) {
+        return mx_row<F, T>(to, static_cast<const T *>(p.q) + batch_elem(p, of, min(l16, of.s.rows - 1), p.q_rs, D), g);
+    };
+
+    FewRun run(p, group);
+    BatchItem it = run.item(), nx = it;
+    FewPiece f, nf;
+    if (!run.next(it, f)) return;
     typename MxOperand<T>::B qf[D / 32];
-    const bool low = mx_row<F, T>(qf, static_cast<const T *>(p.q) + batch_elem(p, it, row, p.q_rs, D), g);
-    if (st < s_hi) {
-        wait_loads<0>();
-        fetch(st + NW, 1);
-        load_k(st, 0);
-        load_v(st, 0);
-    }
-    f32x4 acc[XT];
-#pragma unroll
-    for (int xt = 0; xt < XT; ++xt) acc[xt] = zero4();
-    float m = -INFINITY, lsum = 0.f;
-    unsigned most = 0;
-    // stages before `whole` hold no key that a row does not see
-    const int whole = min(Nk, it.s.pos + 1) / 64;
-    // The wave's next stage: its K goes out once this one's K has been read, with the
-    // blocks of the stage after it, and its V once this one's V has. vmcnt counts in
-    // order: NL loads (this stage's V) follow K, NL + 1 (the blocks and the next K)
-    // follow V. A second buffer for each, with both in flight all the time, was slower (64
-    // sequences, 4 bits: 124 us and 115): the reads are not what waits.
-    auto stage = [&](auto first, auto mask) __attribute__((always_inline)) {
-        const bool more = st + NW < s_hi;
-        wait_loads<NL>();
-        auto after_k = [&]() __attribute__((always_inline)) {
-            wait_lds();
-            if (more) {
-                fetch(st + 2 * NW, n);  // (this stage's blocks: its V is out already)
-                load_k(st + NW, n + 1);
-            }
-        };
-        auto before_v = [&]() __attribute__((always_inline)) {
-            if (more) {
-                wait_loads<NL + 1>();
-            } else {
-                wait_loads<0>();
-            }
-        };
-        const int lim = min(qpos, Nk - 1) - st * 64 - 16 * g;
-        mx_few_stage<F, T, decltype(first)::value, decltype(mask)::value>(acc, m, lsum, most, qf, t.k, t.ke, t.v, t.ve, t.vp,
-                                                                          lim, lane, p.scale_log2, after_k, before_v);
-        wait_lds();
-        if (more) load_v(st + NW, n + 1);
-        st += NW;
-        ++n;
+    bool low;
+    auto begin = [&]() __attribute__((always_inline)) {
+        if (f.lo + wave < f.hi) fetch(t.first, it, f.lo + wave, f.hi);
+        low = load_q(qf, it);
+        mx_arrived<T>(qf);
+        if (f.lo + wave < f.hi) {
+            wait_loads<0>();
+            fetch(t.blk[1], it, f.lo + wave + NW, f.hi);
+            load_k(it, f.lo + wave, t.first);
+            load_v(it, f.lo + wave, t.first);
+        }
     };
-    using std::false_type;
-    using std::true_type;
-    if (st < s_hi) stage(true_type{}, true_type{});
-    while (st < min(s_hi, whole)) stage(false_type{}, false_type{});
-    while (st < s_hi) stage(false_type{}, true_type{});
-    const float lw = xg_sum(lsum);
-    float z = 0.f * lw;
+    if (AHEAD) begin();
+    for (;;) {
+        if (!AHEAD) begin();
+        const bool other = AHEAD && run.next(nx, nf), ahead = other && nf.lo + wave < nf.hi;
+        const int s_hi = f.hi, Nk = it.s.keys;
+        int st = f.lo + wave, n = 0;
+        const int qpos = it.s.pos + min(l16, it.s.rows - 1) / p.group;
+        f32x4 acc[XT];
 #pragma unroll
-    for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt]);
-    const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f || most > kMxMost) != 0 || low;
-    batch_few_finish<T, D, NW, 64 * NW>(
-        p, it, slot, sm.merge, m, lw, bad,
-        [&](int i) __attribute__((always_inline)) { return acc[i] * MxOperand<T>::kDown; },
-        [&](int i) __attribute__((always_inline)) { return 16 * i + 4 * g; },
-        [&](float *part, float *ml) __attribute__((always_inline)) {
-            batch_plain<T, D, ROWS, MxPlainRows<F>>(p, it, 0, s_lo * 64, s_hi * 64, part, ml);
-        });
-}
-template <class F, class T, int NW>
-__device__ __forceinline__ void mx_few_body(const BatchParams &p, int g, MxFewSmem<F, T, NW> &sm) {
-    batch_few_run(p, g, [&](const BatchItem &it, int lo, int hi, int slot) __attribute__((always_inline)) {
-        mx_few_piece<F, T, NW>(p, it, lo, hi, slot, sm);
-    });
+        for (int xt = 0; xt < XT; ++xt) acc[xt] = zero4();
+        float m = -INFINITY, lsum = 0.f;
+        unsigned most = 0;
+        // stages before `whole` hold no key that a row does not see
+        const int whole = min(Nk, it.s.pos + 1) / 64;
+        // what the next piece begins with
+        typename MxOperand<T>::B qn[D / 32];
+        bool lown = false;
+        auto next_up = [&]() __attribute__((always_inline)) {
+            if (ahead) fetch(t.first, nx, nf.lo + wave, nf.hi);
+            if (other) lown = load_q(qn, nx);
+        };
+        // The wave's next stage: its K goes out once this one's K has been read, with the
+        // blocks of the stage after it, and its V once this one's V has; the blocks of the n-th
+        // are in blk[n & 1], of the first in `first`. vmcnt counts in order: NL loads (this stage's
+        // V) follow K, NL + 1 (the blocks and the next K) follow V;
+        // what else goes out in a piece's first stage only makes these waits longer.
+        auto stage = [&](auto first, auto mask) __attribute__((always_inline)) {
+            const bool more = st + NW < s_hi;
+            wait_loads<NL>();
+            auto after_k = [&]() __attribute__((always_inline)) {
+                wait_lds();
+                if (decltype(first)::value) next_up();
+                if (more) {
+                    fetch(t.blk[n & 1], it, st + 2 * NW, s_hi);  // (this stage's: its V is out already)
+                    load_k(it, st + NW, t.blk[(n + 1) & 1]);
+                }
+            };
+            auto before_v = [&]() __attribute__((always_inline)) {
+                if (more) {
+                    wait_loads<NL + 1>();
+                } else {
+                    wait_loads<0>();
+                }
+            };
+            const int lim = min(qpos, Nk - 1) - st * 64 - 16 * g;
+            mx_few_stage<F, T, decltype(first)::value, decltype(mask)::value>(
+                acc, m, lsum, most, qf, t.k, t.e, values.v[wave], values.e[wave], values.power[wave], lim, lane, p.scale_log2,
+                after_k, before_v);
+            wait_lds();
+            if (more) load_v(it, st + NW, t.blk[(n + 1) & 1]);
+            st += NW;
+            ++n;
+        };
+        using std::false_type;
+        using std::true_type;
+        if (st < s_hi) {
+            stage(true_type{}, true_type{});
+        } else {
+            next_up();
+            if constexpr (AHEAD) mx_arrived<T>(qn);
+        }
+        while (st < min(s_hi, whole)) stage(false_type{}, false_type{});
+        while (st < s_hi) stage(false_type{}, true_type{});
+
+        if constexpr (AHEAD) mx_arrived<T>(qn);
+        if (ahead) {
+            wait_loads<0>();
+            fetch(t.blk[1], nx, nf.lo + wave + NW, nf.hi);
+            load_k(nx, nf.lo + wave, t.first);
+            if constexpr (APART) load_v(nx, nf.lo + wave, t.first);
+        }
+        const float lw = xg_sum(lsum);
+        float z = 0.f * lw;
+#pragma unroll
+        for (int xt = 0; xt < XT; ++xt) z += zero_of(acc[xt]);
+        const bool bad = __builtin_amdgcn_ballot_w64(z != 0.f || most > kMxMost) != 0 || low;
+        batch_few_finish<T, D, NW, 64 * NW>(
+            p, it, f.slot, sm.end.merge, m, lw, bad,
+            [&](int i) __attribute__((always_inline)) { return acc[i] * MxOperand<T>::kDown; },
+            [&](int i) __attribute__((always_inline)) { return 16 * i + 4 * g; },
+            [&](float *part, float *ml) __attribute__((always_inline)) {
+                batch_plain<T, D, ROWS, MxPlainRows<F>>(p, it, 0, f.lo * 64, f.hi * 64, part, ml);
+            });
+        if constexpr (AHEAD) {
+            if (!other) return;
+            if constexpr (!APART) {
+                barrier_lds();  // V's tiles are where the waves met
+                if (ahead) load_v(nx, nf.lo + wave, t.first);
+            }
+            it = nx;
+            f = nf;
+            low = lown;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) qf[c] = qn[c];
+        } else {
+            if (!run.next(it, f)) return;
+            barrier_lds();
+        }
+    }
 }
 
 // ----------------------------------------------------------------- the many rows
@@ -677,20 +766,20 @@ __device__ __forceinline__ void mx_many_body(const BatchParams &p, int block, Mx
 template <class F, class T, int QT, int NW>
 __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_groups) {
     __shared__ __attribute__((aligned(16))) union {
-        MxFewSmem<F, T, NW> few;
+        MxFewSmem<F, T, NW, false> few;
         MxManySmem<F::D, NW> many;
     } sm;
     if ((int)blockIdx.x < few_groups) {
-        mx_few_body<F, T, NW>(p, blockIdx.x, sm.few);
+        mx_few_body<F, T, NW, false>(p, blockIdx.x, sm.few);
     } else {
         mx_many_body<F, T, QT, NW>(p, (int)blockIdx.x - few_groups, sm.many);
     }
 }
 
-#define MXFA_BATCH_MX_FEW(NAME, BITS, D, T)                                                                  \
-    extern "C" __global__ __launch_bounds__(64 * kMxFewWaves) void mxfa_batch_##NAME##_few(BatchParams p) {  \
-        __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, T, kMxFewWaves> sm;                   \
-        mx_few_body<Mx<BITS, D>, T, kMxFewWaves>(p, blockIdx.x, sm);                                         \
+#define MXFA_BATCH_MX_FEW(NAME, BITS, D, T, AHEAD)                                                           \
+    extern "C" __global__ __launch_bounds__(64 * kMxFewWaves) void mxfa_batch_##NAME(BatchParams p) {        \
+        __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, T, kMxFewWaves, AHEAD> sm;            \
+        mx_few_body<Mx<BITS, D>, T, kMxFewWaves, AHEAD>(p, blockIdx.x, sm);                                  \
     }
 #define MXFA_BATCH_MX_MANY(MANY, BOTH, BITS, D, T, QT, NW, WPS, BOTH_WPS)                                    \
     extern "C" __global__ __launch_bounds__(64 * NW, WPS) void mxfa_batch_##MANY(BatchParams p) {            \
@@ -701,13 +790,16 @@ __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_group
         mx_both_body<Mx<BITS, D>, T, QT, NW>(p, few_groups);                                                 \
     }
 #define MXFA_BATCH_MX(BITS)                                                                                  \
-    MXFA_BATCH_MX_FEW(x##BITS##b64, BITS, 64, u16)                                                           \
+    MXFA_BATCH_MX_FEW(x##BITS##b64_few, BITS, 64, u16, true)                                                 \
+    MXFA_BATCH_MX_FEW(x##BITS##b64_one, BITS, 64, u16, false)                                                \
     MXFA_BATCH_MX_MANY(x##BITS##b64_many, x##BITS##b64_both, BITS, 64, u16, 2, 4, 3, 3)                      \
     MXFA_BATCH_MX_MANY(x##BITS##b64_many64, x##BITS##b64_both64, BITS, 64, u16, 1, 4, 4, 3)                  \
-    MXFA_BATCH_MX_FEW(x##BITS##b128, BITS, 128, u16)                                                         \
+    MXFA_BATCH_MX_FEW(x##BITS##b128_few, BITS, 128, u16, true)                                               \
+    MXFA_BATCH_MX_FEW(x##BITS##b128_one, BITS, 128, u16, false)                                              \
     MXFA_BATCH_MX_MANY(x##BITS##b128_many, x##BITS##b128_both, BITS, 128, u16, 2, 4, 2, 2)                   \
     MXFA_BATCH_MX_MANY(x##BITS##b128_many64, x##BITS##b128_both64, BITS, 128, u16, 1, 4, 2, 2)               \
-    MXFA_BATCH_MX_FEW(x##BITS##f64, BITS, 64, float)                                                         \
+    MXFA_BATCH_MX_FEW(x##BITS##f64_few, BITS, 64, float, true)                                               \
+    MXFA_BATCH_MX_FEW(x##BITS##f64_one, BITS, 64, float, false)                                              \
     MXFA_BATCH_MX_MANY(x##BITS##f64_many, x##BITS##f64_both, BITS, 64, float, 1, kBatchF32Waves, 4, 4)
 MXFA_BATCH_MX(8)
 MXFA_BATCH_MX(4)

@@ -49,12 +49,12 @@
     X(mxfa_batch_b64_many64) X(mxfa_batch_b64_both64) X(mxfa_batch_b128_many64) X(mxfa_batch_b128_both64)             \
     X(mxfa_batch_f64_few) X(mxfa_batch_f64_many) X(mxfa_batch_f64_join) X(mxfa_batch_f64_both)                       \
     /* attention of a batch over a microscaled cache (fa_batch_mx.hip): x8 or x4, then the type and head dim */ \
-    X(mxfa_batch_x8b64_few) X(mxfa_batch_x8b64_many) X(mxfa_batch_x8b64_both) X(mxfa_batch_x8b64_many64) X(mxfa_batch_x8b64_both64) \
-    X(mxfa_batch_x8b128_few) X(mxfa_batch_x8b128_many) X(mxfa_batch_x8b128_both) X(mxfa_batch_x8b128_many64) X(mxfa_batch_x8b128_both64) \
-    X(mxfa_batch_x8f64_few) X(mxfa_batch_x8f64_many) X(mxfa_batch_x8f64_both) \
-    X(mxfa_batch_x4b64_few) X(mxfa_batch_x4b64_many) X(mxfa_batch_x4b64_both) X(mxfa_batch_x4b64_many64) X(mxfa_batch_x4b64_both64) \
-    X(mxfa_batch_x4b128_few) X(mxfa_batch_x4b128_many) X(mxfa_batch_x4b128_both) X(mxfa_batch_x4b128_many64) X(mxfa_batch_x4b128_both64) \
-    X(mxfa_batch_x4f64_few) X(mxfa_batch_x4f64_many) X(mxfa_batch_x4f64_both) \
+    X(mxfa_batch_x8b64_few) X(mxfa_batch_x8b64_one) X(mxfa_batch_x8b64_many) X(mxfa_batch_x8b64_both) X(mxfa_batch_x8b64_many64) X(mxfa_batch_x8b64_both64) \
+    X(mxfa_batch_x8b128_few) X(mxfa_batch_x8b128_one) X(mxfa_batch_x8b128_many) X(mxfa_batch_x8b128_both) X(mxfa_batch_x8b128_many64) X(mxfa_batch_x8b128_both64) \
+    X(mxfa_batch_x8f64_few) X(mxfa_batch_x8f64_one) X(mxfa_batch_x8f64_many) X(mxfa_batch_x8f64_both) \
+    X(mxfa_batch_x4b64_few) X(mxfa_batch_x4b64_one) X(mxfa_batch_x4b64_many) X(mxfa_batch_x4b64_both) X(mxfa_batch_x4b64_many64) X(mxfa_batch_x4b64_both64) \
+    X(mxfa_batch_x4b128_few) X(mxfa_batch_x4b128_one) X(mxfa_batch_x4b128_many) X(mxfa_batch_x4b128_both) X(mxfa_batch_x4b128_many64) X(mxfa_batch_x4b128_both64) \
+    X(mxfa_batch_x4f64_few) X(mxfa_batch_x4f64_one) X(mxfa_batch_x4f64_many) X(mxfa_batch_x4f64_both) \
     /* its append and its read (fa_mx.hip) */ \
     X(mxfa_append_x8b) X(mxfa_append_x8b1) X(mxfa_append_x8f) X(mxfa_append_x8f1) X(mxfa_read_x8b) X(mxfa_read_x8f) \
     X(mxfa_append_x4b) X(mxfa_append_x4b1) X(mxfa_append_x4f) X(mxfa_append_x4f1) X(mxfa_read_x4b) X(mxfa_read_x4f) \

@@ -94,6 +94,28 @@ def test_many_sequences(n_seq, bits):
 
 
 @pytest.mark.parametrize("bf16,hd,bits", TYPES)
+@pytest.mark.parametrize("bs", [4, 64])
+def test_short_sequences_in_one_run(bs, bf16, hd, bits):
+    """Some ten sequences to a work-group, of fewer stages than it has waves and of more,
+    of none, and of one whose K is NaN: the others' bits stay."""
+    g = torch.Generator().manual_seed(bs)
+    lens = torch.randint(0, 9, (300,), generator=g) ** 3 + torch.randint(0, 90, (300,), generator=g)
+    pairs = [(1 + i % 2, max(int(n), 1 + i % 2)) if i % 7 else (1, 0) for i, n in enumerate(lens)]
+    b = MxBatch(pairs, 16, 8, hd, bs, bits, bf16, seed=bs)
+    out, lse = run(b)
+    check(b, out, lse)
+    # (the 150th, KV head 3, its first token)
+    ke = parts(b.kp, 8, bs, hd, bits)[1]
+    at = int(b.rows[150][0])
+    ke[at // bs, 3, at % bs] = 255
+    got, lse2 = run(b)
+    t0 = sum(n for n, _ in pairs[:150])
+    hit = torch.zeros(out.shape, dtype=torch.bool)
+    hit[t0:t0 + pairs[150][0], 6 * hd:8 * hd] = True
+    assert bool(torch.isnan(got[hit]).all()) and torch.equal(got[~hit], out[~hit])
+
+
+@pytest.mark.parametrize("bf16,hd,bits", TYPES)
 def test_rows_that_see_nothing(bf16, hd, bits):
     b = MxBatch([(0, 50), (3, 0), (5, 2), (0, 0), (40, 10), (2, 90)], 4, 2, hd, 16, bits, bf16, seed=3, extra_rows=6, wide=3)
     out, lse = run(b)
