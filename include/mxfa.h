@@ -505,7 +505,8 @@ size_t mxfa_mx_block_bytes(int block_size, int n_kv_head, int head_dim, int bits
  * the types' range). 32 elements of which one is not finite get E = 255 and
  * read back as NaN. K turns in 64 bits, rounded to 32, so equal tokens get equal
  * codes whatever computes them; factor is one of 64 bits for that. head_dim: a
- * multiple of 32, at most 256. */
+ * multiple of 32, at most 256. The caches must not lie over each other, qkv or q_out
+ * (MXFA_ERR_UNSUPPORTED); they may be columns of the same wider rows. */
 typedef struct {
     int rotary_dim, interleaved;
     double factor;

@@ -1047,7 +1047,8 @@ def _batch_args(q, q_cols, kcache, vcache, out, block_table, block_size, cu_q, l
     n_blocks = kcache.shape[0] // least
     _c_int(n_tok=n_tok, n_blocks=n_blocks, table_stride=ts, q_stride=qs, kv_stride=ks,
            out_stride=os_)
-    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, n_blocks, wide, ts, qs, ks, os_, MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, block_size, n_blocks, wide, ts, qs, ks, os_,
+                        MXFA_BF16 if q.dtype == torch.bfloat16 else MXFA_F32, scale)
     return sh, qp, kp, vp, op, tp, cp, lp
 
 

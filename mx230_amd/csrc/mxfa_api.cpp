@@ -834,8 +834,9 @@ int run_attention(const mxfa_batch_shape *s, int bits, long long pool, long long
     };
     const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, qw = esz * s->n_head * s->head_dim;
     const long long lw = lse == nullptr ? 0 : 4LL * s->n_tok * s->n_head;
-    const Rows all[] = {{q, s->q_stride * esz, qw, s->n_tok}, {kcache, ks, kw, pool}, {vcache, ks, kw, pool}, {out, s->out_stride * esz, qw, s->n_tok},
-                        {lse, lw, lw, 1}, {workspace, (long long)need, (long long)need, 1}};
+    const Rows all[] = {{q, s->q_stride * esz, qw, s->n_tok}, {kcache, ks, kw, pool}, {vcache, ks, kw, pool},
+                        {out, s->out_stride * esz, qw, s->n_tok}, {lse, lw, lw, 1},
+                        {workspace, (long long)need, (long long)need, 1}};
     if (rows_collide(out, s->out_stride * esz, qw, q, s->q_stride * esz, qw, s->n_tok)) return MXFA_ERR_UNSUPPORTED;
     for (int w = 3; w < 6; ++w) {
         for (int r = w == 3 ? 1 : 0; r < w; ++r) {  // (out over q: above)
@@ -956,6 +957,14 @@ int mxfa_run_cache_append_mx(const mxfa_batch_shape *s, int bits, const mxfa_app
     const long long esz = s->dtype == MXFA_BF16 ? 2 : 4, row = esz * s->head_dim;
     if (rows_collide(q_out, s->out_stride * esz, s->n_head * row, qkv, s->q_stride * esz, heads * row, s->n_tok))
         return MXFA_ERR_UNSUPPORTED;
+    const long long bytes = (long long)mxfa_mx_block_bytes(s->block_size, s->n_kv_head, s->head_dim, bits);
+    if (rows_meet(kcache, s->kv_stride, bytes, s->n_blocks, vcache, s->kv_stride, bytes, s->n_blocks))
+        return MXFA_ERR_UNSUPPORTED;
+    for (const void *c : {static_cast<const void *>(kcache), static_cast<const void *>(vcache)}) {
+        if (rows_meet(qkv, s->q_stride * esz, heads * row, s->n_tok, c, s->kv_stride, bytes, s->n_blocks) ||
+            rows_meet(q_out, s->out_stride * esz, s->n_head * row, s->n_tok, c, s->kv_stride, bytes, s->n_blocks))
+            return MXFA_ERR_UNSUPPORTED;
+    }
     mxfa::BatchParams p = batch_params(s, qkv, kcache, vcache, q_out, block_table, cu_q, lens);
     p.bits = bits;
     p.freq = r->frequencies;

@@ -233,3 +233,32 @@ def test_lengths_and_blocks_of_any_kind(bs, entries, bits):
                 rows = [int(table[0, p // bs]) * bs + p % bs for p in (38, 39)]
                 assert not own or torch.equal(k[:2].cpu().double(), held(k2.cpu(), rows, 2, bs, 64, bits))
     assert math.isfinite(float(sound.float().sum()))
+
+
+@pytest.mark.parametrize("bf16,hd,bits", [(True, 64, 8), (True, 128, 4), (False, 64, 4)])
+def test_pools_in_one_tensor(bf16, hd, bits):
+    """K's and V's blocks as columns of the same wider rows: the bytes and the results of
+    pools that lie apart, and nothing else touched; over each other they are refused."""
+    nh, nkv, bs, pairs = 6, 2, 16, [(5, 70), (1, 1), (40, 40), (1, 900)]
+    b = MxBatch(pairs, nh, nkv, hd, bs, bits, bf16, seed=hd)
+    kp, vp, table, cu, lens, qkv = b.cuda("kp", "vp", "table", "cu_q", "lens", "qkv")
+    wide = kp.shape[1]
+    both = torch.full((kp.shape[0], 2 * wide + 48), 0x5a, dtype=torch.uint8, device="cuda")
+    k2, v2 = both[:, 16:16 + wide], both[:, 32 + wide:32 + 2 * wide]
+    k2.copy_(kp)
+    v2.copy_(vp)
+    got = []
+    for k, v in ((kp, vp), (k2, v2)):
+        q, out = (torch.zeros(b.n_tok, nh * hd, dtype=b.dt, device="cuda") for _ in range(2))
+        ko, vo = (torch.zeros(b.n_tok, nkv * hd, dtype=b.dt, device="cuda") for _ in range(2))
+        mx.run_cache_append_mx(qkv, q, k, v, bits, table, bs, cu, lens, nh, nkv, hd)
+        mx.run_prefill_batch_mx(q, k, v, bits, out, table, bs, cu, lens, b.max_q, nh, nkv, hd)
+        mx.run_cache_read_mx(k, v, bits, ko, vo, table, bs, cu, lens, nkv, hd)
+        got.append((q, out, ko, vo))
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and bool(got[0][1].any())
+    assert torch.equal(k2, kp) and torch.equal(v2, vp)
+    for c in (slice(0, 16), slice(16 + wide, 32 + wide), slice(32 + 2 * wide, None)):
+        assert bool((both[:, c] == 0x5a).all())
+    for v in (kp, kp[1:], k2):
+        with pytest.raises((mx.MxfaError, ValueError)):
+            mx.run_cache_append_mx(qkv, q, k2 if v is k2 else kp, v, bits, table, bs, cu, lens, nh, nkv, hd)

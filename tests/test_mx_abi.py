@@ -88,9 +88,9 @@ def test_append_and_read_buffers(lib, bits):  # noqa: F811
     f = ctypes.c_void_p(4096)
     run = lib.mxfa_run_cache_append_mx
 
-    def append(rot=(64, 0, 1.0, f), q_out=p[1], qkv=p[0], k=p[2], sh=s):
+    def append(rot=(64, 0, 1.0, f), q_out=p[1], qkv=p[0], k=p[2], sh=s, v=p[3]):
         r = mx.MxfaAppendRotaryMx(*rot)
-        return run(ctypes.byref(sh), bits, ctypes.byref(r), qkv, q_out, k, p[3], P, P, P, None)
+        return run(ctypes.byref(sh), bits, ctypes.byref(r), qkv, q_out, k, v, P, P, P, None)
     assert append(rot=(64, 0, 1.0, None)) == NULL and append(rot=(66, 0, 1.0, f)) == SHAPE
     assert append(rot=(7, 0, 1.0, f)) == UNSUPPORTED and append(rot=(64, 2, 1.0, f)) == SHAPE
     for x in (math.inf, math.nan, 1e300):
@@ -98,6 +98,10 @@ def test_append_and_read_buffers(lib, bits):  # noqa: F811
     assert append(rot=(64, 0, 1.0, ctypes.c_void_p(4100))) == ALIGN
     assert append(q_out=None) == NULL and append(k=ctypes.c_void_p(FAR[2] + 4)) == ALIGN
     assert append(q_out=ctypes.c_void_p(FAR[0] + 512)) == UNSUPPORTED  # over K's columns
+    for at in (FAR[2], FAR[2] + w // 32 * 16, FAR[2] + 9 * w + 16):  # V, q_out or qkv over K
+        assert append(v=ctypes.c_void_p(at)) == UNSUPPORTED and append(q_out=ctypes.c_void_p(at)) == UNSUPPORTED
+        assert append(qkv=ctypes.c_void_p(at)) == UNSUPPORTED
+    assert append(q_out=ctypes.c_void_p(FAR[3] + 16)) == UNSUPPORTED
     assert append(sh=shape(bits, q_stride=256)) == SHAPE and append(sh=shape(bits, kv_stride=w - 16)) == SHAPE
     assert append(sh=shape(bits, head_dim=48, kv_stride=4096)) == UNSUPPORTED
 
