@@ -15,9 +15,9 @@
 //
 // Measured (us, as in fa_batch.hip; in brackets the ordinary cache, bf16 or fp32):
 //   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: in 8 bits
-//         198 and the join 5 (1.11 GB, 5.6 TB/s), in 4 bits 108 and 5 (0.57 GB, 5.3
+//         195 and the join 5 (1.11 GB, 5.7 TB/s), in 4 bits 107 and 5 (0.57 GB, 5.4
 //         TB/s: a head's 64 bytes of E come as whole lines, 6% more) [391 and 6]; d =
-//         64 122 and 80 in all [248]; fp32 43 and 40 [125]; 512 sequences of 900, d = 128
+//         64 120 and 77 in all [248]; fp32 43 and 40 [125]; 512 sequences of 900, d = 128
 //         186 and 128 in all;
 //         24 sequences of 1 to 4 tokens, to 8192 long, d = 128, 8 bits: 46 and 5;
 //   many: the last 2048 tokens of 32768, 32/8 heads, d = 128, 4 bits: 955 [950]; 1000
@@ -408,6 +408,16 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
     }
 }
 
+// Which of the form's `n` work-groups a block of a launch of its own is: each XCD (blocks 8
+// apart) has them one after another, so the heads of a run, whose E share lines, share
+// an L2. us, 64 sequences of 2000-16384, 32/8 heads, in order and so: d = 128, 4 bits 109 and 107,
+// 8 bits 198 and 195; d = 64 79.6 and 78, 122.7 and 120.8. Beside the many-row form, where they
+// would crowd some XCDs, in order (fp32, 6 tokens and 2 chunks: 30.6 us and 38.5).
+__device__ __forceinline__ int mx_few_group(int block, int n) {
+    const int xcd = block & 7, each = n >> 3, more = n & 7;
+    return xcd * each + min(xcd, more) + (block >> 3);
+}
+
 // A work-group's run of pieces, as batch_few_piece: their loads and waits. AHEAD: a wave
 // that is done with a piece sends for its first stage of the next one before the waves
 // meet, V only where its tiles are not what they meet in (APART); Q has come a piece
@@ -779,7 +789,7 @@ __device__ __forceinline__ void mx_both_body(const BatchParams &p, int few_group
 #define MXFA_BATCH_MX_FEW(NAME, BITS, D, T, AHEAD)                                                           \
     extern "C" __global__ __launch_bounds__(64 * kMxFewWaves) void mxfa_batch_##NAME(BatchParams p) {        \
         __shared__ __attribute__((aligned(16))) MxFewSmem<Mx<BITS, D>, T, kMxFewWaves, AHEAD> sm;            \
-        mx_few_body<Mx<BITS, D>, T, kMxFewWaves, AHEAD>(p, blockIdx.x, sm);                                  \
+        mx_few_body<Mx<BITS, D>, T, kMxFewWaves, AHEAD>(p, mx_few_group(blockIdx.x, gridDim.x), sm);         \
     }
 #define MXFA_BATCH_MX_MANY(MANY, BOTH, BITS, D, T, QT, NW, WPS, BOTH_WPS)                                    \
     extern "C" __global__ __launch_bounds__(64 * NW, WPS) void mxfa_batch_##MANY(BatchParams p) {            \
