@@ -16,9 +16,8 @@
 // Measured (us, as in fa_batch.hip; in brackets the ordinary cache, bf16 or fp32):
 //   few:  64 sequences of one token, 2000-16384 long, 32/8 heads, d = 128: in 8 bits
 //         195 and the join 5 (1.11 GB, 5.7 TB/s), in 4 bits 107 and 5 (0.57 GB, 5.4
-//         TB/s: a head's 64 bytes of E come as whole lines, 6% more) [391 and 6]; d =
-//         64 120 and 77 in all [248]; fp32 43 and 40 [125]; 512 sequences of 900, d = 128
-//         186 and 128 in all;
+//         TB/s, in pieces of 1 KB and 64 bytes) [391 and 6]; d = 64 120 and 77 in all
+//         [248]; fp32 43 and 40 [125]; 512 sequences of 900, d = 128 186 and 128 in all;
 //         24 sequences of 1 to 4 tokens, to 8192 long, d = 128, 8 bits: 46 and 5;
 //   many: the last 2048 tokens of 32768, 32/8 heads, d = 128, 4 bits: 955 [950]; 1000
 //         to 4000 tokens of short contexts 10 to 18% more than the ordinary cache: the
@@ -410,7 +409,8 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
 
 // Which of the form's `n` work-groups a block of a launch of its own is: each XCD (blocks 8
 // apart) has them one after another, so the heads of a run, whose E share lines, share
-// an L2. us, 64 sequences of 2000-16384, 32/8 heads, in order and so: d = 128, 4 bits 109 and 107,
+// an L2: 610 MB read and 574 (4 bits, d = 128), which is what it needs. us, 64
+// sequences of 2000-16384, 32/8 heads, in order and so: d = 128, 4 bits 109 and 107,
 // 8 bits 198 and 195; d = 64 79.6 and 78, 122.7 and 120.8. Beside the many-row form, where they
 // would crowd some XCDs, in order (fp32, 6 tokens and 2 chunks: 30.6 us and 38.5).
 __device__ __forceinline__ int mx_few_group(int block, int n) {
