@@ -92,23 +92,28 @@ struct MxPlainRows {
 // bf16 and (three parts) fp32.
 //
 // bf16: the powers multiply p after it is rounded, by adding to its exponent, two
-// keys at a time: (p + (E << 7)) - (127 << 7) in 16 bits, 0 where that is negative (the
-// result would be below 2^-126). p = 0 becomes 2^(E - 254), as good as 0 beside V's
+// keys at a time: (p + (E + kMxUp << 7)) - (127 << 7) in 16 bits, 0 where that is
+// negative. The sums are held 2^kMxUp times their size (kDown): what is left out is then
+// less than 2^-126 2^-kMxUp times a code, 2^9 at most, and so less than 2^-126 in all over
+// the 2^31 keys that there can be. (Without that, weights below 2^-9 of the running maximum
+// were lost with V near 2^-112.) p = 0 becomes 2^(E - 254), as good as 0 beside V's
 // 2^(E - 127), but not for a key that the row does not see: stages that hold such
-// multiply in fp32. With E up to kMxMost no sum passes 16 bits; a piece that met a larger
-// one (V above 2^63, or NaN) runs in plain arithmetic.
-constexpr unsigned kMxMost = 190;
+// multiply in fp32. With E up to kMxMost no result's exponent passes 254 - 8 (p is at most
+// kLazySum); a piece that met a larger one (V above 2^63, or NaN) or whose sums
+// overflow runs in plain arithmetic.
+constexpr unsigned kMxMost = 190, kMxUp = 40;
 template <class T>
 struct MxOperand;
 template <>
 struct MxOperand<u16> {
     using B = bf16x8;
     using Power = u16;
-    static constexpr float kDown = 1.f;
+    static constexpr float kDown = 0x1p-40f;
+    static_assert(kDown * (float)(1ull << kMxUp) == 1.0f && 16 + kMxMost + kMxUp < 255);
     struct Packed {
         u32x4 w[2];  // keys 2 i, 2 i + 1 in word i
     };
-    __device__ static __forceinline__ Power power(unsigned E) { return (u16)(E << 7); }
+    __device__ static __forceinline__ Power power(unsigned E) { return (u16)((E + kMxUp) << 7); }
     __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) { return PolBF16<64>::mma(a, b, c); }
     __device__ static __forceinline__ Packed prepare(const f32x4 (&p)[4]) {
         return Packed{{__builtin_bit_cast(u32x4, PolBF16<64>::pack(p[0], p[1])), __builtin_bit_cast(u32x4, PolBF16<64>::pack(p[2], p[3]))}};
