@@ -289,8 +289,9 @@ struct MxStage {
 // (g, l16) holds the scores of keys 16 g .. 16 g + 15 of row l16, in order: the 16
 // keys whose codes a transposing read of V brings it. p is relative to the running
 // m, which rises only where a lane's sum of p passes kLazySum (fwd_stage_lazy's
-// reasons), is above 0 while m is still -infinity, or at the wave's FIRST stage. most:
-// the largest E of V so far.
+// reasons), at the wave's FIRST stage, or while m is -infinity for some row: where every
+// score so far overflowed to that, the next may be finite and yet so low that p relative to
+// 0 is 0. most: the largest E of V so far.
 template <class F, class T, bool FIRST, bool MASK, class AfterK, class BeforeV>
 __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, float &lsum, unsigned &most,
                                              const typename MxOperand<T>::B (&qf)[F::D / 32], const char *sk,
@@ -366,7 +367,7 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
     } else {
         const bool none = m == -INFINITY;  // no key seen, or every score so far -infinity
         const float ls = exps(none ? 0.f : m);
-        if (__builtin_amdgcn_ballot_w64(ls > (none ? 0.f : kLazySum)) != 0) {
+        if (__builtin_amdgcn_ballot_w64(none || ls > kLazySum) != 0) {
             raise();
         } else {
             lsum += ls;
