@@ -92,14 +92,17 @@ struct MxPlainRows {
 // bf16 and (three parts) fp32.
 //
 // bf16: the powers multiply p after it is rounded, by adding to its exponent, two
-// keys at a time: (p + (E + kMxUp << 7)) - (127 << 7) in 16 bits, 0 where that is
-// negative. The sums are held 2^kMxUp times their size (kDown): what is left out is then
-// less than 2^-126 2^-kMxUp times a code, 2^9 at most, and so less than 2^-126 in all over
-// the 2^31 keys that there can be. (Without that, weights below 2^-9 of the running maximum
-// were lost with V near 2^-112.) p = 0 becomes 2^(E - 254), as good as 0 beside V's
-// 2^(E - 127), but not for a key that the row does not see: stages that hold such
-// multiply in fp32. With E up to kMxMost no result's exponent passes 254 - 8 (p is at most
-// kLazySum); a piece that met a larger one (V above 2^63, or NaN) or whose sums
+// keys at a time: p + (E + kMxUp - 127 << 7) in 16 bits, 0 where that is negative. The
+// sums are held 2^kMxUp times their size (kDown): what is left out is then less than
+// 2^-126 2^-kMxUp times a code, 2^9 at most, and so less than 2^-126 in all over the 2^31
+// keys that there can be. (Without that, weights below 2^-9 of the running maximum were lost
+// with V near 2^-112.) p = 0 has no exponent to add to: 2^-126 is taken from every p, which
+// makes a 0 the lowest integer, and so 0 with any power (whole calls in us, without, so,
+// and with a branch for where some p is 0: 64 sequences of 2000-16384, d = 128, 8 bits 201.6,
+// 201.5, 205.8, d = 64, 4 bits 75.0, 75.3, 77.4; 512 of 900, d = 128, 4 bits 127.6, 128.6,
+// 129.9). In stages that hold a key that a row does
+// not see all multiply in fp32. With E up to kMxMost no exponent passes 254 - 8 (p is at
+// most kLazySum); a piece that met a larger one (V above 2^63, or NaN) or whose sums
 // overflow runs in plain arithmetic.
 constexpr unsigned kMxMost = 190, kMxUp = 40;
 template <class T>
@@ -113,10 +116,14 @@ struct MxOperand<u16> {
     struct Packed {
         u32x4 w[2];  // keys 2 i, 2 i + 1 in word i
     };
-    __device__ static __forceinline__ Power power(unsigned E) { return (u16)((E + kMxUp) << 7); }
+    // EXACT: the power itself in bf16
+    template <bool EXACT>
+    __device__ static __forceinline__ Power power(unsigned E) { return (u16)((E + kMxUp - (EXACT ? 0 : 127)) << 7); }
     __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) { return PolBF16<64>::mma(a, b, c); }
     __device__ static __forceinline__ Packed prepare(const f32x4 (&p)[4]) {
-        return Packed{{__builtin_bit_cast(u32x4, PolBF16<64>::pack(p[0], p[1])), __builtin_bit_cast(u32x4, PolBF16<64>::pack(p[2], p[3]))}};
+        const float least = 0x1p-126f;
+        return Packed{{__builtin_bit_cast(u32x4, PolBF16<64>::pack(p[0] - least, p[1] - least)),
+                       __builtin_bit_cast(u32x4, PolBF16<64>::pack(p[2] - least, p[3] - least))}};
     }
     template <bool EXACT>
     __device__ static __forceinline__ void scaled(B (&f)[2], const Packed &pk, const f32x4 (&p)[4], const Power *power) {
@@ -134,8 +141,8 @@ struct MxOperand<u16> {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t a = pk.w[h][i], b = e[i];
-                    const u16x2 up = __builtin_bit_cast(u16x2, a) + __builtin_bit_cast(u16x2, b);
-                    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(up, u16x2{127 << 7, 127 << 7}));
+                    const i16x2 x = __builtin_elementwise_add_sat(__builtin_bit_cast(i16x2, a), __builtin_bit_cast(i16x2, b));
+                    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, i16x2{0, 0}));
                 }
                 f[h] = __builtin_bit_cast(B, r);
             }
@@ -149,6 +156,7 @@ struct MxOperand<float> {
     // p times a power of down to 2^-117 keeps its parts (kPartMin)
     static constexpr float kDown = kPartDown;
     struct Packed {};
+    template <bool>
     __device__ static __forceinline__ Power power(unsigned E) { return mx_power(E); }
     __device__ static __forceinline__ f32x4 mma(bf16x8 a, const B &b, f32x4 c) {
         c = PolBF16<64>::mma(a, b.l, c);
@@ -380,10 +388,11 @@ __device__ __forceinline__ void mx_few_stage(f32x4 (&acc)[F::D / 16], float &m, 
     for (int grp = 0; grp < F::SB; ++grp) {
         const unsigned E = (e >> (8 * grp)) & 255u;
         most = max(most, E);
-        vp[grp][lane] = Op::power(E);
+        vp[grp][lane] = Op::template power<MASK>(E);
     }
     wait_lds();
-    const typename Op::Packed pk = Op::prepare(pv);
+    typename Op::Packed pk;
+    if constexpr (!MASK) pk = Op::prepare(pv);
 #pragma unroll
     for (int grp = 0; grp < F::SB; ++grp) {
         typename Op::B pf[2];

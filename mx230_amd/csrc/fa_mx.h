@@ -45,7 +45,6 @@ __host__ __device__ inline MxHead mx_head(const BatchParams &p, int head) {
 #if defined(__HIP_DEVICE_COMPILE__)
 
 typedef short i16x2 __attribute__((ext_vector_type(2)));
-typedef u16 u16x2 __attribute__((ext_vector_type(2)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
