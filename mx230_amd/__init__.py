@@ -1082,12 +1082,17 @@ def run_cache_append(qkv, q_out, kcache, vcache, block_table, block_size: int, c
                                                     _stream(stream)))
 
 
+def _widest(n_seq):
+    """A table width in positions at which a batch's workspace is the largest: 2^17, where
+    every form has all its work-groups, or the widest that is taken of so many sequences."""
+    return max(min(1 << 17, 64 * ((1 << 31) // max(n_seq, 1) - 2)), 1)
+
+
 def prefill_batch_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head: int, n_kv_head: int, head_dim: int = 64,
                                   bf16: bool = True) -> int:
     """mxfa_prefill_batch_workspace_bytes: what run_prefill_batch needs for such a
     batch, whatever its lengths (0 for one it does not take)."""
-    # (a table of any width: at 2^17 positions every form has all its work-groups)
-    w, entries = n_head * head_dim, 1 << 17
+    w, entries = n_head * head_dim, _widest(n_seq)
     _c_int(n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, q_stride=w)
     sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w,
                         n_kv_head * head_dim, w, MXFA_BF16 if bf16 else MXFA_F32, 0.0)
@@ -1218,16 +1223,11 @@ def prefill_batch_mx_workspace_bytes(n_tok: int, n_seq: int, max_q: int, n_head:
                                      bf16: bool = True, bits: int = 8) -> int:
     """mxfa_prefill_batch_mx_workspace_bytes: what run_prefill_batch_mx needs for such a
     batch, whatever its lengths (0 for one it does not take)."""
-    w, lib, block = n_head * head_dim, load_library(), mx_block_bytes(1, n_kv_head, head_dim, bits)
+    w, entries, block = n_head * head_dim, _widest(n_seq), mx_block_bytes(1, n_kv_head, head_dim, bits)
     _c_int(n_tok=n_tok, n_seq=n_seq, max_q=max_q, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, q_stride=w)
-
-    def of(entries):
-        sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w, block, w,
-                            MXFA_BF16 if bf16 else MXFA_F32, 0.0)
-        return int(lib.mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(sh), bits))
-    # (tables of any width: the widest of short contexts, whose units may be smaller and
-    # their shares more, and 2^17 positions, at which every form has all its work-groups)
-    return max(of(64 * ((40 + max(min(max_q, n_tok), 0) // 64) // 2)), of(1 << 17))
+    sh = MxfaBatchShape(n_tok, n_seq, max_q, n_head, n_kv_head, head_dim, 1, 1, entries, entries, w, block, w,
+                        MXFA_BF16 if bf16 else MXFA_F32, 0.0)
+    return int(load_library().mxfa_prefill_batch_mx_workspace_bytes(ctypes.byref(sh), bits))
 
 
 def run_prefill_batch_mx(q, kcache, vcache, bits: int, out, block_table, block_size: int, cu_q, lens, max_q: int,

@@ -1188,13 +1188,18 @@ MXFA_BATCH_MANY(f64_many, f64_both, PolF32, FwdSplitSmem, 2, 64 * kBatchF32Waves
 #undef MXFA_BATCH
 #endif
 
+// Never less for a wider table: over a microscaled cache, where the width has a say in
+// the units' rows (batch_many_rows), what either size of them takes.
 size_t batch_workspace_bytes(const BatchParams &q, int dtype_bf16) {
-    BatchParams p = q;
-    BatchForm f[2];
-    batch_forms(&p, dtype_bf16, f);
-    size_t n = 0;
-    for (const BatchForm &x : f) n += batch_slot_floats(x.slots, x.rows, p.d) + (size_t)x.notes;
-    return std::max<size_t>(n * sizeof(float), 16);
+    auto with = [&](int many_rows) {
+        BatchParams p = q;
+        BatchForm f[2];
+        batch_forms(&p, dtype_bf16, f, many_rows);
+        size_t n = 0;
+        for (const BatchForm &x : f) n += batch_slot_floats(x.slots, x.rows, p.d) + (size_t)x.notes;
+        return std::max<size_t>(n * sizeof(float), 16);
+    };
+    return q.bits != 0 && dtype_bf16 ? std::max(with(64), with(128)) : with(0);
 }
 
 long long batch_groups(const BatchParams &q, int dtype_bf16) {

@@ -377,9 +377,10 @@ inline void batch_plan(BatchParams *p, int dtype_bf16) {
     p->per_item = dtype_bf16 ? 0.024f : 0.007f;
 }
 
-// The forms of a call; groups = 0: not launched.
-inline void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2]) {
+// The forms of a call; groups = 0: not launched. many_rows: 0, or other units than its own.
+inline void batch_forms(BatchParams *p, int dtype_bf16, BatchForm (&f)[2], int many_rows = 0) {
     batch_plan(p, dtype_bf16);
+    if (many_rows > 0) p->many_rows = many_rows;
     f[0] = f[1] = BatchForm{0, 0, 0, 0, 0};
     if (p->few_rows > 0) f[0] = batch_few_form(p);
     if (batch_may_be_many(*p)) f[1] = batch_many_form(p, dtype_bf16);
