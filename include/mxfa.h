@@ -486,7 +486,9 @@ int mxfa_run_cache_append(const mxfa_batch_shape *shape, const mxfa_append_rotar
 /* ---- A microscaled cache: the paged cache in 8 or 4 bits a value. Of each head's
  * row, 32 neighbouring elements share a power of two 2^(E - 127), one byte E;
  * an element is a code of `bits` bits, e4m3 (8) or e2m1 (4; two to a byte, the
- * even element in the low half), and stands for 2^(E - 127) code, exactly a bf16.
+ * even element in the low half), and stands for 2^(E - 127) code, exactly a bf16
+ * (with E from 10 on, which is all that the append writes; of lower ones what is below
+ * 2^-126 may count as 0).
  * kcache and vcache are blocks of bytes, shape.kv_stride BYTES apart (a multiple
  * of 16, at least mxfa_mx_block_bytes); in a block lie the codes [KV head][token]
  * [head_dim bits / 8], then the bytes E [KV head][token][head_dim / 32]. The other

@@ -200,8 +200,10 @@ __device__ __forceinline__ bool mx_row(typename MxOperand<T>::B (&f)[F::D / 32],
 }
 
 // Waits for Q's loads. The compiler knows of no others, and where a use may be the first
-// after them it waits until none of any kind is left: without this in every stage (64
-// sequences of 2000-16384, 32/8 heads, d = 128, 4 bits: 121 us and 110).
+// after them it waits until none of any kind is left: without this in every stage (the
+// kernel in us at the step that brought it, 64 sequences of 2000-16384, 32/8 heads, d = 128, 4
+// bits: 121 and 110; since Q comes a piece ahead, whole calls: 512 sequences of 900, 8 bits,
+// 190 and 185, others the same).
 template <class T, int N>
 __device__ __forceinline__ void mx_arrived(typename MxOperand<T>::B (&f)[N]) {
 #pragma unroll
