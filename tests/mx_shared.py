@@ -15,8 +15,8 @@ BS = 16
 # The launcher gives the few-row form 256 work-groups for all KV heads, which cut the
 # sequences' stages of 64 keys into equal runs, shared by the waves of each (8, beside
 # chunks 4): KV heads and single tokens by which a run is one sequence or a good part
-# of one.
-FORMS = {"one": (64, [1]), "few": (8, [1] * 31 + [2]), "both": (8, [1] * 31 + [40])}
+# of one. A chunk alone has the many-row form to itself.
+FORMS = {"one": (64, [1]), "few": (8, [1] * 31 + [2]), "both": (8, [1] * 31 + [40]), "many": (2, [300])}
 
 
 class Shared:
